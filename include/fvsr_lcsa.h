@@ -1,8 +1,8 @@
 /* fvsr_lcsa.h — C ABI of the MI355X (gfx950) LCSA path: FlashVSR's locality-constrained block-sparse
  * self-attention as called from the DiT self-attention block.
  *
- * Every entry point replaces one piece of the reference's call surface (xocialize/mlx-flashvsr-swift); the
- * reference function is cited beside each declaration. Conventions:
+ * Every entry point replaces one piece of the reference's call surface (xocialize/mlx-flashvsr-swift), and the reference
+ * function is cited beside each declaration, or says that it has no counterpart there. Conventions:
  *   - plain pointers and sizes only; device pointers are HIP device memory owned by the caller;
  *   - `stream` is a hipStream_t passed as void* (NULL = the default stream); no entry point synchronises the
  *     host, except that a call which needs more context workspace than the context holds grows it (hipFree +
@@ -254,6 +254,61 @@ int fvsr_dit_cross_kv(fvsr_ctx* ctx, const fvsr_dit_block_weights* w, int heads,
 int fvsr_dit_block(fvsr_ctx* ctx, fvsr_kv_ring* ring, int layer, const fvsr_dit_block_weights* w, const void* t_mod,
                    void* x, int n_new_slices, int t0, float eps, const float* rope_tables, const uint8_t* local_dev,
                    int topk, int mode, void* stream);
+
+/* ---- (f4) training and serving in 8 bits: layer norm, 8-bit activations, 8-bit linear layers ------------------- */
+/* No reference counterpart. An 8-bit matrix of `rows` x `channels`: each row is cut into runs of 128 channels (the last padded
+ * with zeros); a run has a scale 2^e, the smallest with e >= -127 and max |x| <= 448 * 2^e over its finite values, and each
+ * channel the e4m3 (OCP, no infinities) number nearest to x / 2^e, ties to even; infinities and NaN become NaN. `codes`: (rows,
+ * 128 * runs) bytes, 16-byte aligned; `scales`: the bytes e + 127 (E8M0), (rows, runs rounded up to a multiple of 4), 4-byte
+ * aligned, the bytes past the last run 0. Every value code * 2^e is exact in fp32.
+ * These entry points allocate nothing and use no context workspace: where they need memory beside their operands they take it
+ * as `workspace` (device memory, 16-byte aligned), which is free again when the call's work on `stream` is done. Calls on one
+ * context may therefore overlap, on any streams, and may be captured into HIP graphs. They leave the thread's current device as it
+ * was. Outputs must not overlap inputs or each other (dx may be dy). rows may be 0. */
+size_t fvsr_blocks8_code_bytes(int64_t rows, int channels);
+size_t fvsr_blocks8_scale_bytes(int64_t rows, int channels);
+/* x (rows, channels) `dtype` -> 8 bits; and back, each value rounded once to `dtype` (exact but for bf16's and fp32's range
+ * below 2^-126). channels <= 2^20. */
+int fvsr_quantize8(fvsr_ctx* ctx, int dtype, const void* x, int64_t rows, int channels, void* codes, void* scales,
+                   void* stream);
+int fvsr_dequantize8(fvsr_ctx* ctx, const void* codes, const void* scales, int64_t rows, int channels, int dtype, void* out,
+                     void* stream);
+
+/* Layer norm of each row: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), in fp32, rounded once. weight and
+ * bias (channels), of `param_dtype` (fp32, or the tokens' `dtype`), may be NULL. With weight = 1 + scale and bias = shift it is
+ * the modulated norm of a DiT block. Any of these results may be left out (NULL): y in `dtype`; y in 8 bits, from its fp32
+ * values (y or y_codes must be given); x in 8 bits, a checkpoint for the backward pass; stats, (rows, 2) fp32 mean and rstd.
+ * channels <= 16384. */
+int fvsr_layer_norm(fvsr_ctx* ctx, int dtype, const void* x, int64_t rows, int channels, float eps, int param_dtype,
+                    const void* weight, const void* bias, void* y, void* y_codes, void* y_scales, void* x_codes,
+                    void* x_scales, float* stats, void* stream);
+/* Its gradient. With n = (x - mean) * rstd and g = dy * weight: dx = rstd * (g - mean(g) - n * mean(g * n)) in `dtype`;
+ * dweight = sum over the rows of dy * n and dbias = sum of dy, fp32 (channels), either or both NULL. x as it was (`dtype`), or
+ * in 8 bits (x NULL, x_codes and x_scales given); stats from the forward call. No atomics: the same inputs give the same bits.
+ * With rows = 0, dweight and dbias are zeros. */
+size_t fvsr_layer_norm_backward_workspace(int64_t rows, int channels);
+int fvsr_layer_norm_backward(fvsr_ctx* ctx, int dtype, const void* dy, const void* x, const void* x_codes,
+                             const void* x_scales, const float* stats, int64_t rows, int channels, int param_dtype,
+                             const void* weight, void* dx, float* dweight, float* dbias, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* y = x W^T + bias, optionally through the tanh form of GELU, from 8-bit x (rows, in_features) and W (out_features,
+ * in_features), y (rows, out_features) rounded once to `y_dtype`. Sums are kept in fp32; of 8 neighbouring channels' products
+ * the matrix cores keep 13 bits below the largest one's exponent before they add them (less than half a step of bf16 of the result, but
+ * more than one of an fp32 y). x may be given as tokens of
+ * `x_dtype`: they are quantized into x_codes / x_scales first (which can be kept as the layer's checkpoint); with x NULL those hold
+ * the 8-bit tokens. bias (out_features) of `bias_dtype`, or NULL. The input gradient is the same call: dx = dy (W^T)^T, with
+ * the quantized transpose of W (in_features rows of out_features). */
+size_t fvsr_linear8_workspace(int64_t rows, int in_features, int out_features);
+int fvsr_linear8(fvsr_ctx* ctx, int x_dtype, const void* x, int64_t rows, int in_features, void* x_codes, void* x_scales,
+                 const void* w_codes, const void* w_scales, int out_features, int bias_dtype, const void* bias, int gelu,
+                 int y_dtype, void* y, void* workspace, size_t workspace_bytes, void* stream);
+/* Its weight gradient: dw (out_features, in_features) = dy^T x from bf16 dy (rows, out_features) and the 8-bit x, products and sums
+ * in fp32, `dw_dtype`; db = the sum of dy's rows, fp32 (out_features), or NULL. The same inputs give the same bits. */
+size_t fvsr_linear8_weight_grad_workspace(int64_t rows, int in_features, int out_features);
+int fvsr_linear8_weight_grad(fvsr_ctx* ctx, const void* dy, int64_t rows, int out_features, const void* x_codes,
+                             const void* x_scales, int in_features, int dw_dtype, void* dw, float* db, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ---- (a1) window layout ------------------------------------------------------------------------------------ */
 /* Replace `windowPartition` / `windowReverse` (DiT.swift:113-126): (f*h*w, C) natural <-> window order. */

@@ -123,6 +123,10 @@ struct fvsr_kv_ring {
   int64_t head_stride() const { return (int64_t)layer_tokens() * kHeadDim; }   // elements between heads of a layer
 };
 
+namespace fvsr {
+int ctx_device(const fvsr_ctx* ctx) { return ctx->device; }
+}  // namespace fvsr
+
 #define FVSR_REQUIRE(cond, status, msg) \
   do {                                  \
     if (!(cond)) return set_error((status), (msg)); \

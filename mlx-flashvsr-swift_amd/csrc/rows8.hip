@@ -1,0 +1,411 @@
+// Row operators next to the 8-bit products, for gfx950 (MI355X): tokens to 8 bits and back, and layer norm with its gradient, which
+// write and read the 8-bit form in the passes that hold the row anyway.
+//
+//   y  = n w + b,  n = (x - mean) rstd,  rstd = 1 / sqrt(var + eps)      (mean and var over the row's C channels)
+//   dx = rstd (g - mean(g) - n mean(g n)),  g = dy w
+//   dw = sum over rows of dy n,  db = sum over rows of dy
+//
+// All of them move each row once and compute a few operations a channel: memory-bound. A row's channels stay in registers
+// between the passes over it (sums, then squares, then the result), in 32 bits.
+#include <algorithm>
+
+#include "blocks8.hpp"
+
+namespace fvsr {
+
+struct NormArgs {
+  const void* x;
+  int64_t rows;
+  int C;
+  float eps;
+  const void *w, *b;   // either may be null
+  void* y;             // null: not written
+  Out8 y8, x8;         // codes null: not written
+  float* stats;        // (rows, 2) mean, rstd; may be null
+};
+
+struct NormGradArgs {
+  const void *dy, *x;   // x null: read from x8
+  In8 x8;
+  const float* stats;
+  int64_t rows;
+  int C;
+  const void* w;        // may be null
+  void* dx;
+  float* part;          // (blocks, 2, C) partial dw and db; null: neither is made
+};
+
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// sums over the WAVES waves that share a row, in a fixed order; `sm` holds 2 * WAVES floats and is free for reuse after the
+// call's second barrier only, so successive calls alternate between two areas
+template <int WAVES>
+__device__ __forceinline__ void team_sum2(float& a, float& b, float* sm) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (WAVES > 1) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      sm[2 * wave] = a;
+      sm[2 * wave + 1] = b;
+    }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      a += sm[2 * w];
+      b += sm[2 * w + 1];
+    }
+  }
+}
+
+// One row a team of WAVES waves (a workgroup holds max(WAVES, 4) waves), NV vectors of 8 channels a lane: lane L of the team and
+// vector j hold 8 channels of run 4 * WAVES * j + L / 16.
+template <typename T, typename P, bool VEC, int WAVES, int NV>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kernel(NormArgs a) {
+  __shared__ float sm[2][2 * WAVES];
+  const int l16 = threadIdx.x & 15, C = a.C;
+  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (row >= a.rows) return;   // WAVES > 1: never (one row a workgroup)
+  const int run0 = (WAVES == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x) >> 4;
+  const T* x = (const T*)a.x + row * C;
+  const int runs = runs_of(C), ss = scale_stride(C);
+  float v[NV][8];
+  float sum = 0.f, none = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    load8<T, VEC>(x, (run0 + 4 * WAVES * j) * kRun, l16, C, v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[j][e];
+  }
+  team_sum2<WAVES>(sum, none, sm[0]);
+  const float mean = sum / (float)C;
+  if (a.x8.codes) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int run = run0 + 4 * WAVES * j;
+      uint32_t s;
+      const uint2 c = encode8(v[j], s);
+      if (run < runs) store_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16, c);
+      if (run < ss && l16 == 0) a.x8.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
+    }
+  }
+  float sq = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c0 = (run0 + 4 * WAVES * j) * kRun;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[j][e] = c0 + run_channel<VEC>(l16, e) < C ? v[j][e] - mean : 0.f;
+      sq = fmaf(v[j][e], v[j][e], sq);
+    }
+  }
+  team_sum2<WAVES>(sq, none, sm[1]);
+  const float rstd = 1.f / sqrtf(sq / (float)C + a.eps);
+  if (a.stats && (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) == 0) {
+    a.stats[2 * row] = mean;
+    a.stats[2 * row + 1] = rstd;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int run = run0 + 4 * WAVES * j;
+    float w[8], b[8], y[8];
+    if (a.w) load8<P, VEC>((const P*)a.w, run * kRun, l16, C, w);
+    if (a.b) load8<P, VEC>((const P*)a.b, run * kRun, l16, C, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = v[j][e] * rstd;
+      if (a.w) y[e] *= w[e];
+      if (a.b) y[e] += b[e];
+      if (run * kRun + run_channel<VEC>(l16, e) >= C) y[e] = 0.f;   // also where the row's rstd is not finite
+    }
+    if (a.y) store8<T, VEC>((T*)a.y + row * C, run * kRun, l16, C, y);
+    if (a.y8.codes) {
+      uint32_t s;
+      const uint2 c = encode8(y, s);
+      if (run < runs) store_codes<VEC>(a.y8.codes + (row * runs + run) * kRun, l16, c);
+      if (run < ss && l16 == 0) a.y8.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
+    }
+  }
+}
+
+// The gradient: teams walk over the rows (the grid is a fixed number of workgroups) and keep their part of dw and db in
+// registers; the workgroup's sum goes to `part`, and param_sum_kernel adds the workgroups' up: no atomics, the same result
+// every time.
+template <typename T, typename P, bool VEC, int WAVES, int NV, bool X8>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad_kernel(NormGradArgs a) {
+  __shared__ float sm[2][2 * WAVES];
+  __shared__ float join[WAVES == 1 ? 4 * 64 * 16 : 1];
+  const int l16 = threadIdx.x & 15, lane = threadIdx.x & 63, C = a.C;
+  const int team = WAVES == 1 ? (int)(threadIdx.x >> 6) : 0, teams = WAVES == 1 ? 4 : 1;
+  const int run0 = (WAVES == 1 ? lane : (int)threadIdx.x) >> 4;
+  const int runs = runs_of(C), ss = scale_stride(C);
+  float w[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (a.w) load8<P, VEC>((const P*)a.w, (run0 + 4 * WAVES * j) * kRun, l16, C, w[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!a.w) w[j][e] = 1.f;
+      dw[j][e] = db[j][e] = 0.f;
+    }
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * teams + team; row < a.rows; row += (int64_t)gridDim.x * teams, turn ^= 1) {
+    const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
+    float dy[NV][8], n[NV][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int run = run0 + 4 * WAVES * j;
+      load8<T, VEC>((const T*)a.dy + row * C, run * kRun, l16, C, dy[j]);
+      if constexpr (X8) {
+        if (run < runs) {
+          decode8(load_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16), a.x8.scales[row * ss + run], n[j]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) n[j][e] = 0.f;
+        }
+      } else {
+        load8<T, VEC>((const T*)a.x + row * C, run * kRun, l16, C, n[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        n[j][e] = (n[j][e] - mean) * rstd;   // past C: dy is 0, so the value does not matter (it is finite where the row's are)
+        const float g = dy[j][e] * w[j][e];
+        s1 += g;
+        s2 = fmaf(g, n[j][e], s2);
+        dw[j][e] = fmaf(dy[j][e], n[j][e], dw[j][e]);
+        db[j][e] += dy[j][e];
+      }
+    team_sum2<WAVES>(s1, s2, sm[turn]);
+    const float m1 = s1 / (float)C, m2 = s2 / (float)C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float dx[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dx[e] = rstd * (dy[j][e] * w[j][e] - m1 - n[j][e] * m2);
+      store8<T, VEC>((T*)a.dx + row * C, (run0 + 4 * WAVES * j) * kRun, l16, C, dx);
+    }
+  }
+  if (!a.part) return;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c0 = (run0 + 4 * WAVES * j) * kRun;
+    if constexpr (WAVES == 1) {
+      // the 4 waves hold the same channels: their sums meet in LDS, [wave][16 values][lane]
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        join[(team * 16 + e) * 64 + lane] = dw[j][e];
+        join[(team * 16 + 8 + e) * 64 + lane] = db[j][e];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int k = 4 * team + q;   // value k of lane `lane`: element k % 8 of dw (k < 8) or db
+        const float s = (join[k * 64 + lane] + join[(16 + k) * 64 + lane]) +
+                        (join[(32 + k) * 64 + lane] + join[(48 + k) * 64 + lane]);
+        const int c = c0 + run_channel<VEC>(l16, k & 7);
+        if (c < C) part[(k < 8 ? 0 : C) + c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = c0 + run_channel<VEC>(l16, e);
+        if (c < C) {
+          part[c] = dw[j][e];
+          part[C + c] = db[j][e];
+        }
+      }
+    }
+  }
+}
+
+// out[c] = sum over p < parts of part[p * stride + c], c < n: 64 columns a workgroup, 4 quarters of the parts, in a fixed order
+__global__ __launch_bounds__(256) void param_sum_kernel(const float* __restrict__ part, int parts, int64_t stride, int n,
+                                                        float* __restrict__ out) {
+  __shared__ float sm[256];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < n) {
+    int p = q;
+    for (; p + 12 < parts; p += 16)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(p + 4 * u) * stride + c];
+    for (; p < parts; p += 4) s[0] += part[(int64_t)p * stride + c];
+  }
+  sm[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (q == 0 && c < n) out[c] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
+}
+
+// A wave takes 4 runs of a row (one word of scales), 16 lanes each.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t rows, int C, Out8 o) {
+  const int l16 = threadIdx.x & 15, r4 = (threadIdx.x & 63) >> 4;
+  const int runs = runs_of(C), ss = scale_stride(C), words = ss / 4;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = unit / words;
+  if (row >= rows) return;
+  const int run = (int)(unit - row * words) * 4 + r4;
+  float v[8];
+  load8<T, VEC>(x + row * C, run * kRun, l16, C, v);
+  uint32_t s;
+  const uint2 c = encode8(v, s);
+  if (run < runs) store_codes<VEC>(o.codes + (row * runs + run) * kRun, l16, c);
+  if (l16 == 0) o.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dequantize_kernel(In8 q, int64_t rows, int C, T* __restrict__ out) {
+  const int l16 = threadIdx.x & 15, r4 = (threadIdx.x & 63) >> 4;
+  const int runs = runs_of(C), ss = scale_stride(C), words = ss / 4;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = unit / words;
+  if (row >= rows) return;
+  const int run = (int)(unit - row * words) * 4 + r4;
+  if (run >= runs) return;
+  float v[8];
+  decode8(load_codes<VEC>(q.codes + (row * runs + run) * kRun, l16), q.scales[row * ss + run], v);
+  store8<T, VEC>(out + row * C, run * kRun, l16, C, v);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// launches
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kMaxNormChannels = 16384;
+constexpr int kGradBlocks = 512;   // two workgroups a CU
+
+// a launch's work-items have to stay below 2^32
+static int check_grid(int64_t blocks, int threads) {
+  if (blocks >= (((int64_t)1 << 32) - 1) / threads) return set_error(FVSR_ERR_UNSUPPORTED, "too many rows for one launch");
+  return FVSR_OK;
+}
+
+// f(waves a row, vectors a lane): one wave up to 2048 channels, 4 up to 8192, 16 up to 16384, with just the registers they need
+template <class F>
+static int pick_team(int C, F&& f) {
+  const int nv = (int)ceil_div(C, 512);
+  if (nv <= 4) {
+    switch (nv) {
+      case 1: f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}); break;
+      case 2: f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}); break;
+      case 3: f(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{}); break;
+      default: f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}); break;
+    }
+  } else if (nv <= 16) {
+    switch ((nv + 3) / 4) {
+      case 2: f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
+      case 3: f(std::integral_constant<int, 4>{}, std::integral_constant<int, 3>{}); break;
+      default: f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}); break;
+    }
+  } else {
+    f(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
+  }
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+// f(element type, parameter type, whether rows are read 16 bytes at a time)
+template <class F>
+static int pick_types(int dtype, int param_dtype, bool vec, F&& f) {
+  auto with = [&](auto t, auto p) { return vec ? f(t, p, std::true_type{}) : f(t, p, std::false_type{}); };
+  if (dtype == FVSR_DTYPE_BF16) return param_dtype == FVSR_DTYPE_BF16 ? with(bf16{}, bf16{}) : with(bf16{}, float{});
+  return with(float{}, float{});   // fp32 tokens take fp32 parameters
+}
+
+int max_norm_channels() { return kMaxNormChannels; }
+
+int launch_layer_norm(int dtype, int param_dtype, const void* x, int64_t rows, int C, float eps, const void* w,
+                      const void* b, void* y, Out8 y8, Out8 x8, float* stats, hipStream_t stream) {
+  if (rows <= 0) return FVSR_OK;
+  if (const int rc = check_grid(rows, C <= 2048 ? 64 : C <= 8192 ? 256 : 1024)) return rc;
+  const NormArgs a{x, rows, C, eps, w, b, y, y8, x8, stats};
+  const bool vec = rows_vectorize(x, C) && rows_vectorize(w, C) && rows_vectorize(b, C) && rows_vectorize(y, C);
+  return pick_types(dtype, param_dtype, vec, [&](auto t, auto p, auto v) {
+    return pick_team(C, [&](auto waves, auto nv) {
+      constexpr int W = decltype(waves)::value;
+      hipLaunchKernelGGL((layer_norm_kernel<decltype(t), decltype(p), decltype(v)::value, W, decltype(nv)::value>),
+                         dim3((unsigned)(W == 1 ? ceil_div(rows, 4) : rows)), dim3(W == 1 ? 256 : 64 * W), 0, stream, a);
+    });
+  });
+}
+
+int64_t norm_grad_blocks(int64_t rows, int C) {
+  return std::min<int64_t>(kGradBlocks, C <= 2048 ? ceil_div(rows, 4) : rows);
+}
+
+int launch_layer_norm_grad(int dtype, int param_dtype, const void* dy, const void* x, In8 x8, const float* stats,
+                           int64_t rows, int C, const void* w, void* dx, float* dw, float* db, float* part,
+                           hipStream_t stream) {
+  const bool vec = rows_vectorize(dy, C) && rows_vectorize(x, C) && rows_vectorize(w, C) && rows_vectorize(dx, C);
+  const int64_t blocks = norm_grad_blocks(rows, C);
+  if (blocks > 0) {
+    const NormGradArgs a{dy, x, x8, stats, rows, C, w, dx, dw || db ? part : nullptr};
+    const int rc = pick_types(dtype, param_dtype, vec, [&](auto t, auto p, auto v) {
+      return pick_team(C, [&](auto waves, auto nv) {
+        constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
+        constexpr bool V = decltype(v)::value;
+        const dim3 grid((unsigned)blocks), block(W == 1 ? 256 : 64 * W);
+        if (x8.codes)
+          hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(t), decltype(p), V, W, N, true>), grid, block, 0, stream, a);
+        else
+          hipLaunchKernelGGL((layer_norm_grad_kernel<decltype(t), decltype(p), V, W, N, false>), grid, block, 0, stream, a);
+      });
+    });
+    if (rc) return rc;
+  }
+  const dim3 grid((unsigned)ceil_div(C, 64));
+  if (dw) hipLaunchKernelGGL(param_sum_kernel, grid, dim3(256), 0, stream, part, (int)blocks, (int64_t)2 * C, C, dw);
+  if (db) hipLaunchKernelGGL(param_sum_kernel, grid, dim3(256), 0, stream, part + C, (int)blocks, (int64_t)2 * C, C, db);
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+int launch_param_sum(const float* part, int parts, int64_t stride, int n, float* out, hipStream_t stream) {
+  hipLaunchKernelGGL(param_sum_kernel, dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, stream, part, parts, stride, n, out);
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+int launch_quantize(int dtype, const void* x, int64_t rows, int C, Out8 o, hipStream_t stream) {
+  if (rows <= 0) return FVSR_OK;
+  const bool vec = rows_vectorize(x, C);
+  const int64_t blocks = ceil_div(rows * (scale_stride(C) / 4), 4);
+  if (const int rc = check_grid(blocks, 256)) return rc;
+  auto go = [&](auto t, auto v) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((quantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream,
+                       (const T*)x, rows, C, o);
+  };
+  if (dtype == FVSR_DTYPE_BF16) vec ? go(bf16{}, std::true_type{}) : go(bf16{}, std::false_type{});
+  else vec ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+int launch_dequantize(In8 q, int64_t rows, int C, int dtype, void* out, hipStream_t stream) {
+  if (rows <= 0) return FVSR_OK;
+  const bool vec = rows_vectorize(out, C);
+  const int64_t blocks = ceil_div(rows * (scale_stride(C) / 4), 4);
+  if (const int rc = check_grid(blocks, 256)) return rc;
+  auto go = [&](auto t, auto v) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((dequantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, q, rows,
+                       C, (T*)out);
+  };
+  if (dtype == FVSR_DTYPE_BF16) vec ? go(bf16{}, std::true_type{}) : go(bf16{}, std::false_type{});
+  else vec ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+}  // namespace fvsr

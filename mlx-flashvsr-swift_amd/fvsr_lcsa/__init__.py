@@ -13,6 +13,8 @@ Names mirror the reference's call surface (xocialize/mlx-flashvsr-swift):
   qkv_epilogue                normQ/normK + ropeApply + windowPartition          DiT.swift:34-47,100-118,496-506
   linear                      Linear (+ GELU tanh) on hipBLASLt                  DiT.swift:319-321,371
   DiTBlock                    DiTBlock + blockForward (streaming)               DiT.swift:363-375,491-551
+and, without a counterpart there, what training and serving the dense layers in 8 bits takes (train8.py): Blocks8, quantize8,
+dequantize8, layer_norm, layer_norm_backward, linear8, linear8_weight_grad.
 Token tensors are (L, H*128) or (1, L, H*128), window order, float32 or bfloat16, on a HIP device, contiguous.
 Every call runs the HIP kernels of libfvsr_lcsa.so; there is no CPU fallback.
 """
@@ -30,7 +32,8 @@ from ._abi import (ATTN_AUTO, ATTN_DENSE, ATTN_KERNEL, DTYPE_BF16, DTYPE_F32, LA
 __all__ = ["FVSRError", "Context", "local_block_mask", "draft_block_mask_and_probs", "draft_block_mask",
            "kernel_block_attention", "block_masked_attention", "block_sparse_attention", "FlashVSRAttentionOps",
            "KVRing", "window_partition", "window_reverse", "attention_mode_auto", "workspace_size",
-           "rope_tables", "rope_tables_device", "qkv_epilogue", "linear", "DiTBlock",
+           "rope_tables", "rope_tables_device", "qkv_epilogue", "linear", "DiTBlock", "Blocks8", "quantize8",
+           "dequantize8", "layer_norm", "layer_norm_backward", "linear8", "linear8_weight_grad",
            "ATTN_AUTO", "ATTN_DENSE", "ATTN_KERNEL", "LAYOUT_GRID", "LAYOUT_WINDOWS", "lib"]
 
 HEAD_DIM = 128
@@ -646,3 +649,7 @@ class DiTBlock:
         call("fvsr_dit_block", ring.ctx.handle, ring.handle, layer, C.byref(w), _ptr(tm), _ptr(x2), n_new_slices, t0,
              float(self.eps), _ptr(tab), _ptr(ring.ctx.local_device(local, ring.s)), topk, mode, _stream(stream))
         return x
+
+
+from .train8 import (Blocks8, dequantize8, layer_norm, layer_norm_backward, linear8,  # noqa: E402
+                     linear8_weight_grad, quantize8)

@@ -56,6 +56,17 @@ SIGNATURES = {
     "fvsr_linear": (_i, [_vp, _vp, _i64, _i, _vp, _i, _vp, _i, _vp, _vp]),
     "fvsr_dit_cross_kv": (_i, [_vp, _vp, _i, _vp, _i, C.c_float, _vp, _vp, _vp]),
     "fvsr_dit_block": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, C.c_float, _vp, _vp, _i, _i, _vp]),
+    "fvsr_blocks8_code_bytes": (_sz, [_i64, _i]),
+    "fvsr_blocks8_scale_bytes": (_sz, [_i64, _i]),
+    "fvsr_quantize8": (_i, [_vp, _i, _vp, _i64, _i, _vp, _vp, _vp]),
+    "fvsr_dequantize8": (_i, [_vp, _vp, _vp, _i64, _i, _i, _vp, _vp]),
+    "fvsr_layer_norm": (_i, [_vp, _i, _vp, _i64, _i, C.c_float, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "fvsr_layer_norm_backward_workspace": (_sz, [_i64, _i]),
+    "fvsr_layer_norm_backward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fvsr_linear8_workspace": (_sz, [_i64, _i, _i]),
+    "fvsr_linear8": (_i, [_vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _sz, _vp]),
+    "fvsr_linear8_weight_grad_workspace": (_sz, [_i64, _i, _i]),
+    "fvsr_linear8_weight_grad": (_i, [_vp, _vp, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     "fvsr_window_partition": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _vp]),
     "fvsr_window_reverse": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _vp]),
 }
