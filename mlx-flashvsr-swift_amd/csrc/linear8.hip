@@ -22,13 +22,19 @@ __device__ __forceinline__ u32x4 make_rsrc(const void* base, uint32_t bytes) {
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const lds_char*)p);
 }
-// 16 (or 4) bytes a lane from a buffer straight into LDS at `lds` + 16 (4) * lane; what lies past the buffer's end is stored as
-// 0. The copy is waited for with vmcnt. One wait state has to pass between the write of M0 and its use, hence the s_nop.
-__device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t lds, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
+// 16 (or 4) bytes a lane from a buffer straight into LDS at `lds` + 16 (4) * lane; the address is the lane's offset plus the common
+// one. The copy is waited for with vmcnt. One wait state has to pass between the write of M0 and its use, hence the s_nop.
+// x, not known to be what it was before: what is computed from it in a loop is computed there, and takes no registers across it
+__device__ __forceinline__ uint32_t afresh(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
-__device__ __forceinline__ void copy4(u32x4 rsrc, uint32_t lds, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t lds, uint32_t off, uint32_t common) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off), "s"(rsrc), "s"(uniform(common)));
+}
+__device__ __forceinline__ void copy4(u32x4 rsrc, uint32_t lds, uint32_t off, uint32_t common) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off), "s"(rsrc), "s"(uniform(common)));
 }
 
 struct Linear8Args {
@@ -49,6 +55,44 @@ __device__ __forceinline__ float gelu_tanh(float y) {
   return y * __builtin_amdgcn_rcpf(1.f + e);
 }
 
+// bias (fp32, in LDS, at this lane's first feature), GELU and the store of a wave's fragments: this lane's features n0 + 32 p .. + 7
+// (two fragments) of the tokens row0 + 16 m
+template <int FN, int FM, typename O>
+__device__ __forceinline__ void write_tile(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
+                                           int64_t row0) {
+  float b[FN / 2][8];
+#pragma unroll
+  for (int p = 0; p < FN / 2; ++p) {
+    *(f32x4*)b[p] = *(const f32x4*)(bias + 32 * p);
+    *(f32x4*)(b[p] + 4) = *(const f32x4*)(bias + 32 * p + 4);
+  }
+#pragma unroll
+  for (int m = 0; m < FM; ++m) {
+    const int64_t row = row0 + 16 * m;
+    if (row >= a.rows) continue;
+#pragma unroll
+    for (int p = 0; p < FN / 2; ++p) {
+      const int n = n0 + 32 * p;
+      O v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float s = acc[2 * p + (e >> 2)][m][e & 3] + b[p][e];
+        if (a.gelu) s = gelu_tanh(s);
+        v[e] = (O)s;
+      }
+      O* out = y + row * a.N + n;
+      if (a.vec_out && n + 8 <= a.N) {
+        *(u32x4*)out = *(u32x4*)v;
+        if constexpr (sizeof(O) == 4) ((u32x4*)out)[1] = ((u32x4*)v)[1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < a.N) out[e] = v[e];
+      }
+    }
+  }
+}
+
 // Tile of TN output features x TM tokens, WN x WM waves; a step is one run: 128 codes of every row, and their scales in the
 // matrix instruction.
 //
@@ -64,9 +108,11 @@ __device__ __forceinline__ float gelu_tanh(float y) {
 template <int TN, int TM, int WN, int WM, typename O>
 __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a) {
   constexpr int kWaves = WN * WM, FN = TN / WN / 16, FM = TM / WM / 16;
-  static_assert(FN % 2 == 0 && (TN + TM) % (8 * kWaves) == 0 && (TN + TM) % 64 == 0, "tile");
+  static_assert(FN % 2 == 0 && TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0, "tile");
+  static_assert((TN + TM) / kWaves <= 64 && TN % ((TN + TM) / kWaves) == 0, "a wave's rows of scales belong to one operand");
   constexpr int kStage = (TN + TM) * kRun, kScales = (TN + TM) * 4;
-  __shared__ __align__(1024) char sm[2 * kStage + 2 * kScales];
+  __shared__ __align__(1024) char sm[2 * kStage + 2 * kScales + TN * 4];
+  float* const bias = (float*)(sm + 2 * kStage + 2 * kScales);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // tiles: every XCD a contiguous range, ordered in bands of 8 tiles of tokens so that a band's codes and the weights stay in its L2
   const int t = xcd_remap(blockIdx.x, gridDim.x);
@@ -84,27 +130,33 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
   const u32x4 sx = make_rsrc(a.x.scales + m0 * a.ss, (uint32_t)rows_m * a.ss);
   const uint32_t lds0 = lds_offset(sm);
 
-  auto swz_w = [](int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); };
-  auto swz_x = [](int r) { return (r >> 1) & 7; };
-  auto copy_step = [&](int k) {
-    const uint32_t base = lds0 + (k & 1) * kStage;
-    static_for<0, (TN + TM) / (8 * kWaves)>([&](auto ic) {
-      const int r8 = (decltype(ic)::value * kWaves + wave) * 8;   // 8 rows a wave and copy
-      const int r = r8 + (lane >> 3), c = lane & 7;
-      if (r8 < TN)
-        copy16(rw, base + r8 * kRun, (uint32_t)(r * ld + k * kRun + ((c ^ swz_w(r)) << 4)));
-      else
-        copy16(rx, base + r8 * kRun, (uint32_t)((r - TN) * ld + k * kRun + ((c ^ swz_x(r - TN)) << 4)));
-    });
-    if ((k & 3) == 0) {
-      const uint32_t sbase = lds0 + 2 * kStage + ((k >> 2) & 1) * kScales;
+  auto swz = [](int i, int q) { return ((i >> 1) & 1) | ((q >> 1) << 1) | (((q ^ (q >> 1)) & 1) << 2); };
+  auto swz_w = [&](int r) { return swz(r & 3, (r >> 3) & 3); };
+  auto swz_x = [&](int r) { return swz(r & 3, (r >> 2) & 3); };
+  // a lane's source offsets: of 8 rows a wave and copy, and of a word of scales a row. Rows past the last one read it again (their
+  // results are not stored).
+  constexpr int kCW = TN / (8 * kWaves), kCX = TM / (8 * kWaves), kScaleRows = (TN + TM) / kWaves;
+  uint32_t ow[kCW], ox[kCX];
 #pragma unroll
-      for (int r64 = wave * 64; r64 < TN + TM; r64 += kWaves * 64) {
-        const int r = r64 + lane;
-        if (r64 < TN) copy4(sw, sbase + r64 * 4, (uint32_t)(r * a.ss + k));
-        else copy4(sx, sbase + r64 * 4, (uint32_t)((r - TN) * a.ss + k));
-      }
-    }
+  for (int c = 0; c < kCW; ++c) {
+    const int r = (c * kWaves + wave) * 8 + (lane >> 3);
+    ow[c] = (uint32_t)(min(r, rows_n - 1) * ld + (((lane & 7) ^ swz_w(r)) << 4));
+  }
+#pragma unroll
+  for (int c = 0; c < kCX; ++c) {
+    const int r = (c * kWaves + wave) * 8 + (lane >> 3);
+    ox[c] = (uint32_t)(min(r, rows_m - 1) * ld + (((lane & 7) ^ swz_x(r)) << 4));
+  }
+  const int sr = wave * kScaleRows + (lane & (kScaleRows - 1));   // this lane's row of scales
+  const bool s_of_w = wave * kScaleRows < TN;
+  const uint32_t so = (uint32_t)((s_of_w ? min(sr, rows_n - 1) : min(sr - TN, rows_m - 1)) * a.ss);
+  const u32x4 rs = s_of_w ? sw : sx;
+  auto copy_step = [&](int k) {
+    const uint32_t base = lds0 + (k & 1) * kStage + wave * 8 * kRun;
+    static_for<0, kCW>([&](auto c) { copy16(rw, base + c * kWaves * 8 * kRun, ow[c], k * kRun); });
+    static_for<0, kCX>([&](auto c) { copy16(rx, base + TN * kRun + c * kWaves * 8 * kRun, ox[c], k * kRun); });
+    if ((k & 3) == 0 && lane < kScaleRows)
+      copy4(rs, lds0 + 2 * kStage + ((k >> 2) & 1) * kScales + wave * kScaleRows * 4, so, k);
   };
 
   const int wn = wave % WN, wm = wave / WN, i = lane & 15, g = lane >> 4;
@@ -123,6 +175,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
     for (int m = 0; m < FM; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   copy_step(0);
+  for (int n = threadIdx.x; n < TN; n += 64 * kWaves)
+    bias[n] = !a.bias || n0 + n >= a.N ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n0 + n] : (float)((const bf16*)a.bias)[n0 + n];
   int qw[FN], qx[FM];
   for (int k0 = 0; k0 < a.runs; k0 += 4) {
     static_for<0, 4>([&](auto kc) {
@@ -156,56 +210,270 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
     });
   }
 
-  O* y = (O*)a.y;
-#pragma unroll
-  for (int p = 0; p < FN / 2; ++p) {
-    const int n = n0 + wn * (TN / WN) + 32 * p + 8 * g;
-    float b[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      b[e] = !a.bias || n + e >= a.N ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n + e] : (float)((const bf16*)a.bias)[n + e];
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      const int64_t row = m0 + rx0 + 16 * m;
-      if (row >= a.rows) continue;
-      O v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float s = acc[2 * p + (e >> 2)][m][e & 3] + b[e];
-        if (a.gelu) s = gelu_tanh(s);
-        v[e] = (O)s;
-      }
-      O* out = y + row * a.N + n;
-      if (a.vec_out && n + 8 <= a.N) {
-        *(u32x4*)out = *(u32x4*)v;
-        if constexpr (sizeof(O) == 4) ((u32x4*)out)[1] = ((u32x4*)v)[1];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < a.N) out[e] = v[e];
-      }
-    }
-  }
+  const int fn = wn * (TN / WN) + 8 * g;
+  write_tile(a, acc, (O*)a.y, bias + fn, n0 + fn, m0 + rx0);
 }
 
-size_t linear8_workspace(int64_t, int, int) { return 0; }
+// The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between them. Two groups
+// of four waves, one of each on every SIMD, take turns: while one group's 32 matrix instructions of a step (a run: 128 codes of every
+// row) go, the other reads its operands of the step into registers and asks for later ones. A phase ends with a barrier; steps s are
+// counted across tiles, LDS holds two of them, and wave w of a group computes features 64 w .. 64 w + 63 of the group's 128 tokens:
+//
+//   phase      2s                                       2s + 1
+//   group 0    copy group 1's tokens of s + 1, read(s)  multiply(s)
+//   group 1    multiply(s - 1)                          copy group 0's tokens of s + 2, read(s), copy the weights of s + 2
+//
+// Everything is asked for as soon as its place is free: group 0's tokens of step s have been read when phase 2s ends, group 1's when
+// phase 2s + 1 ends; the weights that wave w of group 1 reads in phase 2s + 1 wave w of group 0 has read before, so it replaces them at
+// once. Each is needed about three phases later, and its wave waits for it at the end of that time, by the count of what it has
+// asked for since (memory operations of a wave complete in order). A group writes its tile, and starts the next one, in its read
+// phase, under the other group's products.
+template <typename O>
+__global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
+  constexpr int FN = 4, FM = 8, kStores = FN / 2 * FM * (int)sizeof(O) / 2;
+  constexpr int kBuf = 256 * kRun;                         // one operand's rows of a step
+  constexpr int kX = 2 * kBuf, kS = 4 * kBuf;              // LDS: weights of two steps, tokens of two steps,
+  constexpr int kScales = 512 * 4, kB = kS + 4 * kScales;  // scales of 4 x 4 steps, biases of 4 tiles
+  __shared__ __align__(1024) char sm[kB + 4 * 1024];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave >> 2, w = wave & 3, i = lane & 15, g = lane >> 4;
+  const int G = a.runs, ld = G * kRun;
+  const uint32_t lds0 = lds_offset(sm);
+  // chunk c of row r of the weights lies at c ^ swz(r % 4, r / 8 % 4), of the tokens at c ^ swz(r % 4, r / 4 % 4): the 16 rows that a cycle
+  // of a 16-byte read serves (of a fragment: features 8 (i / 4) + i % 4, tokens i) then lie on different banks
+  auto swz = [](int r, int q) { return ((r >> 1) & 1) | ((q >> 1) << 1) | (((q ^ (q >> 1)) & 1) << 2); };
+  const int rw0 = w * 64 + ((i >> 2) << 3) + (i & 3), rx0 = group * 128 + i;
+  const char* pw[2];
+  const char* px[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pw[h] = sm + rw0 * kRun + (((2 * g + h) ^ swz(rw0 & 3, (rw0 >> 3) & 3)) << 4);
+    px[h] = sm + kX + rx0 * kRun + (((2 * g + h) ^ swz(rx0 & 3, (rx0 >> 2) & 3)) << 4);
+  }
+  // copies: 8 rows an instruction, this wave's 64 rows of weights and 32 of the other group's tokens; a lane's source of rows 8 c + r8 is
+  // 8 c rows on, its chunk XOR-ed by what c adds to swz
+  const int r8 = lane >> 3, cs = ((lane & 7) ^ ((r8 >> 1) & 1)) << 4;
+  const uint32_t ow = (uint32_t)(r8 * ld + cs), ox = (uint32_t)(r8 * ld + (cs ^ ((r8 >> 2) << 6)));
+  const uint32_t os = (uint32_t)(lane * a.ss);
+
+  // this workgroup's tiles: every XCD walks over a contiguous range of them, in bands of 8 tiles of tokens
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int xcd = blockIdx.x % kXcds, per = (int)gridDim.x / kXcds;   // the grid is a multiple of the XCDs
+  const int first = xcd * (tiles / kXcds) + min(xcd, tiles % kXcds);
+  const int end = first + tiles / kXcds + (xcd < tiles % kXcds ? 1 : 0);
+  int t = first + (int)blockIdx.x / kXcds;
+  if (t >= end) return;   // the whole workgroup
+  auto place = [&](int tile, int64_t& m0, int& n0) __attribute__((always_inline)) {
+    constexpr int kBand = 8;
+    const int band = tile / (kBand * a.tiles_n), in_band = tile % (kBand * a.tiles_n);
+    const int band_m = min(kBand, a.tiles_m - band * kBand);
+    m0 = (int64_t)(band * kBand + in_band % band_m) * 256;
+    n0 = in_band / band_m * 256;
+  };
+
+  // what this wave asks for: step ck of tile ct; rows past the last one lie past the end of a buffer and are read as zeros
+  int ct = t, ck = 0, cn = 0, cs4 = 0;   // cn: tiles, cs4: words of scales asked for before
+  int64_t cm0;
+  int cn0;
+  u32x4 dw, dx, dsw, dsx, db;
+  auto source = [&]() __attribute__((always_inline)) {
+    place(ct, cm0, cn0);
+    auto rows = [&](int64_t have, int64_t at, int most) __attribute__((always_inline)) { return (uint32_t)max((int64_t)0, min(have - at, (int64_t)most)); };
+    const int64_t mx = cm0 + (1 - group) * 128 + w * 32;
+    dx = make_rsrc(a.x.codes + mx * ld, rows(a.rows, mx, 32) * ld);
+    if (group == 1) {
+      const int nw = cn0 + w * 64;
+      dw = make_rsrc(a.w.codes + (int64_t)nw * ld, rows(a.N, nw, 64) * ld);
+      dsw = make_rsrc(a.w.scales + (int64_t)nw * a.ss, rows(a.N, nw, 64) * a.ss);
+      dsx = make_rsrc(a.x.scales + (cm0 + w * 64) * a.ss, rows(a.rows, cm0 + w * 64, 64) * a.ss);
+      db = make_rsrc(a.bias ? (const float*)a.bias + nw : nullptr, a.bias ? rows(a.N, nw, 64) * 4 : 0);
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    if ((ck & 3) == 3 || ck + 1 == G) ++cs4;
+    if (++ck < G) return;
+    ck = 0;
+    ++cn;
+    ct += per;
+    if (ct < end) source();
+  };
+  auto copy_tokens = [&](int par) __attribute__((always_inline)) {   // the other group's, 32 rows
+    const uint32_t to = lds0 + kX + par * kBuf + ((1 - group) * 128 + w * 32) * kRun;
+    const uint32_t o = afresh(ox);
+    static_for<0, 4>([&](auto c) __attribute__((always_inline)) {
+      copy16(dx, to + c * 8 * kRun, (o ^ ((c & 1) * 0x60)) + c * 8 * ld, ck * kRun);
+    });
+  };
+  auto copy_small = [&]() __attribute__((always_inline)) {             // scales and biases (group 1), where the step begins a word or a tile
+    if (ck & 3) return;
+    const uint32_t to = lds0 + kS + (cs4 & 3) * kScales + w * 256;
+    copy4(dsw, to, os, ck);
+    copy4(dsx, to + 1024, os, ck);
+    if (ck == 0) copy4(db, lds0 + kB + (cn & 3) * 1024 + w * 256, lane * 4, 0);
+  };
+  auto copy_weights = [&](int par) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + par * kBuf + w * 64 * kRun;
+    const uint32_t o = afresh(ow);
+    static_for<0, 8>([&](auto c) __attribute__((always_inline)) {
+      constexpr int q = c & 3, m = (q >> 1) | (((q ^ (q >> 1)) & 1) << 1);
+      copy16(dw, to + c * 8 * kRun, (o ^ (m << 5)) + c * 8 * ld, ck * kRun);
+    });
+  };
+
+  i32x8 fw[FN], fx[FM];
+  int qw[FN], qx[FM];
+  f32x4 acc[FN][FM];
+  int par = 0, rs4 = 0;
+  auto read_step = [&](auto kc) __attribute__((always_inline)) {
+    if constexpr (decltype(kc)::value == 0) {
+      const char* s = sm + kS + (rs4 & 3) * kScales;
+      ++rs4;
+#pragma unroll
+      for (int f = 0; f < FN; ++f) qw[f] = *(const int*)(s + 4 * (rw0 + (f >> 1) * 32 + (f & 1) * 4));
+#pragma unroll
+      for (int m = 0; m < FM; ++m) qx[m] = *(const int*)(s + 4 * (256 + rx0 + 16 * m));
+    }
+    const int st = par * kBuf;
+    auto read = [&](const char* const (&p)[2], int off) {
+      const u32x4 lo = *(const u32x4*)(p[0] + st + off), hi = *(const u32x4*)(p[1] + st + off);
+      return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
+#pragma unroll
+    for (int f = 0; f < FN; ++f) fw[f] = read(pw, ((f >> 1) * 32 + (f & 1) * 4) * kRun);
+#pragma unroll
+    for (int m = 0; m < FM; ++m) fx[m] = read(px, 16 * m * kRun);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](auto kc, auto fresh) __attribute__((always_inline)) {
+    constexpr int OP = decltype(kc)::value;
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int m = 0; m < FM; ++m)
+#pragma unroll
+      for (int f = 0; f < FN; ++f) {
+        const f32x4 c = decltype(fresh)::value ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[f][m];
+        acc[f][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[f], fx[m], c, 0, 0, OP, qw[f], OP, qx[m]);
+      }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto turn = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#define FVSR_WAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+
+  int64_t m0 = 0;
+  int n0 = 0, bt = 0;   // the tile being computed, and how many before it
+  bool held = false;    // its predecessor is still in acc
+  // writes the tile in acc; whether it took exactly kStores stores
+  auto write = [&]() __attribute__((always_inline)) {
+    if (!held) return false;
+    const float* b = (const float*)(sm + kB + ((bt - 1) & 3) * 1024);
+    write_tile(a, acc, (O*)a.y, b + w * 64 + 8 * g, n0 + w * 64 + 8 * g, m0 + rx0);
+    return a.vec_out && m0 + 256 <= a.rows && n0 + 256 <= a.N;
+  };
+
+  source();
+  if (group == 0) {
+    copy_tokens(0);
+    advance();
+  } else {
+    for (int s = 0; s < 2 && ct < end; ++s) {
+      copy_small();
+      copy_tokens(s);
+      copy_weights(s);
+      advance();
+    }
+  }
+  FVSR_WAIT(0);
+  turn();
+  if (group == 1) turn();   // phase 0
+  for (; t < end; t += per) {
+    for (int k0 = 0; k0 < G; k0 += 4)
+      static_for<0, 4>([&](auto kc) __attribute__((always_inline)) {
+        const int k = k0 + kc;
+        if (k >= G) return;
+        const bool ask = ct < end;
+        bool wrote = false;
+        if (group == 0) {
+          if (ask) copy_tokens(par ^ 1);
+        } else if (ask) {
+          copy_small();
+          copy_tokens(par);
+        }
+        if constexpr (decltype(kc)::value == 0)
+          if (k == 0) {
+            wrote = write();
+            place(t, m0, n0);
+            held = true;
+            ++bt;
+          }
+        read_step(kc);
+        // what has been asked for since the copies that the next phase needs, and maybe the tile's stores between
+        if (group == 0) {
+          if (!ask) FVSR_WAIT(0);
+          else if (wrote) FVSR_WAIT(4 + kStores);
+          else FVSR_WAIT(4);
+        } else {
+          if (ask) copy_weights(par);
+          if (!ask) FVSR_WAIT(0);
+          else if (wrote) FVSR_WAIT(12 + kStores);
+          else FVSR_WAIT(12);
+        }
+        if (ask) advance();
+        turn();
+        if constexpr (decltype(kc)::value == 0) {
+          if (k == 0) multiply(kc, std::true_type{});
+          else multiply(kc, std::false_type{});
+        } else {
+          multiply(kc, std::false_type{});
+        }
+        par ^= 1;
+        if (group == 0 || k + 1 < G || t + per < end) turn();
+      });
+  }
+  write();
+#undef FVSR_WAIT
+}
+
+__global__ __launch_bounds__(256) void widen_kernel(const bf16* __restrict__ in, int n, float* __restrict__ out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = (float)in[i];
+}
+
+size_t linear8_workspace(int64_t, int, int N) { return (size_t)N * sizeof(float); }
 
 int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, const void* bias, int gelu, int out_dtype,
-                   void* y, void*, hipStream_t stream) {
+                   void* y, void* ws, hipStream_t stream) {
   if (rows <= 0) return FVSR_OK;
   Linear8Args a{};
   a.x = x; a.w = w; a.rows = rows; a.N = N; a.runs = runs_of(K); a.ss = scale_stride(K);
   a.bias = bias; a.bias_f32 = bias_dtype == FVSR_DTYPE_F32; a.gelu = gelu; a.y = y;
   a.vec_out = rows_vectorize(y, N);
-  constexpr int TN = 128, TM = 128;
-  a.tiles_m = (int)ceil_div(rows, TM);
-  a.tiles_n = (int)ceil_div(N, TN);
-  const int64_t tiles = ceil_div(rows, TM) * a.tiles_n;
-  if (tiles >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
-  if (out_dtype == FVSR_DTYPE_BF16)
-    hipLaunchKernelGGL((linear8_kernel<TN, TM, 2, 2, bf16>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((linear8_kernel<TN, TM, 2, 2, float>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+  auto tiles_of = [&](int t) { return ceil_div(rows, t) * ceil_div(N, t); };
+  if (tiles_of(128) >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
+  const bool bf = out_dtype == FVSR_DTYPE_BF16;
+  // A CU does one 256 x 256 tile, or two of 128 x 128 at a time; a round of the former does twice the work of one of the latter in
+  // 1.6 times its time (measured at full rounds, 8192^3: 413 us against 518). So by the rounds that each needs:
+  const bool large = ceil_div(tiles_of(256), 256) * 8 <= ceil_div(tiles_of(128), 512) * 5;
+  const int T = large ? 256 : 128;
+  a.tiles_m = (int)ceil_div(rows, T);
+  a.tiles_n = (int)ceil_div(N, T);
+  const int64_t tiles = tiles_of(T);
+  if (large) {
+    if (bias && !a.bias_f32) {
+      hipLaunchKernelGGL(widen_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, stream, (const bf16*)bias, N, (float*)ws);
+      a.bias = ws;
+    }
+    const dim3 grid((unsigned)std::min<int64_t>(256, ceil_div(tiles, kXcds) * kXcds));
+    if (bf) hipLaunchKernelGGL((linear8_large_kernel<bf16>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((linear8_large_kernel<float>), grid, dim3(512), 0, stream, a);
+  } else {
+    if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, bf16>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+  }
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
 }
@@ -216,10 +484,11 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
 struct WeightGradArgs {
   const bf16* dy;
   In8 x;
-  int64_t rows;
+  int64_t rows, part_rows;   // part_rows: tokens of a part (the work is split over parts where there are few tiles), whole steps
   int N, K, runs, ss;
-  int vec_dy, vec_out;
-  void* dw;
+  int vec_dy;
+  void* dw;                  // (parts, N, K), fp32 where there are more than one
+  float* db;                 // (parts * tiles_k, N) or null
   int tiles_n, tiles_k;
 };
 
@@ -236,6 +505,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int tk = t % a.tiles_k, tn = t / a.tiles_k;
   const int n0 = tn * TN, k0 = tk * TK;
+  const int64_t from = (int64_t)blockIdx.y * a.part_rows, to = min(a.rows, from + a.part_rows);
 
   u32x4 rdy[kDy];
   uint2 rx[kX];
@@ -246,7 +516,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
       const int v = j * kThreads + threadIdx.x, r = v / (TN / 8), c = n0 + v % (TN / 8) * 8;
       const int64_t row = m0 + r;
       rdy[j] = u32x4{0, 0, 0, 0};
-      if (row < a.rows) {
+      if (row < to) {
         const bf16* p = a.dy + row * a.N + c;
         if (a.vec_dy) {
           if (c < a.N) rdy[j] = *(const u32x4*)p;
@@ -264,7 +534,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
       const int64_t row = m0 + r;
       rx[j] = make_uint2(0, 0);
       rs[j] = 0;
-      if (row < a.rows && c < a.runs * kRun) {
+      if (row < to && c < a.runs * kRun) {
         rx[j] = *(const uint2*)(a.x.codes + row * (int64_t)a.runs * kRun + c);
         rs[j] = a.x.scales[row * a.ss + c / kRun];
       }
@@ -295,12 +565,12 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
   for (int f = 0; f < FK; ++f)
 #pragma unroll
     for (int n = 0; n < FN; ++n) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load(0);
+  load(from);
   int turn = 0;
-  for (int64_t m0 = 0; m0 < a.rows; m0 += kTokens, turn ^= 1) {
+  for (int64_t m0 = from; m0 < to; m0 += kTokens, turn ^= 1) {
     put(sm[turn]);
     __syncthreads();
-    if (m0 + kTokens < a.rows) load(m0 + kTokens);
+    if (m0 + kTokens < to) load(m0 + kTokens);
     // lane (g, i): tokens 8 g .. 8 g + 7 of column i of a fragment
     auto read = [&](const char* s, int width, int col) {
       const char* p = s + ((8 * g + (i >> 2)) * width + col + (i & 3) * 4) * 2;
@@ -319,7 +589,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
       for (int n = 0; n < FN; ++n) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fn[n], acc[f][n], 0, 0, 0);
     }
   }
-  O* dw = (O*)a.dw;
+  O* dw = (O*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
 #pragma unroll
   for (int n = 0; n < FN; ++n) {
     const int row = n0 + wn * (TN / WN) + 16 * n + i;
@@ -331,6 +601,234 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (c + e < a.K) out[e] = (O)acc[f][n][e];
+    }
+  }
+}
+
+
+// The large weight gradient: 256 features x 256 channels a workgroup, steps of 64 tokens, two groups of four waves that take turns as in
+// linear8_large_kernel; wave w of group h computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
+//
+//   phase      2s                                             2s + 1
+//   group 0    widen X1(s), ask for codes of s + 2, read(s)   multiply(s)
+//   group 1    multiply(s - 1)                                widen X0(s + 1), ask for codes of s + 3, read(s), ask for dY(s + 2)
+//
+// LDS: dY of two steps, in blocks of 64 features (rows of 128 bytes, a token each): wave w of both groups reads block w, and the later
+// one replaces it. X as bf16, a half (a group's run) of one step each: written in the phases in which it is not read. Codes and scales
+// as they come, two steps: a wave copies, and later widens, its own 16 tokens of the other group's half, so its own count of copies is
+// all it waits for. The 32-byte pairs of a row of token t are XOR-ed by (t / 2 % 2, t / 8 % 2): a half wave's transposing read (4
+// tokens of 16 columns for each 16 lanes) then touches every bank once.
+// Copies past the last token read zeros (and nothing else), so every phase asks for the same number.
+// db: a step's column sums are 8 more products with rows of ones, taken by one of the tiles_k workgroups that read the step.
+template <typename O>
+__global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArgs a) {
+  constexpr int FN = 4, FM = 8, kTokens = 64;
+  constexpr int kBlk = kTokens * 128;                       // 64 columns (bf16) of a step
+  constexpr int kX = 8 * kBlk;                              // LDS: dY 2 x 4 blocks, X 2 halves x 2 blocks,
+  constexpr int kRaw = 12 * kBlk, kSc = kRaw + 2 * 2 * kBlk;   // codes 2 halves x 2 steps, scales 2 halves x 2 steps x 64 words
+  __shared__ __align__(1024) char sm[kSc + 4 * 256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave >> 2, w = wave & 3, i = lane & 15, g = lane >> 4;
+  const uint32_t lds0 = lds_offset(sm);
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int tk = t % a.tiles_k, tn = t / a.tiles_k, n0 = tn * 256 + w * 64, k0 = tk * 256;
+  const int64_t from = (int64_t)blockIdx.y * a.part_rows, to = min(a.rows, from + a.part_rows);
+  const int steps = (int)((to - from + kTokens - 1) / kTokens);
+  const int ldn = a.N * 2, ldk = a.runs * kRun;
+  const int other = 1 - group;
+
+  // copies: 8 tokens an instruction
+  const int r8 = lane >> 3, c8 = lane & 7;
+  const uint32_t od = (uint32_t)((((c8 >> 1) ^ ((r8 >> 1) & 1)) << 5) | ((c8 & 1) << 4));   // in a row of dY's block
+  const uint32_t oc = (uint32_t)((16 * w + r8) * ldk + c8 * 16);
+  const int run = tk * 2 + other;                           // this wave's codes' run
+  auto bytes = [](int64_t x, int64_t most) __attribute__((always_inline)) { return (uint32_t)max((int64_t)0, min(x, most)); };
+  auto copy_dy = [&](int s) __attribute__((always_inline)) {
+    const int64_t m = from + (int64_t)s * kTokens;
+    const int64_t have = m < to ? (to - m) * ldn - (int64_t)n0 * 2 : 0;
+    const u32x4 d = make_rsrc(a.dy + m * a.N + n0, bytes(have, (int64_t)kTokens * ldn));
+    const uint32_t at = lds0 + ((s & 1) * 4 + w) * kBlk;
+    const uint32_t o = afresh(od), r = r8 * ldn;
+    static_for<0, 8>([&](auto c) __attribute__((always_inline)) { copy16(d, at + c * 1024, (o ^ ((c & 1) << 6)) + r + c * 8 * ldn, 0); });
+  };
+  auto copy_codes = [&](int s) __attribute__((always_inline)) {
+    const int64_t m = from + (int64_t)s * kTokens;
+    const int64_t left = m < to ? to - m : 0;
+    const u32x4 d = make_rsrc(a.x.codes + m * ldk + run * kRun, bytes(left * ldk - run * kRun, (int64_t)kTokens * ldk));
+    const u32x4 e = make_rsrc(a.x.scales + m * a.ss + (run & ~3), bytes(left * a.ss - (run & ~3), (int64_t)kTokens * a.ss));
+    const uint32_t at = lds0 + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048;
+    const uint32_t o = afresh(oc);
+    copy16(d, at, o, 0);
+    copy16(d, at + 1024, o + 8 * ldk, 0);
+    if (lane < 16) copy4(e, lds0 + kSc + ((s & 1) * 2 + other) * 256 + w * 64, (16 * w + afresh(lane)) * a.ss, 0);
+  };
+  // codes of step s, this wave's tokens 16 w + 8 j + lane / 8, 16 channels a lane, to bf16
+  auto widen = [&](int s) __attribute__((always_inline)) {
+    const int lane = (int)afresh(threadIdx.x & 63), r8 = lane >> 3, c8 = lane & 7;
+    const char* raw = sm + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048 + lane * 16;
+    const char* sc = sm + kSc + ((s & 1) * 2 + other) * 256 + w * 64 + r8 * 4 + (run & 3);
+    char* out = sm + kX + other * 2 * kBlk + (c8 >> 2) * kBlk + (16 * w + r8) * 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u32x4 c = *(const u32x4*)(raw + j * 1024);
+      const float by = __uint_as_float((uint32_t)*(const uint8_t*)(sc + j * 32) << 23);
+      bf16x2 v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], by, false);
+        v[2 * e + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], by, true);
+      }
+      char* o = out + j * 1024 + (((c8 & 3) ^ ((r8 >> 1) & 1) ^ (j << 1)) << 5);
+      *(u32x4*)o = *(u32x4*)v;
+      *(u32x4*)(o + 16) = *(u32x4*)(v + 4);
+    }
+  };
+
+  // a lane's place in a transposing read: token 8 g + i / 4 (and 4 on), 4 columns of the pair
+  const int at = ((8 * g + (i >> 2)) * 128 + (i & 3) * 8) | ((((i >> 3) & 1) | ((g & 1) << 1)) << 5);
+  const char* const pd = sm + w * kBlk;
+  const char* const px = sm + kX + group * 2 * kBlk;
+  bf16x8 fd[2][FN], fx[2][FM];
+  f32x4 acc[FM][FN], sums = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int f = 0; f < FN; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto read_step = [&](int s) __attribute__((always_inline)) {
+    auto read = [&](const char* p, int pair) __attribute__((always_inline)) {
+      const char* q = p + (at ^ (pair << 5));
+      union { i16x4 h[2]; bf16x8 v; } u;
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)q);
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(q + 512));
+      return u.v;
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int f = 0; f < FN; ++f) fd[h][f] = read(pd + (s & 1) * 4 * kBlk + h * 4096, f);
+#pragma unroll
+      for (int m = 0; m < FM; ++m) fx[h][m] = read(px + (m >> 2) * kBlk + h * 4096, m & 3);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](int s) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int f = 0; f < FN; ++f)
+          acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[h][m], fd[h][f], acc[m][f], 0, 0, 0);
+    if (group == 0 && a.db && s % a.tiles_k == tk) {
+      // row f of the left operand is ones for fragment f: row f of `sums` collects its columns
+#pragma unroll
+      for (int f = 0; f < FN; ++f) {
+        const unsigned o = afresh(i) == (unsigned)f ? 0x3f803f80u : 0u;
+        const u32x4 ones = u32x4{o, o, o, o};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&ones, fd[h][f], sums, 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto turn = []() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#define FVSR_WAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+#define FVSR_READ_DONE() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+
+  if (group == 0) {
+    copy_codes(0);
+    copy_codes(1);
+  } else {
+    copy_dy(0);
+    copy_codes(0);
+    copy_codes(1);
+    FVSR_WAIT(0);
+    widen(0);
+    FVSR_READ_DONE();
+    copy_codes(2);
+    copy_dy(1);
+  }
+  turn();
+  if (group == 1) turn();   // phase 0
+  for (int s = 0; s < steps; ++s) {
+    if (group == 0) {
+      FVSR_WAIT(3);         // codes of s; asked for since: codes of s + 1
+      widen(s);
+      FVSR_READ_DONE();
+      copy_codes(s + 2);
+      read_step(s);
+    } else {
+      FVSR_WAIT(19);        // codes of s + 1; since: dY(s), codes of s + 2, dY(s + 1)
+      widen(s + 1);
+      FVSR_READ_DONE();
+      copy_codes(s + 3);
+      read_step(s);
+      copy_dy(s + 2);
+      FVSR_WAIT(11);        // dY(s + 1); since: codes of s + 3, dY(s + 2)
+    }
+    turn();
+    multiply(s);
+    if (group == 0 || s + 1 < steps) turn();
+  }
+  FVSR_WAIT(0);             // copies (of zeros) into this workgroup's LDS
+#undef FVSR_WAIT
+#undef FVSR_READ_DONE
+
+  O* dw = (O*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
+#pragma unroll
+  for (int f = 0; f < FN; ++f) {
+    const int n = n0 + 16 * f + i;
+    if (n >= a.N) continue;
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      const int c = k0 + group * 128 + 16 * m + 4 * g;
+      O* out = dw + (int64_t)n * a.K + c;
+      if (c + 4 <= a.K && (a.K & 3) == 0 && ((uintptr_t)dw & 15) == 0) {
+        O v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (O)acc[m][f][e];
+        if constexpr (sizeof(O) == 4) *(u32x4*)out = *(u32x4*)v;
+        else *(uint2*)out = *(uint2*)v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.K) out[e] = (O)acc[m][f][e];
+      }
+    }
+    if (group == 0 && a.db && g == 0) a.db[((int64_t)blockIdx.y * a.tiles_k + tk) * a.N + n] = sums[f];
+  }
+}
+
+// dw = the sum over parts of their (N, K) partial results, in order
+template <typename O>
+__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if (n % 4 == 0) {
+    f32x4 s = *(const f32x4*)(part + i);
+    for (int p = 1; p < parts; ++p) s += *(const f32x4*)(part + p * n + i);
+    if (((uintptr_t)dw & 15) == 0) {
+      O v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (O)s[e];
+      if constexpr (sizeof(O) == 4) *(u32x4*)(dw + i) = *(u32x4*)v;
+      else *(uint2*)(dw + i) = *(uint2*)v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dw[i + e] = (O)s[e];
+    }
+  } else {
+    for (int e = 0; e < 4 && i + e < n; ++e) {
+      float s = part[i + e];
+      for (int p = 1; p < parts; ++p) s += part[p * n + i + e];
+      dw[i + e] = (O)s;
     }
   }
 }
@@ -348,35 +846,77 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const bf16* __restrict_
     part[(int64_t)blockIdx.y * N + c] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
 }
 
-int launch_param_sum(const float* part, int parts, int64_t stride, int n, float* out, hipStream_t stream);
+int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);   // rows8.hip
 
+// How a weight gradient is cut up: tiles of 256 x 256 with DMA copies where dY's rows can be read 16 bytes at a time, else of 128 x
+// 128; the tokens into as many parts as fill the card, of at least 8 (16) steps.
+struct WeightGradPlan {
+  bool large;
+  int tiles_n, tiles_k, parts;
+  int64_t part_rows;
+  int sum_parts;   // partial column sums
+};
 constexpr int kSumParts = 64;
+static WeightGradPlan weight_grad_plan(int64_t rows, int N, int K, bool vec_dy) {
+  WeightGradPlan p;
+  p.large = rows > 0 && vec_dy && N > 128 && K > 128;   // (its phases need a step)
+  const int T = p.large ? 256 : 128, step = p.large ? 64 : 32, slots = p.large ? 256 : 512;
+  p.tiles_n = (int)ceil_div(N, T);
+  p.tiles_k = (int)ceil_div(K, T);
+  const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, steps = ceil_div(rows, step);
+  const int64_t parts = std::max<int64_t>(1, std::min(slots / tiles, steps / (p.large ? 8 : 16)));
+  p.part_rows = ceil_div(std::max<int64_t>(steps, 1), parts) * step;
+  p.parts = (int)std::max<int64_t>(1, ceil_div(rows, p.part_rows));
+  p.sum_parts = p.large ? p.parts * p.tiles_k : (int)std::max<int64_t>(1, std::min<int64_t>(kSumParts, ceil_div(rows, 16)));
+  return p;
+}
+static size_t plan_bytes(const WeightGradPlan& p, int N, int K) {
+  return ((size_t)p.sum_parts * N + (p.parts > 1 ? (size_t)p.parts * N * K : 0)) * sizeof(float) + 16;
+}
 size_t weight_grad_workspace(int64_t rows, int N, int K) {
-  (void)rows; (void)K;
-  return (size_t)kSumParts * N * sizeof(float);
+  return std::max(plan_bytes(weight_grad_plan(rows, N, K, false), N, K), plan_bytes(weight_grad_plan(rows, N, K, N % 8 == 0), N, K));
 }
 
 int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int out_dtype, void* dw, float* db, void* ws,
                        hipStream_t stream) {
+  const WeightGradPlan p = weight_grad_plan(rows, N, K, rows_vectorize(dy, N));
+  const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k;
+  if (tiles >= 1 << 22) return set_error(FVSR_ERR_UNSUPPORTED, "linear8_weight_grad: too many output tiles for one launch");
+  float* const sums = (float*)ws;
+  float* const part = (float*)((char*)ws + (((size_t)p.sum_parts * N * sizeof(float) + 15) & ~size_t(15)));
   WeightGradArgs a{};
-  a.dy = (const bf16*)dy; a.x = x; a.rows = rows; a.N = N; a.K = K; a.runs = runs_of(K); a.ss = scale_stride(K);
+  a.dy = (const bf16*)dy; a.x = x; a.rows = rows; a.part_rows = p.part_rows;
+  a.N = N; a.K = K; a.runs = runs_of(K); a.ss = scale_stride(K);
   a.vec_dy = rows_vectorize(dy, N);
-  a.dw = dw;
-  constexpr int TN = 128, TK = 128;
-  a.tiles_n = (int)ceil_div(N, TN);
-  a.tiles_k = (int)ceil_div(K, TK);
-  const int64_t tiles = (int64_t)a.tiles_n * a.tiles_k;
-  if (tiles >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
-  if (out_dtype == FVSR_DTYPE_BF16)
-    hipLaunchKernelGGL((weight_grad_kernel<TN, TK, 2, 2, bf16>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((weight_grad_kernel<TN, TK, 2, 2, float>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+  a.dw = p.parts > 1 ? part : dw;
+  a.db = db && p.large ? sums : nullptr;
+  a.tiles_n = p.tiles_n;
+  a.tiles_k = p.tiles_k;
+  const bool wide = p.parts > 1 || out_dtype == FVSR_DTYPE_F32;
+  const dim3 grid((unsigned)tiles, (unsigned)p.parts);
+  if (p.large) {
+    if (wide) hipLaunchKernelGGL((weight_grad_large_kernel<float>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((weight_grad_large_kernel<bf16>), grid, dim3(512), 0, stream, a);
+  } else {
+    if (wide) hipLaunchKernelGGL((weight_grad_kernel<128, 128, 2, 2, float>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((weight_grad_kernel<128, 128, 2, 2, bf16>), grid, dim3(256), 0, stream, a);
+  }
   FVSR_HIP_CHECK(hipGetLastError());
+  if (p.parts > 1) {
+    const int64_t n = (int64_t)N * K;
+    const dim3 blocks((unsigned)ceil_div(n, 1024));
+    if (out_dtype == FVSR_DTYPE_F32)
+      hipLaunchKernelGGL((weight_grad_join_kernel<float>), blocks, dim3(256), 0, stream, part, p.parts, n, (float*)dw);
+    else
+      hipLaunchKernelGGL((weight_grad_join_kernel<bf16>), blocks, dim3(256), 0, stream, part, p.parts, n, (bf16*)dw);
+    FVSR_HIP_CHECK(hipGetLastError());
+  }
   if (!db) return FVSR_OK;
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSumParts, ceil_div(rows, 16)));
-  hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(N, 64), parts), dim3(256), 0, stream, a.dy, rows, N, (float*)ws);
-  FVSR_HIP_CHECK(hipGetLastError());
-  return launch_param_sum((const float*)ws, parts, N, N, db, stream);
+  if (!p.large) {
+    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(N, 64), (unsigned)p.sum_parts), dim3(256), 0, stream, a.dy, rows, N, sums);
+    FVSR_HIP_CHECK(hipGetLastError());
+  }
+  return launch_param_sum(sums, p.sum_parts, N, N, db, nullptr, stream);
 }
 
 }  // namespace fvsr

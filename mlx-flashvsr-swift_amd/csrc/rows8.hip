@@ -229,9 +229,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad
   }
 }
 
-// out[c] = sum over p < parts of part[p * stride + c], c < n: 64 columns a workgroup, 4 quarters of the parts, in a fixed order
-__global__ __launch_bounds__(256) void param_sum_kernel(const float* __restrict__ part, int parts, int64_t stride, int n,
-                                                        float* __restrict__ out) {
+// The sums over p < parts of part[p * n + c], c < n: columns below `split` go to out, the others to out2 (either may be null); 64
+// columns a workgroup, 4 quarters of the parts, in a fixed order.
+__global__ __launch_bounds__(256) void param_sum_kernel(const float* __restrict__ part, int parts, int n, int split,
+                                                        float* __restrict__ out, float* __restrict__ out2) {
   __shared__ float sm[256];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -239,12 +240,14 @@ __global__ __launch_bounds__(256) void param_sum_kernel(const float* __restrict_
     int p = q;
     for (; p + 12 < parts; p += 16)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(p + 4 * u) * stride + c];
-    for (; p < parts; p += 4) s[0] += part[(int64_t)p * stride + c];
+      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(p + 4 * u) * n + c];
+    for (; p < parts; p += 4) s[0] += part[(int64_t)p * n + c];
   }
   sm[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  if (q == 0 && c < n) out[c] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
+  float* const to = c < split ? out : out2;
+  if (q == 0 && c < n && to)
+    to[c < split ? c : c - split] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
 }
 
 // A wave takes 4 runs of a row (one word of scales), 16 lanes each.
@@ -339,6 +342,12 @@ int launch_layer_norm(int dtype, int param_dtype, const void* x, int64_t rows, i
   });
 }
 
+int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream) {
+  hipLaunchKernelGGL(param_sum_kernel, dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, stream, part, parts, n, split, out, out2);
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
 int64_t norm_grad_blocks(int64_t rows, int C) {
   return std::min<int64_t>(kGradBlocks, C <= 2048 ? ceil_div(rows, 4) : rows);
 }
@@ -363,17 +372,7 @@ int launch_layer_norm_grad(int dtype, int param_dtype, const void* dy, const voi
     });
     if (rc) return rc;
   }
-  const dim3 grid((unsigned)ceil_div(C, 64));
-  if (dw) hipLaunchKernelGGL(param_sum_kernel, grid, dim3(256), 0, stream, part, (int)blocks, (int64_t)2 * C, C, dw);
-  if (db) hipLaunchKernelGGL(param_sum_kernel, grid, dim3(256), 0, stream, part + C, (int)blocks, (int64_t)2 * C, C, db);
-  FVSR_HIP_CHECK(hipGetLastError());
-  return FVSR_OK;
-}
-
-int launch_param_sum(const float* part, int parts, int64_t stride, int n, float* out, hipStream_t stream) {
-  hipLaunchKernelGGL(param_sum_kernel, dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, stream, part, parts, stride, n, out);
-  FVSR_HIP_CHECK(hipGetLastError());
-  return FVSR_OK;
+  return dw || db ? launch_param_sum(part, (int)blocks, 2 * C, C, dw, db, stream) : FVSR_OK;
 }
 
 int launch_quantize(int dtype, const void* x, int64_t rows, int C, Out8 o, hipStream_t stream) {

@@ -16,18 +16,17 @@ allocator on the stream that the call runs on, so calls may overlap on several s
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _abi
-from ._abi import DTYPE_BF16, DTYPE_F32, FVSRError, call, lib
+from ._abi import DTYPE_BF16, DTYPE_F32, FVSRError, lib
 
 __all__ = ["Blocks8", "quantize8", "dequantize8", "layer_norm", "layer_norm_backward", "linear8", "linear8_weight_grad"]
 
 RUN = 128
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _CODE = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+_BF16_ONLY = (torch.bfloat16,)
 
 
 def _refuse(name: str, msg: str, status: int = _abi.ERR_INVALID_ARG):
@@ -73,8 +72,11 @@ class Blocks8:
     @classmethod
     def empty(cls, rows: int, features: int, device) -> "Blocks8":
         c, s = _widths(features)
-        return cls(torch.empty((rows, c), dtype=CODES, device=device),
-                   torch.empty((rows, s), dtype=SCALES, device=device), features)
+        q = cls.__new__(cls)
+        q.codes = torch.empty((rows, c), dtype=CODES, device=device)
+        q.scales = torch.empty((rows, s), dtype=SCALES, device=device)
+        q.features = features
+        return q
 
 
 def _tokens(x, name: str, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tensor:
@@ -92,7 +94,7 @@ def _tokens(x, name: str, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tenso
 
 
 def _same(name: str, shape, want, dtype=None, want_dtype=None):
-    if tuple(shape) != tuple(want) or dtype != want_dtype:
+    if shape != want or dtype != want_dtype:
         _refuse(name, f"expected {tuple(want)} {want_dtype or ''}, got {tuple(shape)} {dtype or ''}")
 
 
@@ -119,25 +121,45 @@ def _one_device(first: torch.Tensor, name: str, *more) -> torch.device:
     return dev
 
 
-def _launch(stream, dev: torch.device):
-    """(stream handle, scope in which the call's tensors are made). Temporaries belong to the stream that the kernels run on,
-    so that the allocator hands their memory on in that stream's order."""
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(device).cuda_stream, without its 2 us
+
+
+def _on_stream(stream, dev: torch.device, make):
+    """(stream handle, make()): `make` allocates the call's tensors. They belong to the stream that the kernels run on, so that
+    the allocator hands their memory on in that stream's order."""
     if stream is None:
-        return torch.cuda.current_stream(dev).cuda_stream, contextlib.nullcontext()
+        return _raw_stream(dev.index), make()
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), dev) if int(stream) else torch.cuda.default_stream(dev)
     if stream.device != dev:
         _refuse("stream", f"a stream of {stream.device} for tensors on {dev}")
-    return stream.cuda_stream, torch.cuda.stream(stream)
+    with torch.cuda.stream(stream):
+        return stream.cuda_stream, make()
+
+
+_contexts: dict = {}
 
 
 def _ctx(dev: torch.device):
-    from . import Context
-    return Context.get(dev).handle
+    h = _contexts.get(dev.index)
+    if h is None:
+        from . import Context
+        h = _contexts[dev.index] = Context.get(dev).handle
+    return h
+
+
+def _check(rc: int, name: str):
+    if rc:
+        raise FVSRError(rc, name, lib.fvsr_last_error().decode(errors="replace"))
 
 
 def _p(t):
-    return 0 if t is None else t.data_ptr()
+    return None if t is None else t.data_ptr()
+
+
+def _p8(q):
+    """(codes, scales) addresses of a Blocks8, or of none."""
+    return (None, None) if q is None else (q.codes.data_ptr(), q.scales.data_ptr())
 
 
 def _param(t, name: str, features: int):
@@ -152,13 +174,12 @@ def _param(t, name: str, features: int):
 
 
 def _params(dtype, *ts):
-    """(type code, parameters): of one type, fp32 or the tokens'; others are widened to fp32 (exact)."""
-    kinds = {t.dtype for t in ts if t is not None}
-    if not kinds:
-        return DTYPE_F32, ts
-    if len(kinds) == 1 and (torch.float32 in kinds or dtype in kinds):
-        return _CODE[kinds.pop()], ts
-    return DTYPE_F32, tuple(None if t is None else t.float() for t in ts)
+    """(type code, *parameters): of one type, fp32 or the tokens'; others are widened to fp32 (exact)."""
+    if all(t is None or t.dtype == torch.float32 for t in ts):
+        return (DTYPE_F32, *ts)
+    if all(t is None or t.dtype == dtype for t in ts):
+        return (_CODE[dtype], *ts)
+    return (DTYPE_F32, *(None if t is None else t.float() for t in ts))
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -173,10 +194,9 @@ def quantize8(x: torch.Tensor, stream=None, out: Blocks8 | None = None) -> Block
     if out is not None:
         _same("out", out.shape, (rows, c))
     dev = _one_device(x2, "x", (out, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        q = Blocks8.empty(rows, c, dev) if out is None else out
-    call("fvsr_quantize8", _ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, q.codes.data_ptr(), q.scales.data_ptr(), handle)
+    handle, q = _on_stream(stream, dev, lambda: Blocks8.empty(rows, c, dev) if out is None else out)
+    _check(lib.fvsr_quantize8(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, q.codes.data_ptr(), q.scales.data_ptr(),
+                              handle), "fvsr_quantize8")
     return q
 
 
@@ -187,11 +207,9 @@ def dequantize8(q: Blocks8, dtype: torch.dtype = torch.bfloat16, stream=None, ou
         _refuse("dequantize8", f"unsupported dtype {dtype} (float32 or bfloat16)")
     o = _out(out, "out", q.shape, dtype)
     dev = _one_device(q.codes, "q", (o, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        o = torch.empty(q.shape, dtype=dtype, device=dev) if o is None else o
-    call("fvsr_dequantize8", _ctx(dev), q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.features, _CODE[dtype],
-         o.data_ptr(), handle)
+    handle, o = _on_stream(stream, dev, lambda: torch.empty(q.shape, dtype=dtype, device=dev) if o is None else o)
+    _check(lib.fvsr_dequantize8(_ctx(dev), q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.features, _CODE[dtype],
+                                o.data_ptr(), handle), "fvsr_dequantize8")
     return o if out is None else out
 
 
@@ -207,27 +225,26 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, want_
     x2 = _tokens(x, "x")
     rows, c = x2.shape
     weight, bias = _param(weight, "weight", c), _param(bias, "bias", c)
-    if quantized:
-        if out is not None:
-            _same("out", out.shape, (rows, c))
-        y, y8 = None, out
-    else:
-        y, y8 = _out(out, "out", (rows, c), x2.dtype), None
+    if not quantized:
+        o = _out(out, "out", (rows, c), x2.dtype)
+    elif out is not None:
+        _same("out", out.shape, (rows, c))
     dev = _one_device(x2, "x", (weight, "weight"), (bias, "bias"), (out, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        kind, (w, b) = _params(x2.dtype, weight, bias)
+
+    def make():
+        kind, w, b = _params(x2.dtype, weight, bias)
         if quantized:
-            y8 = Blocks8.empty(rows, c, dev) if y8 is None else y8
-        elif y is None:
-            y = torch.empty_like(x2)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
-        x8 = Blocks8.empty(rows, c, dev) if want_x8 else None
-    call("fvsr_layer_norm", _ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, float(eps), kind, _p(w), _p(b), _p(y),
-         _p(y8 and y8.codes), _p(y8 and y8.scales), _p(x8 and x8.codes), _p(x8 and x8.scales), _p(stats), handle)
-    if quantized:
-        return y8, stats, x8
-    return (y.reshape(x.shape) if out is None else out), stats, x8
+            y = Blocks8.empty(rows, c, dev) if out is None else out
+        else:
+            y = torch.empty_like(x) if o is None else o
+        return (kind, w, b, y, torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None,
+                Blocks8.empty(rows, c, dev) if want_x8 else None)
+
+    handle, (kind, w, b, y, stats, x8) = _on_stream(stream, dev, make)
+    yp = (None, *_p8(y)) if quantized else (y.data_ptr(), None, None)
+    _check(lib.fvsr_layer_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, eps, kind, _p(w), _p(b), *yp, *_p8(x8),
+                               _p(stats), handle), "fvsr_layer_norm")
+    return (y if out is None else out), stats, x8
 
 
 def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, want_params: bool = True, stream=None,
@@ -248,22 +265,23 @@ def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, w
     if not stats.is_contiguous():
         _refuse("stats", "expected a contiguous tensor")
     weight = _param(weight, "weight", c)
-    dx = _out(out, "out", (rows, c), d2.dtype)
-    dev = _one_device(d2, "dy", (x, "x"), (stats, "stats"), (weight, "weight"), (dx, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        kind, (w,) = _params(d2.dtype, weight)
-        dx = torch.empty_like(d2) if dx is None else dx
-        dw = db = ws = None
-        nbytes = 0
-        if want_params:
-            dw, db = torch.empty((2, c), dtype=torch.float32, device=dev)
-            nbytes = lib.fvsr_layer_norm_backward_workspace(rows, c)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    call("fvsr_layer_norm_backward", _ctx(dev), _CODE[d2.dtype], d2.data_ptr(), _p(x2), _p(kept and kept.codes),
-         _p(kept and kept.scales), stats.data_ptr(), rows, c, kind, _p(w), dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes,
-         handle)
-    return (dx.reshape(dy.shape) if out is None else out), dw, db
+    o = _out(out, "out", (rows, c), d2.dtype)
+    dev = _one_device(d2, "dy", (x, "x"), (stats, "stats"), (weight, "weight"), (o, "out"))
+    nbytes = lib.fvsr_layer_norm_backward_workspace(rows, c) if want_params else 0
+
+    def make():
+        kind, w = _params(d2.dtype, weight)
+        dx = torch.empty_like(dy) if o is None else o
+        if not want_params:
+            return kind, w, dx, None, None, None
+        return (kind, w, dx, torch.empty(c, dtype=torch.float32, device=dev), torch.empty(c, dtype=torch.float32, device=dev),
+                torch.empty(nbytes, dtype=torch.uint8, device=dev))
+
+    handle, (kind, w, dx, dw, db, ws) = _on_stream(stream, dev, make)
+    _check(lib.fvsr_layer_norm_backward(_ctx(dev), _CODE[d2.dtype], d2.data_ptr(), _p(x2), *_p8(kept), stats.data_ptr(), rows,
+                                        c, kind, _p(w), dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes, handle),
+           "fvsr_layer_norm_backward")
+    return (dx if out is None else out), dw, db
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -273,8 +291,8 @@ def linear8(x, weight: Blocks8, bias=None, gelu: bool = False, dtype: torch.dtyp
             out=None) -> torch.Tensor:
     """y = x W^T + bias, then GELU (tanh form) if `gelu`, (rows, out_features) in `dtype`, from 8-bit operands, summed in
     32 bits (the matrix cores cut each product to 13 bits below the largest of 8 neighbouring channels' first, so a float32 y is good
-    to about 2^-12 of its terms' size). x: a Blocks8, or (rows, in_features) float32 or bfloat16 tokens, quantized in the call; weight: quantize8 of
-    the (out_features, in_features) matrix, made once; bias: (out_features), float32 or bfloat16."""
+    to about 2^-12 of its terms' size). x: a Blocks8, or (rows, in_features) float32 or bfloat16 tokens, quantized in the call;
+    weight: quantize8 of the (out_features, in_features) matrix, made once; bias: (out_features), float32 or bfloat16."""
     if dtype not in _CODE:
         _refuse("linear8", f"unsupported dtype {dtype} (float32 or bfloat16)")
     if not isinstance(weight, Blocks8):
@@ -282,29 +300,34 @@ def linear8(x, weight: Blocks8, bias=None, gelu: bool = False, dtype: torch.dtyp
     x8 = x if isinstance(x, Blocks8) else None
     x2 = None if x8 is not None else _tokens(x, "x")
     rows, k = (x8 if x2 is None else x2).shape
-    n = weight.rows
+    n = weight.codes.shape[0]
     if k != weight.features:
         _refuse("linear8", f"x has {k} features, weight expects {weight.features}")
     if n < 1:
         _refuse("weight", "expected at least one row")
     bias = _param(bias, "bias", n)
-    y = _out(out, "out", (rows, n), dtype)
-    first = x8.codes if x2 is None else x2
-    dev = _one_device(first, "x", (weight, "weight"), (bias, "bias"), (y, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        y = torch.empty((rows, n), dtype=dtype, device=dev) if y is None else y
-        if x8 is None:
-            x8 = Blocks8.empty(rows, k, dev)
-        nbytes = lib.fvsr_linear8_workspace(rows, k, n)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    call("fvsr_linear8", _ctx(dev), DTYPE_F32 if x2 is None else _CODE[x2.dtype], _p(x2), rows, k, x8.codes.data_ptr(),
-         x8.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), n,
-         DTYPE_F32 if bias is None else _CODE[bias.dtype], _p(bias), 1 if gelu else 0, _CODE[dtype], y.data_ptr(), _p(ws),
-         nbytes, handle)
-    if out is not None:
-        return out
-    return y.reshape(1, rows, n) if x2 is not None and x.dim() == 3 else y
+    o = _out(out, "out", (rows, n), dtype)
+    dev = _one_device(x8.codes if x2 is None else x2, "x", (weight, "weight"), (bias, "bias"), (o, "out"))
+    shape = (1, rows, n) if x2 is not None and x.dim() == 3 else (rows, n)
+    need = nbytes = lib.fvsr_linear8_workspace(rows, k, n)
+    if x2 is not None:   # the 8-bit tokens live in the same temporary, after the workspace: codes, then scales
+        code_bytes, scale_bytes = _widths(k)
+        at = (need + 255) & ~255
+        nbytes = at + rows * (code_bytes + scale_bytes)
+
+    def make():
+        return (torch.empty(shape, dtype=dtype, device=dev) if o is None else o,
+                torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None)
+
+    handle, (y, ws) = _on_stream(stream, dev, make)
+    wp = _p(ws)
+    if x2 is None:
+        kind, xp, qp = DTYPE_F32, None, _p8(x8)
+    else:
+        kind, xp, qp = _CODE[x2.dtype], x2.data_ptr(), (wp and wp + at, wp and wp + at + rows * code_bytes)
+    _check(lib.fvsr_linear8(_ctx(dev), kind, xp, rows, k, *qp, *_p8(weight), n, DTYPE_F32 if bias is None else _CODE[bias.dtype],
+                            _p(bias), 1 if gelu else 0, _CODE[dtype], y.data_ptr(), wp, need, handle), "fvsr_linear8")
+    return y if out is None else out
 
 
 def linear8_weight_grad(dy: torch.Tensor, x8: Blocks8, dtype: torch.dtype = torch.float32, want_bias: bool = True, stream=None,
@@ -316,19 +339,21 @@ def linear8_weight_grad(dy: torch.Tensor, x8: Blocks8, dtype: torch.dtype = torc
         _refuse("linear8_weight_grad", f"unsupported dtype {dtype} (float32 or bfloat16)")
     if not isinstance(x8, Blocks8):
         _refuse("x8", "expected the Blocks8 that the layer read")
-    d2 = _tokens(dy, "dy", (torch.bfloat16,))
+    d2 = _tokens(dy, "dy", _BF16_ONLY)
     rows, n = d2.shape
-    if x8.rows != rows:
+    if x8.codes.shape[0] != rows:
         _refuse("x8", f"{x8.rows} rows, dy has {rows}")
     k = x8.features
-    dw = _out(out, "out", (n, k), dtype)
-    dev = _one_device(d2, "dy", (x8, "x8"), (dw, "out"))
-    handle, scope = _launch(stream, dev)
-    with scope:
-        dw = torch.empty((n, k), dtype=dtype, device=dev) if dw is None else dw
-        db = torch.empty(n, dtype=torch.float32, device=dev) if want_bias else None
-        nbytes = lib.fvsr_linear8_weight_grad_workspace(rows, k, n)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    call("fvsr_linear8_weight_grad", _ctx(dev), d2.data_ptr(), rows, n, x8.codes.data_ptr(), x8.scales.data_ptr(), k,
-         _CODE[dtype], dw.data_ptr(), _p(db), _p(ws), nbytes, handle)
+    o = _out(out, "out", (n, k), dtype)
+    dev = _one_device(d2, "dy", (x8, "x8"), (o, "out"))
+    nbytes = lib.fvsr_linear8_weight_grad_workspace(rows, k, n)
+
+    def make():
+        return (torch.empty((n, k), dtype=dtype, device=dev) if o is None else o,
+                torch.empty(n, dtype=torch.float32, device=dev) if want_bias else None,
+                torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None)
+
+    handle, (dw, db, ws) = _on_stream(stream, dev, make)
+    _check(lib.fvsr_linear8_weight_grad(_ctx(dev), d2.data_ptr(), rows, n, *_p8(x8), k, _CODE[dtype], dw.data_ptr(), _p(db),
+                                        _p(ws), nbytes, handle), "fvsr_linear8_weight_grad")
     return (dw if out is None else out), db
