@@ -167,6 +167,7 @@ int fvsr_linear8(fvsr_ctx* ctx, int x_dtype, const void* x, int64_t rows, int in
   int rc = check_rows(ctx, rows, in_features, kMaxFeatures);
   if (rc) return rc;
   FVSR_REQUIRE(out_features > 0, FVSR_ERR_INVALID_ARG, "out_features must be > 0");
+  FVSR_REQUIRE(out_features <= kMaxFeatures, FVSR_ERR_UNSUPPORTED, "at most " + std::to_string(kMaxFeatures) + " out_features");
   FVSR_REQUIRE(!x || dtype_ok(x_dtype), FVSR_ERR_INVALID_ARG, "x_dtype must be FVSR_DTYPE_F32 or FVSR_DTYPE_BF16");
   FVSR_REQUIRE(!bias || dtype_ok(bias_dtype), FVSR_ERR_INVALID_ARG, "bias_dtype must be FVSR_DTYPE_F32 or FVSR_DTYPE_BF16");
   FVSR_REQUIRE(dtype_ok(y_dtype), FVSR_ERR_INVALID_ARG, "y_dtype must be FVSR_DTYPE_F32 or FVSR_DTYPE_BF16");
@@ -194,6 +195,7 @@ int fvsr_linear8_weight_grad(fvsr_ctx* ctx, const void* dy, int64_t rows, int ou
   int rc = check_rows(ctx, rows, in_features, kMaxFeatures);
   if (rc) return rc;
   FVSR_REQUIRE(out_features > 0, FVSR_ERR_INVALID_ARG, "out_features must be > 0");
+  FVSR_REQUIRE(out_features <= kMaxFeatures, FVSR_ERR_UNSUPPORTED, "at most " + std::to_string(kMaxFeatures) + " out_features");
   FVSR_REQUIRE(dtype_ok(dw_dtype), FVSR_ERR_INVALID_ARG, "dw_dtype must be FVSR_DTYPE_F32 or FVSR_DTYPE_BF16");
   FVSR_REQUIRE(dw != nullptr, FVSR_ERR_INVALID_ARG, "dw is NULL");
   if (rows > 0) {

@@ -340,9 +340,9 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
     };
 #pragma unroll
     for (int f = 0; f < FN; ++f) fw[f] = read(pw, ((f >> 1) * 32 + (f & 1) * 4) * kRun);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < FM; ++m) fx[m] = read(px, 16 * m * kRun);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](auto kc, auto fresh) __attribute__((always_inline)) {
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
   };
   auto turn = [] {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_barrier" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 #define FVSR_WAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
@@ -397,12 +397,6 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
         if (k >= G) return;
         const bool ask = ct < end;
         bool wrote = false;
-        if (group == 0) {
-          if (ask) copy_tokens(par ^ 1);
-        } else if (ask) {
-          copy_small();
-          copy_tokens(par);
-        }
         if constexpr (decltype(kc)::value == 0)
           if (k == 0) {
             wrote = write();
@@ -411,13 +405,20 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
             ++bt;
           }
         read_step(kc);
-        // what has been asked for since the copies that the next phase needs, and maybe the tile's stores between
+        // then what has been asked for since the copies that the next phase needs may be outstanding: this step's, and maybe stores
         if (group == 0) {
+          if (ask) copy_tokens(par ^ 1);
           if (!ask) FVSR_WAIT(0);
           else if (wrote) FVSR_WAIT(4 + kStores);
           else FVSR_WAIT(4);
         } else {
-          if (ask) copy_weights(par);
+          if (ask) {
+            copy_small();
+            copy_tokens(par);
+            // the weights were read first: with 15 of the 24 reads outstanding, their place is free
+            asm volatile("s_waitcnt lgkmcnt(15)" ::: "memory");
+            copy_weights(par);
+          }
           if (!ask) FVSR_WAIT(0);
           else if (wrote) FVSR_WAIT(12 + kStores);
           else FVSR_WAIT(12);
@@ -609,15 +610,16 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
 // The large weight gradient: 256 features x 256 channels a workgroup, steps of 64 tokens, two groups of four waves that take turns as in
 // linear8_large_kernel; wave w of group h computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
 //
-//   phase      2s                                             2s + 1
-//   group 0    widen X1(s), ask for codes of s + 2, read(s)   multiply(s)
-//   group 1    multiply(s - 1)                                widen X0(s + 1), ask for codes of s + 3, read(s), ask for dY(s + 2)
+//   phase      2s                                                          2s + 1
+//   group 0    widen X1(s), read(s), ask for dY(s + 1) and codes of s + 2  multiply(s)
+//   group 1    multiply(s - 1)                                             widen X0(s + 1), read(s), ask for codes of s + 3
 //
-// LDS: dY of two steps, in blocks of 64 features (rows of 128 bytes, a token each): wave w of both groups reads block w, and the later
-// one replaces it. X as bf16, a half (a group's run) of one step each: written in the phases in which it is not read. Codes and scales
-// as they come, two steps: a wave copies, and later widens, its own 16 tokens of the other group's half, so its own count of copies is
-// all it waits for. The 32-byte pairs of a row of token t are XOR-ed by (t / 2 % 2, t / 8 % 2): a half wave's transposing read (4
-// tokens of 16 columns for each 16 lanes) then touches every bank once.
+// LDS: dY of two steps, in blocks of 64 features (rows of 128 bytes, a token each). X as bf16, a half (a group's run) of one step each:
+// written in the phases in which it is not read. Codes and scales as they come, two steps: a wave copies, and later widens, its own 16
+// tokens of the other group's half, so its own count of copies is all it waits for. The 32-byte pairs of a row of token t are XOR-ed by
+// (t / 2 % 2, t / 8 % 2): a half wave's transposing read (4 tokens of 16 columns for each 16 lanes) then touches every bank once.
+// dY's copies stand between the reads from LDS: behind them, at the phase's end, their issue was what the other group waited for
+// (497 us at 17280 x 1536 x 8960).
 // Copies past the last token read zeros (and nothing else), so every phase asks for the same number.
 // db: a step's column sums are 8 more products with rows of ones, taken by one of the tiles_k workgroups that read the step.
 template <typename O>
@@ -642,45 +644,61 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
   const uint32_t od = (uint32_t)((((c8 >> 1) ^ ((r8 >> 1) & 1)) << 5) | ((c8 & 1) << 4));   // in a row of dY's block
   const uint32_t oc = (uint32_t)((16 * w + r8) * ldk + c8 * 16);
   const int run = tk * 2 + other;                           // this wave's codes' run
-  auto bytes = [](int64_t x, int64_t most) __attribute__((always_inline)) { return (uint32_t)max((int64_t)0, min(x, most)); };
-  auto copy_dy = [&](int s) __attribute__((always_inline)) {
-    const int64_t m = from + (int64_t)s * kTokens;
-    const int64_t have = m < to ? (to - m) * ldn - (int64_t)n0 * 2 : 0;
-    const u32x4 d = make_rsrc(a.dy + m * a.N + n0, bytes(have, (int64_t)kTokens * ldn));
-    const uint32_t at = lds0 + ((s & 1) * 4 + w) * kBlk;
-    const uint32_t o = afresh(od), r = r8 * ldn;
-    static_for<0, 8>([&](auto c) __attribute__((always_inline)) { copy16(d, at + c * 1024, (o ^ ((c & 1) << 6)) + r + c * 8 * ldn, 0); });
+  const int count = (int)(to - from);                       // tokens (a part has fewer than 2^31)
+  auto left = [&](int s) __attribute__((always_inline)) { return max(0, min(kTokens, count - s * kTokens)); };
+  u32x4 dd, dc, ds;    // dY, codes and scales of the steps that are asked for, and their places
+  uint32_t dy_at = 0, codes_at = 0, scales_at = 0;
+  const char* const dy0 = (const char*)(a.dy + from * a.N + n0);
+  const uint8_t* const codes0 = a.x.codes + from * ldk + run * kRun;
+  const uint8_t* const scales0 = a.x.scales + from * a.ss + (run & ~3);
+  auto place_dy = [&](int s) __attribute__((always_inline)) {
+    dd = make_rsrc(dy0 + (int64_t)s * (kTokens * ldn), (uint32_t)max(0, left(s) * ldn - n0 * 2));
+    dy_at = lds0 + ((s & 1) * 4 + w) * kBlk;
   };
-  auto copy_codes = [&](int s) __attribute__((always_inline)) {
-    const int64_t m = from + (int64_t)s * kTokens;
-    const int64_t left = m < to ? to - m : 0;
-    const u32x4 d = make_rsrc(a.x.codes + m * ldk + run * kRun, bytes(left * ldk - run * kRun, (int64_t)kTokens * ldk));
-    const u32x4 e = make_rsrc(a.x.scales + m * a.ss + (run & ~3), bytes(left * a.ss - (run & ~3), (int64_t)kTokens * a.ss));
-    const uint32_t at = lds0 + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048;
-    const uint32_t o = afresh(oc);
-    copy16(d, at, o, 0);
-    copy16(d, at + 1024, o + 8 * ldk, 0);
-    if (lane < 16) copy4(e, lds0 + kSc + ((s & 1) * 2 + other) * 256 + w * 64, (16 * w + afresh(lane)) * a.ss, 0);
+  auto place_codes = [&](int s) __attribute__((always_inline)) {
+    dc = make_rsrc(codes0 + (int64_t)s * (kTokens * ldk), (uint32_t)max(0, left(s) * ldk - run * kRun));
+    ds = make_rsrc(scales0 + (int64_t)s * (kTokens * a.ss), (uint32_t)max(0, left(s) * a.ss - (run & ~3)));
+    codes_at = lds0 + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048;
+    scales_at = lds0 + kSc + ((s & 1) * 2 + other) * 256 + w * 64;
+  };
+  auto copy_dy = [&](auto c) __attribute__((always_inline)) {   // 8 of its 64 tokens
+    copy16(dd, dy_at + c * 1024, (afresh(od) ^ ((c & 1) << 6)) + (r8 + c * 8) * ldn, 0);
+  };
+  auto copy_codes = [&](auto c) __attribute__((always_inline)) {   // 0, 1: 8 tokens' codes; 2: this wave's 16 scales
+    if constexpr (decltype(c)::value < 2) copy16(dc, codes_at + c * 1024, afresh(oc) + c * 8 * ldk, 0);
+    else if (lane < 16) copy4(ds, scales_at, (16 * w + afresh(lane)) * a.ss, 0);
   };
   // codes of step s, this wave's tokens 16 w + 8 j + lane / 8, 16 channels a lane, to bf16
-  auto widen = [&](int s) __attribute__((always_inline)) {
-    const int lane = (int)afresh(threadIdx.x & 63), r8 = lane >> 3, c8 = lane & 7;
-    const char* raw = sm + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048 + lane * 16;
-    const char* sc = sm + kSc + ((s & 1) * 2 + other) * 256 + w * 64 + r8 * 4 + (run & 3);
-    char* out = sm + kX + other * 2 * kBlk + (c8 >> 2) * kBlk + (16 * w + r8) * 128;
+  u32x4 raw[2];
+  uint32_t raw_scale[2];
+  auto read_codes = [&](int s) __attribute__((always_inline)) {
+    const int l = (int)afresh(threadIdx.x & 63);
+    const char* r = sm + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048 + l * 16;
+    const char* sc = sm + kSc + ((s & 1) * 2 + other) * 256 + w * 64 + (l >> 3) * 4 + (run & 3);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const u32x4 c = *(const u32x4*)(raw + j * 1024);
-      const float by = __uint_as_float((uint32_t)*(const uint8_t*)(sc + j * 32) << 23);
+      raw[j] = *(const u32x4*)(r + j * 1024);
+      raw_scale[j] = *(const uint8_t*)(sc + j * 32);
+    }
+  };
+  auto widen = [&]() __attribute__((always_inline)) {
+    const int l = (int)afresh(threadIdx.x & 63), r = l >> 3, c = l & 7;
+    char* out = sm + kX + other * 2 * kBlk + (c >> 2) * kBlk + (16 * w + r) * 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float by = __uint_as_float(raw_scale[j] << 23);
       bf16x2 v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[2 * e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], by, false);
-        v[2 * e + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], by, true);
+        v[2 * e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j][e], by, false);
+        v[2 * e + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j][e], by, true);
       }
-      char* o = out + j * 1024 + (((c8 & 3) ^ ((r8 >> 1) & 1) ^ (j << 1)) << 5);
-      *(u32x4*)o = *(u32x4*)v;
-      *(u32x4*)(o + 16) = *(u32x4*)(v + 4);
+      // the lanes of one block write the lower halves of their pairs first, those of the other, on the same banks, the upper ones
+      char* o = out + j * 1024 + (((c & 3) ^ ((r >> 1) & 1) ^ (j << 1)) << 5);
+      const bool up = c >> 2;
+      const u32x4 lo = *(u32x4*)v, hi = *(u32x4*)(v + 4);
+      *(u32x4*)(o + (up ? 16 : 0)) = up ? hi : lo;
+      *(u32x4*)(o + (up ? 0 : 16)) = up ? lo : hi;
     }
   };
 
@@ -694,7 +712,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
   for (int m = 0; m < FM; ++m)
 #pragma unroll
     for (int f = 0; f < FN; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto read_step = [&](int s) __attribute__((always_inline)) {
+  auto read_step = [&](int s, auto with_dy) __attribute__((always_inline)) {   // and the copies, between the reads
     auto read = [&](const char* p, int pair) __attribute__((always_inline)) {
       const char* q = p + (at ^ (pair << 5));
       union { i16x4 h[2]; bf16x8 v; } u;
@@ -702,14 +720,14 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
       u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(q + 512));
       return u.v;
     };
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int f = 0; f < FN; ++f) fd[h][f] = read(pd + (s & 1) * 4 * kBlk + h * 4096, f);
-#pragma unroll
-      for (int m = 0; m < FM; ++m) fx[h][m] = read(px + (m >> 2) * kBlk + h * 4096, m & 3);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    static_for<0, 2 * (FN + FM)>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value, h = j / (FN + FM), r = j % (FN + FM);
+      if constexpr (r < FN) fd[h][r] = read(pd + (s & 1) * 4 * kBlk + h * 4096, r);
+      else fx[h][r - FN] = read(px + ((r - FN) >> 2) * kBlk + h * 4096, (r - FN) & 3);
+      if constexpr (decltype(with_dy)::value && j % 2 == 0 && j < 16) copy_dy(std::integral_constant<int, j / 2>{});
+      if constexpr (j % 2 == 1 && j >= 17 && j < 23) copy_codes(std::integral_constant<int, (j - 17) / 2>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
     __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](int s) __attribute__((always_inline)) {
@@ -743,38 +761,43 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
 #define FVSR_READ_DONE() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
   if (group == 0) {
-    copy_codes(0);
-    copy_codes(1);
-  } else {
-    copy_dy(0);
-    copy_codes(0);
-    copy_codes(1);
-    FVSR_WAIT(0);
-    widen(0);
+    place_dy(0);
+    static_for<0, 8>(copy_dy);
+  }
+  for (int s = 0; s < 2; ++s) {
+    place_codes(s);
+    static_for<0, 3>(copy_codes);
+  }
+  FVSR_WAIT(0);
+  if (group == 1) {
+    read_codes(0);
     FVSR_READ_DONE();
-    copy_codes(2);
-    copy_dy(1);
+    widen();
+    place_codes(2);
+    static_for<0, 3>(copy_codes);
   }
   turn();
   if (group == 1) turn();   // phase 0
   for (int s = 0; s < steps; ++s) {
     if (group == 0) {
-      FVSR_WAIT(3);         // codes of s; asked for since: codes of s + 1
-      widen(s);
-      FVSR_READ_DONE();
-      copy_codes(s + 2);
-      read_step(s);
+      FVSR_WAIT(11);        // codes of s; asked for since: dY(s), codes of s + 1
+      read_codes(s);
+      place_dy(s + 1);
+      place_codes(s + 2);
+      FVSR_READ_DONE();     // their place is free
+      widen();
+      read_step(s, std::true_type{});
     } else {
-      FVSR_WAIT(19);        // codes of s + 1; since: dY(s), codes of s + 2, dY(s + 1)
-      widen(s + 1);
+      FVSR_WAIT(3);         // codes of s + 1; since: codes of s + 2
+      read_codes(s + 1);
+      place_codes(s + 3);
       FVSR_READ_DONE();
-      copy_codes(s + 3);
-      read_step(s);
-      copy_dy(s + 2);
-      FVSR_WAIT(11);        // dY(s + 1); since: codes of s + 3, dY(s + 2)
+      widen();
+      read_step(s, std::false_type{});
     }
     turn();
     multiply(s);
+    if (group == 0) FVSR_WAIT(3);   // dY(s + 1); since: codes of s + 2
     if (group == 0 || s + 1 < steps) turn();
   }
   FVSR_WAIT(0);             // copies (of zeros) into this workgroup's LDS
@@ -879,6 +902,7 @@ size_t weight_grad_workspace(int64_t rows, int N, int K) {
 
 int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int out_dtype, void* dw, float* db, void* ws,
                        hipStream_t stream) {
+  if (rows >= (int64_t)1 << 31) return set_error(FVSR_ERR_UNSUPPORTED, "linear8_weight_grad: too many rows");
   const WeightGradPlan p = weight_grad_plan(rows, N, K, rows_vectorize(dy, N));
   const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k;
   if (tiles >= 1 << 22) return set_error(FVSR_ERR_UNSUPPORTED, "linear8_weight_grad: too many output tiles for one launch");
