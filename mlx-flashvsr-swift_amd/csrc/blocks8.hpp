@@ -90,31 +90,38 @@ __device__ __forceinline__ int run_channel(int l16, int e) {
   return VEC ? l16 * 8 + e : l16 + 16 * e;
 }
 
+// 8 elements as they lie in memory, zeros past the row's end: loaded now, widened when they are needed
+template <typename T>
+struct Raw8 {
+  T v[8];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c0, int l16, int C, float (&v)[8]) {
+__device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c0, int l16, int C) {
+  Raw8<T> r;
   if constexpr (VEC) {
     const int c = c0 + l16 * 8;
+    u32x4* const to = (u32x4*)r.v;
     if (c < C) {
-      T t[8];
-      if constexpr (sizeof(T) == 2) {
-        *(u32x4*)t = *(const u32x4*)(row + c);
-      } else {
-        ((u32x4*)t)[0] = ((const u32x4*)(row + c))[0];
-        ((u32x4*)t)[1] = ((const u32x4*)(row + c))[1];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+      to[0] = *(const u32x4*)(row + c);
+      if constexpr (sizeof(T) == 4) to[1] = *(const u32x4*)(row + c + 4);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      to[0] = u32x4{0, 0, 0, 0};
+      if constexpr (sizeof(T) == 4) to[1] = u32x4{0, 0, 0, 0};
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int c = c0 + l16 + 16 * e;
-      v[e] = c < C ? (float)row[c] : 0.f;
+      r.v[e] = c < C ? row[c] : (T)0.f;
     }
   }
+  return r;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int c0, int l16, int C, float (&v)[8]) {
+  const Raw8<T> r = load_raw8<T, VEC>(row, c0, l16, C);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)r.v[e];
 }
 
 template <typename T, bool VEC>

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
 // registers; the workgroup's sum goes to `part`, and param_sum_kernel adds the workgroups' up: no atomics, the same result
 // every time.
 template <typename T, typename P, bool VEC, int WAVES, int NV, bool X8>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 2 : 1) void layer_norm_grad_kernel(NormGradArgs a) {
   __shared__ float sm[2][2 * WAVES];
   __shared__ float join[WAVES == 1 ? 4 * 64 * 16 : 1];
   const int l16 = threadIdx.x & 15, lane = threadIdx.x & 63, C = a.C;
@@ -153,31 +153,49 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad
       dw[j][e] = db[j][e] = 0.f;
     }
   }
+  // the next row is on its way while one is worked on
+  Raw8<T> rdy[NV], rx[NV];
+  uint2 rc[NV];
+  uint32_t rs[NV];
+  float mean = 0.f, rstd = 0.f;
+  auto load = [&](int64_t row) {
+    mean = a.stats[2 * row];
+    rstd = a.stats[2 * row + 1];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int run = run0 + 4 * WAVES * j;
+      rdy[j] = load_raw8<T, VEC>((const T*)a.dy + row * C, run * kRun, l16, C);
+      if constexpr (X8) {
+        rc[j] = run < runs ? load_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16) : make_uint2(0, 0);
+        rs[j] = run < runs ? a.x8.scales[row * ss + run] : 0;
+      } else {
+        rx[j] = load_raw8<T, VEC>((const T*)a.x + row * C, run * kRun, l16, C);
+      }
+    }
+  };
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * teams + team; row < a.rows; row += (int64_t)gridDim.x * teams, turn ^= 1) {
-    const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
+  const int64_t step = (int64_t)gridDim.x * teams;
+  int64_t row = (int64_t)blockIdx.x * teams + team;
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step, turn ^= 1) {
+    const float mu = mean, r = rstd;
     float dy[NV][8], n[NV][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int run = run0 + 4 * WAVES * j;
-      load8<T, VEC>((const T*)a.dy + row * C, run * kRun, l16, C, dy[j]);
-      if constexpr (X8) {
-        if (run < runs) {
-          decode8(load_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16), a.x8.scales[row * ss + run], n[j]);
-        } else {
+      if constexpr (X8) decode8(rc[j], rs[j], n[j]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) n[j][e] = 0.f;
-        }
-      } else {
-        load8<T, VEC>((const T*)a.x + row * C, run * kRun, l16, C, n[j]);
+      for (int e = 0; e < 8; ++e) {
+        dy[j][e] = (float)rdy[j].v[e];
+        if constexpr (!X8) n[j][e] = (float)rx[j].v[e];
       }
     }
+    if (row + step < a.rows) load(row + step);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[j][e] = (n[j][e] - mean) * rstd;   // past C: dy is 0, so the value does not matter (it is finite where the row's are)
+        n[j][e] = (n[j][e] - mu) * r;   // past C: dy is 0, so the value does not matter (it is finite where the row's are)
         const float g = dy[j][e] * w[j][e];
         s1 += g;
         s2 = fmaf(g, n[j][e], s2);
@@ -190,7 +208,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad
     for (int j = 0; j < NV; ++j) {
       float dx[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dx[e] = rstd * (dy[j][e] * w[j][e] - m1 - n[j][e] * m2);
+      for (int e = 0; e < 8; ++e) dx[e] = r * (dy[j][e] * w[j][e] - m1 - n[j][e] * m2);
       store8<T, VEC>((T*)a.dx + row * C, (run0 + 4 * WAVES * j) * kRun, l16, C, dx);
     }
   }
@@ -229,25 +247,30 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_grad
   }
 }
 
-// The sums over p < parts of part[p * n + c], c < n: columns below `split` go to out, the others to out2 (either may be null); 64
-// columns a workgroup, 4 quarters of the parts, in a fixed order.
-__global__ __launch_bounds__(256) void param_sum_kernel(const float* __restrict__ part, int parts, int n, int split,
-                                                        float* __restrict__ out, float* __restrict__ out2) {
-  __shared__ float sm[256];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+// The sums over p < parts of part[p * n + c], c < n: columns below `split` go to out, the others to out2 (either may be null). 64
+// columns a workgroup, a sixteenth of the parts a wave, joined in a fixed order: the parts' addresses are known at once, so the time is
+// that of a few loads in a row (512 parts of 2 x 1536 columns: 12 us with a quarter a wave).
+__global__ __launch_bounds__(1024) void param_sum_kernel(const float* __restrict__ part, int parts, int n, int split,
+                                                         float* __restrict__ out, float* __restrict__ out2) {
+  __shared__ float sm[16][64];
+  const int l = threadIdx.x & 63, c = blockIdx.x * 64 + l, q = threadIdx.x >> 6;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < n) {
     int p = q;
-    for (; p + 12 < parts; p += 16)
+    for (; p + 48 < parts; p += 64)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(p + 4 * u) * n + c];
-    for (; p < parts; p += 4) s[0] += part[(int64_t)p * n + c];
+      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(p + 16 * u) * n + c];
+    for (; p < parts; p += 16) s[0] += part[(int64_t)p * n + c];
   }
-  sm[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  sm[q][l] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
   float* const to = c < split ? out : out2;
-  if (q == 0 && c < n && to)
-    to[c < split ? c : c - split] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
+  if (q == 0 && c < n && to) {
+    float t = 0.f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) t += sm[u][l];
+    to[c < split ? c : c - split] = t;
+  }
 }
 
 // A wave takes 4 runs of a row (one word of scales), 16 lanes each.
@@ -343,13 +366,14 @@ int launch_layer_norm(int dtype, int param_dtype, const void* x, int64_t rows, i
 }
 
 int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream) {
-  hipLaunchKernelGGL(param_sum_kernel, dim3((unsigned)ceil_div(n, 64)), dim3(256), 0, stream, part, parts, n, split, out, out2);
+  hipLaunchKernelGGL(param_sum_kernel, dim3((unsigned)ceil_div(n, 64)), dim3(1024), 0, stream, part, parts, n, split, out, out2);
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
 }
 
+// a workgroup's rows are at least two for each of its teams: its parts of dw and db cost as much as a row
 int64_t norm_grad_blocks(int64_t rows, int C) {
-  return std::min<int64_t>(kGradBlocks, C <= 2048 ? ceil_div(rows, 4) : rows);
+  return std::min<int64_t>(kGradBlocks, C <= 2048 ? ceil_div(rows, 8) : ceil_div(rows, 2));
 }
 
 int launch_layer_norm_grad(int dtype, int param_dtype, const void* dy, const void* x, In8 x8, const float* stats,
