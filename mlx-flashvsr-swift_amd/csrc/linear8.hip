@@ -45,6 +45,7 @@ struct Linear8Args {
   int bias_f32, gelu, vec_out;
   void* y;
   int tiles_m, tiles_n;
+  int part_runs;         // runs of a part, whole words of scales (linear8_kernel; part p writes its own rows x N sums at y)
 };
 
 // 0.5 y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) = y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))), the exponential in base 2:
@@ -174,17 +175,18 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
 #pragma unroll
     for (int m = 0; m < FM; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  copy_step(0);
+  const int k_from = blockIdx.y * a.part_runs, k_to = min(a.runs, k_from + a.part_runs);
+  copy_step(k_from);
   for (int n = threadIdx.x; n < TN; n += 64 * kWaves)
     bias[n] = !a.bias || n0 + n >= a.N ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n0 + n] : (float)((const bf16*)a.bias)[n0 + n];
   int qw[FN], qx[FM];
-  for (int k0 = 0; k0 < a.runs; k0 += 4) {
+  for (int k0 = k_from; k0 < k_to; k0 += 4) {
     static_for<0, 4>([&](auto kc) {
       constexpr int OP = decltype(kc)::value;
       const int k = k0 + OP;
-      if (k >= a.runs) return;
+      if (k >= k_to) return;
       wait_all_and_sync();   // step k is in LDS, and nobody reads step k - 1 any more
-      if (k + 1 < a.runs) copy_step(k + 1);
+      if (k + 1 < k_to) copy_step(k + 1);
       if constexpr (OP == 0) {
         const char* ps = sm + 2 * kStage + ((k >> 2) & 1) * kScales;
 #pragma unroll
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
   }
 
   const int fn = wn * (TN / WN) + 8 * g;
-  write_tile(a, acc, (O*)a.y, bias + fn, n0 + fn, m0 + rx0);
+  write_tile(a, acc, (O*)a.y + blockIdx.y * a.rows * a.N, bias + fn, n0 + fn, m0 + rx0);
 }
 
 // The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between them. Two groups
@@ -444,36 +446,146 @@ __global__ __launch_bounds__(256) void widen_kernel(const bf16* __restrict__ in,
   if (i < n) out[i] = (float)in[i];
 }
 
-size_t linear8_workspace(int64_t, int, int N) { return (size_t)N * sizeof(float); }
+// y = the sum over parts of their (rows, N) sums, bias, GELU
+template <typename O>
+__global__ __launch_bounds__(256) void linear8_join_kernel(const float* __restrict__ part, int parts, int64_t n, int N,
+                                                           const void* __restrict__ bias, int bias_f32, int gelu, O* __restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = part[i];
+  for (int p = 1; p < parts; ++p) s += part[p * n + i];
+  if (bias) s += bias_f32 ? ((const float*)bias)[i % N] : (float)((const bf16*)bias)[i % N];
+  if (gelu) s = gelu_tanh(s);
+  y[i] = (O)s;
+}
+
+// The product of a few tokens (16 * FM at most), bound by reading the weights: 16 features a workgroup, its four waves take every
+// fourth run and read their operands straight into registers, all of them asked for at once as far as the registers go; the waves' sums
+// meet in LDS. 1 x 1536 x 9216: ___ us, 128 x 128 tiles 9.9.
+template <int FM, typename O>
+__global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a) {
+  __shared__ float sm[4][FM][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, ld = a.runs * kRun;
+  const int rows = (int)a.rows;
+  // rows past the last one read it again: their results are not stored
+  const int n = min(n0 + i, a.N - 1);
+  const uint8_t* const w = a.w.codes + (int64_t)n * ld + g * 32;
+  const uint8_t* const ws = a.w.scales + (int64_t)n * a.ss;
+  f32x4 acc[FM];
+#pragma unroll
+  for (int m = 0; m < FM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 3
+  for (int k = wave; k < a.runs; k += 4) {
+    const u32x4 lo = *(const u32x4*)(w + k * kRun), hi = *(const u32x4*)(w + k * kRun + 16);
+    const i32x8 fw = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    const int qw = ws[k];
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      const int row = min(16 * m + i, rows - 1);
+      const uint8_t* x = a.x.codes + (int64_t)row * ld + g * 32 + k * kRun;
+      const u32x4 xl = *(const u32x4*)x, xh = *(const u32x4*)(x + 16);
+      const i32x8 fx = i32x8{(int)xl[0], (int)xl[1], (int)xl[2], (int)xl[3], (int)xh[0], (int)xh[1], (int)xh[2], (int)xh[3]};
+      acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, acc[m], 0, 0, 0, qw, 0, (int)a.x.scales[(int64_t)row * a.ss + k]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sm[wave][m][i][4 * g + e] = acc[m][e];   // token i, feature 4 g + e
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < FM; ++m) {
+    const int token = threadIdx.x >> 4, f = threadIdx.x & 15, row = 16 * m + token;
+    if (row >= rows || n0 + f >= a.N) continue;
+    float s = (sm[0][m][token][f] + sm[1][m][token][f]) + (sm[2][m][token][f] + sm[3][m][token][f]);
+    if (a.bias) s += a.bias_f32 ? ((const float*)a.bias)[n0 + f] : (float)((const bf16*)a.bias)[n0 + f];
+    if (a.gelu) s = gelu_tanh(s);
+    ((O*)a.y)[(int64_t)row * a.N + n0 + f] = (O)s;
+  }
+}
+
+// How a product is cut up. A few tokens: by 16 features. Else tiles of 256 x 256, one a CU, or of 128 x 128, two a CU: a round of the
+// former does twice the work of one of the latter in 1.6 times its time (full rounds, 8192^3: 405 us against 518), so by the rounds
+// that each needs. Where there are few of the latter, each row's runs are cut into parts of at least 8 (512 x 4096 x 1536, 48 tiles: ___
+// us in 4 parts and the join, 25 in one).
+struct Linear8Plan {
+  bool few, large;
+  int64_t tiles;
+  int parts, part_runs;
+};
+static Linear8Plan linear8_plan(int64_t rows, int K, int N) {
+  auto tiles_of = [&](int t) { return ceil_div(rows, t) * ceil_div(N, t); };
+  Linear8Plan p{};
+  p.few = rows <= 64;
+  p.large = ceil_div(tiles_of(256), 256) * 8 <= ceil_div(tiles_of(128), 512) * 5;
+  p.tiles = tiles_of(p.large ? 256 : 128);
+  const int runs = runs_of(K);
+  int64_t parts = 1;
+  if (!p.few && !p.large && p.tiles < 256) parts = std::max<int64_t>(1, std::min<int64_t>(256 / p.tiles, runs / 8));
+  p.part_runs = (int)ceil_div(ceil_div(runs, 4), parts) * 4;
+  p.parts = (int)ceil_div(runs, p.part_runs);
+  return p;
+}
+
+size_t linear8_workspace(int64_t rows, int K, int N) {
+  const Linear8Plan p = linear8_plan(rows, K, N);
+  if (p.few) return 0;
+  return p.large ? (size_t)N * sizeof(float) : p.parts > 1 ? (size_t)p.parts * rows * N * sizeof(float) : 0;
+}
 
 int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, const void* bias, int gelu, int out_dtype,
                    void* y, void* ws, hipStream_t stream) {
   if (rows <= 0) return FVSR_OK;
+  const Linear8Plan p = linear8_plan(rows, K, N);
   Linear8Args a{};
   a.x = x; a.w = w; a.rows = rows; a.N = N; a.runs = runs_of(K); a.ss = scale_stride(K);
   a.bias = bias; a.bias_f32 = bias_dtype == FVSR_DTYPE_F32; a.gelu = gelu; a.y = y;
   a.vec_out = rows_vectorize(y, N);
-  auto tiles_of = [&](int t) { return ceil_div(rows, t) * ceil_div(N, t); };
-  if (tiles_of(128) >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
+  a.part_runs = p.part_runs;
+  if (!p.few && p.tiles >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
   const bool bf = out_dtype == FVSR_DTYPE_BF16;
-  // A CU does one 256 x 256 tile, or two of 128 x 128 at a time; a round of the former does twice the work of one of the latter in
-  // 1.6 times its time (measured at full rounds, 8192^3: 413 us against 518). So by the rounds that each needs:
-  const bool large = ceil_div(tiles_of(256), 256) * 8 <= ceil_div(tiles_of(128), 512) * 5;
-  const int T = large ? 256 : 128;
+  const int T = p.large ? 256 : 128;
   a.tiles_m = (int)ceil_div(rows, T);
   a.tiles_n = (int)ceil_div(N, T);
-  const int64_t tiles = tiles_of(T);
-  if (large) {
+  if (p.few) {
+    const dim3 grid((unsigned)ceil_div(N, 16));
+    auto go = [&](auto fm) {
+      constexpr int FM = decltype(fm)::value;
+      if (bf) hipLaunchKernelGGL((linear8_few_kernel<FM, bf16>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((linear8_few_kernel<FM, float>), grid, dim3(256), 0, stream, a);
+    };
+    if (rows <= 16) go(std::integral_constant<int, 1>{});
+    else if (rows <= 32) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+  } else if (p.large) {
     if (bias && !a.bias_f32) {
       hipLaunchKernelGGL(widen_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, stream, (const bf16*)bias, N, (float*)ws);
       a.bias = ws;
     }
-    const dim3 grid((unsigned)std::min<int64_t>(256, ceil_div(tiles, kXcds) * kXcds));
+    const dim3 grid((unsigned)std::min<int64_t>(256, ceil_div(p.tiles, kXcds) * kXcds));
     if (bf) hipLaunchKernelGGL((linear8_large_kernel<bf16>), grid, dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((linear8_large_kernel<float>), grid, dim3(512), 0, stream, a);
+  } else if (p.parts > 1) {
+    Linear8Args part = a;
+    part.bias = nullptr;
+    part.gelu = 0;
+    part.y = ws;
+    part.vec_out = N % 8 == 0;
+    hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(256), 0, stream, part);
+    FVSR_HIP_CHECK(hipGetLastError());
+    const int64_t n = rows * N;
+    const dim3 grid((unsigned)ceil_div(n, 256));
+    if (bf)
+      hipLaunchKernelGGL((linear8_join_kernel<bf16>), grid, dim3(256), 0, stream, (const float*)ws, p.parts, n, N, bias, a.bias_f32,
+                         gelu, (bf16*)y);
+    else
+      hipLaunchKernelGGL((linear8_join_kernel<float>), grid, dim3(256), 0, stream, (const float*)ws, p.parts, n, N, bias, a.bias_f32,
+                         gelu, (float*)y);
   } else {
-    if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, bf16>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+    const dim3 grid((unsigned)p.tiles);
+    if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, bf16>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), grid, dim3(256), 0, stream, a);
   }
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
@@ -872,7 +984,7 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const bf16* __restrict_
 int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);   // rows8.hip
 
 // How a weight gradient is cut up: tiles of 256 x 256 with DMA copies where dY's rows can be read 16 bytes at a time, else of 128 x
-// 128; the tokens into as many parts as fill the card, of at least 8 (16) steps.
+// 128; the tokens into as many parts as fill the card, of at least 4 steps.
 struct WeightGradPlan {
   bool large;
   int tiles_n, tiles_k, parts;
@@ -887,7 +999,7 @@ static WeightGradPlan weight_grad_plan(int64_t rows, int N, int K, bool vec_dy) 
   p.tiles_n = (int)ceil_div(N, T);
   p.tiles_k = (int)ceil_div(K, T);
   const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, steps = ceil_div(rows, step);
-  const int64_t parts = std::max<int64_t>(1, std::min(slots / tiles, steps / (p.large ? 8 : 16)));
+  const int64_t parts = std::max<int64_t>(1, std::min(slots / tiles, steps / 4));
   p.part_rows = ceil_div(std::max<int64_t>(steps, 1), parts) * step;
   p.parts = (int)std::max<int64_t>(1, ceil_div(rows, p.part_rows));
   p.sum_parts = p.large ? p.parts * p.tiles_k : (int)std::max<int64_t>(1, std::min<int64_t>(kSumParts, ceil_div(rows, 16)));
