@@ -12,7 +12,8 @@ A training pass of a linear layer keeps nothing but what its forward pass read:
   dx = linear8(dy, quantize8(w.t().contiguous())); dw, db = linear8_weight_grad(dy, x8)
 
 Tokens are (L, C) or (1, L, C), contiguous, on a HIP device; L may be 0. The calls keep no state: temporaries come from torch's
-allocator on the stream that the call runs on, so calls may overlap on several streams and be captured into graphs.
+allocator on the stream that the call runs on (the current one, or `stream`), so calls may overlap on several streams and be
+captured into graphs.
 """
 from __future__ import annotations
 
@@ -73,8 +74,8 @@ class Blocks8:
     def empty(cls, rows: int, features: int, device) -> "Blocks8":
         c, s = _widths(features)
         q = cls.__new__(cls)
-        q.codes = torch.empty((rows, c), dtype=CODES, device=device)
-        q.scales = torch.empty((rows, s), dtype=SCALES, device=device)
+        q.codes = torch.empty(rows, c, dtype=CODES, device=device)
+        q.scales = torch.empty(rows, s, dtype=SCALES, device=device)
         q.features = features
         return q
 
@@ -124,17 +125,18 @@ def _one_device(first: torch.Tensor, name: str, *more) -> torch.device:
 _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(device).cuda_stream, without its 2 us
 
 
-def _on_stream(stream, dev: torch.device, make):
-    """(stream handle, make()): `make` allocates the call's tensors. They belong to the stream that the kernels run on, so that
-    the allocator hands their memory on in that stream's order."""
-    if stream is None:
-        return _raw_stream(dev.index), make()
+def _current(stream, t):
+    """The scope in which `stream` (a torch stream, or a hipStream_t as an integer) is the current one: a call given a stream runs
+    itself in it, so that its temporaries belong to the stream that its kernels run on, and the allocator hands their memory on in
+    that stream's order."""
+    dev = t.device
+    if dev.type != "cuda":
+        _refuse("stream", f"a stream for tensors on {dev}")
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), dev) if int(stream) else torch.cuda.default_stream(dev)
     if stream.device != dev:
         _refuse("stream", f"a stream of {stream.device} for tensors on {dev}")
-    with torch.cuda.stream(stream):
-        return stream.cuda_stream, make()
+    return torch.cuda.stream(stream)
 
 
 _contexts: dict = {}
@@ -173,13 +175,13 @@ def _param(t, name: str, features: int):
     return t
 
 
-def _params(dtype, *ts):
-    """(type code, *parameters): of one type, fp32 or the tokens'; others are widened to fp32 (exact)."""
-    if all(t is None or t.dtype == torch.float32 for t in ts):
-        return (DTYPE_F32, *ts)
-    if all(t is None or t.dtype == dtype for t in ts):
-        return (_CODE[dtype], *ts)
-    return (DTYPE_F32, *(None if t is None else t.float() for t in ts))
+def _params(dtype, w, b=None):
+    """(type code, w, b): of one type, fp32 or the tokens'; others are widened to fp32 (exact)."""
+    if (w is None or w.dtype == torch.float32) and (b is None or b.dtype == torch.float32):
+        return DTYPE_F32, w, b
+    if (w is None or w.dtype == dtype) and (b is None or b.dtype == dtype):
+        return _CODE[dtype], w, b
+    return DTYPE_F32, None if w is None else w.float(), None if b is None else b.float()
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -189,27 +191,35 @@ def quantize8(x: torch.Tensor, stream=None, out: Blocks8 | None = None) -> Block
     """x (rows, features), float32 or bfloat16, in 8 bits: of each run of 128 channels of a row, the scale is the smallest power
     of two 2^e, e >= -127, with max |x| <= 448 * 2^e, and a channel's code the e4m3 number nearest to x / 2^e, ties to even.
     Infinities and NaN become NaN and do not count for the scale."""
+    if stream is not None:
+        with _current(stream, x):
+            return quantize8(x, out=out)
     x2 = _tokens(x, "x")
     rows, c = x2.shape
     if out is not None:
         _same("out", out.shape, (rows, c))
     dev = _one_device(x2, "x", (out, "out"))
-    handle, q = _on_stream(stream, dev, lambda: Blocks8.empty(rows, c, dev) if out is None else out)
+    q = Blocks8.empty(rows, c, dev) if out is None else out
     _check(lib.fvsr_quantize8(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, q.codes.data_ptr(), q.scales.data_ptr(),
-                              handle), "fvsr_quantize8")
+                              _raw_stream(dev.index)), "fvsr_quantize8")
     return q
 
 
 def dequantize8(q: Blocks8, dtype: torch.dtype = torch.bfloat16, stream=None, out=None) -> torch.Tensor:
     """The values that q stands for, (rows, features) in `dtype`. From bfloat16 or float32 tokens the round trip is off by at most
     2^-4 relative to a channel's value, or 2^-17 relative to its run's largest, whichever is more."""
+    if stream is not None:
+        with _current(stream, q):
+            return dequantize8(q, dtype, out=out)
     if dtype not in _CODE:
         _refuse("dequantize8", f"unsupported dtype {dtype} (float32 or bfloat16)")
-    o = _out(out, "out", q.shape, dtype)
+    rows, c = q.shape
+    o = _out(out, "out", (rows, c), dtype)
     dev = _one_device(q.codes, "q", (o, "out"))
-    handle, o = _on_stream(stream, dev, lambda: torch.empty(q.shape, dtype=dtype, device=dev) if o is None else o)
-    _check(lib.fvsr_dequantize8(_ctx(dev), q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.features, _CODE[dtype],
-                                o.data_ptr(), handle), "fvsr_dequantize8")
+    if o is None:
+        o = torch.empty(rows, c, dtype=dtype, device=dev)
+    _check(lib.fvsr_dequantize8(_ctx(dev), q.codes.data_ptr(), q.scales.data_ptr(), rows, c, _CODE[dtype], o.data_ptr(),
+                                _raw_stream(dev.index)), "fvsr_dequantize8")
     return o if out is None else out
 
 
@@ -222,29 +232,32 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, want_
     x's dtype; with `quantized`, y is a Blocks8 made from the 32-bit values. stats, (rows, 2) float32 mean and 1 / sqrt(var +
     eps), and x8, the rows as they came in 8 bits, are what layer_norm_backward reads (None unless wanted). weight and bias:
     (channels), float32 or bfloat16. The modulated norm of a DiT block is weight = 1 + scale, bias = shift."""
+    if stream is not None:
+        with _current(stream, x):
+            return layer_norm(x, weight, bias, eps, want_stats, want_x8, quantized, out=out)
     x2 = _tokens(x, "x")
     rows, c = x2.shape
     weight, bias = _param(weight, "weight", c), _param(bias, "bias", c)
     if not quantized:
-        o = _out(out, "out", (rows, c), x2.dtype)
+        y = _out(out, "out", (rows, c), x2.dtype)
     elif out is not None:
         _same("out", out.shape, (rows, c))
     dev = _one_device(x2, "x", (weight, "weight"), (bias, "bias"), (out, "out"))
-
-    def make():
-        kind, w, b = _params(x2.dtype, weight, bias)
-        if quantized:
-            y = Blocks8.empty(rows, c, dev) if out is None else out
-        else:
-            y = torch.empty_like(x) if o is None else o
-        return (kind, w, b, y, torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None,
-                Blocks8.empty(rows, c, dev) if want_x8 else None)
-
-    handle, (kind, w, b, y, stats, x8) = _on_stream(stream, dev, make)
-    yp = (None, *_p8(y)) if quantized else (y.data_ptr(), None, None)
-    _check(lib.fvsr_layer_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, eps, kind, _p(w), _p(b), *yp, *_p8(x8),
-                               _p(stats), handle), "fvsr_layer_norm")
-    return (y if out is None else out), stats, x8
+    kind, w, b = _params(x2.dtype, weight, bias)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if want_stats else None
+    x8 = Blocks8.empty(rows, c, dev) if want_x8 else None
+    if quantized:
+        result = Blocks8.empty(rows, c, dev) if out is None else out
+        yp, (yc, ys) = None, _p8(result)
+    else:
+        result = out
+        if y is None:
+            result = y = torch.empty_like(x)
+        yp, yc, ys = y.data_ptr(), None, None
+    xc, xs = _p8(x8)
+    _check(lib.fvsr_layer_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, eps, kind, _p(w), _p(b), yp, yc, ys, xc, xs,
+                               _p(stats), _raw_stream(dev.index)), "fvsr_layer_norm")
+    return result, stats, x8
 
 
 def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, want_params: bool = True, stream=None,
@@ -252,6 +265,9 @@ def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, w
     """(dx, dweight, dbias) of layer_norm: x is the tensor that it normed (dy's dtype) or the Blocks8 kept of it, stats what it
     returned, weight the one that it was given. dweight and dbias are float32 (channels), None without `want_params`; they are
     summed in a fixed order. `out` may be dy itself."""
+    if stream is not None:
+        with _current(stream, dy):
+            return layer_norm_backward(dy, x, stats, weight, want_params, out=out)
     d2 = _tokens(dy, "dy")
     rows, c = d2.shape
     kept = x if isinstance(x, Blocks8) else None
@@ -267,19 +283,18 @@ def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, w
     weight = _param(weight, "weight", c)
     o = _out(out, "out", (rows, c), d2.dtype)
     dev = _one_device(d2, "dy", (x, "x"), (stats, "stats"), (weight, "weight"), (o, "out"))
-    nbytes = lib.fvsr_layer_norm_backward_workspace(rows, c) if want_params else 0
-
-    def make():
-        kind, w = _params(d2.dtype, weight)
-        dx = torch.empty_like(dy) if o is None else o
-        if not want_params:
-            return kind, w, dx, None, None, None
-        return (kind, w, dx, torch.empty(c, dtype=torch.float32, device=dev), torch.empty(c, dtype=torch.float32, device=dev),
-                torch.empty(nbytes, dtype=torch.uint8, device=dev))
-
-    handle, (kind, w, dx, dw, db, ws) = _on_stream(stream, dev, make)
-    _check(lib.fvsr_layer_norm_backward(_ctx(dev), _CODE[d2.dtype], d2.data_ptr(), _p(x2), *_p8(kept), stats.data_ptr(), rows,
-                                        c, kind, _p(w), dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes, handle),
+    kind, w, _ = _params(d2.dtype, weight)
+    dx = torch.empty_like(dy) if o is None else o
+    dw = db = ws = None
+    nbytes = 0
+    if want_params:
+        nbytes = lib.fvsr_layer_norm_backward_workspace(rows, c)
+        dw = torch.empty(c, dtype=torch.float32, device=dev)
+        db = torch.empty_like(dw)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    xc, xs = _p8(kept)
+    _check(lib.fvsr_layer_norm_backward(_ctx(dev), _CODE[d2.dtype], d2.data_ptr(), _p(x2), xc, xs, stats.data_ptr(), rows, c, kind,
+                                        _p(w), dx.data_ptr(), _p(dw), _p(db), _p(ws), nbytes, _raw_stream(dev.index)),
            "fvsr_layer_norm_backward")
     return (dx if out is None else out), dw, db
 
@@ -293,6 +308,9 @@ def linear8(x, weight: Blocks8, bias=None, gelu: bool = False, dtype: torch.dtyp
     32 bits (the matrix cores cut each product to 13 bits below the largest of 8 neighbouring channels' first, so a float32 y is good
     to about 2^-12 of its terms' size). x: a Blocks8, or (rows, in_features) float32 or bfloat16 tokens, quantized in the call;
     weight: quantize8 of the (out_features, in_features) matrix, made once; bias: (out_features), float32 or bfloat16."""
+    if stream is not None:
+        with _current(stream, x):
+            return linear8(x, weight, bias, gelu, dtype, out=out)
     if dtype not in _CODE:
         _refuse("linear8", f"unsupported dtype {dtype} (float32 or bfloat16)")
     if not isinstance(weight, Blocks8):
@@ -315,18 +333,17 @@ def linear8(x, weight: Blocks8, bias=None, gelu: bool = False, dtype: torch.dtyp
         at = (need + 255) & ~255
         nbytes = at + rows * (code_bytes + scale_bytes)
 
-    def make():
-        return (torch.empty(shape, dtype=dtype, device=dev) if o is None else o,
-                torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None)
-
-    handle, (y, ws) = _on_stream(stream, dev, make)
+    y = torch.empty(shape, dtype=dtype, device=dev) if o is None else o
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     wp = _p(ws)
     if x2 is None:
-        kind, xp, qp = DTYPE_F32, None, _p8(x8)
+        kind, xp, (qc, qs) = DTYPE_F32, None, _p8(x8)
     else:
-        kind, xp, qp = _CODE[x2.dtype], x2.data_ptr(), (wp and wp + at, wp and wp + at + rows * code_bytes)
-    _check(lib.fvsr_linear8(_ctx(dev), kind, xp, rows, k, *qp, *_p8(weight), n, DTYPE_F32 if bias is None else _CODE[bias.dtype],
-                            _p(bias), 1 if gelu else 0, _CODE[dtype], y.data_ptr(), wp, need, handle), "fvsr_linear8")
+        kind, xp = _CODE[x2.dtype], x2.data_ptr()
+        qc, qs = (wp and wp + at), (wp and wp + at + rows * code_bytes)
+    _check(lib.fvsr_linear8(_ctx(dev), kind, xp, rows, k, qc, qs, weight.codes.data_ptr(), weight.scales.data_ptr(), n,
+                            DTYPE_F32 if bias is None else _CODE[bias.dtype], _p(bias), 1 if gelu else 0, _CODE[dtype],
+                            y.data_ptr(), wp, need, _raw_stream(dev.index)), "fvsr_linear8")
     return y if out is None else out
 
 
@@ -335,6 +352,9 @@ def linear8_weight_grad(dy: torch.Tensor, x8: Blocks8, dtype: torch.dtype = torc
     """(dW, db) of linear8: dW = dY^T X, (out_features, in_features) in `dtype`, from bfloat16 dY (rows, out_features) and the
     8-bit X that the layer read; db the sum of dY's rows, float32 (None without `want_bias`). Products and sums in 32 bits, in
     a fixed order."""
+    if stream is not None:
+        with _current(stream, dy):
+            return linear8_weight_grad(dy, x8, dtype, want_bias, out=out)
     if dtype not in _CODE:
         _refuse("linear8_weight_grad", f"unsupported dtype {dtype} (float32 or bfloat16)")
     if not isinstance(x8, Blocks8):
@@ -348,12 +368,10 @@ def linear8_weight_grad(dy: torch.Tensor, x8: Blocks8, dtype: torch.dtype = torc
     dev = _one_device(d2, "dy", (x8, "x8"), (o, "out"))
     nbytes = lib.fvsr_linear8_weight_grad_workspace(rows, k, n)
 
-    def make():
-        return (torch.empty((n, k), dtype=dtype, device=dev) if o is None else o,
-                torch.empty(n, dtype=torch.float32, device=dev) if want_bias else None,
-                torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None)
-
-    handle, (dw, db, ws) = _on_stream(stream, dev, make)
-    _check(lib.fvsr_linear8_weight_grad(_ctx(dev), d2.data_ptr(), rows, n, *_p8(x8), k, _CODE[dtype], dw.data_ptr(), _p(db),
-                                        _p(ws), nbytes, handle), "fvsr_linear8_weight_grad")
+    dw = torch.empty(n, k, dtype=dtype, device=dev) if o is None else o
+    db = torch.empty(n, dtype=torch.float32, device=dev) if want_bias else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _check(lib.fvsr_linear8_weight_grad(_ctx(dev), d2.data_ptr(), rows, n, x8.codes.data_ptr(), x8.scales.data_ptr(), k,
+                                        _CODE[dtype], dw.data_ptr(), _p(db), _p(ws), nbytes, _raw_stream(dev.index)),
+           "fvsr_linear8_weight_grad")
     return (dw if out is None else out), db
