@@ -56,33 +56,48 @@ __device__ __forceinline__ float gelu_tanh(float y) {
   return y * __builtin_amdgcn_rcpf(1.f + e);
 }
 
+// of 8 values, the steps side by side: an exponential or a reciprocal is used three instructions after it was asked for at the least
+__device__ __forceinline__ void gelu_tanh8(float (&y)[8]) {
+  constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
+  float e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = k * y[i] * fmaf(0.044715f * y[i], y[i], 1.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_rcpf(1.f + e[i]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= e[i];
+}
+
 // bias (fp32, in LDS, at this lane's first feature), GELU and the store of a wave's fragments: this lane's features n0 + 32 p .. + 7
-// (two fragments) of the tokens row0 + 16 m
-template <int FN, int FM, typename O>
-__device__ __forceinline__ void write_tile(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
-                                           int64_t row0) {
+// (two fragments) of the tokens row0 + 16 m. WHOLE: every feature and token is inside, and rows can be written 16 bytes at a time.
+template <bool GELU, bool WHOLE, int FN, int FM, typename O>
+__device__ __forceinline__ void write_fragments(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
+                                                int64_t row0) {
   float b[FN / 2][8];
 #pragma unroll
   for (int p = 0; p < FN / 2; ++p) {
     *(f32x4*)b[p] = *(const f32x4*)(bias + 32 * p);
     *(f32x4*)(b[p] + 4) = *(const f32x4*)(bias + 32 * p + 4);
   }
+  O* out0 = y + row0 * a.N + n0;
+  const int64_t step = (int64_t)16 * a.N;
 #pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    const int64_t row = row0 + 16 * m;
-    if (row >= a.rows) continue;
+  for (int m = 0; m < FM; ++m, out0 += step) {
+    if (!WHOLE && row0 + 16 * m >= a.rows) continue;
 #pragma unroll
     for (int p = 0; p < FN / 2; ++p) {
-      const int n = n0 + 32 * p;
+      float s[8];
       O v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float s = acc[2 * p + (e >> 2)][m][e & 3] + b[p][e];
-        if (a.gelu) s = gelu_tanh(s);
-        v[e] = (O)s;
-      }
-      O* out = y + row * a.N + n;
-      if (a.vec_out && n + 8 <= a.N) {
+      for (int e = 0; e < 8; ++e) s[e] = acc[2 * p + (e >> 2)][m][e & 3] + b[p][e];
+      if constexpr (GELU) gelu_tanh8(s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (O)s[e];
+      O* const out = out0 + 32 * p;
+      const int n = n0 + 32 * p;
+      if (WHOLE || (a.vec_out && n + 8 <= a.N)) {
         *(u32x4*)out = *(u32x4*)v;
         if constexpr (sizeof(O) == 4) ((u32x4*)out)[1] = ((u32x4*)v)[1];
       } else {
@@ -92,6 +107,14 @@ __device__ __forceinline__ void write_tile(const Linear8Args& a, const f32x4 (&a
       }
     }
   }
+}
+// true: by whole vectors (FN / 2 * FM * sizeof(O) / 2 stores)
+template <bool GELU, int FN, int FM, typename O>
+__device__ __forceinline__ bool write_tile(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
+                                           int64_t row0, bool whole) {
+  if (whole) write_fragments<GELU, true>(a, acc, y, bias, n0, row0);
+  else write_fragments<GELU, false>(a, acc, y, bias, n0, row0);
+  return whole;
 }
 
 // Tile of TN output features x TM tokens, WN x WM waves; a step is one run: 128 codes of every row, and their scales in the
@@ -106,7 +129,7 @@ __device__ __forceinline__ void write_tile(const Linear8Args& a, const f32x4 (&a
 // LDS holds two steps: rows of 128 bytes, the 16-byte chunks XOR-ed by a number of the row under which the 16 rows that one
 // instruction reads fall on 16 places of the 64 banks; copies go from memory to LDS directly (the XOR is on the source side), the
 // next step's while this one's products run. A word of scales holds 4 steps.
-template <int TN, int TM, int WN, int WM, typename O>
+template <int TN, int TM, int WN, int WM, bool GELU, typename O>
 __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a) {
   constexpr int kWaves = WN * WM, FN = TN / WN / 16, FM = TM / WM / 16;
   static_assert(FN % 2 == 0 && TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0, "tile");
@@ -213,7 +236,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
   }
 
   const int fn = wn * (TN / WN) + 8 * g;
-  write_tile(a, acc, (O*)a.y + blockIdx.y * a.rows * a.N, bias + fn, n0 + fn, m0 + rx0);
+  write_tile<GELU>(a, acc, (O*)a.y + blockIdx.y * a.rows * a.N, bias + fn, n0 + fn, m0 + rx0,
+                   a.vec_out && rows_m == TM && rows_n == TN);
 }
 
 // The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between them. Two groups
@@ -230,7 +254,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
 // once. Each is needed about three phases later, and its wave waits for it at the end of that time, by the count of what it has
 // asked for since (memory operations of a wave complete in order). A group writes its tile, and starts the next one, in its read
 // phase, under the other group's products.
-template <typename O>
+template <bool GELU, typename O>
 __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
   constexpr int FN = 4, FM = 8, kStores = FN / 2 * FM * (int)sizeof(O) / 2;
   constexpr int kBuf = 256 * kRun;                         // one operand's rows of a step
@@ -373,8 +397,8 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
   auto write = [&]() __attribute__((always_inline)) {
     if (!held) return false;
     const float* b = (const float*)(sm + kB + ((bt - 1) & 3) * 1024);
-    write_tile(a, acc, (O*)a.y, b + w * 64 + 8 * g, n0 + w * 64 + 8 * g, m0 + rx0);
-    return a.vec_out && m0 + 256 <= a.rows && n0 + 256 <= a.N;
+    return write_tile<GELU>(a, acc, (O*)a.y, b + w * 64 + 8 * g, n0 + w * 64 + 8 * g, m0 + rx0,
+                            a.vec_out && m0 + 256 <= a.rows && n0 + 256 <= a.N);
   };
 
   source();
@@ -460,8 +484,7 @@ __global__ __launch_bounds__(256) void linear8_join_kernel(const float* __restri
 }
 
 // The product of a few tokens (16 * FM at most), bound by reading the weights: 16 features a workgroup, its four waves take every
-// fourth run and read their operands straight into registers, all of them asked for at once as far as the registers go; the waves' sums
-// meet in LDS. 1 x 1536 x 9216: ___ us, 128 x 128 tiles 9.9.
+// fourth run and read their operands straight into registers, up to three runs asked for at once; the waves' sums meet in LDS. 1 x 1536 x 9216: ___ us, 128 x 128 tiles 9.9.
 template <int FM, typename O>
 __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a) {
   __shared__ float sm[4][FM][16][17];
@@ -475,19 +498,32 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a) {
   f32x4 acc[FM];
 #pragma unroll
   for (int m = 0; m < FM; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 3
-  for (int k = wave; k < a.runs; k += 4) {
-    const u32x4 lo = *(const u32x4*)(w + k * kRun), hi = *(const u32x4*)(w + k * kRun + 16);
-    const i32x8 fw = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    const int qw = ws[k];
+  constexpr int U = FM < 4 ? 3 : 2;   // runs asked for at once
+  for (int k0 = wave; k0 < a.runs; k0 += 4 * U) {
+    i32x8 fw[U], fx[U][FM];
+    int qw[U], qx[U][FM];
+    auto load = [](const uint8_t* p) {
+      const u32x4 lo = *(const u32x4*)p, hi = *(const u32x4*)(p + 16);
+      return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
 #pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      const int row = min(16 * m + i, rows - 1);
-      const uint8_t* x = a.x.codes + (int64_t)row * ld + g * 32 + k * kRun;
-      const u32x4 xl = *(const u32x4*)x, xh = *(const u32x4*)(x + 16);
-      const i32x8 fx = i32x8{(int)xl[0], (int)xl[1], (int)xl[2], (int)xl[3], (int)xh[0], (int)xh[1], (int)xh[2], (int)xh[3]};
-      acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, acc[m], 0, 0, 0, qw, 0, (int)a.x.scales[(int64_t)row * a.ss + k]);
+    for (int u = 0; u < U; ++u) {
+      const int k = min(k0 + 4 * u, a.runs - 1);   // past the last one: asked for again, and not used
+      fw[u] = load(w + k * kRun);
+      qw[u] = ws[k];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        const int64_t row = min(16 * m + i, rows - 1);
+        fx[u][m] = load(a.x.codes + row * ld + g * 32 + k * kRun);
+        qx[u][m] = a.x.scales[row * a.ss + k];
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + 4 * u < a.runs)
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+          acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u], fx[u][m], acc[m], 0, 0, 0, qw[u], 0, qx[u][m]);
   }
 #pragma unroll
   for (int m = 0; m < FM; ++m)
@@ -564,15 +600,20 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
       a.bias = ws;
     }
     const dim3 grid((unsigned)std::min<int64_t>(256, ceil_div(p.tiles, kXcds) * kXcds));
-    if (bf) hipLaunchKernelGGL((linear8_large_kernel<bf16>), grid, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((linear8_large_kernel<float>), grid, dim3(512), 0, stream, a);
+    auto go = [&](auto g) {
+      constexpr bool G = decltype(g)::value;
+      if (bf) hipLaunchKernelGGL((linear8_large_kernel<G, bf16>), grid, dim3(512), 0, stream, a);
+      else hipLaunchKernelGGL((linear8_large_kernel<G, float>), grid, dim3(512), 0, stream, a);
+    };
+    if (gelu) go(std::true_type{});
+    else go(std::false_type{});
   } else if (p.parts > 1) {
     Linear8Args part = a;
     part.bias = nullptr;
     part.gelu = 0;
     part.y = ws;
     part.vec_out = N % 8 == 0;
-    hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(256), 0, stream, part);
+    hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(256), 0, stream, part);
     FVSR_HIP_CHECK(hipGetLastError());
     const int64_t n = rows * N;
     const dim3 grid((unsigned)ceil_div(n, 256));
@@ -584,8 +625,13 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
                          gelu, (float*)y);
   } else {
     const dim3 grid((unsigned)p.tiles);
-    if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, bf16>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, float>), grid, dim3(256), 0, stream, a);
+    auto go = [&](auto g) {
+      constexpr bool G = decltype(g)::value;
+      if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, G, bf16>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, G, float>), grid, dim3(256), 0, stream, a);
+    };
+    if (gelu) go(std::true_type{});
+    else go(std::false_type{});
   }
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;

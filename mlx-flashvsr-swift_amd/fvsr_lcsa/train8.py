@@ -255,7 +255,7 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, want_
             result = y = torch.empty_like(x)
         yp, yc, ys = y.data_ptr(), None, None
     xc, xs = _p8(x8)
-    _check(lib.fvsr_layer_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, eps, kind, _p(w), _p(b), yp, yc, ys, xc, xs,
+    _check(lib.fvsr_layer_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, float(eps), kind, _p(w), _p(b), yp, yc, ys, xc, xs,
                                _p(stats), _raw_stream(dev.index)), "fvsr_layer_norm")
     return result, stats, x8
 
