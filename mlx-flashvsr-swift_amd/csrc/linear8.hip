@@ -613,7 +613,7 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
     part.gelu = 0;
     part.y = ws;
     part.vec_out = N % 8 == 0;
-    hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(256), 0, stream, part);
+    hipLaunchKernelGGL((linear8_kernel<128, 128, 4, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(512), 0, stream, part);
     FVSR_HIP_CHECK(hipGetLastError());
     const int64_t n = rows * N;
     const dim3 grid((unsigned)ceil_div(n, 256));
@@ -624,14 +624,17 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
       hipLaunchKernelGGL((linear8_join_kernel<float>), grid, dim3(256), 0, stream, (const float*)ws, p.parts, n, N, bias, a.bias_f32,
                          gelu, (float*)y);
   } else {
+    // where a CU has one workgroup at most, 8 waves of it: two on each SIMD, whose reads and products overlap
     const dim3 grid((unsigned)p.tiles);
-    auto go = [&](auto g) {
+    auto go = [&](auto wn, auto g) {
+      constexpr int WN = decltype(wn)::value;
       constexpr bool G = decltype(g)::value;
-      if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, G, bf16>), grid, dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((linear8_kernel<128, 128, 2, 2, G, float>), grid, dim3(256), 0, stream, a);
+      if (bf) hipLaunchKernelGGL((linear8_kernel<128, 128, WN, 2, G, bf16>), grid, dim3(128 * WN), 0, stream, a);
+      else hipLaunchKernelGGL((linear8_kernel<128, 128, WN, 2, G, float>), grid, dim3(128 * WN), 0, stream, a);
     };
-    if (gelu) go(std::true_type{});
-    else go(std::false_type{});
+    auto with = [&](auto wn) { gelu ? go(wn, std::true_type{}) : go(wn, std::false_type{}); };
+    if (p.tiles <= 256) with(std::integral_constant<int, 4>{});
+    else with(std::integral_constant<int, 2>{});
   }
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
@@ -803,21 +806,42 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
   const uint32_t oc = (uint32_t)((16 * w + r8) * ldk + c8 * 16);
   const int run = tk * 2 + other;                           // this wave's codes' run
   const int count = (int)(to - from);                       // tokens (a part has fewer than 2^31)
-  auto left = [&](int s) __attribute__((always_inline)) { return max(0, min(kTokens, count - s * kTokens)); };
-  u32x4 dd, dc, ds;    // dY, codes and scales of the steps that are asked for, and their places
-  uint32_t dy_at = 0, codes_at = 0, scales_at = 0;
-  const char* const dy0 = (const char*)(a.dy + from * a.N + n0);
-  const uint8_t* const codes0 = a.x.codes + from * ldk + run * kRun;
-  const uint8_t* const scales0 = a.x.scales + from * a.ss + (run & ~3);
-  auto place_dy = [&](int s) __attribute__((always_inline)) {
-    dd = make_rsrc(dy0 + (int64_t)s * (kTokens * ldn), (uint32_t)max(0, left(s) * ldn - n0 * 2));
-    dy_at = lds0 + ((s & 1) * 4 + w) * kBlk;
+  // dY, codes and scales of the step that is asked for next, and their places in LDS: steps are asked for in order, so all that a step
+  // costs is three sums (its 64-bit products and minima each time cost 60 us of 445)
+  auto records = [&](int left, int ld, int off) __attribute__((always_inline)) {
+    return (uint32_t)max(0, max(0, min(kTokens, left)) * ld - off);
   };
-  auto place_codes = [&](int s) __attribute__((always_inline)) {
-    dc = make_rsrc(codes0 + (int64_t)s * (kTokens * ldk), (uint32_t)max(0, left(s) * ldk - run * kRun));
-    ds = make_rsrc(scales0 + (int64_t)s * (kTokens * a.ss), (uint32_t)max(0, left(s) * a.ss - (run & ~3)));
-    codes_at = lds0 + kRaw + ((s & 1) * 2 + other) * kBlk + w * 2048;
-    scales_at = lds0 + kSc + ((s & 1) * 2 + other) * 256 + w * 64;
+  auto move = [](u32x4& d, int by) __attribute__((always_inline)) {
+    const uint64_t b = (((uint64_t)d[1] << 32) | d[0]) + (uint64_t)by;
+    d[0] = (uint32_t)b;
+    d[1] = (uint32_t)(b >> 32);
+  };
+  int dy_left = count, codes_left = count;
+  u32x4 dd = make_rsrc(a.dy + from * a.N + n0, records(count, ldn, n0 * 2));
+  u32x4 dc = make_rsrc(a.x.codes + from * ldk + run * kRun, records(count, ldk, run * kRun));
+  u32x4 ds = make_rsrc(a.x.scales + from * a.ss + (run & ~3), records(count, a.ss, run & ~3));
+  uint32_t dy_at = lds0 + w * kBlk, dy_flip = 4 * kBlk;
+  uint32_t codes_at = lds0 + kRaw + other * kBlk + w * 2048, codes_flip = 2 * kBlk;
+  uint32_t scales_at = lds0 + kSc + other * 256 + w * 64, scales_flip = 2 * 256;
+  auto next_dy = [&]() __attribute__((always_inline)) {
+    move(dd, kTokens * ldn);
+    dy_left -= kTokens;
+    if (dy_left < kTokens) dd[2] = records(dy_left, ldn, n0 * 2);
+    dy_at += dy_flip;
+    dy_flip = 0u - dy_flip;
+  };
+  auto next_codes = [&]() __attribute__((always_inline)) {
+    move(dc, kTokens * ldk);
+    move(ds, kTokens * a.ss);
+    codes_left -= kTokens;
+    if (codes_left < kTokens) {
+      dc[2] = records(codes_left, ldk, run * kRun);
+      ds[2] = records(codes_left, a.ss, run & ~3);
+    }
+    codes_at += codes_flip;
+    codes_flip = 0u - codes_flip;
+    scales_at += scales_flip;
+    scales_flip = 0u - scales_flip;
   };
   auto copy_dy = [&](auto c) __attribute__((always_inline)) {   // 8 of its 64 tokens
     copy16(dd, dy_at + c * 1024, (afresh(od) ^ ((c & 1) << 6)) + (r8 + c * 8) * ldn, 0);
@@ -918,21 +942,18 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
 #define FVSR_WAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 #define FVSR_READ_DONE() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
-  if (group == 0) {
-    place_dy(0);
-    static_for<0, 8>(copy_dy);
-  }
+  if (group == 0) static_for<0, 8>(copy_dy);
   for (int s = 0; s < 2; ++s) {
-    place_codes(s);
     static_for<0, 3>(copy_codes);
+    next_codes();
   }
   FVSR_WAIT(0);
   if (group == 1) {
     read_codes(0);
     FVSR_READ_DONE();
     widen();
-    place_codes(2);
     static_for<0, 3>(copy_codes);
+    next_codes();
   }
   turn();
   if (group == 1) turn();   // phase 0
@@ -940,18 +961,18 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
     if (group == 0) {
       FVSR_WAIT(11);        // codes of s; asked for since: dY(s), codes of s + 1
       read_codes(s);
-      place_dy(s + 1);
-      place_codes(s + 2);
+      next_dy();
       FVSR_READ_DONE();     // their place is free
       widen();
       read_step(s, std::true_type{});
+      next_codes();
     } else {
       FVSR_WAIT(3);         // codes of s + 1; since: codes of s + 2
       read_codes(s + 1);
-      place_codes(s + 3);
       FVSR_READ_DONE();
       widen();
       read_step(s, std::false_type{});
+      next_codes();
     }
     turn();
     multiply(s);
