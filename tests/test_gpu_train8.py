@@ -283,6 +283,41 @@ def test_linear8(dev, rows, k, n):
     assert torch.equal(f.linear8(xf[None], w8, b), f.linear8(x8, w8, b)[None])
 
 
+@pytest.mark.parametrize("rows,k,n", [(3000, 300, 3000), (2950, 128, 3001), (9000, 400, 3000), (2900, 1100, 2840), (600, 2100, 520),
+                                      (300, 4200, 131)])
+def test_linear8_of_many_tiles(dev, rows, k, n):
+    """Enough tiles that a workgroup takes whole CUs, one or several tiles each, ragged ones among them and 1 to 9 runs deep; and few
+    tiles of many runs, which are cut into parts."""
+    _, x, w, b = linear_case(rows, k, n, dev)
+    w8, x8 = f.quantize8(w), f.quantize8(x)
+    a64, w64 = quantize64(x)[0], quantize64(w)[0]
+    for bias, gelu, dtype in ((b, True, bf), (b.to(bf), False, bf), (None, False, f32), (b.to(bf), True, f32)):
+        print(f"  linear8 {rows} x {k} x {n} gelu {gelu} {dtype}", flush=True)
+        y = f.linear8(x8, w8, bias, gelu=gelu, dtype=dtype)
+        check_linear(y, a64, w64, bias, gelu)
+        assert torch.equal(f.linear8(x, w8, bias, gelu=gelu, dtype=dtype), y)
+    o = unaligned(torch.zeros((rows, n), dtype=f32, device=dev))
+    assert torch.equal(f.linear8(x8, w8, b.to(bf), gelu=True, dtype=f32, out=o), y)
+
+
+def test_blocks8_with_a_scale_of_nan(dev):
+    """A scale byte of 255 stands for NaN: its run's values are, and what is made of them."""
+    for rows in (40, 300):
+        x8 = f.quantize8(tokens(gen_of(rows), rows, 300, bf, dev))
+        w8 = f.quantize8(tokens(gen_of(5), 264, 300, bf, dev))
+        dy = tokens(gen_of(6), rows, 264, bf, dev)
+        x8.scales.view(torch.uint8)[7, 1] = 255
+        v = f.dequantize8(x8).isnan()
+        assert v[7, 128:256].all() and v.sum() == 128
+        y = f.linear8(x8, w8).isnan()
+        assert y[7].all() and y.sum() == 264
+        for d in (dy, unaligned(dy)):
+            dw = f.linear8_weight_grad(d, x8)[0].isnan()
+            assert dw[:, 128:256].all() and dw.sum() == 128 * 264
+        dx = f.layer_norm_backward(dy[:, :1].expand(rows, 300).contiguous(), x8, torch.ones((rows, 2), device=dev))[0].isnan()
+        assert dx[7].all() and dx.sum() == 300
+
+
 def test_linear8_of_rows_with_nan(dev):
     """A NaN token takes its row of y, a NaN weight its column; no other value."""
     _, x, w, b = linear_case(150, 300, 140, dev)
@@ -314,13 +349,14 @@ def test_linear8_past_32_bits(dev):
     within(db, dy.double().sum(0), (rows + 8) * U * dy.double().abs().sum(0), "dbias")
 
 
-@pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES + [(1000, 136, 200), (5000, 256, 264), (40, 2304, 2000)])
+@pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES + [(1000, 136, 200), (5000, 256, 264), (40, 2304, 2000),
+                                                      (129, 1000, 4200), (20000, 300, 520)])
 def test_linear8_weight_grad(dev, rows, k, n):
     g, x, _, _ = linear_case(rows, k, n, dev)
     dy = torch.randn((rows, n), generator=g).to(bf).to(dev)
     x8, a = f.quantize8(x), quantize64(x)[0]
     want, mag = dy.double().t() @ a, dy.double().abs().t() @ a.abs()
-    for dtype, d in ((f32, dy), (bf, unaligned(dy))):
+    for dtype, d in ((f32, dy), (bf, dy), (bf, unaligned(dy))):
         print(f"  linear8_weight_grad {rows} x {k} x {n} {dtype}", flush=True)
         dw, db = f.linear8_weight_grad(d, x8, dtype)
         within(dw, want, ((rows + 8) * U * mag + HALF[dtype] * want.abs()) * (1 + 2.0 ** -7), "dweight")
