@@ -794,7 +794,8 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
 // dY's copies stand between the reads from LDS: behind them, at the phase's end, their issue was what the other group waited for
 // (497 us at 17280 x 1536 x 8960).
 // Copies past the last token read zeros (and nothing else), so every phase asks for the same number.
-// db: a step's column sums are 8 more products with rows of ones, taken by one of the tiles_k workgroups that read the step.
+// db: a step's column sums are taken by one of the tiles_k workgroups that read the step, from the fragments in registers, under the
+// products (a column a lane; as products with rows of ones and zeros an infinity would reach other columns).
 template <typename O>
 __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArgs a) {
   constexpr int FN = 4, FM = 8, kTokens = 64;
@@ -901,7 +902,8 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
   const char* const pd = sm + w * kBlk;
   const char* const px = sm + kX + group * 2 * kBlk;
   bf16x8 fd[2][FN], fx[2][FM];
-  f32x4 acc[FM][FN], sums = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[FM][FN];
+  float sums[FN] = {0.f, 0.f, 0.f, 0.f};   // of this lane's tokens of column i of each fragment
 #pragma unroll
   for (int m = 0; m < FM; ++m)
 #pragma unroll
@@ -934,15 +936,13 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
         for (int f = 0; f < FN; ++f)
           acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[h][m], fd[h][f], acc[m][f], 0, 0, 0);
     if (group == 0 && a.db && s % a.tiles_k == tk) {
-      // row f of the left operand is ones for fragment f: row f of `sums` collects its columns
 #pragma unroll
-      for (int f = 0; f < FN; ++f) {
-        const unsigned o = afresh(i) == (unsigned)f ? 0x3f803f80u : 0u;
-        const u32x4 ones = u32x4{o, o, o, o};
+      for (int f = 0; f < FN; ++f)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&ones, fd[h][f], sums, 0, 0, 0);
-      }
+        for (int h = 0; h < 2; ++h) {
+          const bf16x8 d = fd[h][f];
+          sums[f] += (((float)d[0] + (float)d[1]) + ((float)d[2] + (float)d[3])) + (((float)d[4] + (float)d[5]) + ((float)d[6] + (float)d[7]));
+        }
     }
     __builtin_amdgcn_s_setprio(0);
   };
@@ -995,6 +995,11 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
 #undef FVSR_WAIT
 #undef FVSR_READ_DONE
 
+#pragma unroll
+  for (int f = 0; f < FN; ++f) {   // over the lanes (g, i) of a column
+    sums[f] += __shfl_xor(sums[f], 16);
+    sums[f] += __shfl_xor(sums[f], 32);
+  }
   O* dw = (O*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
 #pragma unroll
   for (int f = 0; f < FN; ++f) {

@@ -366,6 +366,24 @@ def test_linear8_weight_grad(dev, rows, k, n):
         assert got is o and none is None and torch.equal(o, dw)
 
 
+@pytest.mark.parametrize("rows,k,n", [(200, 300, 264), (50, 100, 130), (700, 300, 520)])
+def test_linear8_weight_grad_of_infinities(dev, rows, k, n):
+    """An infinity or NaN in dY takes its row of dW and its value of db; no other value."""
+    g, x, _, _ = linear_case(rows, k, n, dev)
+    dy = torch.randn((rows, n), generator=g).to(bf).to(dev)
+    x8 = f.quantize8(x)
+    for layout in (lambda t: t, unaligned):
+        dw, db = f.linear8_weight_grad(layout(dy), x8)
+        bad = dy.clone()
+        bad[7, 16], bad[rows - 1, 40], bad[3, n - 1] = math.inf, math.nan, -math.inf
+        gw, gb = f.linear8_weight_grad(layout(bad), x8)
+        hit = torch.zeros(n, dtype=torch.bool, device=dev)
+        hit[[16, 40, n - 1]] = True
+        assert gb[16] == math.inf and gb[40].isnan() and gb[n - 1] == -math.inf
+        assert torch.equal(gb[~hit], db[~hit]) and torch.equal(gw[~hit], dw[~hit])
+        assert not gw[hit].isfinite().any()
+
+
 def test_linear8_input_gradient(dev):
     """dx = linear8(dy, quantize8(W^T)) against the 8-bit values' product."""
     g, x, w, _ = linear_case(333, 520, 270, dev)
