@@ -13,7 +13,8 @@ A training pass of a linear layer keeps nothing but what its forward pass read:
 
 Tokens are (L, C) or (1, L, C), contiguous, on a HIP device; L may be 0. The calls keep no state: temporaries come from torch's
 allocator on the stream that the call runs on (the current one, or `stream`), so calls may overlap on several streams and be
-captured into graphs.
+captured into graphs. They are plain functions: gradients are asked for by name, and no result is part of an autograd graph. An `out`
+must not overlap what the call reads (but layer_norm_backward's may be dy). Norms take up to 16384 channels, the others 2^20.
 """
 from __future__ import annotations
 
@@ -42,8 +43,8 @@ def _widths(features: int):
 
 class Blocks8:
     """A (rows, features) matrix in 8 bits. `codes`: (rows, 128 * runs) float8_e4m3fn; `scales`: (rows, runs rounded up to a
-    multiple of 4) float8_e8m0fnu; both contiguous. A channel's value is code * scale of its run of 128 (dequantize8); what lies
-    past the last channel is 0. Rows can be taken out of one: Blocks8(q.codes[a:b], q.scales[a:b], q.features)."""
+    multiple of 4) float8_e8m0fnu; both contiguous. A channel's value is code * scale of its run of 128 (dequantize8), NaN where the
+    scale is; the codes past the last channel are 0, and have to be (products read whole runs). Rows can be taken out of one: Blocks8(q.codes[a:b], q.scales[a:b], q.features)."""
     __slots__ = ("codes", "scales", "features")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int):
