@@ -303,8 +303,8 @@ size_t fvsr_linear8_workspace(int64_t rows, int in_features, int out_features);
 int fvsr_linear8(fvsr_ctx* ctx, int x_dtype, const void* x, int64_t rows, int in_features, void* x_codes, void* x_scales,
                  const void* w_codes, const void* w_scales, int out_features, int bias_dtype, const void* bias, int gelu,
                  int y_dtype, void* y, void* workspace, size_t workspace_bytes, void* stream);
-/* Its weight gradient: dw (out_features, in_features) = dy^T x from bf16 dy (rows, out_features) and the 8-bit x, products and sums
- * in fp32, `dw_dtype`; db = the sum of dy's rows, fp32 (out_features), or NULL. The same inputs give the same bits. */
+/* Its weight gradient: dw (out_features, in_features) = dy^T x from bf16 dy (rows, out_features; 16-byte aligned where out_features is
+ * a multiple of 8) and the 8-bit x, products and sums in fp32, `dw_dtype`; db = the sum of dy's rows, fp32 (out_features), or NULL. The same inputs give the same bits. */
 size_t fvsr_linear8_weight_grad_workspace(int64_t rows, int in_features, int out_features);
 int fvsr_linear8_weight_grad(fvsr_ctx* ctx, const void* dy, int64_t rows, int out_features, const void* x_codes,
                              const void* x_scales, int in_features, int dw_dtype, void* dw, float* db, void* workspace,

@@ -200,6 +200,8 @@ int fvsr_linear8_weight_grad(fvsr_ctx* ctx, const void* dy, int64_t rows, int ou
   FVSR_REQUIRE(dw != nullptr, FVSR_ERR_INVALID_ARG, "dw is NULL");
   if (rows > 0) {
     FVSR_REQUIRE(dy != nullptr, FVSR_ERR_INVALID_ARG, "dy is NULL");
+    FVSR_REQUIRE(out_features % 8 != 0 || aligned(dy, 16), FVSR_ERR_INVALID_ARG,
+                 "dy must be 16-byte aligned where out_features is a multiple of 8");
     if ((rc = check_8(x_codes, x_scales, "x"))) return rc;
   }
   const size_t need = fvsr_linear8_weight_grad_workspace(rows, in_features, out_features);

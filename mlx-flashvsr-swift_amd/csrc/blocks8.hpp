@@ -17,6 +17,12 @@ namespace fvsr {
 constexpr int kRun = 128;
 constexpr int kMaxFeatures = 1 << 20;   // channels of a row: a tile's 256 rows of codes stay below 2^31 bytes
 
+// vectors of whole elements at any address: the hardware reads and writes global memory unaligned, in one instruction
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 any16 __attribute__((aligned(2)));
+typedef u32x2 any8 __attribute__((aligned(2)));
+typedef f32x4 any_f32x4 __attribute__((aligned(4)));
+
 struct In8 {
   const uint8_t* codes;
   const uint8_t* scales;

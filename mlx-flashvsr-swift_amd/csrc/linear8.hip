@@ -42,7 +42,7 @@ struct Linear8Args {
   int64_t rows;
   int N, runs, ss;       // output features; runs and scale bytes a row of both operands
   const void* bias;      // may be null
-  int bias_f32, gelu, vec_out;
+  int bias_f32, gelu;
   void* y;
   int tiles_m, tiles_n;
   int part_runs;         // runs of a part, whole words of scales (linear8_kernel; part p writes its own rows x N sums at y)
@@ -71,7 +71,7 @@ __device__ __forceinline__ void gelu_tanh8(float (&y)[8]) {
 }
 
 // bias (fp32, in LDS, at this lane's first feature), GELU and the store of a wave's fragments: this lane's features n0 + 32 p .. + 7
-// (two fragments) of the tokens row0 + 16 m. WHOLE: every feature and token is inside, and rows can be written 16 bytes at a time.
+// (two fragments) of the tokens row0 + 16 m. WHOLE: every feature and token is inside.
 template <bool GELU, bool WHOLE, int FN, int FM, typename O>
 __device__ __forceinline__ void write_fragments(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
                                                 int64_t row0) {
@@ -97,9 +97,9 @@ __device__ __forceinline__ void write_fragments(const Linear8Args& a, const f32x
       for (int e = 0; e < 8; ++e) v[e] = (O)s[e];
       O* const out = out0 + 32 * p;
       const int n = n0 + 32 * p;
-      if (WHOLE || (a.vec_out && n + 8 <= a.N)) {
-        *(u32x4*)out = *(u32x4*)v;
-        if constexpr (sizeof(O) == 4) ((u32x4*)out)[1] = ((u32x4*)v)[1];
+      if (WHOLE || n + 8 <= a.N) {
+        *(any16*)out = *(u32x4*)v;
+        if constexpr (sizeof(O) == 4) ((any16*)out)[1] = ((u32x4*)v)[1];
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
 
   const int fn = wn * (TN / WN) + 8 * g;
   write_tile<GELU>(a, acc, (O*)a.y + blockIdx.y * a.rows * a.N, bias + fn, n0 + fn, m0 + rx0,
-                   a.vec_out && rows_m == TM && rows_n == TN);
+                   rows_m == TM && rows_n == TN);
 }
 
 // The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between them. Two groups
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
     if (!held) return false;
     const float* b = (const float*)(sm + kB + ((bt - 1) & 3) * 1024);
     return write_tile<GELU>(a, acc, (O*)a.y, b + w * 64 + 8 * g, n0 + w * 64 + 8 * g, m0 + rx0,
-                            a.vec_out && m0 + 256 <= a.rows && n0 + 256 <= a.N);
+                            m0 + 256 <= a.rows && n0 + 256 <= a.N);
   };
 
   source();
@@ -583,7 +583,6 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
   Linear8Args a{};
   a.x = x; a.w = w; a.rows = rows; a.N = N; a.runs = runs_of(K); a.ss = scale_stride(K);
   a.bias = bias; a.bias_f32 = bias_dtype == FVSR_DTYPE_F32; a.gelu = gelu; a.y = y;
-  a.vec_out = rows_vectorize(y, N);
   a.part_runs = p.part_runs;
   if (!p.few && p.tiles >= 1 << 24) return set_error(FVSR_ERR_UNSUPPORTED, "linear8: too many output tiles for one launch");
   const bool bf = out_dtype == FVSR_DTYPE_BF16;
@@ -618,7 +617,6 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
     part.bias = nullptr;
     part.gelu = 0;
     part.y = ws;
-    part.vec_out = N % 8 == 0;
     hipLaunchKernelGGL((linear8_kernel<128, 128, 4, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(512), 0, stream, part);
     FVSR_HIP_CHECK(hipGetLastError());
     const int64_t n = rows * N;
@@ -657,131 +655,35 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
 // ------------------------------------------------------------------------------------------------------------
 struct WeightGradArgs {
   const bf16* dy;
+  int ld;                    // elements from one of its rows to the next
   In8 x;
   int64_t rows, part_rows;   // part_rows: tokens of a part (the work is split over parts where there are few tiles), whole steps
   int N, K, runs, ss;
-  int vec_dy;
   void* dw;                  // (parts, N, K), fp32 where there are more than one
   float* db;                 // (parts * tiles_k, N) or null
   int tiles_n, tiles_k;
 };
 
-// dW (N, K) = dY^T X: a tile of TN x TK, steps of 32 tokens. Both operands lie token-major, so the product's depth runs across rows:
-// the tiles are stored in LDS as they come, [token][column] in bf16 (codes times scales are exact in bf16), and
-// ds_read_b64_tr_b16 hands a lane 4 tokens of one column: 16 lanes read 4 rows of 16 columns, lane i gets column i of the four.
-template <int TN, int TK, int WN, int WK, typename O>
-__global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGradArgs a) {
-  constexpr int kThreads = 64 * WN * WK, kTokens = 32, FN = TN / WN / 16, FK = TK / WK / 16;
-  constexpr int kDy = kTokens * TN / 8 / kThreads, kX = kTokens * TK / 8 / kThreads;   // 8-element vectors a thread
-  static_assert(kDy > 0 && kX > 0, "tile");
-  __shared__ __align__(1024) char sm[2][kTokens * (TN + TK) * 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
-  const int tk = t % a.tiles_k, tn = t / a.tiles_k;
-  const int n0 = tn * TN, k0 = tk * TK;
-  const int64_t from = (int64_t)blockIdx.y * a.part_rows, to = min(a.rows, from + a.part_rows);
-
-  u32x4 rdy[kDy];
-  uint2 rx[kX];
-  uint32_t rs[kX];
-  auto load = [&](int64_t m0) {
+// the first `n` of 4 results, at any address
+template <typename O>
+__device__ __forceinline__ void store4(O* out, f32x4 x, int n) {
+  O v[4];
 #pragma unroll
-    for (int j = 0; j < kDy; ++j) {
-      const int v = j * kThreads + threadIdx.x, r = v / (TN / 8), c = n0 + v % (TN / 8) * 8;
-      const int64_t row = m0 + r;
-      rdy[j] = u32x4{0, 0, 0, 0};
-      if (row < to) {
-        const bf16* p = a.dy + row * a.N + c;
-        if (a.vec_dy) {
-          if (c < a.N) rdy[j] = *(const u32x4*)p;
-        } else {
-          bf16* d = (bf16*)&rdy[j];
+  for (int e = 0; e < 4; ++e) v[e] = (O)x[e];
+  if (n >= 4) {
+    if constexpr (sizeof(O) == 4) *(any16*)out = *(u32x4*)v;
+    else *(any8*)out = *(u32x2*)v;
+  } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c + e < a.N) d[e] = p[e];
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kX; ++j) {
-      const int v = j * kThreads + threadIdx.x, r = v / (TK / 8), c = k0 + v % (TK / 8) * 8;
-      const int64_t row = m0 + r;
-      rx[j] = make_uint2(0, 0);
-      rs[j] = 0;
-      if (row < to && c < a.runs * kRun) {
-        rx[j] = *(const uint2*)(a.x.codes + row * (int64_t)a.runs * kRun + c);
-        rs[j] = a.x.scales[row * a.ss + c / kRun];
-      }
-    }
-  };
-  auto put = [&](char* s) {
-#pragma unroll
-    for (int j = 0; j < kDy; ++j) {
-      const int v = j * kThreads + threadIdx.x, r = v / (TN / 8), c = v % (TN / 8) * 8;
-      *(u32x4*)(s + (r * TN + c) * 2) = rdy[j];
-    }
-#pragma unroll
-    for (int j = 0; j < kX; ++j) {
-      const int v = j * kThreads + threadIdx.x, r = v / (TK / 8), c = v % (TK / 8) * 8;
-      const float by = __uint_as_float(rs[j] << 23);
-      bf16x2 q[4];
-      q[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rx[j].x, by, false);
-      q[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rx[j].x, by, true);
-      q[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rx[j].y, by, false);
-      q[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rx[j].y, by, true);
-      *(u32x4*)(s + kTokens * TN * 2 + (r * TK + c) * 2) = *(u32x4*)q;
-    }
-  };
-
-  const int wn = wave % WN, wk = wave / WN, i = lane & 15, g = lane >> 4;
-  f32x4 acc[FK][FN];
-#pragma unroll
-  for (int f = 0; f < FK; ++f)
-#pragma unroll
-    for (int n = 0; n < FN; ++n) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load(from);
-  int turn = 0;
-  for (int64_t m0 = from; m0 < to; m0 += kTokens, turn ^= 1) {
-    put(sm[turn]);
-    __syncthreads();
-    if (m0 + kTokens < to) load(m0 + kTokens);
-    // lane (g, i): tokens 8 g .. 8 g + 7 of column i of a fragment
-    auto read = [&](const char* s, int width, int col) {
-      const char* p = s + ((8 * g + (i >> 2)) * width + col + (i & 3) * 4) * 2;
-      union { i16x4 h[2]; bf16x8 v; } u;
-      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
-      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 4 * width * 2));
-      return u.v;
-    };
-    bf16x8 fn[FN];
-#pragma unroll
-    for (int n = 0; n < FN; ++n) fn[n] = read(sm[turn], TN, wn * (TN / WN) + 16 * n);
-#pragma unroll
-    for (int f = 0; f < FK; ++f) {
-      const bf16x8 fk = read(sm[turn] + kTokens * TN * 2, TK, wk * (TK / WK) + 16 * f);
-#pragma unroll
-      for (int n = 0; n < FN; ++n) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fn[n], acc[f][n], 0, 0, 0);
-    }
-  }
-  O* dw = (O*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
-#pragma unroll
-  for (int n = 0; n < FN; ++n) {
-    const int row = n0 + wn * (TN / WN) + 16 * n + i;
-    if (row >= a.N) continue;
-#pragma unroll
-    for (int f = 0; f < FK; ++f) {
-      const int c = k0 + wk * (TK / WK) + 16 * f + 4 * g;
-      O* out = dw + (int64_t)row * a.K + c;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < a.K) out[e] = (O)acc[f][n][e];
-    }
+    for (int e = 0; e < 3; ++e)
+      if (e < n) out[e] = v[e];
   }
 }
 
-
-// The large weight gradient: 256 features x 256 channels a workgroup, steps of 64 tokens, two groups of four waves that take turns as in
-// linear8_large_kernel; wave w of group h computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
+// dW (N, K) = dY^T X, 256 features x 256 channels a workgroup, steps of 64 tokens. Both operands lie token-major, so the product's depth
+// runs across rows: they are kept in LDS as they come, [token][column], in bf16 (codes times scales are exact in it), and
+// ds_read_b64_tr_b16 hands a lane 4 tokens of one column: 16 lanes read 4 rows of 16 columns, lane i gets column i of the four.
+// Two groups of four waves take turns as in linear8_large_kernel; wave w of group h computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
 //
 //   phase      2s                                                          2s + 1
 //   group 0    widen X1(s), read(s), ask for dY(s + 1) and codes of s + 2  multiply(s)
@@ -797,7 +699,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void weight_grad_kernel(WeightGrad
 // db: a step's column sums are taken by one of the tiles_k workgroups that read the step, from the fragments in registers, under the
 // products (a column a lane; as products with rows of ones and zeros an infinity would reach other columns).
 template <typename O>
-__global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArgs a) {
+__global__ __launch_bounds__(512, 2) void weight_grad_kernel(WeightGradArgs a) {
   constexpr int FN = 4, FM = 8, kTokens = 64;
   constexpr int kBlk = kTokens * 128;                       // 64 columns (bf16) of a step
   constexpr int kX = 8 * kBlk;                              // LDS: dY 2 x 4 blocks, X 2 halves x 2 blocks,
@@ -810,7 +712,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
   const int tk = t % a.tiles_k, tn = t / a.tiles_k, n0 = tn * 256 + w * 64, k0 = tk * 256;
   const int64_t from = (int64_t)blockIdx.y * a.part_rows, to = min(a.rows, from + a.part_rows);
   const int steps = (int)((to - from + kTokens - 1) / kTokens);
-  const int ldn = a.N * 2, ldk = a.runs * kRun;
+  const int ldn = a.ld * 2, ldk = a.runs * kRun;
   const int other = 1 - group;
 
   // copies: 8 tokens an instruction
@@ -830,7 +732,7 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
     d[1] = (uint32_t)(b >> 32);
   };
   int dy_left = count, codes_left = count;
-  u32x4 dd = make_rsrc(a.dy + from * a.N + n0, records(count, ldn, n0 * 2));
+  u32x4 dd = make_rsrc(a.dy + from * a.ld + n0, records(count, ldn, n0 * 2));
   u32x4 dc = make_rsrc(a.x.codes + from * ldk + run * kRun, records(count, ldk, run * kRun));
   u32x4 ds = make_rsrc(a.x.scales + from * a.ss + (run & ~3), records(count, a.ss, run & ~3));
   uint32_t dy_at = lds0 + w * kBlk, dy_flip = 4 * kBlk;
@@ -1008,123 +910,123 @@ __global__ __launch_bounds__(512, 2) void weight_grad_large_kernel(WeightGradArg
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
       const int c = k0 + group * 128 + 16 * m + 4 * g;
-      O* out = dw + (int64_t)n * a.K + c;
-      if (c + 4 <= a.K && (a.K & 3) == 0 && ((uintptr_t)dw & 15) == 0) {
-        O v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (O)acc[m][f][e];
-        if constexpr (sizeof(O) == 4) *(u32x4*)out = *(u32x4*)v;
-        else *(uint2*)out = *(uint2*)v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < a.K) out[e] = (O)acc[m][f][e];
-      }
+      store4(dw + (int64_t)n * a.K + c, acc[m][f], a.K - c);
     }
     if (group == 0 && a.db && g == 0) a.db[((int64_t)blockIdx.y * a.tiles_k + tk) * a.N + n] = sums[f];
   }
 }
 
-// dw = the sum over parts of their (N, K) partial results, in order
-template <typename O>
-__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  if (n % 4 == 0) {
-    f32x4 s = *(const f32x4*)(part + i);
-    for (int p = 1; p < parts; ++p) s += *(const f32x4*)(part + p * n + i);
-    if (((uintptr_t)dw & 15) == 0) {
-      O v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (O)s[e];
-      if constexpr (sizeof(O) == 4) *(u32x4*)(dw + i) = *(u32x4*)v;
-      else *(uint2*)(dw + i) = *(uint2*)v;
+// rows of N elements, N not a multiple of 8, to rows of N rounded up to one (the rest zeros)
+__global__ __launch_bounds__(256) void pad_rows_kernel(const bf16* __restrict__ in, int64_t rows, int N, bf16* __restrict__ out) {
+  const int vectors = (N + 7) / 8;
+  const int64_t n = rows * vectors;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / vectors;
+    const int c = (int)(i - row * vectors) * 8;
+    const bf16* p = in + row * N + c;
+    u32x4 v = u32x4{0, 0, 0, 0};
+    if (c + 8 <= N) {
+      v = *(const any16*)p;
     } else {
+      bf16* d = (bf16*)&v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dw[i + e] = (O)s[e];
+      for (int e = 0; e < 8; ++e)
+        if (c + e < N) d[e] = p[e];
     }
-  } else {
-    for (int e = 0; e < 4 && i + e < n; ++e) {
-      float s = part[i + e];
-      for (int p = 1; p < parts; ++p) s += part[p * n + i + e];
-      dw[i + e] = (O)s;
-    }
+    ((u32x4*)out)[i] = v;
   }
 }
 
-// partial column sums of dy: workgroup (x, y) adds rows y, y + gridDim.y, .. of 4 waves' worth of 64 columns each
-__global__ __launch_bounds__(256) void column_sum_kernel(const bf16* __restrict__ dy, int64_t rows, int N, float* __restrict__ part) {
-  __shared__ float sm[256];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-  float s = 0.f;
-  if (c < N)
-    for (int64_t r = (int64_t)blockIdx.y * 4 + q; r < rows; r += (int64_t)gridDim.y * 4) s += (float)dy[r * N + c];
-  sm[threadIdx.x] = s;
-  __syncthreads();
-  if (q == 0 && c < N)
-    part[(int64_t)blockIdx.y * N + c] = (sm[threadIdx.x] + sm[64 + threadIdx.x]) + (sm[128 + threadIdx.x] + sm[192 + threadIdx.x]);
+// dw = the sum over parts of their (N, K) partial results, in order (zeros if there are none)
+template <typename O>
+__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int have = (int)min((int64_t)4, n - i);
+    for (int p = 0; p < parts; ++p) {
+      const float* from = part + p * n + i;
+      if (have == 4) s += *(const any_f32x4*)from;
+      else
+        for (int e = 0; e < have; ++e) s[e] += from[e];
+    }
+    store4(dw + i, s, have);
+  }
 }
 
 int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);   // rows8.hip
 
-// How a weight gradient is cut up: tiles of 256 x 256 with DMA copies where dY's rows can be read 16 bytes at a time, else of 128 x
-// 128; the tokens into as many parts as fill the card, of at least 4 steps.
+// How a weight gradient is cut up: the tokens of a tile into as many parts as fill the card, of at least kMinSteps steps. Rows of dY
+// that are not whole 16 bytes, which the copies into LDS need, are copied to such first (4000 x 1536 x 4500: 95 us; tiles of 128 that
+// read them as they are, without such copies, 310).
 struct WeightGradPlan {
-  bool large;
+  bool pad;
   int tiles_n, tiles_k, parts;
   int64_t part_rows;
   int sum_parts;   // partial column sums
 };
-constexpr int kSumParts = 64;
-static WeightGradPlan weight_grad_plan(int64_t rows, int N, int K, bool vec_dy) {
+constexpr int kMinSteps = 4;
+static WeightGradPlan weight_grad_plan(int64_t rows, int N, int K) {
   WeightGradPlan p;
-  p.large = rows > 0 && vec_dy && N > 128 && K > 128;   // (its phases need a step)
-  const int T = p.large ? 256 : 128, step = p.large ? 64 : 32, slots = p.large ? 256 : 512;
-  p.tiles_n = (int)ceil_div(N, T);
-  p.tiles_k = (int)ceil_div(K, T);
-  const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, steps = ceil_div(rows, step);
-  const int64_t parts = std::max<int64_t>(1, std::min(slots / tiles, steps / 4));
-  p.part_rows = ceil_div(std::max<int64_t>(steps, 1), parts) * step;
-  p.parts = (int)std::max<int64_t>(1, ceil_div(rows, p.part_rows));
-  p.sum_parts = p.large ? p.parts * p.tiles_k : (int)std::max<int64_t>(1, std::min<int64_t>(kSumParts, ceil_div(rows, 16)));
+  p.pad = N % 8 != 0;
+  p.tiles_n = (int)ceil_div(N, 256);
+  p.tiles_k = (int)ceil_div(K, 256);
+  const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, steps = ceil_div(rows, 64);
+  const int64_t parts = std::max<int64_t>(1, std::min(256 / tiles, steps / kMinSteps));
+  p.part_rows = ceil_div(steps, parts) * 64;
+  p.parts = rows > 0 ? (int)ceil_div(rows, p.part_rows) : 0;
+  p.sum_parts = p.parts * p.tiles_k;
   return p;
 }
-static size_t plan_bytes(const WeightGradPlan& p, int N, int K) {
-  return ((size_t)p.sum_parts * N + (p.parts > 1 ? (size_t)p.parts * N * K : 0)) * sizeof(float) + 16;
+// the workspace: partial column sums, partial products, the copy of dY, each 16-byte aligned
+struct WeightGradSpace {
+  size_t part, dy, bytes;
+};
+static WeightGradSpace weight_grad_space(const WeightGradPlan& p, int64_t rows, int N, int K) {
+  auto up = [](size_t n) { return (n + 15) & ~size_t(15); };
+  WeightGradSpace s;
+  s.part = up((size_t)p.sum_parts * N * sizeof(float));
+  s.dy = s.part + (p.parts > 1 ? up((size_t)p.parts * N * K * sizeof(float)) : 0);
+  s.bytes = s.dy + (p.pad ? (size_t)rows * ceil_div(N, 8) * 16 : 0);
+  return s;
 }
 size_t weight_grad_workspace(int64_t rows, int N, int K) {
-  return std::max(plan_bytes(weight_grad_plan(rows, N, K, false), N, K), plan_bytes(weight_grad_plan(rows, N, K, N % 8 == 0), N, K));
+  return weight_grad_space(weight_grad_plan(rows, N, K), rows, N, K).bytes;
 }
 
 int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int out_dtype, void* dw, float* db, void* ws,
                        hipStream_t stream) {
   if (rows >= (int64_t)1 << 31) return set_error(FVSR_ERR_UNSUPPORTED, "linear8_weight_grad: too many rows");
-  const WeightGradPlan p = weight_grad_plan(rows, N, K, rows_vectorize(dy, N));
+  const WeightGradPlan p = weight_grad_plan(rows, N, K);
+  const WeightGradSpace space = weight_grad_space(p, rows, N, K);
   const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k;
   if (tiles >= 1 << 22) return set_error(FVSR_ERR_UNSUPPORTED, "linear8_weight_grad: too many output tiles for one launch");
   float* const sums = (float*)ws;
-  float* const part = (float*)((char*)ws + (((size_t)p.sum_parts * N * sizeof(float) + 15) & ~size_t(15)));
+  float* const part = (float*)((char*)ws + space.part);
   WeightGradArgs a{};
-  a.dy = (const bf16*)dy; a.x = x; a.rows = rows; a.part_rows = p.part_rows;
+  a.dy = (const bf16*)dy; a.ld = N; a.x = x; a.rows = rows; a.part_rows = p.part_rows;
   a.N = N; a.K = K; a.runs = runs_of(K); a.ss = scale_stride(K);
-  a.vec_dy = rows_vectorize(dy, N);
   a.dw = p.parts > 1 ? part : dw;
-  a.db = db && p.large ? sums : nullptr;
+  a.db = db ? sums : nullptr;
   a.tiles_n = p.tiles_n;
   a.tiles_k = p.tiles_k;
   const bool wide = p.parts > 1 || out_dtype == FVSR_DTYPE_F32;
   const dim3 grid((unsigned)tiles, (unsigned)p.parts);
-  if (p.large) {
-    if (wide) hipLaunchKernelGGL((weight_grad_large_kernel<float>), grid, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((weight_grad_large_kernel<bf16>), grid, dim3(512), 0, stream, a);
-  } else {
-    if (wide) hipLaunchKernelGGL((weight_grad_kernel<128, 128, 2, 2, float>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((weight_grad_kernel<128, 128, 2, 2, bf16>), grid, dim3(256), 0, stream, a);
+  if (p.parts > 0 && p.pad) {
+    a.ld = (int)ceil_div(N, 8) * 8;
+    a.dy = (const bf16*)((char*)ws + space.dy);
+    const int64_t blocks = ceil_div(rows * (a.ld / 8), 256);
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream, (const bf16*)dy, rows, N,
+                       (bf16*)((char*)ws + space.dy));
+    FVSR_HIP_CHECK(hipGetLastError());
   }
-  FVSR_HIP_CHECK(hipGetLastError());
-  if (p.parts > 1) {
+  if (p.parts > 0) {
+    if (wide) hipLaunchKernelGGL((weight_grad_kernel<float>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((weight_grad_kernel<bf16>), grid, dim3(512), 0, stream, a);
+    FVSR_HIP_CHECK(hipGetLastError());
+  }
+  if (p.parts != 1) {   // also no token: zeros
     const int64_t n = (int64_t)N * K;
-    const dim3 blocks((unsigned)ceil_div(n, 1024));
+    const dim3 blocks((unsigned)std::min<int64_t>(ceil_div(n, 1024), 1 << 20));
     if (out_dtype == FVSR_DTYPE_F32)
       hipLaunchKernelGGL((weight_grad_join_kernel<float>), blocks, dim3(256), 0, stream, part, p.parts, n, (float*)dw);
     else
@@ -1132,10 +1034,6 @@ int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int ou
     FVSR_HIP_CHECK(hipGetLastError());
   }
   if (!db) return FVSR_OK;
-  if (!p.large) {
-    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(N, 64), (unsigned)p.sum_parts), dim3(256), 0, stream, a.dy, rows, N, sums);
-    FVSR_HIP_CHECK(hipGetLastError());
-  }
   return launch_param_sum(sums, p.sum_parts, N, N, db, nullptr, stream);
 }
 

@@ -368,7 +368,8 @@ def linear8_weight_grad(dy: torch.Tensor, x8: Blocks8, dtype: torch.dtype = torc
     o = _out(out, "out", (n, k), dtype)
     dev = _one_device(d2, "dy", (x8, "x8"), (o, "out"))
     nbytes = lib.fvsr_linear8_weight_grad_workspace(rows, k, n)
-
+    if n % 8 == 0 and d2.data_ptr() & 15:   # a view that starts inside 16 bytes
+        d2 = d2.clone()
     dw = torch.empty(n, k, dtype=dtype, device=dev) if o is None else o
     db = torch.empty(n, dtype=torch.float32, device=dev) if want_bias else None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
