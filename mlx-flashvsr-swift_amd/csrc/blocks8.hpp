@@ -35,10 +35,6 @@ struct Out8 {
 __host__ __device__ __forceinline__ int runs_of(int channels) { return (channels + kRun - 1) / kRun; }
 __host__ __device__ __forceinline__ int scale_stride(int channels) { return (runs_of(channels) + 3) & ~3; }
 
-// An element type code of the C ABI as a byte count, and whether a buffer can be read and written 16 bytes at a time in rows
-// of C elements (8 elements a lane: one access for bf16, two for fp32).
-__host__ __forceinline__ bool rows_vectorize(const void* p, int C) { return C % 8 == 0 && ((uintptr_t)p & 15) == 0; }
-
 // max over each 16 lanes of a wave (every lane active, x >= 0), in every one of them: DPP rotations within the rows of 16
 __device__ __forceinline__ float max16(float x) {
   auto rot = [](float v, auto ctrl) {
@@ -89,88 +85,55 @@ __device__ __forceinline__ void decode8(uint2 c, uint32_t scale, float (&v)[8]) 
   v[6] = p[0]; v[7] = p[1];
 }
 
-// The 8 channels of a run that a lane (l16 = lane % 16) holds, element e: 8 adjacent ones where rows can be read 16 bytes at a time
-// (VEC), else every 16th, so that the lanes of an access read adjacent elements.
-template <bool VEC>
-__device__ __forceinline__ int run_channel(int l16, int e) {
-  return VEC ? l16 * 8 + e : l16 + 16 * e;
-}
-
-// 8 elements as they lie in memory, zeros past the row's end: loaded now, widened when they are needed
+// A lane (l16 = lane % 16) holds 8 adjacent channels of a run, 8 l16 .. 8 l16 + 7. As they lie in memory, zeros past the row's end: loaded
+// now, widened when they are needed. Rows of any length and alignment are read and written by whole vectors, but for a last part of 8;
+// EIGHTS: rows have none (C is a multiple of 8), and no registers are spent on it.
 template <typename T>
 struct Raw8 {
   T v[8];
 };
-template <typename T, bool VEC>
+template <typename T, bool EIGHTS>
 __device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c0, int l16, int C) {
   Raw8<T> r;
-  if constexpr (VEC) {
-    const int c = c0 + l16 * 8;
-    u32x4* const to = (u32x4*)r.v;
-    if (c < C) {
-      to[0] = *(const u32x4*)(row + c);
-      if constexpr (sizeof(T) == 4) to[1] = *(const u32x4*)(row + c + 4);
-    } else {
-      to[0] = u32x4{0, 0, 0, 0};
-      if constexpr (sizeof(T) == 4) to[1] = u32x4{0, 0, 0, 0};
-    }
-  } else {
+  const int c = c0 + l16 * 8;
+  u32x4* const to = (u32x4*)r.v;
+  to[0] = u32x4{0, 0, 0, 0};
+  if constexpr (sizeof(T) == 4) to[1] = u32x4{0, 0, 0, 0};
+  if (c + 8 <= C) {
+    to[0] = *(const any16*)(row + c);
+    if constexpr (sizeof(T) == 4) to[1] = *(const any16*)(row + c + 4);
+  } else if (!EIGHTS && c < C) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = c0 + l16 + 16 * e;
-      r.v[e] = c < C ? row[c] : (T)0.f;
-    }
+    for (int e = 0; e < 7; ++e)
+      if (c + e < C) r.v[e] = row[c + e];
   }
   return r;
 }
-template <typename T, bool VEC>
+template <typename T, bool EIGHTS>
 __device__ __forceinline__ void load8(const T* row, int c0, int l16, int C, float (&v)[8]) {
-  const Raw8<T> r = load_raw8<T, VEC>(row, c0, l16, C);
+  const Raw8<T> r = load_raw8<T, EIGHTS>(row, c0, l16, C);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (float)r.v[e];
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int c0, int l16, int C, const float (&v)[8]) {
-  if constexpr (VEC) {
-    const int c = c0 + l16 * 8;
-    if (c >= C) return;
-    T t[8];
+// the other way: channels c .. c + 7, but for the first `skip` and those past the row's end
+template <typename T, bool EIGHTS>
+__device__ __forceinline__ void store8(T* row, int c, int skip, int C, const float (&v)[8]) {
+  T t[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
-    if constexpr (sizeof(T) == 2) {
-      *(u32x4*)(row + c) = *(u32x4*)t;
-    } else {
-      ((u32x4*)(row + c))[0] = ((u32x4*)t)[0];
-      ((u32x4*)(row + c))[1] = ((u32x4*)t)[1];
-    }
-  } else {
+  for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+  if (c + 8 <= C && (EIGHTS || skip == 0)) {
+    *(any16*)(row + c) = *(u32x4*)t;
+    if constexpr (sizeof(T) == 4) *(any16*)(row + c + 4) = ((u32x4*)t)[1];
+  } else if (!EIGHTS) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = c0 + l16 + 16 * e;
-      if (c < C) row[c] = (T)v[e];
-    }
+    for (int e = 0; e < 8; ++e)
+      if (e >= skip && c + e < C) row[c + e] = t[e];
   }
 }
 
 // the 8 codes of a lane of a run that starts at `run` (whole runs are stored: what lies past the last channel is 0)
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* run, int l16, uint2 c) {
-  if constexpr (VEC) {
-    *(uint2*)(run + l16 * 8) = c;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) run[l16 + 16 * e] = (uint8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3)));
-  }
-}
-
-template <bool VEC>
-__device__ __forceinline__ uint2 load_codes(const uint8_t* run, int l16) {
-  if constexpr (VEC) return *(const uint2*)(run + l16 * 8);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)run[l16 + 16 * e] << (8 * (e & 3));
-  return make_uint2(w[0], w[1]);
-}
+__device__ __forceinline__ void store_codes(uint8_t* run, int l16, uint2 c) { *(uint2*)(run + l16 * 8) = c; }
+__device__ __forceinline__ uint2 load_codes(const uint8_t* run, int l16) { return *(const uint2*)(run + l16 * 8); }
 
 }  // namespace fvsr

@@ -64,7 +64,7 @@ __device__ __forceinline__ void team_sum2(float& a, float& b, float* sm) {
 
 // One row a team of WAVES waves (a workgroup holds max(WAVES, 4) waves), NV vectors of 8 channels a lane: lane L of the team and
 // vector j hold 8 channels of run 4 * WAVES * j + L / 16.
-template <typename T, typename P, bool VEC, int WAVES, int NV>
+template <typename T, typename P, bool EIGHTS, int WAVES, int NV>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kernel(NormArgs a) {
   __shared__ float sm[2][2 * WAVES];
   const int l16 = threadIdx.x & 15, C = a.C;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
   float sum = 0.f, none = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    load8<T, VEC>(x, (run0 + 4 * WAVES * j) * kRun, l16, C, v[j]);
+    load8<T, EIGHTS>(x, (run0 + 4 * WAVES * j) * kRun, l16, C, v[j]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum += v[j][e];
   }
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
       const int run = run0 + 4 * WAVES * j;
       uint32_t s;
       const uint2 c = encode8(v[j], s);
-      if (run < runs) store_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16, c);
+      if (run < runs) store_codes(a.x8.codes + (row * runs + run) * kRun, l16, c);
       if (run < ss && l16 == 0) a.x8.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
     }
   }
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
     const int c0 = (run0 + 4 * WAVES * j) * kRun;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[j][e] = c0 + run_channel<VEC>(l16, e) < C ? v[j][e] - mean : 0.f;
+      v[j][e] = c0 + l16 * 8 + e < C ? v[j][e] - mean : 0.f;
       sq = fmaf(v[j][e], v[j][e], sq);
     }
   }
@@ -113,20 +113,20 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
   for (int j = 0; j < NV; ++j) {
     const int run = run0 + 4 * WAVES * j;
     float w[8], b[8], y[8];
-    if (a.w) load8<P, VEC>((const P*)a.w, run * kRun, l16, C, w);
-    if (a.b) load8<P, VEC>((const P*)a.b, run * kRun, l16, C, b);
+    if (a.w) load8<P, EIGHTS>((const P*)a.w, run * kRun, l16, C, w);
+    if (a.b) load8<P, EIGHTS>((const P*)a.b, run * kRun, l16, C, b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       y[e] = v[j][e] * rstd;
       if (a.w) y[e] *= w[e];
       if (a.b) y[e] += b[e];
-      if (run * kRun + run_channel<VEC>(l16, e) >= C) y[e] = 0.f;   // also where the row's rstd is not finite
+      if (run * kRun + l16 * 8 + e >= C) y[e] = 0.f;   // also where the row's rstd is not finite
     }
-    if (a.y) store8<T, VEC>((T*)a.y + row * C, run * kRun, l16, C, y);
+    if (a.y) store8<T, EIGHTS>((T*)a.y + row * C, run * kRun + l16 * 8, 0, C, y);
     if (a.y8.codes) {
       uint32_t s;
       const uint2 c = encode8(y, s);
-      if (run < runs) store_codes<VEC>(a.y8.codes + (row * runs + run) * kRun, l16, c);
+      if (run < runs) store_codes(a.y8.codes + (row * runs + run) * kRun, l16, c);
       if (run < ss && l16 == 0) a.y8.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
     }
   }
@@ -134,9 +134,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
 
 // The gradient: teams walk over the rows (the grid is a fixed number of workgroups) and keep their part of dw and db in
 // registers; the workgroup's sum goes to `part`, and param_sum_kernel adds the workgroups' up: no atomics, the same result
-// every time.
-template <typename T, typename P, bool VEC, int WAVES, int NV, bool X8>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 2 : 1) void layer_norm_grad_kernel(NormGradArgs a) {
+// every time. Where C is not a multiple of 8 (not EIGHTS), the lane of the row's end takes its last 8 channels, and skips the first `dup`
+// of them, which its neighbour has too: one load, which nothing waits for before its row is worked on.
+template <typename T, typename P, bool EIGHTS, int WAVES, int NV, bool X8>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16 ? 2 : 1) void layer_norm_grad_kernel(NormGradArgs a) {
   __shared__ float sm[2][2 * WAVES];
   __shared__ float join[WAVES == 1 ? 4 * 64 * 16 : 1];
   const int l16 = threadIdx.x & 15, lane = threadIdx.x & 63, C = a.C;
@@ -144,9 +145,31 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
   const int run0 = (WAVES == 1 ? lane : (int)threadIdx.x) >> 4;
   const int runs = runs_of(C), ss = scale_stride(C);
   float w[NV][8], dw[NV][8], db[NV][8];
+  auto first = [&](int j) { return (run0 + 4 * WAVES * j) * kRun + l16 * 8; };   // the lane's channels of vector j
+  auto held = [&](int j) { return EIGHTS ? first(j) : min(first(j), max(0, C - 8)); };
+  auto dup = [&](int j) { return first(j) - held(j); };                          // 8 or more past the row's end
+  auto load_held = [&](auto* p, int j) {
+    using E = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+    Raw8<E> r;
+    u32x4* const to = (u32x4*)r.v;
+    to[0] = u32x4{0, 0, 0, 0};
+    if constexpr (sizeof(E) == 4) to[1] = u32x4{0, 0, 0, 0};
+    if (first(j) >= C) return r;
+    if (EIGHTS || C >= 8) {
+      to[0] = *(const any16*)(p + held(j));
+      if constexpr (sizeof(E) == 4) to[1] = *(const any16*)(p + held(j) + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < C) r.v[e] = p[e];
+    }
+    return r;
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (a.w) load8<P, VEC>((const P*)a.w, (run0 + 4 * WAVES * j) * kRun, l16, C, w[j]);
+    const Raw8<P> rw = a.w ? load_held((const P*)a.w, j) : Raw8<P>{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[j][e] = (float)rw.v[e];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (!a.w) w[j][e] = 1.f;
@@ -155,7 +178,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
   }
   // the next row is on its way while one is worked on
   Raw8<T> rdy[NV], rx[NV];
-  uint2 rc[NV];
+  u32x2 rc[NV];
   uint32_t rs[NV];
   float mean = 0.f, rstd = 0.f;
   auto load = [&](int64_t row) {
@@ -164,12 +187,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int run = run0 + 4 * WAVES * j;
-      rdy[j] = load_raw8<T, VEC>((const T*)a.dy + row * C, run * kRun, l16, C);
+      rdy[j] = load_held((const T*)a.dy + row * C, j);
       if constexpr (X8) {
-        rc[j] = run < runs ? load_codes<VEC>(a.x8.codes + (row * runs + run) * kRun, l16) : make_uint2(0, 0);
+        rc[j] = u32x2{0, 0};
+        if (run < runs && first(j) < C) rc[j] = *(const any8*)(a.x8.codes + row * runs * kRun + held(j));
         rs[j] = run < runs ? a.x8.scales[row * ss + run] : 0;
       } else {
-        rx[j] = load_raw8<T, VEC>((const T*)a.x + row * C, run * kRun, l16, C);
+        rx[j] = load_held((const T*)a.x + row * C, j);
       }
     }
   };
@@ -183,10 +207,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if constexpr (X8) decode8(rc[j], rs[j], n[j]);
+      if constexpr (X8) decode8(make_uint2(rc[j][0], rc[j][1]), rs[j], n[j]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        dy[j][e] = (float)rdy[j].v[e];
+        dy[j][e] = EIGHTS || e >= dup(j) ? (float)rdy[j].v[e] : 0.f;
         if constexpr (!X8) n[j][e] = (float)rx[j].v[e];
       }
     }
@@ -195,7 +219,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[j][e] = (n[j][e] - mu) * r;   // past C: dy is 0, so the value does not matter (it is finite where the row's are)
+        n[j][e] = (n[j][e] - mu) * r;
+        if (!EIGHTS && e < dup(j)) n[j][e] = 0.f;   // (codes of another run, maybe); past C: dy is 0, and this finite where the row is
         const float g = dy[j][e] * w[j][e];
         s1 += g;
         s2 = fmaf(g, n[j][e], s2);
@@ -209,14 +234,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
       float dx[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) dx[e] = r * (dy[j][e] * w[j][e] - m1 - n[j][e] * m2);
-      store8<T, VEC>((T*)a.dx + row * C, (run0 + 4 * WAVES * j) * kRun, l16, C, dx);
+      store8<T, EIGHTS>((T*)a.dx + row * C, held(j), dup(j), C, dx);
     }
   }
   if (!a.part) return;
   float* part = a.part + (int64_t)blockIdx.x * 2 * C;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c0 = (run0 + 4 * WAVES * j) * kRun;
+    auto put = [&](float* to, int e0, f32x4 v) {   // elements e0 .. e0 + 3 of vector j
+      if (first(j) + 8 <= C) {
+        *(any_f32x4*)(to + held(j) + e0) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e0 + e >= dup(j) && held(j) + e0 + e < C) to[held(j) + e0 + e] = v[e];
+      }
+    };
     if constexpr (WAVES == 1) {
       // the 4 waves hold the same channels: their sums meet in LDS, [wave][16 values][lane]
       __syncthreads();
@@ -226,22 +259,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, VEC && WAVES < 16 ? 
         join[(team * 16 + 8 + e) * 64 + lane] = db[j][e];
       }
       __syncthreads();
+      f32x4 s;   // values 4 team .. + 3 of lane `lane`: elements 4 (team % 2) .. + 3 of dw (team < 2) or db
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int k = 4 * team + q;   // value k of lane `lane`: element k % 8 of dw (k < 8) or db
-        const float s = (join[k * 64 + lane] + join[(16 + k) * 64 + lane]) +
-                        (join[(32 + k) * 64 + lane] + join[(48 + k) * 64 + lane]);
-        const int c = c0 + run_channel<VEC>(l16, k & 7);
-        if (c < C) part[(k < 8 ? 0 : C) + c] = s;
+        const int k = 4 * team + q;
+        s[q] = (join[k * 64 + lane] + join[(16 + k) * 64 + lane]) + (join[(32 + k) * 64 + lane] + join[(48 + k) * 64 + lane]);
       }
+      put(part + (team < 2 ? 0 : C), 4 * (team & 1), s);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = c0 + run_channel<VEC>(l16, e);
-        if (c < C) {
-          part[c] = dw[j][e];
-          part[C + c] = db[j][e];
-        }
+      for (int h = 0; h < 8; h += 4) {
+        put(part, h, f32x4{dw[j][h], dw[j][h + 1], dw[j][h + 2], dw[j][h + 3]});
+        put(part + C, h, f32x4{db[j][h], db[j][h + 1], db[j][h + 2], db[j][h + 3]});
       }
     }
   }
@@ -274,7 +303,7 @@ __global__ __launch_bounds__(1024) void param_sum_kernel(const float* __restrict
 }
 
 // A wave takes 4 runs of a row (one word of scales), 16 lanes each.
-template <typename T, bool VEC>
+template <typename T, bool EIGHTS>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t rows, int C, Out8 o) {
   const int l16 = threadIdx.x & 15, r4 = (threadIdx.x & 63) >> 4;
   const int runs = runs_of(C), ss = scale_stride(C), words = ss / 4;
@@ -283,14 +312,14 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
   if (row >= rows) return;
   const int run = (int)(unit - row * words) * 4 + r4;
   float v[8];
-  load8<T, VEC>(x + row * C, run * kRun, l16, C, v);
+  load8<T, EIGHTS>(x + row * C, run * kRun, l16, C, v);
   uint32_t s;
   const uint2 c = encode8(v, s);
-  if (run < runs) store_codes<VEC>(o.codes + (row * runs + run) * kRun, l16, c);
+  if (run < runs) store_codes(o.codes + (row * runs + run) * kRun, l16, c);
   if (l16 == 0) o.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool EIGHTS>
 __global__ __launch_bounds__(256) void dequantize_kernel(In8 q, int64_t rows, int C, T* __restrict__ out) {
   const int l16 = threadIdx.x & 15, r4 = (threadIdx.x & 63) >> 4;
   const int runs = runs_of(C), ss = scale_stride(C), words = ss / 4;
@@ -300,8 +329,8 @@ __global__ __launch_bounds__(256) void dequantize_kernel(In8 q, int64_t rows, in
   const int run = (int)(unit - row * words) * 4 + r4;
   if (run >= runs) return;
   float v[8];
-  decode8(load_codes<VEC>(q.codes + (row * runs + run) * kRun, l16), q.scales[row * ss + run], v);
-  store8<T, VEC>(out + row * C, run * kRun, l16, C, v);
+  decode8(load_codes(q.codes + (row * runs + run) * kRun, l16), q.scales[row * ss + run], v);
+  store8<T, EIGHTS>(out + row * C, run * kRun + l16 * 8, 0, C, v);
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -340,10 +369,10 @@ static int pick_team(int C, F&& f) {
   return FVSR_OK;
 }
 
-// f(element type, parameter type, whether rows are read 16 bytes at a time)
+// f(element type, parameter type, whether C is a multiple of 8)
 template <class F>
-static int pick_types(int dtype, int param_dtype, bool vec, F&& f) {
-  auto with = [&](auto t, auto p) { return vec ? f(t, p, std::true_type{}) : f(t, p, std::false_type{}); };
+static int pick_types(int dtype, int param_dtype, int C, F&& f) {
+  auto with = [&](auto t, auto p) { return C % 8 == 0 ? f(t, p, std::true_type{}) : f(t, p, std::false_type{}); };
   if (dtype == FVSR_DTYPE_BF16) return param_dtype == FVSR_DTYPE_BF16 ? with(bf16{}, bf16{}) : with(bf16{}, float{});
   return with(float{}, float{});   // fp32 tokens take fp32 parameters
 }
@@ -355,8 +384,7 @@ int launch_layer_norm(int dtype, int param_dtype, const void* x, int64_t rows, i
   if (rows <= 0) return FVSR_OK;
   if (const int rc = check_grid(rows, C <= 2048 ? 64 : C <= 8192 ? 256 : 1024)) return rc;
   const NormArgs a{x, rows, C, eps, w, b, y, y8, x8, stats};
-  const bool vec = rows_vectorize(x, C) && rows_vectorize(w, C) && rows_vectorize(b, C) && rows_vectorize(y, C);
-  return pick_types(dtype, param_dtype, vec, [&](auto t, auto p, auto v) {
+  return pick_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
     return pick_team(C, [&](auto waves, auto nv) {
       constexpr int W = decltype(waves)::value;
       hipLaunchKernelGGL((layer_norm_kernel<decltype(t), decltype(p), decltype(v)::value, W, decltype(nv)::value>),
@@ -379,11 +407,10 @@ int64_t norm_grad_blocks(int64_t rows, int C) {
 int launch_layer_norm_grad(int dtype, int param_dtype, const void* dy, const void* x, In8 x8, const float* stats,
                            int64_t rows, int C, const void* w, void* dx, float* dw, float* db, float* part,
                            hipStream_t stream) {
-  const bool vec = rows_vectorize(dy, C) && rows_vectorize(x, C) && rows_vectorize(w, C) && rows_vectorize(dx, C);
   const int64_t blocks = norm_grad_blocks(rows, C);
   if (blocks > 0) {
     const NormGradArgs a{dy, x, x8, stats, rows, C, w, dx, dw || db ? part : nullptr};
-    const int rc = pick_types(dtype, param_dtype, vec, [&](auto t, auto p, auto v) {
+    const int rc = pick_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
       return pick_team(C, [&](auto waves, auto nv) {
         constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
         constexpr bool V = decltype(v)::value;
@@ -401,32 +428,30 @@ int launch_layer_norm_grad(int dtype, int param_dtype, const void* dy, const voi
 
 int launch_quantize(int dtype, const void* x, int64_t rows, int C, Out8 o, hipStream_t stream) {
   if (rows <= 0) return FVSR_OK;
-  const bool vec = rows_vectorize(x, C);
   const int64_t blocks = ceil_div(rows * (scale_stride(C) / 4), 4);
   if (const int rc = check_grid(blocks, 256)) return rc;
   auto go = [&](auto t, auto v) {
     using T = decltype(t);
-    hipLaunchKernelGGL((quantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                       (const T*)x, rows, C, o);
+    hipLaunchKernelGGL((quantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, rows, C, o);
   };
-  if (dtype == FVSR_DTYPE_BF16) vec ? go(bf16{}, std::true_type{}) : go(bf16{}, std::false_type{});
-  else vec ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+  auto with = [&](auto t) { C % 8 == 0 ? go(t, std::true_type{}) : go(t, std::false_type{}); };
+  if (dtype == FVSR_DTYPE_BF16) with(bf16{});
+  else with(float{});
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
 }
 
 int launch_dequantize(In8 q, int64_t rows, int C, int dtype, void* out, hipStream_t stream) {
   if (rows <= 0) return FVSR_OK;
-  const bool vec = rows_vectorize(out, C);
   const int64_t blocks = ceil_div(rows * (scale_stride(C) / 4), 4);
   if (const int rc = check_grid(blocks, 256)) return rc;
   auto go = [&](auto t, auto v) {
     using T = decltype(t);
-    hipLaunchKernelGGL((dequantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, q, rows,
-                       C, (T*)out);
+    hipLaunchKernelGGL((dequantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, q, rows, C, (T*)out);
   };
-  if (dtype == FVSR_DTYPE_BF16) vec ? go(bf16{}, std::true_type{}) : go(bf16{}, std::false_type{});
-  else vec ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+  auto with = [&](auto t) { C % 8 == 0 ? go(t, std::true_type{}) : go(t, std::false_type{}); };
+  if (dtype == FVSR_DTYPE_BF16) with(bf16{});
+  else with(float{});
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
 }
