@@ -7,6 +7,10 @@
 //
 // All of them move each row once and compute a few operations a channel: memory-bound. A row's channels stay in registers
 // between the passes over it (sums, then squares, then the result), in 32 bits.
+//
+// bf16, against 4.8 TB/s that a copy of 4 GB reaches here: 17280 x 1536 norm 21.4 us (106 MB: 5.0 TB/s), norm with its statistics and x in
+// 8 bits 30.6 (133 MB, 4.3), gradient from them 25.8 (133 MB, 5.1) and 4.2 to add the parts; 17280 x 8960 quantize 93-102 us (466 MB,
+// 4.6-5.0), dequantize 79 (5.9: part of the codes is still in the memory-side cache). One row of 1536: 3.2 us, a chain of two round trips.
 #include <algorithm>
 
 #include "blocks8.hpp"

@@ -7,8 +7,8 @@ Tolerances, per value, with U = 2^-24 (half a step of fp32) and h half a step of
       rstd; the variance by about 64 U of itself, rstd by 40 U; with the last products and sums below 64 U |n w| + 4 U |b|
   its gradient (stats are inputs): n is off by 3 U |n| + U rstd |mean|-sized roundings of x - mean (U rstd |x - mean| = U |n|) and of
       the product: 4 U |n|; m1 and m2 by 70 U of their sums of magnitudes over C: with the rest below 80 U rstd (|g| + mean|g| +
-      |n| mean|g n|), plus h |dx|; dweight and dbias: at most rows / 2048 + 8 values in a lane, 4 waves, 128 workgroups' parts in a
-      thread, 4 threads: (rows / 2048 + 160) U of the sum of magnitudes
+      |n| mean|g n|), plus h |dx|; dweight and dbias: at most rows / 2048 + 8 values in a lane, 4 waves, 32 workgroups' parts in a
+      thread, 16 threads: below (rows / 2048 + 160) U of the sum of magnitudes
   weight gradients: exact factors, products added in some order, each addition at most U of the sum of magnitudes: (rows + 8) U
       sum |a b|, plus h |dW|
   8-bit products: the matrix cores add the products of 8 neighbouring channels after cutting each to a multiple of 2^(E - 13), E the
@@ -205,6 +205,63 @@ def test_layer_norm_backward(dev, dtype, rows, c):
     same = dy.clone()
     assert f.layer_norm_backward(same, x, stats, w, out=same)[0] is same
     assert torch.equal(same, f.layer_norm_backward(dy, x, stats, w)[0])
+
+
+@pytest.mark.parametrize("dtype", [bf, f32])
+@pytest.mark.parametrize("c", [2, 5, 9, 15, 121, 130, 135, 385, 1031, 1537, 2047, 2049, 4100, 8195, 16383])
+def test_layer_norm_backward_of_odd_rows(dev, dtype, c):
+    """Rows whose last 8 channels straddle two lanes, runs, waves."""
+    rows = 21
+    g = gen_of(rows, c, 5)
+    x = tokens(g, rows, c, dtype, dev)
+    dy = torch.randn((rows, c), generator=g).to(dtype).to(dev)
+    w = torch.randn(c, generator=g).to(dtype).to(dev)
+    _, stats, x8 = f.layer_norm(x, want_stats=True, want_x8=True)
+    for kept in (x, x8):
+        dx, dw, db = f.layer_norm_backward(dy, kept, stats, w)
+        check_norm_grad(dy, x if kept is x else quantize64(x)[0], stats, w, dx, dw, db)
+    same = dy.clone()
+    f.layer_norm_backward(same, x8, stats, w, out=same)
+    assert torch.equal(same, dx)
+
+
+def test_layer_norm_backward_of_neighbouring_runs(dev):
+    """A row's last channel alone in a run of 2^-127's scale, beside a run of the largest one: neither reaches the other."""
+    x = torch.ones((4, 129), device=dev)
+    x[1, :128], x[1, 128] = 1.2e19, 0
+    x[2, 128] = 3e38
+    dy = torch.randn((4, 129), generator=gen_of(3)).to(dev)
+    x8 = f.quantize8(x)
+    stats = torch.tensor([[0.0, 1e-25]], device=dev).repeat(4, 1)
+    dx, dw, db = f.layer_norm_backward(dy, x8, stats)
+    check_norm_grad(dy, quantize64(x)[0], stats, None, dx, dw, db)
+
+
+def test_nothing_is_written_past_the_ends(dev):
+    """Results of odd widths in the middle of a larger buffer, whose other elements stay as they were."""
+    rows, k, n = 133, 261, 267
+
+    def ends(call, shape, dtype):
+        size = shape[0] * shape[1]
+        buf = torch.full((size + 64,), 7.5, dtype=dtype, device=dev)
+        call(buf[31:31 + size].view(shape))
+        assert (buf[:31] == 7.5).all() and (buf[31 + size:] == 7.5).all() and not (buf[31:31 + size] == 7.5).all()
+
+    for dtype in (bf, f32):
+        x = tokens(gen_of(8), rows, k, dtype, dev)
+        x8, w8 = f.quantize8(x), f.quantize8(tokens(gen_of(9), n, k, bf, dev))
+        _, stats, _ = f.layer_norm(x, want_stats=True)
+        dy = tokens(gen_of(10), rows, n, bf, dev)
+        ends(lambda o: f.layer_norm(x, out=o), (rows, k), dtype)
+        ends(lambda o: f.layer_norm_backward(x, x8, stats, out=o), (rows, k), dtype)
+        ends(lambda o: f.dequantize8(x8, dtype, out=o), (rows, k), dtype)
+        ends(lambda o: f.linear8_weight_grad(dy, x8, dtype, out=o), (n, k), dtype)
+        for m in (3, 70, rows):
+            q = f.Blocks8(x8.codes[:m], x8.scales[:m], k)
+            ends(lambda o: f.linear8(q, w8, dtype=dtype, out=o), (m, n), dtype)
+        many = f.quantize8(tokens(gen_of(11), 2900, k, bf, dev))
+        wide = f.quantize8(tokens(gen_of(12), 3001, k, bf, dev))
+        ends(lambda o: f.linear8(many, wide, dtype=dtype, out=o), (2900, 3001), dtype)
 
 
 def test_layer_norm_backward_against_differences(dev):

@@ -154,3 +154,11 @@ def test_c_entry_points_refuse_bad_arguments():
     need = _abi.lib.fvsr_linear8_weight_grad_workspace(1, 8, 8)
     if need:
         assert wg(ctx, p, 1, 8, p, p, 8, F32, p, p, p, need - 1, None)[0] == inv
+
+
+def test_c_weight_gradient_wants_whole_rows_aligned():
+    """dY's rows are copied 16 bytes at a time where they are whole 16 bytes: then it starts at a multiple of 16."""
+    mem = C.create_string_buffer(4096)
+    p = (C.addressof(mem) + 255) & ~255
+    rc, msg = _rc("fvsr_linear8_weight_grad", p, p + 2, 1, 8, p, p, 8, _abi.DTYPE_F32, p, None, p, 1 << 20, None)
+    assert rc == _abi.ERR_INVALID_ARG and "16-byte aligned" in msg
