@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
 // phase, under the other group's products.
 //
 // 8192^3 in 382 us (2.9 PFLOP/s), 17280 x 8960 x 1536 in 207 (2.3, 408 tiles: a round and 152 over), 17280 x 1536 x 8960 in 228 (2.1, 12
-// steps a tile) and with GELU 237, the matrix cores busy 44 % of the cycles in the last; no bank conflicts. What bounds it is the
+// steps a tile) and with GELU 237, the matrix cores busy 45 % of the cycles in the last; no bank conflicts. What bounds it is the
 // issue of the copies and the reads from LDS side by side: without the copies of one operand (of both) the first takes 330 (303) us,
 // without any wait for them 372.
 template <bool GELU, typename O>
