@@ -951,10 +951,25 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16* __restrict__ 
   }
 }
 
-// dw = the sum over parts of their (N, K) partial results, in order (zeros if there are none)
+// dw = the sum over parts of their (N, K) partial results, in order (zeros if there are none), by the first `blocks` workgroups; the others,
+// if any, add up `sums` partial column sums, 64 columns each, a fourth of them a wave
 template <typename O>
-__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw) {
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw,
+                                                               int blocks, const float* __restrict__ col, int sums, int N,
+                                                               float* __restrict__ db) {
+  if ((int)blockIdx.x >= blocks) {
+    __shared__ float sm[4][64];
+    const int l = threadIdx.x & 63, q = threadIdx.x >> 6, c = ((int)blockIdx.x - blocks) * 64 + l;
+    float s = 0.f;
+    if (c < N)
+#pragma unroll 4
+      for (int p = q; p < sums; p += 4) s += col[(int64_t)p * N + c];
+    sm[q][l] = s;
+    __syncthreads();
+    if (q == 0 && c < N) db[c] = (sm[0][l] + sm[1][l]) + (sm[2][l] + sm[3][l]);
+    return;
+  }
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)blocks * 1024) {
     f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
     const int have = (int)min((int64_t)4, n - i);
     for (int p = 0; p < parts; ++p) {
@@ -1040,12 +1055,14 @@ int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int ou
   }
   if (p.parts != 1) {   // also no token: zeros
     const int64_t n = (int64_t)N * K;
-    const dim3 blocks((unsigned)std::min<int64_t>(ceil_div(n, 1024), 1 << 20));
+    const int blocks = (int)std::min<int64_t>(ceil_div(n, 1024), 1 << 20);
+    const dim3 join((unsigned)(blocks + (db ? ceil_div(N, 64) : 0)));
     if (out_dtype == FVSR_DTYPE_F32)
-      hipLaunchKernelGGL((weight_grad_join_kernel<float>), blocks, dim3(256), 0, stream, part, p.parts, n, (float*)dw);
+      hipLaunchKernelGGL((weight_grad_join_kernel<float>), join, dim3(256), 0, stream, part, p.parts, n, (float*)dw, blocks, sums, p.sum_parts, N, db);
     else
-      hipLaunchKernelGGL((weight_grad_join_kernel<bf16>), blocks, dim3(256), 0, stream, part, p.parts, n, (bf16*)dw);
+      hipLaunchKernelGGL((weight_grad_join_kernel<bf16>), join, dim3(256), 0, stream, part, p.parts, n, (bf16*)dw, blocks, sums, p.sum_parts, N, db);
     FVSR_HIP_CHECK(hipGetLastError());
+    return FVSR_OK;
   }
   if (!db) return FVSR_OK;
   return launch_param_sum(sums, p.sum_parts, N, N, db, nullptr, stream);
