@@ -39,9 +39,17 @@ struct NormGradArgs {
   float* part;          // (blocks, 2, C) partial dw and db; null: neither is made
 };
 
+// the sum over a wave (every lane active), by DPP rotations within its rows of 16 lanes and a lane of each row: no LDS round trips
 __device__ __forceinline__ float wave_sum(float x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  auto rot = [](float v, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x += rot(x, std::integral_constant<int, 0x128>{});   // row_ror:8
+  x += rot(x, std::integral_constant<int, 0x124>{});
+  x += rot(x, std::integral_constant<int, 0x122>{});
+  x += rot(x, std::integral_constant<int, 0x121>{});
+  auto row = [&](int r) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16 * r)); };
+  return (row(0) + row(1)) + (row(2) + row(3));
 }
 
 // sums over the WAVES waves that share a row, in a fixed order; `sm` holds 2 * WAVES floats and is free for reuse after the
