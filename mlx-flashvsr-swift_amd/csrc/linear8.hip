@@ -984,8 +984,10 @@ __global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __re
 
 int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);   // rows8.hip
 
-// How a weight gradient is cut up: the tokens of a tile into as many parts as fill the card, of at least kMinSteps steps. Rows of dY
-// that are not whole 16 bytes, which the copies into LDS need, are copied to such first (4000 x 1536 x 4500: 95 us; tiles of 128 that
+// How a weight gradient is cut up: the tokens of a tile into parts of at least kMinSteps steps, by what the whole takes: rounds of 256
+// workgroups, of 1.6 us a step and 6 us to start and end one, then the parts' sums at the copy's rate. As many as fill the card, or up to 4
+// that even out a ragged last round, if that gains a twelfth (4096 x 4608, 288 tiles: 17280 tokens 846 us whole, 695 in 3 parts; 2048
+// 121, 142 in 2: whole. 1400 x 5700, 138 tiles, 17280 tokens: 515, 416 in 3). Rows of dY that are not whole 16 bytes, which the copies into LDS need, are copied to such first (4000 x 1536 x 4500: 95 us; tiles of 128 that
 // read them as they are, without such copies, 310).
 struct WeightGradPlan {
   bool pad;
@@ -1000,7 +1002,15 @@ static WeightGradPlan weight_grad_plan(int64_t rows, int N, int K) {
   p.tiles_n = (int)ceil_div(N, 256);
   p.tiles_k = (int)ceil_div(K, 256);
   const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k, steps = ceil_div(rows, 64);
-  const int64_t parts = std::max<int64_t>(1, std::min(256 / tiles, steps / kMinSteps));
+  const int64_t most = std::max<int64_t>(1, steps / kMinSteps);
+  auto ns = [&](int64_t parts) {
+    return ceil_div(tiles * parts, 256) * (ceil_div(steps, parts) * 1600 + 6000) + (parts > 1 ? parts * N * K / 600 + 3000 : 0);
+  };
+  const int64_t fill = std::min(most, std::max<int64_t>(1, 256 / tiles));
+  int64_t parts = fill;
+  for (int64_t p = 1; p <= std::min<int64_t>(4, most); ++p)
+    if (ns(p) < ns(parts)) parts = p;
+  if (ns(parts) * 12 > ns(fill) * 11) parts = fill;
   p.part_rows = ceil_div(steps, parts) * 64;
   p.parts = rows > 0 ? (int)ceil_div(rows, p.part_rows) : 0;
   p.sum_parts = p.parts * p.tiles_k;

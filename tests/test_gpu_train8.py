@@ -423,6 +423,19 @@ def test_linear8_weight_grad(dev, rows, k, n):
         assert got is o and none is None and torch.equal(o, dw)
 
 
+@pytest.mark.parametrize("rows,k,n", [(9000, 3900, 4100), (9000, 1400, 5700)])
+def test_linear8_weight_grad_of_many_tiles(dev, rows, k, n):
+    """More tiles than workgroups run at once, or more than half as many, their tokens cut into parts all the same."""
+    g = gen_of(rows, k)
+    x8 = f.quantize8((torch.randn((rows, k), generator=g)).to(bf).to(dev))
+    dy = torch.randn((rows, n), generator=g).to(bf).to(dev)
+    dw, db = f.linear8_weight_grad(dy, x8)
+    a = values(x8)[:, :k]
+    within(dw, dy.double().t() @ a, (rows + 8) * U * (dy.double().abs().t() @ a.abs()) * (1 + 2.0 ** -7), "dweight")
+    within(db, dy.double().sum(0), (rows + 8) * U * dy.double().abs().sum(0), "dbias")
+    assert torch.equal(f.linear8_weight_grad(dy, x8, want_bias=False)[0], dw)
+
+
 @pytest.mark.parametrize("rows,k,n", [(200, 300, 264), (50, 100, 130), (700, 300, 520)])
 def test_linear8_weight_grad_of_infinities(dev, rows, k, n):
     """An infinity or NaN in dY takes its row of dW and its value of db; no other value."""
