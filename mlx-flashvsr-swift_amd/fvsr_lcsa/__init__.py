@@ -21,6 +21,7 @@ Every call runs the HIP kernels of libfvsr_lcsa.so; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 import torch
@@ -118,6 +119,7 @@ def _stream(stream) -> C.c_void_p:
 class Context:
     """One fvsr_ctx per device (workspace + device binding). Not re-entrant, like the reference's modules."""
     _by_device: dict[int, "Context"] = {}
+    _create = threading.Lock()
 
     def __init__(self, device: int = 0):
         self.device = device
@@ -132,9 +134,13 @@ class Context:
             device = torch.cuda.current_device()
         if isinstance(device, torch.device):
             device = device.index if device.index is not None else torch.cuda.current_device()
-        if device not in cls._by_device:
-            cls._by_device[device] = Context(device)
-        return cls._by_device[device]
+        found = cls._by_device.get(device)
+        if found is None:
+            with cls._create:   # one context per device, whichever thread asks first: a second one would replace it, and end it in use
+                found = cls._by_device.get(device)
+                if found is None:
+                    found = cls._by_device[device] = Context(device)
+        return found
 
     def reserve(self, nbytes: int):
         call("fvsr_ctx_reserve", self.handle, nbytes)

@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _abi
+from . import Context, _abi
 from ._abi import DTYPE_BF16, DTYPE_F32, FVSRError, lib
 
 __all__ = ["Blocks8", "quantize8", "dequantize8", "layer_norm", "layer_norm_backward", "linear8", "linear8_weight_grad"]
@@ -140,15 +140,9 @@ def _current(stream, t):
     return torch.cuda.stream(stream)
 
 
-_contexts: dict = {}
-
-
 def _ctx(dev: torch.device):
-    h = _contexts.get(dev.index)
-    if h is None:
-        from . import Context
-        h = _contexts[dev.index] = Context.get(dev).handle
-    return h
+    found = Context._by_device.get(dev.index)
+    return (Context.get(dev) if found is None else found).handle
 
 
 def _check(rc: int, name: str):
