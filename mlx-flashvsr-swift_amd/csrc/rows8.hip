@@ -52,8 +52,8 @@ __device__ __forceinline__ float wave_sum(float x) {
   return (row(0) + row(1)) + (row(2) + row(3));
 }
 
-// sums over the WAVES waves that share a row, in a fixed order; `sm` holds 2 * WAVES floats and is free for reuse after the
-// call's second barrier only, so successive calls alternate between two areas
+// sums over the WAVES waves that share a row, in a fixed order; `sm` holds 2 * WAVES floats, which a wave may
+// still read when another has left the call: successive calls alternate between two areas
 template <int WAVES>
 __device__ __forceinline__ void team_sum2(float& a, float& b, float* sm) {
   a = wave_sum(a);
@@ -228,17 +228,21 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16
     }
     if (row + step < a.rows) load(row + step);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      // Past the row's end dy is 0, and n has to be 0 too: the mean times rstd may pass the largest number where no channel's n
+      // does. Only the last vector reaches past it; a row of less than 8 channels has no neighbour's to take.
+      const float m = EIGHTS && j == NV - 1 && first(j) >= C ? 0.f : mu;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[j][e] = (n[j][e] - mu) * r;
-        if (!EIGHTS && e < dup(j)) n[j][e] = 0.f;   // (codes of another run, maybe); past C: dy is 0, and this finite where the row is
+        n[j][e] = (n[j][e] - m) * r;
+        if (!EIGHTS && (e < dup(j) || (WAVES * NV == 1 && e >= C))) n[j][e] = 0.f;   // the neighbour's, or codes of another run
         const float g = dy[j][e] * w[j][e];
         s1 += g;
         s2 = fmaf(g, n[j][e], s2);
         dw[j][e] = fmaf(dy[j][e], n[j][e], dw[j][e]);
         db[j][e] += dy[j][e];
       }
+    }
     team_sum2<WAVES>(s1, s2, sm[turn]);
     const float m1 = s1 / (float)C, m2 = s2 / (float)C;
 #pragma unroll
