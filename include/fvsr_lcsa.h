@@ -258,10 +258,11 @@ int fvsr_dit_block(fvsr_ctx* ctx, fvsr_kv_ring* ring, int layer, const fvsr_dit_
 /* ---- (f4) training and serving in 8 bits: layer norm, 8-bit activations, 8-bit linear layers ------------------- */
 /* No reference counterpart. An 8-bit matrix of `rows` x `channels`: each row is cut into runs of 128 channels (the last padded
  * with zeros); a run has a scale 2^e, the smallest with e >= -127 and max |x| <= 448 * 2^e over its finite values, and each
- * channel the e4m3 (OCP, no infinities) number nearest to x / 2^e, ties to even; infinities and NaN become NaN. `codes`: (rows,
+ * channel the e4m3 (OCP, no infinities) number nearest to x / 2^e, ties to even, but at most 240 under the largest scale, 2^120
+ * (256 there would stand for 2^128: what is finite comes back finite); infinities and NaN become NaN. `codes`: (rows,
  * 128 * runs) bytes, 16-byte aligned; `scales`: the bytes e + 127 (E8M0), (rows, runs rounded up to a multiple of 4), 4-byte
- * aligned, the bytes past the last run 0. Every value code * 2^e is exact in fp32. A scale byte of 255, which quantize8 does not
- * write, makes its run NaN. Codes past the last channel have to be 0: the products read whole runs.
+ * aligned, the bytes past the last run 0. Every value code * 2^e that quantize8 writes is exact in fp32. A scale byte of 255, which
+ * it does not write, makes its run NaN. Codes past the last channel have to be 0: the products read whole runs.
  * These entry points allocate nothing and use no context workspace: where they need memory beside their operands they take it
  * as `workspace` (device memory, 16-byte aligned), which is free again when the call's work on `stream` is done. Calls on one
  * context may therefore overlap, on any streams, and may be captured into HIP graphs. They leave the thread's current device as it

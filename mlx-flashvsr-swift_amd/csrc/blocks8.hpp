@@ -2,7 +2,8 @@
 //
 // A row of C channels is cut into runs of 128 (the last padded with zeros). A run has a scale 2^e, the smallest with e >= -127
 // and max |x| <= 448 * 2^e over its finite values, and each channel a code: the e4m3 number nearest to x / 2^e, ties to
-// even; an infinity or NaN becomes NaN. Codes are stored (rows, 128 * runs), scales as the byte e + 127 (E8M0), (rows,
+// even, but at most 240 under the largest scale, 2^120, where the next number, 256, would stand for 2^128 (so what is finite
+// comes back finite, and within 2^-4 of what it was: 240 * 2^120 is 15 / 16 of 2^128); an infinity or NaN becomes NaN. Codes are stored (rows, 128 * runs), scales as the byte e + 127 (E8M0), (rows,
 // runs rounded up to 4), the bytes past the last run 0.
 //
 // Why a power of two: x / 2^e is exact, so the codes do not depend on how the quotient is formed; an element's value
@@ -48,16 +49,16 @@ __device__ __forceinline__ float max16(float x) {
 }
 
 // Encodes a run held by 16 lanes, 8 values each: the codes of this lane's values in order, and the run's scale byte. With top =
-// 1.f * 2^(E - 127), the smallest e is E - 127 - 8, one more where 1.f > 1.75 (448 = 1.75 * 2^8).
+// 1.f * 2^(E - 127), the smallest e is E - 127 - 8, one more where 1.f > 1.75 (448 = 1.75 * 2^8). Magnitudes above 240 * 2^120 exist
+// under the scale 2^120 only, and are cut to that: it changes no other value's code.
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& scale) {
   float top = 0.f;
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float a = fabsf(v[e]);
-    const bool finite = a <= 3.402823466e38f;   // false for NaN
-    top = fmaxf(top, finite ? a : 0.f);
-    f[e] = finite ? v[e] : __uint_as_float(0x7fc00000u);
+    const bool finite = fabsf(v[e]) <= 3.402823466e38f;   // false for NaN
+    f[e] = finite ? __builtin_amdgcn_fmed3f(v[e], -0x1.ep127f, 0x1.ep127f) : __uint_as_float(0x7fc00000u);
+    top = fmaxf(top, fabsf(f[e]));                        // the other one where f is NaN
   }
   const uint32_t bits = __float_as_uint(max16(top));
   const int s = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);

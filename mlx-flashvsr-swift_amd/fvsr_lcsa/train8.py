@@ -184,8 +184,8 @@ def _params(dtype, w, b=None):
 # ----------------------------------------------------------------------------------------------------------------------
 def quantize8(x: torch.Tensor, stream=None, out: Blocks8 | None = None) -> Blocks8:
     """x (rows, features), float32 or bfloat16, in 8 bits: of each run of 128 channels of a row, the scale is the smallest power
-    of two 2^e, e >= -127, with max |x| <= 448 * 2^e, and a channel's code the e4m3 number nearest to x / 2^e, ties to even.
-    Infinities and NaN become NaN and do not count for the scale."""
+    of two 2^e, e >= -127, with max |x| <= 448 * 2^e, and a channel's code the e4m3 number nearest to x / 2^e, ties to even (at
+    most 240 under the largest scale, 2^120, so that every finite value comes back finite). Infinities and NaN become NaN and do not count for the scale."""
     if stream is not None:
         with _current(stream, x):
             return quantize8(x, out=out)
@@ -202,7 +202,8 @@ def quantize8(x: torch.Tensor, stream=None, out: Blocks8 | None = None) -> Block
 
 def dequantize8(q: Blocks8, dtype: torch.dtype = torch.bfloat16, stream=None, out=None) -> torch.Tensor:
     """The values that q stands for, (rows, features) in `dtype`. From bfloat16 or float32 tokens the round trip is off by at most
-    2^-4 relative to a channel's value, or 2^-17 relative to its run's largest, whichever is more."""
+    2^-4 relative to a channel's value, or 2^-17 relative to its run's largest, whichever is more (in a run whose largest
+    value is below 2^-119 by 2^-137 instead, and bfloat16 rounds what is below 2^-126 once more)."""
     if stream is not None:
         with _current(stream, q):
             return dequantize8(q, dtype, out=out)
