@@ -18,6 +18,8 @@ must not overlap what the call reads (but layer_norm_backward's may be dy). Norm
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import Context, _abi
@@ -48,6 +50,12 @@ class Blocks8:
     __slots__ = ("codes", "scales", "features")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, features: int):
+        try:
+            features = operator.index(features)
+        except TypeError:
+            _refuse("Blocks8", f"expected a whole number of features, got {type(features).__name__}")
+        for t in (codes, scales):
+            _kind(t, "Blocks8", torch.Tensor)
         if codes.dtype != CODES or scales.dtype != SCALES:
             _refuse("Blocks8", f"expected float8_e4m3fn codes and float8_e8m0fnu scales, got {codes.dtype} and {scales.dtype}")
         if features < 1 or codes.dim() != 2 or scales.dim() != 2 or codes.shape[0] != scales.shape[0] or \
@@ -100,10 +108,25 @@ def _same(name: str, shape, want, dtype=None, want_dtype=None):
         _refuse(name, f"expected {tuple(want)} {want_dtype or ''}, got {tuple(shape)} {dtype or ''}")
 
 
+def _kind(t, name: str, kind):
+    """t, which has to be a `kind` (a tensor or a Blocks8)."""
+    if not isinstance(t, kind):
+        _refuse(name, f"expected a {kind.__name__}, got {type(t).__name__}")
+    return t
+
+
+def _out8(out, name: str, shape):
+    """A caller's 8-bit output (or None) of exactly this shape."""
+    if out is not None:
+        _same(name, _kind(out, name, Blocks8).shape, shape)
+    return out
+
+
 def _out(out, name: str, shape, dtype):
     """A caller's output tensor (or None) of exactly this shape, contiguous; a batch-1 3-D view is taken too."""
     if out is None:
         return None
+    _kind(out, name, torch.Tensor)
     o = out[0] if out.dim() == 3 and out.shape[0] == 1 else out
     _same(name, o.shape, shape, o.dtype, dtype)
     if not o.is_contiguous():
@@ -130,6 +153,8 @@ def _current(stream, t):
     """The scope in which `stream` (a torch stream, or a hipStream_t as an integer) is the current one: a call given a stream runs
     itself in it, so that its temporaries belong to the stream that its kernels run on, and the allocator hands their memory on in
     that stream's order."""
+    if not isinstance(t, (torch.Tensor, Blocks8)):
+        _refuse("stream", f"a stream for a {type(t).__name__} in a tensor's or Blocks8's place")
     dev = t.device
     if dev.type != "cuda":
         _refuse("stream", f"a stream for tensors on {dev}")
@@ -163,7 +188,7 @@ def _param(t, name: str, features: int):
     """A weight or bias of a norm or linear layer: (features) values, fp32 or bf16."""
     if t is None:
         return None
-    if t.dtype not in _CODE:
+    if _kind(t, name, torch.Tensor).dtype not in _CODE:
         _refuse(name, f"unsupported dtype {t.dtype} (float32 or bfloat16)")
     if t.numel() != features or not t.is_contiguous():
         _refuse(name, f"expected {features} contiguous elements, got {tuple(t.shape)}")
@@ -191,8 +216,7 @@ def quantize8(x: torch.Tensor, stream=None, out: Blocks8 | None = None) -> Block
             return quantize8(x, out=out)
     x2 = _tokens(x, "x")
     rows, c = x2.shape
-    if out is not None:
-        _same("out", out.shape, (rows, c))
+    _out8(out, "out", (rows, c))
     dev = _one_device(x2, "x", (out, "out"))
     q = Blocks8.empty(rows, c, dev) if out is None else out
     _check(lib.fvsr_quantize8(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), rows, c, q.codes.data_ptr(), q.scales.data_ptr(),
@@ -209,7 +233,7 @@ def dequantize8(q: Blocks8, dtype: torch.dtype = torch.bfloat16, stream=None, ou
             return dequantize8(q, dtype, out=out)
     if dtype not in _CODE:
         _refuse("dequantize8", f"unsupported dtype {dtype} (float32 or bfloat16)")
-    rows, c = q.shape
+    rows, c = _kind(q, "q", Blocks8).shape
     o = _out(out, "out", (rows, c), dtype)
     dev = _one_device(q.codes, "q", (o, "out"))
     if o is None:
@@ -234,10 +258,7 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, want_
     x2 = _tokens(x, "x")
     rows, c = x2.shape
     weight, bias = _param(weight, "weight", c), _param(bias, "bias", c)
-    if not quantized:
-        y = _out(out, "out", (rows, c), x2.dtype)
-    elif out is not None:
-        _same("out", out.shape, (rows, c))
+    y = _out8(out, "out", (rows, c)) if quantized else _out(out, "out", (rows, c), x2.dtype)
     dev = _one_device(x2, "x", (weight, "weight"), (bias, "bias"), (out, "out"))
     kind, w, b = _params(x2.dtype, weight, bias)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if want_stats else None
@@ -273,7 +294,7 @@ def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, w
     else:
         x2 = None
         _same("x", kept.shape, (rows, c))
-    _same("stats", stats.shape, (rows, 2), stats.dtype, torch.float32)
+    _same("stats", _kind(stats, "stats", torch.Tensor).shape, (rows, 2), stats.dtype, torch.float32)
     if not stats.is_contiguous():
         _refuse("stats", "expected a contiguous tensor")
     weight = _param(weight, "weight", c)

@@ -1,6 +1,8 @@
-"""CPU checks of how the 8-bit training operators are called: the context that calls of several threads share."""
+"""CPU checks of how the 8-bit training operators are called: the context that calls of several threads share, operands of a
+wrong kind."""
 import threading
 
+import pytest
 import torch
 
 import fvsr_lcsa as f
@@ -37,3 +39,39 @@ def test_first_calls_of_two_threads_share_one_context(monkeypatch):
         f.Context._by_device.pop(device.index, None)
         getattr(train8, "_contexts", {}).pop(device.index, None)
     assert ended == [1]
+
+
+def test_operands_of_a_wrong_kind_are_refused_by_name():
+    """A tensor in a Blocks8's place, the other way round, None and numbers: the framework's error, with the operand's name."""
+    bf = torch.bfloat16
+    x, w, st = torch.zeros((4, 256), dtype=bf), torch.ones(256), torch.zeros((4, 2))
+    q, w8, dy = f.Blocks8.empty(4, 256, "cpu"), f.Blocks8.empty(24, 256, "cpu"), torch.zeros((4, 24), dtype=bf)
+    for name, call in (
+            ("out", lambda: f.quantize8(x, out=x)),
+            ("q", lambda: f.dequantize8(x)),
+            ("q", lambda: f.dequantize8(None)),
+            ("out", lambda: f.dequantize8(q, out=q)),
+            ("out", lambda: f.layer_norm(x, out=q)),
+            ("out", lambda: f.layer_norm(x, quantized=True, out=x)),
+            ("weight", lambda: f.layer_norm(x, 1.0)),
+            ("bias", lambda: f.layer_norm(x, w, [0.0] * 256)),
+            ("x", lambda: f.layer_norm(q)),
+            ("stats", lambda: f.layer_norm_backward(x, x, None)),
+            ("stats", lambda: f.layer_norm_backward(x, q, (0.0, 1.0))),
+            ("x", lambda: f.layer_norm_backward(x, None, st)),
+            ("dy", lambda: f.layer_norm_backward(q, x, st)),
+            ("out", lambda: f.layer_norm_backward(x, x, st, out=q)),
+            ("x", lambda: f.linear8(None, w8)),
+            ("weight", lambda: f.linear8(x, None)),
+            ("bias", lambda: f.linear8(x, w8, 0.5)),
+            ("out", lambda: f.linear8(x, w8, out=q)),
+            ("x8", lambda: f.linear8_weight_grad(dy, None)),
+            ("dy", lambda: f.linear8_weight_grad(q, q)),
+            ("out", lambda: f.linear8_weight_grad(dy, q, out=w8)),
+            ("Blocks8", lambda: f.Blocks8(None, q.scales, 256)),
+            ("Blocks8", lambda: f.Blocks8(q.codes, 1, 256)),
+            ("Blocks8", lambda: f.Blocks8(q.codes, q.scales, 256.0)),
+            ("stream", lambda: f.quantize8(None, stream=0)),
+            ("stream", lambda: f.linear8([1.0], w8, stream=0))):
+        with pytest.raises(f.FVSRError, match=f"^{name} failed"):
+            call()
