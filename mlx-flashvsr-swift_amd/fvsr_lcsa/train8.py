@@ -13,8 +13,9 @@ A training pass of a linear layer keeps nothing but what its forward pass read:
 
 Tokens are (L, C) or (1, L, C), contiguous, on a HIP device; L may be 0. The calls keep no state: temporaries come from torch's
 allocator on the stream that the call runs on (the current one, or `stream`), so calls may overlap on several streams and be
-captured into graphs. They are plain functions: gradients are asked for by name, and no result is part of an autograd graph. An `out`
-must not overlap what the call reads (but layer_norm_backward's may be dy). Norms take up to 16384 channels, the others 2^20.
+captured into graphs. They are plain functions: gradients are asked for by name, and no result is part of an autograd graph; a tensor
+that requires a gradient is refused where autograd records (call them under torch.no_grad() or inside an autograd function). An `out` must
+not overlap what the call reads (but layer_norm_backward's may be dy). Norms take up to 16384 channels, the others 2^20.
 """
 from __future__ import annotations
 
@@ -89,11 +90,20 @@ class Blocks8:
         return q
 
 
+def _detached(t: torch.Tensor, name: str):
+    """Refuses a tensor that requires a gradient where autograd records: the gradient would be lost without a word, for these calls are no
+    part of a graph. Under torch.no_grad(), and so inside an autograd function's forward and backward, it is taken as it is."""
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(name, "requires a gradient, which this call would drop: call it under torch.no_grad(), or on .detach()",
+                _abi.ERR_UNSUPPORTED)
+
+
 def _tokens(x, name: str, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tensor:
     if not isinstance(x, torch.Tensor):
         _refuse(name, f"expected a tensor, got {type(x).__name__}")
     if x.dtype not in dtypes:
         _refuse(name, f"unsupported dtype {x.dtype} ({' or '.join(str(d)[6:] for d in dtypes)})")
+    _detached(x, name)
     if x.dim() == 3:
         if x.shape[0] != 1:
             _refuse(name, "batch 1 only (flatten the batch into the tokens)", _abi.ERR_UNSUPPORTED)
@@ -126,7 +136,7 @@ def _out(out, name: str, shape, dtype):
     """A caller's output tensor (or None) of exactly this shape, contiguous; a batch-1 3-D view is taken too."""
     if out is None:
         return None
-    _kind(out, name, torch.Tensor)
+    _detached(_kind(out, name, torch.Tensor), name)
     o = out[0] if out.dim() == 3 and out.shape[0] == 1 else out
     _same(name, o.shape, shape, o.dtype, dtype)
     if not o.is_contiguous():
@@ -190,6 +200,7 @@ def _param(t, name: str, features: int):
         return None
     if _kind(t, name, torch.Tensor).dtype not in _CODE:
         _refuse(name, f"unsupported dtype {t.dtype} (float32 or bfloat16)")
+    _detached(t, name)
     if t.numel() != features or not t.is_contiguous():
         _refuse(name, f"expected {features} contiguous elements, got {tuple(t.shape)}")
     return t
@@ -295,6 +306,7 @@ def layer_norm_backward(dy: torch.Tensor, x, stats: torch.Tensor, weight=None, w
         x2 = None
         _same("x", kept.shape, (rows, c))
     _same("stats", _kind(stats, "stats", torch.Tensor).shape, (rows, 2), stats.dtype, torch.float32)
+    _detached(stats, "stats")
     if not stats.is_contiguous():
         _refuse("stats", "expected a contiguous tensor")
     weight = _param(weight, "weight", c)

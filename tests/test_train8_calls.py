@@ -1,5 +1,5 @@
 """CPU checks of how the 8-bit training operators are called: the context that calls of several threads share, operands of a
-wrong kind."""
+wrong kind, tensors that require a gradient."""
 import threading
 
 import pytest
@@ -75,3 +75,41 @@ def test_operands_of_a_wrong_kind_are_refused_by_name():
             ("stream", lambda: f.linear8([1.0], w8, stream=0))):
         with pytest.raises(f.FVSRError, match=f"^{name} failed"):
             call()
+
+
+def test_a_gradient_is_not_dropped_without_a_word():
+    """Where autograd records, a tensor that requires a gradient is refused; under no_grad, and inside an autograd function, the call
+    goes on (here as far as the check of its device)."""
+    bf = torch.bfloat16
+    x, w, st = torch.zeros((4, 256), dtype=bf), torch.ones(256), torch.zeros((4, 2))
+    q, w8, dy, b = f.Blocks8.empty(4, 256, "cpu"), f.Blocks8.empty(24, 256, "cpu"), torch.zeros((4, 24), dtype=bf), torch.zeros(24)
+    r = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = (("x", lambda: f.quantize8(r(x))),
+             ("out", lambda: f.dequantize8(q, out=r(x))),
+             ("x", lambda: f.layer_norm(r(x)[None], w)),
+             ("weight", lambda: f.layer_norm(x, r(w))),
+             ("bias", lambda: f.layer_norm(x, w, torch.nn.Parameter(w), quantized=True)),
+             ("out", lambda: f.layer_norm(x, out=r(x))),
+             ("dy", lambda: f.layer_norm_backward(r(x), x, st)),
+             ("x", lambda: f.layer_norm_backward(x, r(x), st)),
+             ("stats", lambda: f.layer_norm_backward(x, q, r(st))),
+             ("weight", lambda: f.layer_norm_backward(x, q, st, r(w))),
+             ("x", lambda: f.linear8(r(x), w8)),
+             ("bias", lambda: f.linear8(q, w8, r(b))),
+             ("dy", lambda: f.linear8_weight_grad(r(dy), q)))
+    for name, call in calls:
+        with pytest.raises(f.FVSRError, match=f"^{name} failed.*requires a gradient") as e:
+            call()
+        assert e.value.status == f._abi.ERR_UNSUPPORTED
+
+    class Inside(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return f.layer_norm(t, w)[0]
+
+    with torch.no_grad():
+        for _, call in calls:
+            with pytest.raises(f.FVSRError, match="HIP device"):
+                call()
+    with pytest.raises(f.FVSRError, match="HIP device"):
+        Inside.apply(r(x))
