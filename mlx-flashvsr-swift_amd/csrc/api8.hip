@@ -1,7 +1,7 @@
-// extern "C" entry points of the row operators and products with 8-bit operands (declared in include/fvsr_lcsa.h, section f4):
-// argument validation before any device work, then launches on the caller's stream. They allocate nothing and keep nothing: what
-// they need beside their operands is the caller's `workspace`, so calls on one context may overlap, on any streams, and may be
-// captured into graphs.
+// extern "C" entry points of the row operators and products with 8-bit operands (declared in include/fvsr_lcsa.h,
+// section f4): argument validation before any device work, then launches on the caller's stream. They allocate nothing
+// and keep nothing: what they need beside their operands is the caller's `workspace`, so calls on one context may
+// overlap, on any streams, and may be captured into graphs.
 #include "blocks8.hpp"
 
 namespace fvsr {
@@ -150,7 +150,8 @@ int fvsr_layer_norm_backward(fvsr_ctx* ctx, int dtype, const void* dy, const voi
     FVSR_REQUIRE((!dweight && !dbias) ||
                      (workspace && aligned(workspace, 16) &&
                       workspace_bytes >= fvsr_layer_norm_backward_workspace(rows, channels)),
-                 FVSR_ERR_INVALID_ARG, "dweight and dbias need a 16-byte aligned workspace of fvsr_layer_norm_backward_workspace bytes");
+                 FVSR_ERR_INVALID_ARG,
+                 "dweight and dbias need a 16-byte aligned workspace of fvsr_layer_norm_backward_workspace bytes");
   }
   FVSR_ON_DEVICE(ctx);
   return launch_layer_norm_grad(dtype, param_dtype, dy, x, In8{(const uint8_t*)x_codes, (const uint8_t*)x_scales}, stats,

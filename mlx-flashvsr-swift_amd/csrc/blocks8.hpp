@@ -1,15 +1,17 @@
-// The 8-bit form of a matrix of tokens or weights, shared by the kernels that write and read it (rows8.hip, linear8.hip).
+// The 8-bit form of a matrix of tokens or weights, shared by the kernels that write and read it (rows8.hip,
+// linear8.hip).
 //
-// A row of C channels is cut into runs of 128 (the last padded with zeros). A run has a scale 2^e, the smallest with e >= -127
-// and max |x| <= 448 * 2^e over its finite values, and each channel a code: the e4m3 number nearest to x / 2^e, ties to
-// even, but at most 240 under the largest scale, 2^120, where the next number, 256, would stand for 2^128 (so what is finite
-// comes back finite, and within 2^-4 of what it was: 240 * 2^120 is 15 / 16 of 2^128); an infinity or NaN becomes NaN. Codes are stored (rows, 128 * runs), scales as the byte e + 127 (E8M0), (rows,
-// runs rounded up to 4), the bytes past the last run 0.
+// A row of C channels is cut into runs of 128 (the last padded with zeros). A run has a scale 2^e, the smallest with e
+// >= -127 and max |x| <= 448 * 2^e over its finite values, and each channel a code: the e4m3 number nearest to x / 2^e,
+// ties to even, but at most 240 under the largest scale, 2^120, where the next number, 256, would stand for 2^128 (so
+// what is finite comes back finite, and within 2^-4 of what it was: 240 * 2^120 is 15 / 16 of 2^128); an infinity or
+// NaN becomes NaN. Codes are stored (rows, 128 * runs), scales as the byte e + 127 (E8M0), (rows, runs rounded up to
+// 4), the bytes past the last run 0.
 //
 // Why a power of two: x / 2^e is exact, so the codes do not depend on how the quotient is formed; an element's value
-// code * 2^e has 4 significant bits and is exact in bf16 and fp32; and the matrix cores' scaled products take the byte as
-// it is, so no vector instruction ever multiplies by a scale. e4m3 being a floating format, a scale up to twice the tightest
-// one costs no relative precision above its subnormals.
+// code * 2^e has 4 significant bits and is exact in bf16 and fp32; and the matrix cores' scaled products take the byte
+// as it is, so no vector instruction ever multiplies by a scale. e4m3 being a floating format, a scale up to twice the
+// tightest one costs no relative precision above its subnormals.
 #pragma once
 #include "common.hpp"
 
@@ -36,7 +38,8 @@ struct Out8 {
 __host__ __device__ __forceinline__ int runs_of(int channels) { return (channels + kRun - 1) / kRun; }
 __host__ __device__ __forceinline__ int scale_stride(int channels) { return (runs_of(channels) + 3) & ~3; }
 
-// max over each 16 lanes of a wave (every lane active, x >= 0), in every one of them: DPP rotations within the rows of 16
+// max over each 16 lanes of a wave (every lane active, x >= 0), in every one of them: DPP rotations within the rows of
+// 16
 __device__ __forceinline__ float max16(float x) {
   auto rot = [](float v, auto ctrl) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false));
@@ -48,9 +51,9 @@ __device__ __forceinline__ float max16(float x) {
   return x;
 }
 
-// Encodes a run held by 16 lanes, 8 values each: the codes of this lane's values in order, and the run's scale byte. With top =
-// 1.f * 2^(E - 127), the smallest e is E - 127 - 8, one more where 1.f > 1.75 (448 = 1.75 * 2^8). Magnitudes above 240 * 2^120 exist
-// under the scale 2^120 only, and are cut to that: it changes no other value's code.
+// Encodes a run held by 16 lanes, 8 values each: the codes of this lane's values in order, and the run's scale byte.
+// With top = 1.f * 2^(E - 127), the smallest e is E - 127 - 8, one more where 1.f > 1.75 (448 = 1.75 * 2^8). Magnitudes
+// above 240 * 2^120 exist under the scale 2^120 only, and are cut to that: it changes no other value's code.
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& scale) {
   float top = 0.f;
   float f[8];
@@ -86,9 +89,10 @@ __device__ __forceinline__ void decode8(uint2 c, uint32_t scale, float (&v)[8]) 
   v[6] = p[0]; v[7] = p[1];
 }
 
-// A lane (l16 = lane % 16) holds 8 adjacent channels of a run, 8 l16 .. 8 l16 + 7. As they lie in memory, zeros past the row's end: loaded
-// now, widened when they are needed. Rows of any length and alignment are read and written by whole vectors, but for a last part of 8;
-// EIGHTS: rows have none (C is a multiple of 8), and no registers are spent on it.
+// A lane (l16 = lane % 16) holds 8 adjacent channels of a run, 8 l16 .. 8 l16 + 7. As they lie in memory, zeros past
+// the row's end: loaded now, widened when they are needed. Rows of any length and alignment are read and written by
+// whole vectors, but for a last part of 8; EIGHTS: rows have none (C is a multiple of 8), and no registers are spent on
+// it.
 template <typename T>
 struct Raw8 {
   T v[8];

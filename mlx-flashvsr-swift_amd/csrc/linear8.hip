@@ -1,5 +1,5 @@
-// Products with 8-bit operands for gfx950 (MI355X): the linear layer y = x W^T + b (+ GELU) from 8-bit tokens and weights, and
-// its weight gradient dW = dY^T X from bf16 gradients and the 8-bit tokens that the layer read.
+// Products with 8-bit operands for gfx950 (MI355X): the linear layer y = x W^T + b (+ GELU) from 8-bit tokens and
+// weights, and its weight gradient dW = dY^T X from bf16 gradients and the 8-bit tokens that the layer read.
 #include <algorithm>
 
 #include "blocks8.hpp"
@@ -22,19 +22,23 @@ __device__ __forceinline__ u32x4 make_rsrc(const void* base, uint32_t bytes) {
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const lds_char*)p);
 }
-// x, not known to be what it was before: what is computed from it in a loop is computed there, and takes no registers across it
+// x, not known to be what it was before: what is computed from it in a loop is computed there, and takes no registers
+// across it
 __device__ __forceinline__ uint32_t afresh(uint32_t x) {
   asm volatile("" : "+v"(x));
   return x;
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
-// 16 (or 4) bytes a lane from a buffer straight into LDS at `lds` + 16 (4) * lane; the address is the lane's offset plus the common
-// one. The copy is waited for with vmcnt. One wait state has to pass between the write of M0 and its use, hence the s_nop.
+// 16 (or 4) bytes a lane from a buffer straight into LDS at `lds` + 16 (4) * lane; the address is the lane's offset
+// plus the common one. The copy is waited for with vmcnt. One wait state has to pass between the write of M0 and its
+// use, hence the s_nop.
 __device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t lds, uint32_t off, uint32_t common) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off), "s"(rsrc), "s"(uniform(common)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off),
+               "s"(rsrc), "s"(uniform(common)));
 }
 __device__ __forceinline__ void copy4(u32x4 rsrc, uint32_t lds, uint32_t off, uint32_t common) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off), "s"(rsrc), "s"(uniform(common)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(off),
+               "s"(rsrc), "s"(uniform(common)));
 }
 
 struct Linear8Args {
@@ -48,15 +52,16 @@ struct Linear8Args {
   int part_runs;         // runs of a part, whole words of scales (linear8_kernel; part p writes its own rows x N sums at y)
 };
 
-// 0.5 y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) = y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))), the exponential in base 2:
-// its argument overflows to +inf (the result then is 0) only where y is far below zero
+// 0.5 y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) = y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))), the
+// exponential in base 2: its argument overflows to +inf (the result then is 0) only where y is far below zero
 __device__ __forceinline__ float gelu_tanh(float y) {
   constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
   const float e = __builtin_amdgcn_exp2f(k * y * fmaf(0.044715f * y, y, 1.f));
   return y * __builtin_amdgcn_rcpf(1.f + e);
 }
 
-// of 8 values, the steps side by side: an exponential or a reciprocal is used three instructions after it was asked for at the least
+// of 8 values, the steps side by side: an exponential or a reciprocal is used three instructions after it was asked for
+// at the least
 __device__ __forceinline__ void gelu_tanh8(float (&y)[8]) {
   constexpr float k = -2.f * 0.7978845608028654f * 1.4426950408889634f;
   float e[8];
@@ -70,8 +75,8 @@ __device__ __forceinline__ void gelu_tanh8(float (&y)[8]) {
   for (int i = 0; i < 8; ++i) y[i] *= e[i];
 }
 
-// bias (fp32, in LDS, at this lane's first feature), GELU and the store of a wave's fragments: this lane's features n0 + 32 p .. + 7
-// (two fragments) of the tokens row0 + 16 m. WHOLE: every feature and token is inside.
+// bias (fp32, in LDS, at this lane's first feature), GELU and the store of a wave's fragments: this lane's features n0
+// + 32 p .. + 7 (two fragments) of the tokens row0 + 16 m. WHOLE: every feature and token is inside.
 template <bool GELU, bool WHOLE, int FN, int FM, typename O>
 __device__ __forceinline__ void write_fragments(const Linear8Args& a, const f32x4 (&acc)[FN][FM], O* y, const float* bias, int n0,
                                                 int64_t row0) {
@@ -117,25 +122,28 @@ __device__ __forceinline__ bool write_tile(const Linear8Args& a, const f32x4 (&a
   return whole;
 }
 
-// Tile of TN output features x TM tokens, WN x WM waves; a step is one run: 128 codes of every row, and their scales in the
-// matrix instruction.
+// Tile of TN output features x TM tokens, WN x WM waves; a step is one run: 128 codes of every row, and their scales in
+// the matrix instruction.
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4 D (16 x 16) += A (16 x 128) B (128 x 16): lane l gives 32 codes of row l % 16 of A and of
-// column l % 16 of B, and the scale byte of its 32 codes, taken from byte OP of a register; all of a run have one scale, so which 32
-// codes go with which lane does not matter as long as A and B agree. A is the weights: a lane's 4 results are then 4 features of
-// one token. Fragment f of a wave holds the features 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4, i = 0 .. 15, so that two fragments
-// leave a lane 8 adjacent features: 16-byte stores, 64 bytes a token and instruction.
+// v_mfma_scale_f32_16x16x128_f8f6f4 D (16 x 16) += A (16 x 128) B (128 x 16): lane l gives 32 codes of row l % 16 of A
+// and of column l % 16 of B, and the scale byte of its 32 codes, taken from byte OP of a register; all of a run have
+// one scale, so which 32 codes go with which lane does not matter as long as A and B agree. A is the weights: a lane's
+// 4 results are then 4 features of one token. Fragment f of a wave holds the features 32 (f / 2) + 8 (i / 4) + 4 (f %
+// 2) + i % 4, i = 0 .. 15, so that two fragments leave a lane 8 adjacent features: 16-byte stores, 64 bytes a token and
+// instruction.
 //
-// LDS holds two steps: rows of 128 bytes, the 16-byte chunks XOR-ed by a number of the row under which the 16 rows that one
-// instruction reads fall on 16 places of the 64 banks; copies go from memory to LDS directly (the XOR is on the source side), the
-// next step's while this one's products run. A word of scales holds 4 steps.
+// LDS holds two steps: rows of 128 bytes, the 16-byte chunks XOR-ed by a number of the row under which the 16 rows that
+// one instruction reads fall on 16 places of the 64 banks; copies go from memory to LDS directly (the XOR is on the
+// source side), the next step's while this one's products run. A word of scales holds 4 steps.
 //
-// Sums are fp32. Before it adds them, the matrix core cuts each of the 8 products of an octet (8 adjacent codes of a lane) toward zero to a
-// multiple of 2^(E - 13), E the largest sum of two code exponents among them (found by comparing 102400 random octets bit by bit; the
-// 32 x 32 x 64 form and the unscaled ones do the same). The rate of these instructions is why the layer is kept in 8 bits at all, a bf16 y
-// hides the cut, and an fp32 y carries it.
+// Sums are fp32. Before it adds them, the matrix core cuts each of the 8 products of an octet (8 adjacent codes of a
+// lane) toward zero to a multiple of 2^(E - 13), E the largest sum of two code exponents among them (found by comparing
+// 102400 random octets bit by bit; the 32 x 32 x 64 form and the unscaled ones do the same), so an octet is off by less
+// than 2^-10 of its largest product. The rate of these instructions is why the layer is kept in 8 bits at all. Of a
+// layer of random operands the fp32 sums are off by 5e-5 to 8e-5 (root mean square, relative), which an fp32 y carries
+// and which moves 1 in 40 values of a bf16 y to the next number.
 //
-// Bound by latency where there is little work: 512 x 4096 x 1536, 12.6 us in 4 parts of 8 steps, 0.5 PFLOP/s.
+// Bound by latency where there is little work: 512 x 4096 x 1536, 12.3 us in 4 parts of 8 steps, 0.5 PFLOP/s.
 template <int TN, int TM, int WN, int WM, bool GELU, typename O>
 __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a) {
   constexpr int kWaves = WN * WM, FN = TN / WN / 16, FM = TM / WM / 16;
@@ -145,7 +153,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
   __shared__ __align__(1024) char sm[2 * kStage + 2 * kScales + TN * 4];
   float* const bias = (float*)(sm + 2 * kStage + 2 * kScales);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // tiles: every XCD a contiguous range, ordered in bands of 8 tiles of tokens so that a band's codes and the weights stay in its L2
+  // tiles: every XCD a contiguous range, ordered in bands of 8 tiles of tokens so that a band's codes and the weights
+  // stay in its L2
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   constexpr int kBand = 8;
   const int band = t / (kBand * a.tiles_n), in_band = t % (kBand * a.tiles_n);
@@ -164,8 +173,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
   auto swz = [](int i, int q) { return ((i >> 1) & 1) | ((q >> 1) << 1) | (((q ^ (q >> 1)) & 1) << 2); };
   auto swz_w = [&](int r) { return swz(r & 3, (r >> 3) & 3); };
   auto swz_x = [&](int r) { return swz(r & 3, (r >> 2) & 3); };
-  // a lane's source offsets: of 8 rows a wave and copy, and of a word of scales a row. Rows past the last one read it again (their
-  // results are not stored).
+  // a lane's source offsets: of 8 rows a wave and copy, and of a word of scales a row. Rows past the last one read it
+  // again (their results are not stored).
   constexpr int kCW = TN / (8 * kWaves), kCX = TM / (8 * kWaves), kScaleRows = (TN + TM) / kWaves;
   uint32_t ow[kCW], ox[kCX];
 #pragma unroll
@@ -247,25 +256,27 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear8_kernel(Linear8Args a)
                    rows_m == TM && rows_n == TN);
 }
 
-// The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between them. Two groups
-// of four waves, one of each on every SIMD, take turns: while one group's 32 matrix instructions of a step (a run: 128 codes of every
-// row) go, the other reads its operands of the step into registers and asks for later ones. A phase ends with a barrier; steps s are
-// counted across tiles, LDS holds two of them, and wave w of a group computes features 64 w .. 64 w + 63 of the group's 128 tokens:
+// The large product: 256 features x 256 tokens a tile, one workgroup a CU walking over tiles without a break between
+// them. Two groups of four waves, one of each on every SIMD, take turns: while one group's 32 matrix instructions of a
+// step (a run: 128 codes of every row) go, the other reads its operands of the step into registers and asks for later
+// ones. A phase ends with a barrier; steps s are counted across tiles, LDS holds two of them, and wave w of a group
+// computes features 64 w .. 64 w + 63 of the group's 128 tokens:
 //
 //   phase      2s                                       2s + 1
 //   group 0    copy group 1's tokens of s + 1, read(s)  multiply(s)
 //   group 1    multiply(s - 1)                          copy group 0's tokens of s + 2, read(s), copy the weights of s + 2
 //
-// Everything is asked for as soon as its place is free: group 0's tokens of step s have been read when phase 2s ends, group 1's when
-// phase 2s + 1 ends; the weights that wave w of group 1 reads in phase 2s + 1 wave w of group 0 has read before, so it replaces them at
-// once. Each is needed about three phases later, and its wave waits for it at the end of that time, by the count of what it has
-// asked for since (memory operations of a wave complete in order). A group writes its tile, and starts the next one, in its read
-// phase, under the other group's products.
+// Everything is asked for as soon as its place is free: group 0's tokens of step s have been read when phase 2s ends,
+// group 1's when phase 2s + 1 ends; the weights that wave w of group 1 reads in phase 2s + 1 wave w of group 0 has read
+// before, so it replaces them at once. Each is needed about three phases later, and its wave waits for it at the end of
+// that time, by the count of what it has asked for since (memory operations of a wave complete in order). A group
+// writes its tile, and starts the next one, in its read phase, under the other group's products.
 //
-// 8192^3 in 382 us (2.9 PFLOP/s), 17280 x 8960 x 1536 in 207 (2.3, 408 tiles: a round and 152 over), 17280 x 1536 x 8960 in 228 (2.1, 12
-// steps a tile) and with GELU 237, the matrix cores busy 45 % of the cycles in the last; no bank conflicts. What bounds it is the
-// issue of the copies and the reads from LDS side by side: without the copies of one operand (of both) the first takes 330 (303) us,
-// without any wait for them 372.
+// 8192^3 in 382-394 us by part (2.8-2.9 PFLOP/s), 17280 x 8960 x 1536 in 207-210 (2.3, 408 tiles: a round and 152
+// over), 17280 x 1536 x 8960 in 228 (2.1, 12 steps a tile) and with GELU 237-247, the matrix cores busy 44 % of the
+// cycles in the last; no bank conflicts. What bounds the first, 64 steps a tile, is the issue of the copies and the
+// reads from LDS side by side: where it took 382, without the copies of one operand (of both) 330 (303) us, without any
+// wait for them 372. At 12 steps a tile this was not told apart.
 template <bool GELU, typename O>
 __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
   constexpr int FN = 4, FM = 8, kStores = FN / 2 * FM * (int)sizeof(O) / 2;
@@ -277,8 +288,9 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
   const int group = wave >> 2, w = wave & 3, i = lane & 15, g = lane >> 4;
   const int G = a.runs, ld = G * kRun;
   const uint32_t lds0 = lds_offset(sm);
-  // chunk c of row r of the weights lies at c ^ swz(r % 4, r / 8 % 4), of the tokens at c ^ swz(r % 4, r / 4 % 4): the 16 rows that a cycle
-  // of a 16-byte read serves (of a fragment: features 8 (i / 4) + i % 4, tokens i) then lie on different banks
+  // chunk c of row r of the weights lies at c ^ swz(r % 4, r / 8 % 4), of the tokens at c ^ swz(r % 4, r / 4 % 4): the
+  // 16 rows that a cycle of a 16-byte read serves (of a fragment: features 8 (i / 4) + i % 4, tokens i) then lie on
+  // different banks
   auto swz = [](int r, int q) { return ((r >> 1) & 1) | ((q >> 1) << 1) | (((q ^ (q >> 1)) & 1) << 2); };
   const int rw0 = w * 64 + ((i >> 2) << 3) + (i & 3), rx0 = group * 128 + i;
   const char* pw[2];
@@ -288,8 +300,8 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
     pw[h] = sm + rw0 * kRun + (((2 * g + h) ^ swz(rw0 & 3, (rw0 >> 3) & 3)) << 4);
     px[h] = sm + kX + rx0 * kRun + (((2 * g + h) ^ swz(rx0 & 3, (rx0 >> 2) & 3)) << 4);
   }
-  // copies: 8 rows an instruction, this wave's 64 rows of weights and 32 of the other group's tokens; a lane's source of rows 8 c + r8 is
-  // 8 c rows on, its chunk XOR-ed by what c adds to swz
+  // copies: 8 rows an instruction, this wave's 64 rows of weights and 32 of the other group's tokens; a lane's source
+  // of rows 8 c + r8 is 8 c rows on, its chunk XOR-ed by what c adds to swz
   const int r8 = lane >> 3, cs = ((lane & 7) ^ ((r8 >> 1) & 1)) << 4;
   const uint32_t ow = (uint32_t)(r8 * ld + cs), ox = (uint32_t)(r8 * ld + (cs ^ ((r8 >> 2) << 6)));
   const uint32_t os = (uint32_t)(lane * a.ss);
@@ -309,14 +321,17 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
     n0 = in_band / band_m * 256;
   };
 
-  // what this wave asks for: step ck of tile ct; rows past the last one lie past the end of a buffer and are read as zeros
+  // what this wave asks for: step ck of tile ct; rows past the last one lie past the end of a buffer and are read as
+  // zeros
   int ct = t, ck = 0, cn = 0, cs4 = 0;   // cn: tiles, cs4: words of scales asked for before
   int64_t cm0;
   int cn0;
   u32x4 dw, dx, dsw, dsx, db;
   auto source = [&]() __attribute__((always_inline)) {
     place(ct, cm0, cn0);
-    auto rows = [&](int64_t have, int64_t at, int most) __attribute__((always_inline)) { return (uint32_t)max((int64_t)0, min(have - at, (int64_t)most)); };
+    auto rows = [&](int64_t have, int64_t at, int most) __attribute__((always_inline)) {
+      return (uint32_t)max((int64_t)0, min(have - at, (int64_t)most));
+    };
     const int64_t mx = cm0 + (1 - group) * 128 + w * 32;
     dx = make_rsrc(a.x.codes + mx * ld, rows(a.rows, mx, 32) * ld);
     if (group == 1) {
@@ -342,7 +357,7 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
       copy16(dx, to + c * 8 * kRun, (o ^ ((c & 1) * 0x60)) + c * 8 * ld, ck * kRun);
     });
   };
-  auto copy_small = [&]() __attribute__((always_inline)) {             // scales and biases (group 1), where the step begins a word or a tile
+  auto copy_small = [&]() __attribute__((always_inline)) {   // scales and biases (group 1), where a word or a tile begins
     if (ck & 3) return;
     const uint32_t to = lds0 + kS + (cs4 & 3) * kScales + w * 256;
     copy4(dsw, to, os, ck);
@@ -443,7 +458,8 @@ __global__ __launch_bounds__(512, 2) void linear8_large_kernel(Linear8Args a) {
             ++bt;
           }
         read_step(kc);
-        // then what has been asked for since the copies that the next phase needs may be outstanding: this step's, and maybe stores
+        // then what has been asked for since the copies that the next phase needs may be outstanding: this step's, and
+        // maybe stores
         if (group == 0) {
           if (ask) copy_tokens(par ^ 1);
           if (!ask) FVSR_WAIT(0);
@@ -485,7 +501,8 @@ __global__ __launch_bounds__(256) void widen_kernel(const bf16* __restrict__ in,
 // y = the sum over parts of their (rows, N) sums, bias, GELU; V elements a thread (4 where N is a multiple of 4)
 template <int V, typename O>
 __global__ __launch_bounds__(256) void linear8_join_kernel(const float* __restrict__ part, int parts, int64_t n, int N,
-                                                           const void* __restrict__ bias, int bias_f32, int gelu, O* __restrict__ y) {
+                                                           const void* __restrict__ bias, int bias_f32, int gelu,
+                                                           O* __restrict__ y) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= n) return;
   typedef float fv __attribute__((ext_vector_type(V)));
@@ -501,9 +518,9 @@ __global__ __launch_bounds__(256) void linear8_join_kernel(const float* __restri
   }
 }
 
-// The product of a few tokens (16 * FM at most), bound by reading the weights: 16 features a workgroup, its four waves take every
-// fourth run and read their operands straight into registers, up to three runs asked for at once; the waves' sums meet in LDS. 1 x 1536 x
-// 9216: 5.8 us, 2.5 TB/s (a chain of three round trips; in tiles of 128 x 128 9.9 us).
+// The product of a few tokens (16 * FM at most), bound by reading the weights: 16 features a workgroup, its four waves
+// take every fourth run and read their operands straight into registers, up to three runs asked for at once; the waves'
+// sums meet in LDS. 1 x 1536 x 9216: 5.8 us, 2.5 TB/s (a chain of three round trips; in tiles of 128 x 128 9.9 us).
 template <int FM, typename O>
 __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a) {
   __shared__ float sm[4][FM][16][17];
@@ -560,10 +577,11 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a) {
   }
 }
 
-// How a product is cut up. A few tokens: by 16 features. Else tiles of 256 x 256, one a CU, or of 128 x 128, two a CU: a round of the
-// former does twice the work of one of the latter in 1.5 to 1.6 times its time (8192^3, 4 rounds against 8: 382 us, 518; 4096 x 1536 x 6144,
-// 2 against 3: 48 us, 46), so by the rounds that each needs. Where there are few of the latter,
-// each row's runs are cut into parts of at least 8 (512 x 4096 x 1536, 48 tiles: 12.6 us in 4 parts and 4.8 to join them, 25 in one).
+// How a product is cut up. A few tokens: by 16 features. Else tiles of 256 x 256, one a CU, or of 128 x 128, two a CU:
+// a round of the former does twice the work of one of the latter in 1.5 to 1.6 times its time (8192^3, 4 rounds against
+// 8: 382 us, 518; 4096 x 1536 x 6144, 2 against 3: 48 us, 46), so by the rounds that each needs. Where there are few of
+// the latter, each row's runs are cut into parts of at least 8 (512 x 4096 x 1536, 48 tiles: 12.3 us in 4 parts and 4.2
+// to join them, 25 in one).
 struct Linear8Plan {
   bool few, large;
   int64_t tiles;
@@ -630,7 +648,8 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
     part.bias = nullptr;
     part.gelu = 0;
     part.y = ws;
-    hipLaunchKernelGGL((linear8_kernel<128, 128, 4, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(512), 0, stream, part);
+    hipLaunchKernelGGL((linear8_kernel<128, 128, 4, 2, false, float>), dim3((unsigned)p.tiles, (unsigned)p.parts), dim3(512),
+                       0, stream, part);
     FVSR_HIP_CHECK(hipGetLastError());
     const int64_t n = rows * N;
     auto join = [&](auto v, auto o) {
@@ -646,8 +665,8 @@ int launch_linear8(In8 x, int64_t rows, int K, In8 w, int N, int bias_dtype, con
     if (bf) with(bf16{});
     else with(float{});
   } else {
-    // where a CU has one workgroup at most, 8 waves of it: two on each SIMD, whose reads and products overlap (512 x 1536 x 1536, 12
-    // steps: 9.8 us with 8 waves, 10.5 with 4)
+    // where a CU has one workgroup at most, 8 waves of it: two on each SIMD, whose reads and products overlap (512 x
+    // 1536 x 1536, 12 steps: 9.8 us with 8 waves, 10.5 with 4)
     const dim3 grid((unsigned)p.tiles);
     auto go = [&](auto wn, auto g) {
       constexpr int WN = decltype(wn)::value;
@@ -693,24 +712,26 @@ __device__ __forceinline__ void store4(O* out, f32x4 x, int n) {
   }
 }
 
-// dW (N, K) = dY^T X, 256 features x 256 channels a workgroup, steps of 64 tokens. Both operands lie token-major, so the product's depth
-// runs across rows: they are kept in LDS as they come, [token][column], in bf16 (codes times scales are exact in it), and
-// ds_read_b64_tr_b16 hands a lane 4 tokens of one column: 16 lanes read 4 rows of 16 columns, lane i gets column i of the four.
-// Two groups of four waves take turns as in linear8_large_kernel; wave w of group h computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
+// dW (N, K) = dY^T X, 256 features x 256 channels a workgroup, steps of 64 tokens. Both operands lie token-major, so
+// the product's depth runs across rows: they are kept in LDS as they come, [token][column], in bf16 (codes times scales
+// are exact in it), and ds_read_b64_tr_b16 hands a lane 4 tokens of one column: 16 lanes read 4 rows of 16 columns,
+// lane i gets column i of the four. Two groups of four waves take turns as in linear8_large_kernel; wave w of group h
+// computes features 64 w .. 64 w + 63 and channels 128 h .. 128 h + 127, a run:
 //
 //   phase      2s                                                          2s + 1
 //   group 0    widen X1(s), read(s), ask for dY(s + 1) and codes of s + 2  multiply(s)
 //   group 1    multiply(s - 1)                                             widen X0(s + 1), read(s), ask for codes of s + 3
 //
-// LDS: dY of two steps, in blocks of 64 features (rows of 128 bytes, a token each). X as bf16, a half (a group's run) of one step each:
-// written in the phases in which it is not read. Codes and scales as they come, two steps: a wave copies, and later widens, its own 16
-// tokens of the other group's half, so its own count of copies is all it waits for. The 32-byte pairs of a row of token t are XOR-ed by
-// (t / 2 % 2, t / 8 % 2): a half wave's transposing read (4 tokens of 16 columns for each 16 lanes) then touches every bank once.
-// dY's copies stand between the reads from LDS: behind them, at the phase's end, their issue was what the other group waited for
-// (497 us at 17280 x 1536 x 8960, now 436: 1.1 PFLOP/s on 210 of 256 CUs, which alone allows 1.3 of the 1.58 that a library product of
-// 16384^3 reaches; matrix cores busy 54 % of those CUs' cycles).
-// Copies past the last token read zeros (and nothing else), so every phase asks for the same number.
-// db: a step's column sums are taken by one of the tiles_k workgroups that read the step, from the fragments in registers, under the
+// LDS: dY of two steps, in blocks of 64 features (rows of 128 bytes, a token each). X as bf16, a half (a group's run)
+// of one step each: written in the phases in which it is not read. Codes and scales as they come, two steps: a wave
+// copies, and later widens, its own 16 tokens of the other group's half, so its own count of copies is all it waits
+// for. The 32-byte pairs of a row of token t are XOR-ed by (t / 2 % 2, t / 8 % 2): a half wave's transposing read (4
+// tokens of 16 columns for each 16 lanes) then touches every bank once. dY's copies stand between the reads from LDS:
+// behind them, at the phase's end, their issue was what the other group waited for (497 us at 17280 x 1536 x 8960, now
+// 434: 1.1 PFLOP/s on 210 of 256 CUs, which alone allows 1.3 of the 1.58 that a library product of 16384^3 reaches;
+// matrix cores busy 53 % of those CUs' cycles).
+// Copies past the last token read zeros (and nothing else), so every phase asks for the same number. db: a step's
+// column sums are taken by one of the tiles_k workgroups that read the step, from the fragments in registers, under the
 // products (a column a lane; as products with rows of ones and zeros an infinity would reach other columns).
 template <typename O>
 __global__ __launch_bounds__(512, 2) void weight_grad_kernel(WeightGradArgs a) {
@@ -735,8 +756,8 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(WeightGradArgs a) {
   const uint32_t oc = (uint32_t)((16 * w + r8) * ldk + c8 * 16);
   const int run = tk * 2 + other;                           // this wave's codes' run
   const int count = (int)(to - from);                       // tokens (a part has fewer than 2^31)
-  // dY, codes and scales of the step that is asked for next, and their places in LDS: steps are asked for in order, so all that a step
-  // costs is three sums (its 64-bit products and minima each time cost 60 us of 445)
+  // dY, codes and scales of the step that is asked for next, and their places in LDS: steps are asked for in order, so
+  // all that a step costs is three sums (its 64-bit products and minima each time cost 60 us of 445)
   auto records = [&](int left, int ld, int off) __attribute__((always_inline)) {
     return (uint32_t)max(0, max(0, min(kTokens, left)) * ld - off);
   };
@@ -804,7 +825,8 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(WeightGradArgs a) {
         v[2 * e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j][e], by, false);
         v[2 * e + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[j][e], by, true);
       }
-      // the lanes of one block write the lower halves of their pairs first, those of the other, on the same banks, the upper ones
+      // the lanes of one block write the lower halves of their pairs first, those of the other, on the same banks, the
+      // upper ones
       char* o = out + j * 1024 + (((c & 3) ^ ((r >> 1) & 1) ^ (j << 1)) << 5);
       const bool up = c >> 2;
       const u32x4 lo = *(u32x4*)v, hi = *(u32x4*)(v + 4);
@@ -857,7 +879,8 @@ __global__ __launch_bounds__(512, 2) void weight_grad_kernel(WeightGradArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const bf16x8 d = fd[h][f];
-          sums[f] += (((float)d[0] + (float)d[1]) + ((float)d[2] + (float)d[3])) + (((float)d[4] + (float)d[5]) + ((float)d[6] + (float)d[7]));
+          sums[f] += (((float)d[0] + (float)d[1]) + ((float)d[2] + (float)d[3])) +
+                     (((float)d[4] + (float)d[5]) + ((float)d[6] + (float)d[7]));
         }
     }
     __builtin_amdgcn_s_setprio(0);
@@ -951,11 +974,12 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16* __restrict__ 
   }
 }
 
-// dw = the sum over parts of their (N, K) partial results, in order (zeros if there are none), by the first `blocks` workgroups; the others,
-// if any, add up `sums` partial column sums, 64 columns each, a fourth of them a wave
+// dw = the sum over parts of their (N, K) partial results, in order (zeros if there are none), by the first `blocks`
+// workgroups; the others, if any, add up `sums` partial column sums, 64 columns each, a fourth of them a wave
 template <typename O>
-__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n, O* __restrict__ dw,
-                                                               int blocks, const float* __restrict__ col, int sums, int N,
+__global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __restrict__ part, int parts, int64_t n,
+                                                               O* __restrict__ dw, int blocks,
+                                                               const float* __restrict__ col, int sums, int N,
                                                                float* __restrict__ db) {
   if ((int)blockIdx.x >= blocks) {
     __shared__ float sm[4][64];
@@ -984,11 +1008,12 @@ __global__ __launch_bounds__(256) void weight_grad_join_kernel(const float* __re
 
 int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);   // rows8.hip
 
-// How a weight gradient is cut up: the tokens of a tile into parts of at least kMinSteps steps, by what the whole takes: rounds of 256
-// workgroups, of 1.6 us a step and 6 us to start and end one, then the parts' sums at the copy's rate. As many as fill the card, or up to 4
-// that even out a ragged last round, if that gains a twelfth (4096 x 4608, 288 tiles: 17280 tokens 846 us whole, 695 in 3 parts; 2048
-// 121, 142 in 2: whole. 1400 x 5700, 138 tiles, 17280 tokens: 515, 416 in 3). Rows of dY that are not whole 16 bytes, which the copies into LDS need, are copied to such first (4000 x 1536 x 4500: 95 us; tiles of 128 that
-// read them as they are, without such copies, 310).
+// How a weight gradient is cut up: the tokens of a tile into parts of at least kMinSteps steps, by what the whole
+// takes: rounds of 256 workgroups, of 1.6 us a step and 6 us to start and end one, then the parts' sums at the copy's
+// rate. As many as fill the card, or up to 4 that even out a ragged last round, if that gains a twelfth (4096 x 4608,
+// 288 tiles: 17280 tokens 844 us whole, 659 in 3 parts; 2048 117, 142 in 2: whole. 1400 x 5700, 138 tiles, 17280
+// tokens: 515, 415 in 3). Rows of dY that are not whole 16 bytes, which the copies into LDS need, are copied to such
+// first (4000 x 1536 x 4500: 90 us; tiles of 128 that read them as they are, without such copies, 310).
 struct WeightGradPlan {
   bool pad;
   int tiles_n, tiles_k, parts;
@@ -1054,8 +1079,8 @@ int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int ou
     a.ld = (int)ceil_div(N, 8) * 8;
     a.dy = (const bf16*)((char*)ws + space.dy);
     const int64_t blocks = ceil_div(rows * (a.ld / 8), 256);
-    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream, (const bf16*)dy, rows, N,
-                       (bf16*)((char*)ws + space.dy));
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, stream,
+                       (const bf16*)dy, rows, N, (bf16*)((char*)ws + space.dy));
     FVSR_HIP_CHECK(hipGetLastError());
   }
   if (p.parts > 0) {
@@ -1068,9 +1093,11 @@ int launch_weight_grad(const void* dy, int64_t rows, int N, In8 x, int K, int ou
     const int blocks = (int)std::min<int64_t>(ceil_div(n, 1024), 1 << 20);
     const dim3 join((unsigned)(blocks + (db ? ceil_div(N, 64) : 0)));
     if (out_dtype == FVSR_DTYPE_F32)
-      hipLaunchKernelGGL((weight_grad_join_kernel<float>), join, dim3(256), 0, stream, part, p.parts, n, (float*)dw, blocks, sums, p.sum_parts, N, db);
+      hipLaunchKernelGGL((weight_grad_join_kernel<float>), join, dim3(256), 0, stream, part, p.parts, n, (float*)dw, blocks,
+                         sums, p.sum_parts, N, db);
     else
-      hipLaunchKernelGGL((weight_grad_join_kernel<bf16>), join, dim3(256), 0, stream, part, p.parts, n, (bf16*)dw, blocks, sums, p.sum_parts, N, db);
+      hipLaunchKernelGGL((weight_grad_join_kernel<bf16>), join, dim3(256), 0, stream, part, p.parts, n, (bf16*)dw, blocks,
+                         sums, p.sum_parts, N, db);
     FVSR_HIP_CHECK(hipGetLastError());
     return FVSR_OK;
   }

@@ -1,16 +1,18 @@
-// Row operators next to the 8-bit products, for gfx950 (MI355X): tokens to 8 bits and back, and layer norm with its gradient, which
-// write and read the 8-bit form in the passes that hold the row anyway.
+// Row operators next to the 8-bit products, for gfx950 (MI355X): tokens to 8 bits and back, and layer norm with its
+// gradient, which write and read the 8-bit form in the passes that hold the row anyway.
 //
 //   y  = n w + b,  n = (x - mean) rstd,  rstd = 1 / sqrt(var + eps)      (mean and var over the row's C channels)
 //   dx = rstd (g - mean(g) - n mean(g n)),  g = dy w
 //   dw = sum over rows of dy n,  db = sum over rows of dy
 //
-// All of them move each row once and compute a few operations a channel: memory-bound. A row's channels stay in registers
-// between the passes over it (sums, then squares, then the result), in 32 bits.
+// All of them move each row once and compute a few operations a channel: memory-bound. A row's channels stay in
+// registers between the passes over it (sums, then squares, then the result), in 32 bits.
 //
-// bf16, against 4.8 TB/s that a copy of 4 GB reaches here: 17280 x 1536 norm 21.4 us (106 MB: 5.0 TB/s), norm with its statistics and x in
-// 8 bits 30.6 (133 MB, 4.3), gradient from them 25.8 (133 MB, 5.1) and 4.2 to add the parts; 17280 x 8960 quantize 93-102 us (466 MB,
-// 4.6-5.0), dequantize 79 (5.9: part of the codes is still in the memory-side cache). One row of 1536: 3.2 us, a chain of two round trips.
+// bf16, against 4.8 TB/s that a copy of 4 GB reaches here, over buffers of more than the memory-side cache: 17280 x
+// 1536 norm 26.4 us (106 MB, 4.0 TB/s; 21.3 where each pass writes the same output, part of which stays in that cache),
+// with its statistics and x in 8 bits 30.5 (133 MB, 4.3), to 8 bits 24.1 (80 MB, 3.3; 30-33 right behind a product
+// whose output still drains), gradient from 8 bits 27.4 (133 MB, 4.9) and 5-6 to add the parts; 17280 x 8960 quantize
+// 84-95 us (466 MB, 4.9-5.5), dequantize 75-81 (5.7-6.2). One row of 1536: 3.0 us, a chain of two round trips.
 #include <algorithm>
 
 #include "blocks8.hpp"
@@ -39,7 +41,8 @@ struct NormGradArgs {
   float* part;          // (blocks, 2, C) partial dw and db; null: neither is made
 };
 
-// the sum over a wave (every lane active), by DPP rotations within its rows of 16 lanes and a lane of each row: no LDS round trips
+// the sum over a wave (every lane active), by DPP rotations within its rows of 16 lanes and a lane of each row: no LDS
+// round trips
 __device__ __forceinline__ float wave_sum(float x) {
   auto rot = [](float v, auto ctrl) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false));
@@ -74,8 +77,8 @@ __device__ __forceinline__ void team_sum2(float& a, float& b, float* sm) {
   }
 }
 
-// One row a team of WAVES waves (a workgroup holds max(WAVES, 4) waves), NV vectors of 8 channels a lane: lane L of the team and
-// vector j hold 8 channels of run 4 * WAVES * j + L / 16.
+// One row a team of WAVES waves (a workgroup holds max(WAVES, 4) waves), NV vectors of 8 channels a lane: lane L of the
+// team and vector j hold 8 channels of run 4 * WAVES * j + L / 16.
 template <typename T, typename P, bool EIGHTS, int WAVES, int NV>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kernel(NormArgs a) {
   __shared__ float sm[2][2 * WAVES];
@@ -145,11 +148,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void layer_norm_kern
 }
 
 // The gradient: teams walk over the rows (the grid is a fixed number of workgroups) and keep their part of dw and db in
-// registers; the workgroup's sum goes to `part`, and param_sum_kernel adds the workgroups' up: no atomics, the same result
-// every time. Where C is not a multiple of 8 (not EIGHTS), the lane of the row's end takes its last 8 channels, and skips the first `dup`
-// of them, which its neighbour has too: one load, which nothing waits for before its row is worked on.
+// registers; the workgroup's sum goes to `part`, and param_sum_kernel adds the workgroups' up: no atomics, the same
+// result every time. Where C is not a multiple of 8 (not EIGHTS), the lane of the row's end takes its last 8 channels,
+// and skips the first `dup` of them, which its neighbour has too: one load, which nothing waits for before its row is
+// worked on.
 template <typename T, typename P, bool EIGHTS, int WAVES, int NV, bool X8>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16 ? 2 : 1) void layer_norm_grad_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16 ? 2 : 1)
+void layer_norm_grad_kernel(NormGradArgs a) {
   __shared__ float sm[2][2 * WAVES];
   __shared__ float join[WAVES == 1 ? 4 * 64 * 16 : 1];
   const int l16 = threadIdx.x & 15, lane = threadIdx.x & 63, C = a.C;
@@ -229,8 +234,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16
     if (row + step < a.rows) load(row + step);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      // Past the row's end dy is 0, and n has to be 0 too: the mean times rstd may pass the largest number where no channel's n
-      // does. Only the last vector reaches past it; a row of less than 8 channels has no neighbour's to take.
+      // Past the row's end dy is 0, and n has to be 0 too: the mean times rstd may pass the largest number where no
+      // channel's n does. Only the last vector reaches past it; a row of less than 8 channels has no neighbour's to
+      // take.
       const float m = EIGHTS && j == NV - 1 && first(j) >= C ? 0.f : mu;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -292,9 +298,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, EIGHTS && WAVES < 16
   }
 }
 
-// The sums over p < parts of part[p * n + c], c < n: columns below `split` go to out, the others to out2 (either may be null). 64
-// columns a workgroup, a sixteenth of the parts a wave, joined in a fixed order: the parts' addresses are known at once, so the time is
-// that of a few loads in a row (512 parts of 2 x 1536 columns: 12 us with a quarter a wave).
+// The sums over p < parts of part[p * n + c], c < n: columns below `split` go to out, the others to out2 (either may be
+// null). 64 columns a workgroup, a sixteenth of the parts a wave, joined in a fixed order: the parts' addresses are
+// known at once, so the time is that of a few loads in a row (512 parts of 2 x 1536 columns: 12 us with a quarter a
+// wave).
 __global__ __launch_bounds__(1024) void param_sum_kernel(const float* __restrict__ part, int parts, int n, int split,
                                                          float* __restrict__ out, float* __restrict__ out2) {
   __shared__ float sm[16][64];
@@ -361,7 +368,14 @@ static int check_grid(int64_t blocks, int threads) {
   return FVSR_OK;
 }
 
-// f(waves a row, vectors a lane): one wave up to 2048 channels, 4 up to 8192, 16 up to 16384, with just the registers they need
+// f(waves a row, vectors a lane): one wave up to 2048 channels, 4 up to 8192, 16 up to 16384. Few waves a row share its
+// work with few barriers and wave sums; many leave each lane fewer registers to hold. This rule against 4 waves from
+// 1025 channels and 16 from 4097 (one or two vectors a lane): bf16 17280 x 1536 norm 26.4 us against 31.9, to 8 bits
+// 24.3 against 35.9, gradient from 8 bits 27.5 against 37.7; 4000 x 8192 34.4 against 35.9, 31.9 against 38.6, 33.4
+// against 34.4. It costs fp32 gradients of 4 vectors a lane, which spill 26-61 registers: 8192 x 2048 from x 62.1
+// against 38.2, 4000 x 8192 119 against 73. Above 8192 channels every gradient spills 30-98 (bf16 from 8 bits, 3800 x
+// 8960 104 us, 1.6 TB/s; 2000 x 16384 74, 2.2), and odd rows of 4 vectors a lane run one wave a SIMD (8000 x 2047 24.5,
+// 3.4).
 template <class F>
 static int pick_team(int C, F&& f) {
   const int nv = (int)ceil_div(C, 512);
@@ -448,7 +462,8 @@ int launch_quantize(int dtype, const void* x, int64_t rows, int C, Out8 o, hipSt
   if (const int rc = check_grid(blocks, 256)) return rc;
   auto go = [&](auto t, auto v) {
     using T = decltype(t);
-    hipLaunchKernelGGL((quantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, rows, C, o);
+    hipLaunchKernelGGL((quantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x,
+                       rows, C, o);
   };
   auto with = [&](auto t) { C % 8 == 0 ? go(t, std::true_type{}) : go(t, std::false_type{}); };
   if (dtype == FVSR_DTYPE_BF16) with(bf16{});
@@ -463,7 +478,8 @@ int launch_dequantize(In8 q, int64_t rows, int C, int dtype, void* out, hipStrea
   if (const int rc = check_grid(blocks, 256)) return rc;
   auto go = [&](auto t, auto v) {
     using T = decltype(t);
-    hipLaunchKernelGGL((dequantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, q, rows, C, (T*)out);
+    hipLaunchKernelGGL((dequantize_kernel<T, decltype(v)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, q, rows, C,
+                       (T*)out);
   };
   auto with = [&](auto t) { C % 8 == 0 ? go(t, std::true_type{}) : go(t, std::false_type{}); };
   if (dtype == FVSR_DTYPE_BF16) with(bf16{});
