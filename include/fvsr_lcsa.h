@@ -317,6 +317,74 @@ int fvsr_linear8_weight_grad(fvsr_ctx* ctx, const void* dy, int64_t rows, int ou
                              const void* x_scales, int in_features, int dw_dtype, void* dw, float* db, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ---- (f5) training and serving the self-attention: norm, positions, packed sequences ---------------------------- */
+/* No reference counterpart as such: what is between the projections and the o projection, for a DiT block that is trained, or
+ * serves whole or causal sequences of any lengths. As in (f4): nothing is allocated, memory beside the operands is the caller's
+ * `workspace` (16-byte aligned), calls on one context may overlap and be captured into HIP graphs, the thread's current device
+ * stays, no atomics: the same inputs give the same bits. Outputs must not overlap inputs or each other but where it says so. */
+
+/* Root-mean-square norm of each row, after the residual's addition: s = x + residual rounded to `dtype`, s = x where residual is
+ * NULL; y = s * rstd * weight, rstd = 1 / sqrt(mean(s^2) + eps), in fp32, rounded once. x: rows of `channels`, x_stride elements
+ * apart (>= channels); everything else contiguous. weight (channels) of `param_dtype` (fp32, or the tokens' `dtype`), may be
+ * NULL. Results, each may be NULL but one of y and y_codes: y in `dtype`; y in 8 bits (as fvsr_quantize8, from its fp32 values);
+ * sum, s in `dtype`; rstd, (rows) fp32. y may be x or residual, sum may be x or residual (x then contiguous). channels <= 16384. */
+int fvsr_rms_norm(fvsr_ctx* ctx, int dtype, const void* x, int64_t x_stride, const void* residual, int64_t rows, int channels,
+                  float eps, int param_dtype, const void* weight, void* y, void* y_codes, void* y_scales, void* sum, float* rstd,
+                  void* stream);
+/* Its gradient, of x and of residual alike: with n = s * rstd and g = dy * weight, dx = dsum + rstd * (g - n * mean(g * n)) in
+ * `dtype`, where dsum is the gradient that reached the sum from elsewhere (NULL: none); dweight = sum over the rows of dy * n,
+ * fp32 (channels), or NULL. s (rows s_stride apart) and rstd as the forward call left them. dx may be dy or dsum. */
+size_t fvsr_rms_norm_backward_workspace(int64_t rows, int channels);
+int fvsr_rms_norm_backward(fvsr_ctx* ctx, int dtype, const void* dy, const void* s, int64_t s_stride, const float* rstd,
+                           const void* dsum, int64_t rows, int channels, int param_dtype, const void* weight, void* dx,
+                           float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* (tokens, heads, channels) with contiguous channels: strides in elements, so that q, k and v may be parts of the rows that one
+ * projection wrote. */
+typedef struct fvsr_heads {
+  void* data;
+  int heads;
+  int64_t token_stride, head_stride;
+} fvsr_heads;
+
+/* Rotary positions: of each head (channels wide, even), pair i turns by positions[axis of i][token] * frequencies[i] radians: (a, b)
+ * becomes (a cos - b sin, a sin + b cos), or with `back` (the gradient) (a cos + b sin, b cos - a sin). Pairs are channels (2 i,
+ * 2 i + 1), or with `halves` (i, pairs + i); the first axis_pairs[0] pairs are of axis 0, and so on (1 to 3 axes); channels
+ * past the pairs are copied. Angles in 64 bits (positions below 2^53 in magnitude), the rest in fp32, rounded once. positions:
+ * (axes, tokens), int32, or int64 with positions64; frequencies: (pairs) fp64. k and k_out may be NULL. An output may be its
+ * input. */
+int fvsr_rotary(fvsr_ctx* ctx, int dtype, const fvsr_heads* q, const fvsr_heads* q_out, const fvsr_heads* k,
+                const fvsr_heads* k_out, int64_t tokens, int channels, const void* positions, int positions64,
+                const double* frequencies, int axes, const int32_t* axis_pairs, int halves, int back, void* stream);
+
+/* Sequences packed one behind another. Sequence b has the queries cu_q[b] .. cu_q[b + 1] - 1 of tokens_q and the keys cu_k[b] ..
+ * cu_k[b + 1] - 1 of tokens_k, the first used_k[b] of them where used_k is given (a cache with room for more). Offsets are device
+ * int32 and do not fall; they are read when the kernels run (a captured call follows them), and taken into the tensors' range
+ * where they leave it. Query i of m sees all n keys, or with `causal` the first i + 1 + n - m; one that sees none gives zeros (and an
+ * lse of -inf). `scale` (> 0) multiplies the scores. channels a head: a multiple of 8, at most 128. */
+typedef struct fvsr_packed {
+  const int32_t *cu_q, *cu_k, *used_k;
+  int sequences;
+  int64_t tokens_q, tokens_k;
+  int channels;
+  int causal;
+  float scale;
+} fvsr_packed;
+
+/* o = softmax(scale q k^T) v, bf16; lse (heads, tokens_q) fp32, log(sum exp(scores)), or NULL. k and v have the same heads, q and o a
+ * multiple of them, whose neighbours share one. Data 16-byte and strides 8-element aligned, 128 tokens' strides below 2^31 bytes.
+ * Rows of no sequence are left as they were, or with `clear` zeros (lse -inf). */
+size_t fvsr_packed_attention_workspace(const fvsr_packed* p, int heads, int kv_heads);
+int fvsr_packed_attention(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads* q, const fvsr_heads* k, const fvsr_heads* v,
+                          const fvsr_heads* o, float* lse, int clear, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradient: dq, dk, dv from d_o and what the forward call read and wrote. Keys past used_k, and those that no query sees, have
+ * gradients of zero; rows of no sequence as above. */
+size_t fvsr_packed_attention_backward_workspace(const fvsr_packed* p, int heads, int kv_heads);
+int fvsr_packed_attention_backward(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads* d_o, const fvsr_heads* q,
+                                   const fvsr_heads* k, const fvsr_heads* v, const fvsr_heads* o, const float* lse,
+                                   const fvsr_heads* dq, const fvsr_heads* dk, const fvsr_heads* dv, int clear, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 /* ---- (a1) window layout ------------------------------------------------------------------------------------ */
 /* Replace `windowPartition` / `windowReverse` (DiT.swift:113-126): (f*h*w, C) natural <-> window order. */
 int fvsr_window_partition(int dtype, const void* x, void* out, int f, int h, int w, int channels, void* stream);

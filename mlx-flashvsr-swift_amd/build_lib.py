@@ -19,7 +19,7 @@ LIB = os.path.join(LIB_DIR, "libfvsr_lcsa.so")
 PROBE = os.path.join(LIB_DIR, "fvsr_probe_attn")
 
 SOURCES = ["api.hip", "lcsa_attn.hip", "lcsa_select.hip", "kv_ring.hip", "qkv_epilogue.hip", "dit_block.hip",
-           "rows8.hip", "linear8.hip", "api8.hip"]
+           "rows8.hip", "linear8.hip", "api8.hip", "rms_norm.hip", "rotary.hip", "packed_attn.hip", "api_packed.hip"]
 # Packed-FP32 VALU forms are disabled: hipcc -O3 would otherwise emit v_pk_{add,mul,fma}_f32 from float code.
 # MFMA builtins get the VGPR form (results in VGPRs, where the VALU reads them without v_accvgpr_read); every MFMA
 # of the attention kernels, the output accumulation included, is a compiler builtin.

@@ -1,0 +1,890 @@
+// Attention over packed sequences for gfx950 (MI355X), causal or whole, query heads in groups that share a key and value
+// head, with its gradient.
+//
+//   S = scale Q K^T,  P = softmax(S) over the keys that a query sees,  O = P V,  lse = log(sum exp(S))
+//   delta = sum over channels of dO O,  dP = dO V^T,  dS = P (dP - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO          (dK and dV summed over the group's query heads)
+//
+// Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys from cu_k[b] on. Query i of m sees all n keys, or, causal, the
+// first i + 1 + n - m. The lengths are on the device only: a workgroup finds its sequence from the number of its block (a
+// sequence of m rows takes the slots from cu[b] / rows + b on, rows being the block's, so that slots never collide and the
+// grid is known from the totals).
+//
+// bf16 operands, fp32 sums on v_mfma_f32_32x32x16_bf16: S^T = K Q^T, so a lane owns a query, P packed to bf16 goes
+// straight back in as the operand of O^T += V^T P^T, V^T read transposed from row-major LDS (ds_read_b64_tr_b16). P and dS are
+// rounded to bf16 for those products (off by at most 2^-9 of themselves each); sums of P, the softmax and delta stay fp32.
+#include <algorithm>
+
+#include "attn_tile.hpp"
+#include "packed_attn.hpp"
+#include "teams.hpp"
+
+namespace fvsr {
+namespace {
+
+constexpr int kRows = 128;      // rows of a block: 4 waves of 32
+constexpr int kTile = 32;       // rows of a tile of the other side
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// A tile of 32 rows of HD channels in LDS (D <= HD, zeros past D): rows of 2 HD bytes, whose 16-byte chunks are XOR-swizzled by
+// row so that both reads of a tile spread over all banks: 16 rows of one chunk (ds_read_b128), and 4 neighbouring rows (a
+// multiple of 4 first) of 4 adjacent chunks (ds_read_b64_tr_b16).
+template <int HD>
+struct Tile {
+  static constexpr int kRow = 2 * HD, kBytes = kTile * kRow, kChunks = HD / 8;
+  static constexpr int kCopies = kBytes / 1024, kCopyRows = 1024 / kRow;   // a copy: 64 lanes of 16 bytes
+  static constexpr int kT = HD / 16, kD = HD / 32;                         // products over the channels, blocks of channels
+  static __device__ __forceinline__ int swz(int r) {
+    return HD == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
+  }
+};
+
+// byte offset, for copy p of a tile, of the lane's chunk in rows `stride` bytes apart; past every buffer where the channels
+// are past D
+template <int HD>
+__device__ __forceinline__ int copy_off(int p, int lane, int stride, int D) {
+  using T = Tile<HD>;
+  const int r = p * T::kCopyRows + lane / T::kChunks, chunk = lane % T::kChunks ^ T::swz(r);
+  return chunk * 8 < D ? r * stride + chunk * 16 : (int)0x80000000;
+}
+
+// The buffer of rows row0 .. of a head whose rows end at `end`: what is past it reads as zeros. The base is 64 bits wide, so
+// offsets of long caches do not wrap; 32 rows stay below 2^31 bytes.
+__device__ __forceinline__ u32x4 rows_rsrc(const bf16* base, int64_t stride, int row0, int end, int D) {
+  const int left = min(end - row0, kTile);
+  const uint64_t at = (uint64_t)(base + (int64_t)row0 * stride);
+  const uint32_t bytes = left <= 0 ? 0 : (uint32_t)((left - 1) * (int)stride + D) * 2;
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+
+// the compiler moves no memory access across it
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+// all of this wave's copies have landed, and every wave is past its reads
+__device__ __forceinline__ void wait_and_sync() {
+  fence();
+  FVSR_WAIT_VM_LGKM0(0);
+  __builtin_amdgcn_s_barrier();
+  fence();
+}
+
+// LDS offsets of a lane's operands within a tile
+template <int HD>
+struct Lanes {
+  int row[Tile<HD>::kT];        // A operand of (tile rows) x (channels): row lane % 32, channels 16 t + 8 (lane / 32) ..
+  int tr[2][Tile<HD>::kD];      // A operand of (channels) x (tile rows), transposed: rows 16 u + 8 ab + ..
+  __device__ __forceinline__ Lanes() {
+    using T = Tile<HD>;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, G = lane >> 4, mm = lane & 15;
+#pragma unroll
+    for (int t = 0; t < T::kT; ++t) row[t] = l32 * T::kRow + ((2 * t + g) ^ T::swz(l32)) * 16;
+#pragma unroll
+    for (int ab = 0; ab < 2; ++ab) {
+      const int r = 8 * ab + 4 * (G >> 1) + (mm >> 2);
+#pragma unroll
+      for (int d = 0; d < T::kD; ++d) tr[ab][d] = r * T::kRow + ((4 * d + 2 * (G & 1) + (mm >> 1 & 1)) ^ T::swz(r)) * 16 + (mm & 1) * 8;
+    }
+  }
+};
+
+// (32 tile rows) x (32 columns, one a lane pair): the tile's rows times the lane's row b. Element i of the result is tile row
+// 8 (i / 4) + 4 (lane / 32) + i % 4.
+template <int HD>
+__device__ __forceinline__ f32x16 rows_times(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&b)[Tile<HD>::kT]) {
+  f32x16 s = f32x16{};
+#pragma unroll
+  for (int t = 0; t < Tile<HD>::kT; ++t)
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const lds_bf16x8*)(tile + at.row[t]), b[t], s, 0, 0, 0);
+  return s;
+}
+
+// acc (channels x columns) += tile^T w, w packed from elements laid out as above
+template <int HD>
+__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&w)[2], f32x16 (&acc)[Tile<HD>::kD]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int d = 0; d < Tile<HD>::kD; ++d) {
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr[0][d] + 16 * u * Tile<HD>::kRow));
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr[1][d] + 16 * u * Tile<HD>::kRow));
+      // whole-vector concatenation: element-wise assembly of the operand is mis-lowered (one dword duplicated)
+      const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w[u], acc[d], 0, 0, 0);
+    }
+}
+
+// The same one tile row after another, without those that the lane's column does not see: 0 times an infinity or NaN there
+// would be NaN. `seen`: a bit a tile row. Slow, and reached only where such a value was met.
+template <int HD>
+__device__ __forceinline__ void add_seen(lds_char* tile, const f32x16& w, uint32_t seen, f32x16 (&acc)[Tile<HD>::kD]) {
+  using T = Tile<HD>;
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+  for (int r = 0; r < kTile; ++r) {
+    const int i = (r >> 3) * 4 + (r & 3);
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x = e == i ? w[e] : x;
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float p = __uint_as_float((r >> 2 & 1) ? both[1] : both[0]);   // held by the half of lanes that owns row r
+    const bool see = seen >> r & 1;
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int chunk = 4 * d + c;   // channels 32 d + 8 c + 4 g ..
+        const bf16x4 v = *(const __attribute__((address_space(3))) bf16x4*)(tile + r * T::kRow + (chunk ^ T::swz(r)) * 16 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][4 * c + e] = see ? fmaf(p, (float)v[e], acc[d][4 * c + e]) : acc[d][4 * c + e];
+      }
+  }
+}
+
+// a bit for each tile row from a function of the row
+template <class F>
+__device__ __forceinline__ uint32_t row_bits(F&& f) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int r = 0; r < kTile; ++r) b |= f(r) ? 1u << r : 0;
+  return b;
+}
+
+__device__ __forceinline__ void pack(const f32x16& p, bf16x8 (&w)[2]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (bf16)p[i];
+}
+
+template <int N>
+__device__ __forceinline__ bool any_nan(const f32x16 (&acc)[N]) {
+  bool bad = false;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= acc[d][i] != acc[d][i];
+  return bad;
+}
+
+// the lane's row (channels 16 t + 8 (lane / 32) .. of it) as the other operand; zeros where there is none
+template <int HD>
+__device__ __forceinline__ void load_row(const bf16* row, bool there, int D, bf16x8 (&b)[Tile<HD>::kT]) {
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int t = 0; t < Tile<HD>::kT; ++t) {
+    b[t] = bf16x8{};
+    if (there && 16 * t + 8 * g < D) b[t] = *(const bf16x8*)(row + 16 * t + 8 * g);
+  }
+}
+
+// and back: acc (channels x columns) times `by` into the lane's row
+template <int HD>
+__device__ __forceinline__ void store_row(bf16* row, int D, const f32x16 (&acc)[Tile<HD>::kD], float by) {
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int d = 0; d < Tile<HD>::kD; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int ch = 32 * d + 8 * c;
+      bf16x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (bf16)(acc[d][4 * c + e] * by);
+      if (ch < D) *(bf16x4*)(row + ch + 4 * g) = x;
+    }
+}
+
+// ---- sequences ---------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int within(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// Rows of a sequence, whatever the offsets hold: inside the tensors.
+struct Span {
+  int q0, nq, k0, nk, room;   // room: keys up to the next sequence's, nk of them in use
+};
+__device__ __forceinline__ Span span_of(const PackedArgs& a, int b) {
+  Span s;
+  s.q0 = within(uniform(a.cu_q[b]), 0, a.tq);
+  s.nq = within(uniform(a.cu_q[b + 1]), s.q0, a.tq) - s.q0;
+  s.k0 = within(uniform(a.cu_k[b]), 0, a.tk);
+  s.room = within(uniform(a.cu_k[b + 1]), s.k0, a.tk) - s.k0;
+  s.nk = a.used_k ? within(uniform(a.used_k[b]), 0, s.room) : s.room;
+  return s;
+}
+
+// The block of kRows rows in `slot`: of sequence b (then its first row, `row`, in the sequence), or rows of no sequence: then
+// [lo, hi), which are cleared where the call asks for it.
+struct Block {
+  int b, row;
+  int lo, hi;
+};
+__device__ __forceinline__ Block block_of(const int32_t* cu, int total, int seqs, int slot) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int i = 0; i <= seqs; i += 64) {
+    const bool before = i + lane <= seqs && within(cu[min(i + lane, seqs)], 0, total) / kRows + i + lane <= slot;
+    n += __popcll(__ballot(before));
+  }
+  Block x;
+  x.b = uniform(n) - 1;
+  const int first = within(uniform(cu[max(x.b, 0)]), 0, total);   // of the sequence, or behind the last one
+  x.row = x.b < 0 ? 0 : (slot - (first / kRows + x.b)) * kRows;
+  x.lo = x.hi = 0;
+  if (x.b < 0) {
+    x.lo = slot * kRows;
+    x.hi = min(x.lo + kRows, first);
+  } else if (x.b == seqs) {
+    x.lo = min(first + max(x.row, 0), total);
+    x.hi = min(x.lo + kRows, total);
+  } else if (x.b == 0 && x.row == 0) {   // the rest of the rows before the first sequence
+    x.lo = first / kRows * kRows;
+    x.hi = first;
+  }
+  if (x.row < 0) x.b = seqs;   // offsets that fall: nothing here
+  return x;
+}
+
+__device__ __forceinline__ void clear_rows(HeadView<bf16> o, int head, int lo, int hi, int D) {
+  for (int e = threadIdx.x; e < (hi - lo) * (D / 8); e += blockDim.x)
+    *(u32x4*)(o.p + (int64_t)(lo + e / (D / 8)) * o.t + head * o.h + e % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+}
+
+// the keys that query i of a sequence sees (rows past the last query: as many as that one)
+__device__ __forceinline__ int keys_seen(const PackedArgs& a, const Span& s, int i) {
+  return a.causal ? within(min(i, s.nq - 1) + 1 + s.nk - s.nq, 0, s.nk) : s.nk;
+}
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+// A softmax in progress for the lane's query: reference m (log2 units), sum l of this lane's half of the keys, unnormalised
+// output (channels x queries).
+template <int HD>
+struct Soft {
+  float m, l;
+  f32x16 acc[Tile<HD>::kD];
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < Tile<HD>::kD; ++d) acc[d] = f32x16{};
+  }
+  // a tile of keys k0 .. k0 + 31, of which the lane's query sees those below `lim`
+  template <bool EXACT>
+  __device__ __forceinline__ void tile(lds_char* kt, lds_char* vt, const Lanes<HD>& at, const bf16x8 (&q)[Tile<HD>::kT], int k0,
+                                       int lim, bool masked, float c) {
+    const int g = (threadIdx.x & 63) >> 5;
+    f32x16 s = rows_times<HD>(kt, at, q);
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = k0 + 8 * (i >> 2) + 4 * g + (i & 3) < lim ? s[i] : -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    const float to = fmaxf(m, pair_max(mx) * c);
+    const float ref = to == -INFINITY ? 0.f : to;   // nothing seen yet
+    const float by = __builtin_amdgcn_exp2f(m - ref);
+    m = to;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
+      sum += s[i];
+    }
+    l = fmaf(l, by, sum);
+#pragma unroll
+    for (int d = 0; d < Tile<HD>::kD; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= by;
+    if (EXACT && masked) {
+      add_seen<HD>(vt, s, row_bits([&](int r) { return k0 + r < lim; }), acc);
+    } else {
+      bf16x8 w[2];
+      pack(s, w);
+      add_times<HD>(vt, at, w, acc);
+    }
+  }
+};
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
+  using T = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][K, V]
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
+  // a sequence's last rows, which see most where it is causal, come first
+  const Block blk = block_of(a.cu_q, a.tq, a.seqs, slots - 1 - (int)(blockIdx.x / a.heads));
+  if (a.clear && blk.hi > blk.lo) {
+    clear_rows(a.o, head, blk.lo, blk.hi, a.D);
+    if (a.lse)
+      for (int r = blk.lo + (int)threadIdx.x; r < blk.hi; r += 256) a.lse[(int64_t)head * a.tq + r] = -INFINITY;
+  }
+  if (blk.b < 0 || blk.b >= a.seqs) return;
+  const Span s = span_of(a, blk.b);
+  if (blk.row >= s.nq) return;
+  const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
+  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile;
+
+  bf16x8 q[T::kT];
+  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
+  const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + head / a.group * a.k.h;
+  const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + head / a.group * a.v.h;
+  constexpr int kMine = T::kCopies / 4;   // copies of a tile a wave makes
+  int koff[kMine], voff[kMine];
+#pragma unroll
+  for (int p = 0; p < kMine; ++p) {
+    koff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.k.t * 2, a.D);
+    voff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.v.t * 2, a.D);
+  }
+  const uint32_t base = lds_addr(smem);
+  lds_char* const lds = (lds_char*)(uintptr_t)base;
+  auto issue = [&](int t) {
+    const u32x4 kr = rows_rsrc(kb, a.k.t, t * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, t * kTile, s.nk, a.D);
+    const uint32_t to = base + (t & 1) * 2 * T::kBytes + wave * kMine * 1024;
+    static_for<0, kMine>([&](auto p) {
+      dma16<p * 1024>(kr, to, koff[p], 0);
+      dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
+    });
+  };
+  const Lanes<HD> at;
+  Soft<HD> soft;
+  auto walk = [&](auto exact) {
+    soft.clear();
+    if (tiles > 0) issue(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_and_sync();
+      if (t + 1 < tiles) issue(t + 1);
+      lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
+      if (t * kTile < lim_max)
+        soft.template tile<decltype(exact)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, t * kTile + kTile > lim_min, a.c);
+    }
+    wait_and_sync();
+  };
+  walk(std::false_type{});
+  // An infinity or NaN in a key's V that a row of its tile does not see makes that row NaN. Where a result is NaN, the walk is
+  // done again with those tiles' products without what is not seen.
+  if (a.causal && __syncthreads_or(any_nan(soft.acc))) walk(std::true_type{});
+  if (i >= s.nq) return;
+  const float l = pair_sum(soft.l);
+  store_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, a.D, soft.acc, l == 0.f ? 0.f : 1.f / l);
+  if (a.lse && g == 0)
+    a.lse[(int64_t)head * a.tq + s.q0 + i] = l == 0.f ? -INFINITY : (soft.m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- few queries a sequence: the keys split over the workgroups ------------------------------------------------------------
+// A row is (query, head of the group), 32 to an item, so that K and V are read once for a group. All items' tiles of 32 keys
+// stand in one order (sequence, key head, item, tile) and are cut into equal parts, one a workgroup, whatever the lengths are:
+// a part begins and ends inside items, whose results it leaves for packed_join_kernel, and finishes those in between. Of an
+// item's tiles each of the 4 waves takes every fourth, with a ring of its own and no barrier.
+struct Parts {
+  int work, parts;   // tiles of all items; workgroups that share them
+  __device__ __forceinline__ int begin(int w) const { return (int)((int64_t)work * w / parts); }
+  __device__ __forceinline__ int owner(int tile) const { return (int)((((int64_t)tile + 1) * parts - 1) / work); }
+};
+__device__ __forceinline__ int items_of(const PackedArgs& a, const Span& s) { return (s.nq * a.group + kTile - 1) / kTile; }
+__device__ __forceinline__ int tiles_of(const Span& s) { return max(1, (s.nk + kTile - 1) / kTile); }
+__device__ __forceinline__ Span lane_span(const PackedArgs& a, int b) {   // span_of, for a sequence of the lane's own
+  Span s;
+  s.q0 = within(a.cu_q[b], 0, a.tq);
+  s.nq = within(a.cu_q[b + 1], s.q0, a.tq) - s.q0;
+  s.k0 = within(a.cu_k[b], 0, a.tk);
+  s.room = within(a.cu_k[b + 1], s.k0, a.tk) - s.k0;
+  s.nk = a.used_k ? within(a.used_k[b], 0, s.room) : s.room;
+  return s;
+}
+
+constexpr int kMinTiles = 8;          // tiles a part, at the least: two a wave
+constexpr int kMostWork = 1 << 30;    // tiles of a call (split)
+
+// The parts, and for the tile `of(parts)` its sequence and that one's first tile. Called by the whole workgroup of 256;
+// `sm` is LDS for 12 ints. The sequence is -1 where there is no such tile. Offsets that fall could make sequences overlap and
+// their work pass 31 bits: none is done then.
+template <class F>
+__device__ __forceinline__ Parts find_tile(const PackedArgs& a, int* sm, F&& of, int& tile, int& b, int& first) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.seqs + 255) / 256, b0 = min(tid * per, a.seqs), b1 = min(b0 + per, a.seqs);
+  auto work_of = [&](int i) {
+    const Span s = lane_span(a, i);
+    return items_of(a, s) * tiles_of(s) * a.kv_heads;
+  };
+  int mine = 0;
+  float about = 0.f;
+  for (int i = b0; i < b1; ++i) {
+    const int n = work_of(i);
+    mine += n;
+    about += (float)n;
+  }
+  about = wave_sum(about);
+  int at = wave_scan_dpp(mine);
+  if (lane == 63) {
+    sm[wave] = at;
+    sm[8 + wave] = __float_as_int(about);
+  }
+  if (tid == 0) sm[4] = -1;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) at += sm[w];
+  at -= mine;
+  Parts p;
+  p.work = uniform(sm[0] + sm[1] + sm[2] + sm[3]);
+  about = __int_as_float(sm[8]) + __int_as_float(sm[9]) + __int_as_float(sm[10]) + __int_as_float(sm[11]);
+  if (about > 1.5f * kMostWork) p.work = 0;
+  p.parts = max(1, min(a.max_parts, p.work / kMinTiles));
+  tile = p.work > 0 ? of(p) : -1;
+  if (tile >= at && tile < at + mine) {
+    for (int i = b0; i < b1; ++i) {
+      const int n = work_of(i);
+      if (tile < at + n) {
+        sm[4] = i;
+        sm[5] = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  b = uniform(sm[4]);
+  first = uniform(sm[5]);
+  __syncthreads();
+  return p;
+}
+
+// partial results: of slot x, 32 rows of HD floats, then the rows' references and sums
+template <int HD>
+struct Partial {
+  static constexpr int kFloats = kTile * HD + 2 * kTile;
+};
+
+template <int HD>
+__global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
+  using T = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char smem[4][4 * T::kBytes];   // [wave][buffer][K, V]
+  __shared__ float ml[4][2][kTile];
+  __shared__ int sm[12];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(tid >> 6);
+  if (a.clear) {   // rows of no sequence, a head a turn
+    const int lo = within(uniform(a.cu_q[0]), 0, a.tq), hi = within(uniform(a.cu_q[a.seqs]), lo, a.tq);
+    for (int h = blockIdx.x; h < a.heads; h += gridDim.x) {
+      clear_rows(a.o, h, 0, lo, a.D);
+      clear_rows(a.o, h, hi, a.tq, a.D);
+      if (a.lse)
+        for (int r = tid; r < a.tq; r += 256)
+          if (r < lo || r >= hi) a.lse[(int64_t)h * a.tq + r] = -INFINITY;
+    }
+  }
+  int tile, b, first;
+  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return (int)blockIdx.x < p.parts ? p.begin(blockIdx.x) : -1; }, tile, b, first);
+  if (b < 0) return;
+  const int begin = tile, end = parts.begin(blockIdx.x + 1);
+  const uint32_t base = lds_addr(smem[wave]);
+  lds_char* const lds = (lds_char*)(uintptr_t)base;
+  const Lanes<HD> at;
+  int koff[T::kCopies], voff[T::kCopies];
+#pragma unroll
+  for (int p = 0; p < T::kCopies; ++p) {
+    koff[p] = copy_off<HD>(p, lane, (int)a.k.t * 2, a.D);
+    voff[p] = copy_off<HD>(p, lane, (int)a.v.t * 2, a.D);
+  }
+  Span s = span_of(a, b);
+  for (; tile < end;) {
+    int items = items_of(a, s), tiles = tiles_of(s);
+    while (tile - first >= items * tiles * a.kv_heads) {   // on to the next sequence; there is one, since tile < end <= work
+      first += items * tiles * a.kv_heads;
+      s = span_of(a, ++b);
+      items = items_of(a, s);
+      tiles = tiles_of(s);
+    }
+    const int unit = (tile - first) / tiles, t0 = (tile - first) - unit * tiles, t1 = min(tiles, t0 + end - tile);
+    const int hk = unit / items, r0 = (unit - hk * items) * kTile, rows = s.nq * a.group;
+    // the lane's row: query i, head h
+    const int r = r0 + l32, i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) % a.group;
+    const int lim = keys_seen(a, s, i), lim_min = keys_seen(a, s, r0 / a.group);
+    bf16x8 q[T::kT];
+    load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + h * a.q.h, r < rows, a.D, q);
+    const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + hk * a.k.h;
+    const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + hk * a.v.h;
+    auto issue = [&](int t, int buf) {
+      const u32x4 kr = rows_rsrc(kb, a.k.t, t * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, t * kTile, s.nk, a.D);
+      const uint32_t to = base + buf * 2 * T::kBytes;
+      static_for<0, T::kCopies>([&](auto p) { dma16<p * 1024>(kr, to, koff[p], 0); });
+      static_for<0, T::kCopies>([&](auto p) { dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0); });
+    };
+    Soft<HD> soft;
+    auto walk = [&](auto exact) {
+      soft.clear();
+      int buf = 0;
+      if (t0 + wave < t1) issue(t0 + wave, 0);
+      for (int t = t0 + wave; t < t1; t += 4, buf ^= 1) {
+        if (t + 4 < t1) {
+          issue(t + 4, buf ^ 1);
+          FVSR_WAIT_VM_LGKM0(2 * T::kCopies);
+        } else {
+          FVSR_WAIT_VM_LGKM0(0);
+        }
+        fence();
+        lds_char* const kt = lds + buf * 2 * T::kBytes;
+        soft.template tile<decltype(exact)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, t * kTile + kTile > lim_min, a.c);
+        fence();
+        FVSR_WAIT_VM_LGKM0(63);   // its reads are done before the next copies into this buffer
+      }
+    };
+    walk(std::false_type{});
+    if (a.causal && __ballot(any_nan(soft.acc)) != 0) walk(std::true_type{});   // as in packed_forward_kernel
+    // the waves' results meet in LDS: each its rows x channels in its own ring
+    {
+      const float l = pair_sum(soft.l);
+      if (g == 0) {
+        ml[wave][0][l32] = soft.m;
+        ml[wave][1][l32] = l;
+      }
+      float* const mine = (float*)smem[wave];
+#pragma unroll
+      for (int d = 0; d < T::kD; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {   // 16-byte pieces of a row, XOR-swizzled by row
+          const int piece = (8 * d + 2 * c + g) ^ (l32 & 7);
+          *(f32x4*)(mine + l32 * HD + 4 * piece) = f32x4{soft.acc[d][4 * c], soft.acc[d][4 * c + 1], soft.acc[d][4 * c + 2], soft.acc[d][4 * c + 3]};
+        }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == tiles;
+    float* const part = a.part + (int64_t)(2 * blockIdx.x + (tile == begin ? 0 : 1)) * Partial<HD>::kFloats;
+    const int here = min(kTile, rows - r0);
+    for (int e = tid; e < here * (HD / 4); e += 256) {
+      const int row = e / (HD / 4), piece = e % (HD / 4);
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][0][row]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float by = __builtin_amdgcn_exp2f(ml[w][0][row] - ref), lw = ml[w][1][row];
+        if (lw == 0.f) continue;   // a wave without keys for the row
+        l = fmaf(lw, by, l);
+        const f32x4 y = *(const f32x4*)((const float*)smem[w] + row * HD + 4 * (piece ^ (row & 7)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(y[j], by, x[j]);
+      }
+      if (whole) {
+        const int qi = (r0 + row) / a.group, qh = hk * a.group + (r0 + row) % a.group;
+        const float by = l == 0.f ? 0.f : 1.f / l;
+        if (4 * piece < a.D) {
+          bf16x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = (bf16)(x[j] * by);
+          *(bf16x4*)(a.o.p + (int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + 4 * piece) = o;
+        }
+        if (a.lse && piece == 0)
+          a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+      } else {
+        *(f32x4*)(part + row * HD + 4 * piece) = x;
+        if (piece == 0) {
+          part[kTile * HD + row] = m;
+          part[kTile * HD + kTile + row] = l;
+        }
+      }
+    }
+    __syncthreads();
+    tile += t1 - t0;
+  }
+}
+
+// Workgroup (x, y): the item cut by part x + 1's beginning, if that is the item's first cut; 256 of its rows' channels.
+template <int HD>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
+  __shared__ int sm[12];
+  int tile, b, first;
+  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return (int)blockIdx.x + 1 < p.parts ? p.begin(blockIdx.x + 1) : -1; }, tile, b, first);
+  if (b < 0) return;
+  const Span s = span_of(a, b);
+  const int items = items_of(a, s), tiles = tiles_of(s);
+  const int unit = (tile - first) / tiles, begin = first + unit * tiles;
+  if (begin == tile || parts.owner(begin) != (int)blockIdx.x) return;   // no cut, or not the first one
+  const int last = parts.owner(begin + tiles - 1), hk = unit / items, r0 = (unit - hk * items) * kTile;
+  const int row = ((int)blockIdx.y * 256 + (int)threadIdx.x) / HD, ch = threadIdx.x % HD;
+  if (row >= min(kTile, s.nq * a.group - r0)) return;
+  auto part = [&](int w) {
+    return a.part + (int64_t)(2 * w + (w == (int)blockIdx.x && parts.begin(w) < begin ? 1 : 0)) * Partial<HD>::kFloats;
+  };
+  float m = -INFINITY;
+  for (int w = blockIdx.x; w <= last; ++w) m = fmaxf(m, part(w)[kTile * HD + row]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, x = 0.f;
+#pragma unroll 4
+  for (int w = blockIdx.x; w <= last; ++w) {
+    const float* p = part(w);
+    const float by = __builtin_amdgcn_exp2f(p[kTile * HD + row] - ref), lw = p[kTile * HD + kTile + row];
+    l = lw == 0.f ? l : fmaf(lw, by, l);
+    x = lw == 0.f ? x : fmaf(p[row * HD + ch], by, x);
+  }
+  const int qi = (r0 + row) / a.group, qh = hk * a.group + (r0 + row) % a.group;
+  if (ch < a.D) a.o.p[(int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + ch] = (bf16)(l == 0.f ? 0.f : x / l);
+  if (a.lse && ch == 0) a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------
+// Two kernels, so that nothing is added with atomics: dQ walks over the keys like the forward pass (and leaves delta), dK and dV
+// walk over the queries of the group's heads. Each makes S and dP again: 7 products in all where one kernel would make 5.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
+  using T = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][K, V]
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
+  const Block blk = block_of(a.cu_q, a.tq, a.seqs, slots - 1 - (int)(blockIdx.x / a.heads));
+  if (a.clear && blk.hi > blk.lo) clear_rows(a.dq, head, blk.lo, blk.hi, a.D);
+  if (blk.b < 0 || blk.b >= a.seqs) return;
+  const Span s = span_of(a, blk.b);
+  if (blk.row >= s.nq) return;
+  const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
+  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile;
+
+  bf16x8 q[T::kT], d_o[T::kT];
+  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
+  load_row<HD>(a.d_o.p + (int64_t)(s.q0 + i) * a.d_o.t + head * a.d_o.h, i < s.nq, a.D, d_o);
+  float lse2 = 0.f, delta = 0.f;
+  {
+    bf16x8 o[T::kT];
+    load_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, i < s.nq, a.D, o);
+#pragma unroll
+    for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)d_o[t][e], (float)o[t][e], delta);
+    delta = pair_sum(delta);
+    if (i < s.nq) {
+      const int64_t at = (int64_t)head * a.tq + s.q0 + i;
+      lse2 = a.lse[at] * kLog2e;
+      if (g == 0) a.delta[at] = delta;
+    }
+  }
+  const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + head / a.group * a.k.h;
+  const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + head / a.group * a.v.h;
+  constexpr int kMine = T::kCopies / 4;
+  int koff[kMine], voff[kMine];
+#pragma unroll
+  for (int p = 0; p < kMine; ++p) {
+    koff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.k.t * 2, a.D);
+    voff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.v.t * 2, a.D);
+  }
+  const uint32_t base = lds_addr(smem);
+  lds_char* const lds = (lds_char*)(uintptr_t)base;
+  auto issue = [&](int t) {
+    const u32x4 kr = rows_rsrc(kb, a.k.t, t * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, t * kTile, s.nk, a.D);
+    const uint32_t to = base + (t & 1) * 2 * T::kBytes + wave * kMine * 1024;
+    static_for<0, kMine>([&](auto p) {
+      dma16<p * 1024>(kr, to, koff[p], 0);
+      dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
+    });
+  };
+  const Lanes<HD> at;
+  f32x16 acc[T::kD];
+  auto walk = [&](auto exact) {
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
+    if (tiles > 0) issue(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_and_sync();
+      if (t + 1 < tiles) issue(t + 1);
+      lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
+      const int k0 = t * kTile;
+      if (k0 >= lim_max) continue;
+      const bool masked = k0 + kTile > lim_min;
+      f32x16 p = rows_times<HD>(kt, at, q);
+      f32x16 dp = rows_times<HD>(kt + T::kBytes, at, d_o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(fmaf(p[e], a.c, -lse2)) * (dp[e] - delta);
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = k0 + 8 * (e >> 2) + 4 * g + (e & 3) < lim ? dp[e] : 0.f;
+      }
+      if (decltype(exact)::value && masked) {
+        add_seen<HD>(kt, dp, row_bits([&](int r) { return k0 + r < lim; }), acc);
+      } else {
+        bf16x8 w[2];
+        pack(dp, w);
+        add_times<HD>(kt, at, w, acc);
+      }
+    }
+    wait_and_sync();
+  };
+  walk(std::false_type{});
+  if (a.causal && __syncthreads_or(any_nan(acc))) walk(std::true_type{});
+  if (i < s.nq) store_row<HD>(a.dq.p + (int64_t)(s.q0 + i) * a.dq.t + head * a.dq.h, a.D, acc, a.scale);
+}
+
+template <int HD>
+__global__ __launch_bounds__(256, 1) void packed_dkv_kernel(PackedArgs a) {
+  using T = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][Q, dO]
+  __shared__ __attribute__((aligned(16))) float stat[4][2][kTile];      // [wave][lse (log2 units), delta] of a tile's queries
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int hk = blockIdx.x % a.kv_heads;
+  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.kv_heads);   // the first keys, which most queries see, first
+  if (a.clear && blk.hi > blk.lo) {
+    clear_rows(a.dk, hk, blk.lo, blk.hi, a.D);
+    clear_rows(a.dv, hk, blk.lo, blk.hi, a.D);
+  }
+  if (blk.b < 0 || blk.b >= a.seqs) return;
+  const Span s = span_of(a, blk.b);
+  if (blk.row >= s.room) return;
+  const int j0 = blk.row + wave * 32, j = j0 + l32;
+  const int off = s.nk - s.nq;   // causal: query i sees keys j <= i + off
+  // tiles of queries; none for keys that are not in use
+  const int tiles = blk.row < s.nk ? (s.nq + kTile - 1) / kTile : 0;
+  const int t0 = a.causal ? min(tiles, max(0, blk.row - off) / kTile) : 0;
+  const int steps = (tiles - t0) * a.group;
+
+  bf16x8 k[T::kT], v[T::kT];
+  load_row<HD>(a.k.p + (int64_t)(s.k0 + j) * a.k.t + hk * a.k.h, j < s.nk, a.D, k);
+  load_row<HD>(a.v.p + (int64_t)(s.k0 + j) * a.v.t + hk * a.v.h, j < s.nk, a.D, v);
+  constexpr int kMine = T::kCopies / 4;
+  int qoff[kMine], ooff[kMine];
+#pragma unroll
+  for (int p = 0; p < kMine; ++p) {
+    qoff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.q.t * 2, a.D);
+    ooff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.d_o.t * 2, a.D);
+  }
+  const uint32_t base = lds_addr(smem);
+  lds_char* const lds = (lds_char*)(uintptr_t)base;
+  auto issue = [&](int h, int t, int buf) {
+    const bf16* const qb = a.q.p + (int64_t)s.q0 * a.q.t + h * a.q.h;
+    const bf16* const ob = a.d_o.p + (int64_t)s.q0 * a.d_o.t + h * a.d_o.h;
+    const u32x4 qr = rows_rsrc(qb, a.q.t, t * kTile, s.nq, a.D), dr = rows_rsrc(ob, a.d_o.t, t * kTile, s.nq, a.D);
+    const uint32_t to = base + buf * 2 * T::kBytes + wave * kMine * 1024;
+    static_for<0, kMine>([&](auto p) {
+      dma16<p * 1024>(qr, to, qoff[p], 0);
+      dma16<p * 1024>(dr, to + T::kBytes, ooff[p], 0);
+    });
+  };
+  // lanes 0-31: lse, lanes 32-63: delta, of the tile's queries
+  auto stat_of = [&](int h, int t) {
+    const int64_t at = (int64_t)h * a.tq + s.q0 + min(t * kTile + l32, s.nq - 1);
+    return g ? a.delta[at] : a.lse[at] * kLog2e;
+  };
+  const Lanes<HD> at;
+  f32x16 dk[T::kD], dv[T::kD];
+  auto walk = [&](auto exact) {
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d) dk[d] = dv[d] = f32x16{};
+    int h = hk * a.group, t = t0;
+    float next = 0.f;
+    if (steps > 0) {
+      issue(h, t, 0);
+      next = stat_of(h, t);
+    }
+    for (int n = 0; n < steps; ++n) {
+      wait_and_sync();
+      const int q0 = t * kTile;
+      stat[wave][g][l32] = next;
+      if (++t == tiles) {
+        t = t0;
+        ++h;
+      }
+      if (n + 1 < steps) {
+        issue(h, t, (n + 1) & 1);
+        next = stat_of(h, t);
+      }
+      lds_char* const qt = lds + (n & 1) * 2 * T::kBytes;
+      lds_char* const ot = qt + T::kBytes;
+      const bool causal_edge = a.causal && j0 + 31 > q0 + off, masked = causal_edge || q0 + kTile > s.nq;
+      if (a.causal && j0 > q0 + 31 + off) continue;   // no query of the tile sees a key of the wave
+      auto sees = [&](int r) { return q0 + r < s.nq && (!a.causal || j <= q0 + r + off); };
+      f32x16 p = rows_times<HD>(qt, at, k);
+      f32x16 ds = rows_times<HD>(ot, at, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const f32x4 lse2 = *(const f32x4*)&stat[wave][0][8 * c + 4 * g], delta = *(const f32x4*)&stat[wave][1][8 * c + 4 * g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(p[4 * c + e], a.c, -lse2[e]));
+          p[4 * c + e] = x;
+          ds[4 * c + e] = x * (ds[4 * c + e] - delta[e]);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool see = sees(8 * (e >> 2) + 4 * g + (e & 3));
+          p[e] = see ? p[e] : 0.f;
+          ds[e] = see ? ds[e] : 0.f;
+        }
+      }
+      if (decltype(exact)::value && masked) {
+        const uint32_t seen = row_bits(sees);
+        add_seen<HD>(ot, p, seen, dv);
+        add_seen<HD>(qt, ds, seen, dk);
+      } else {
+        bf16x8 w[2];
+        pack(p, w);
+        add_times<HD>(ot, at, w, dv);
+        pack(ds, w);
+        add_times<HD>(qt, at, w, dk);
+      }
+    }
+    wait_and_sync();
+  };
+  walk(std::false_type{});
+  if (a.causal && __syncthreads_or(any_nan(dk) || any_nan(dv))) walk(std::true_type{});
+  if (j >= s.room) return;
+  if (j >= s.nk) {   // not in use: seen by none
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d) dk[d] = dv[d] = f32x16{};
+  }
+  store_row<HD>(a.dk.p + (int64_t)(s.k0 + j) * a.dk.t + hk * a.dk.h, a.D, dk, a.scale);
+  store_row<HD>(a.dv.p + (int64_t)(s.k0 + j) * a.dv.t + hk * a.dv.h, a.D, dv, 1.f);
+}
+
+int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
+
+constexpr int kMaxParts = 256;   // workgroups of the split walk: its rings leave room for one on a compute unit
+
+// Whether the keys are split over the workgroups: where there are few queries a sequence, so that a block of 128 rows would be
+// mostly empty, and the lengths' products stay below kMostWork.
+bool split(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
+  const int64_t group = heads / kv_heads;
+  if (tq * group > (int64_t)64 * seqs) return false;
+  return (ceil_div(tq * group, kTile) + seqs) * (ceil_div(tk, kTile) + seqs) * kv_heads < kMostWork;
+}
+
+}  // namespace
+
+size_t packed_forward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D) {
+  if (!split(seqs, tq, tk, heads, kv_heads)) return 0;
+  return (size_t)2 * kMaxParts * (D <= 64 ? Partial<64>::kFloats : Partial<128>::kFloats) * sizeof(float);
+}
+
+int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
+  auto go = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    if (split(a.seqs, a.tq, a.tk, a.heads, a.kv_heads)) {
+      a.part = (float*)ws;
+      a.max_parts = kMaxParts;
+      hipLaunchKernelGGL((packed_split_kernel<HD>), dim3(kMaxParts), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(kMaxParts - 1, kTile * HD / 256), dim3(256), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((packed_forward_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
+    }
+  };
+  if (a.D <= 64) go(std::integral_constant<int, 64>{});
+  else go(std::integral_constant<int, 128>{});
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+size_t packed_backward_workspace(int64_t tq, int heads) { return (size_t)tq * heads * sizeof(float); }
+
+int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {
+  a.delta = (float*)ws;
+  auto go = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3((unsigned)(slots(a.tk, a.seqs) * a.kv_heads)), dim3(256), 0, stream, a);
+  };
+  if (a.D <= 64) go(std::integral_constant<int, 64>{});
+  else go(std::integral_constant<int, 128>{});
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+}  // namespace fvsr

@@ -1,0 +1,281 @@
+// Root-mean-square norm of tokens with the residual's addition before it, and its gradient, for gfx950 (MI355X).
+//
+//   s  = x + residual (rounded to the tokens' type, as the next layers read it; x itself without a residual)
+//   y  = n w,  n = s rstd,  rstd = 1 / sqrt(mean(s^2) + eps)               (the mean over the row's C channels)
+//   dx = ds + rstd (g - n mean(g n)),  g = dy w;  the same for both addends
+//   dw = sum over rows of dy n
+//
+// Each row moves once and stays in registers between the pass that sums and the one that writes, in 32 bits: memory-bound.
+// A row belongs to a team: 16 lanes up to 128 channels (a head's width), a wave, 4 or 16 waves beyond.
+#include <algorithm>
+
+#include "blocks8.hpp"
+#include "teams.hpp"
+
+namespace fvsr {
+
+int launch_param_sum(const float* part, int parts, int n, int split, float* out, float* out2, hipStream_t stream);
+
+struct RmsArgs {
+  const void* x;
+  int64_t x_stride;      // elements between x's rows
+  const void* r;         // residual, may be null
+  int64_t rows;
+  int C;
+  float eps;
+  const void* w;         // may be null
+  void* y;               // null: not written
+  Out8 y8;               // codes null: not written
+  void* s;               // null: not written
+  float* rstd;           // may be null
+};
+
+struct RmsGradArgs {
+  const void *dy, *s;
+  int64_t s_stride;
+  const float* rstd;
+  const void* ds;        // may be null
+  int64_t rows;
+  int C;
+  const void* w;         // may be null
+  void* dx;
+  float* part;           // (blocks, C) partial dw; null: not made
+};
+
+// lanes of a team, teams of a workgroup, threads of a workgroup
+template <int WAVES>
+struct Team {
+  static constexpr int kLanes = WAVES == 0 ? 16 : 64 * WAVES;
+  static constexpr int kThreads = WAVES <= 1 ? 256 : 64 * WAVES;
+  static constexpr int kTeams = kThreads / kLanes;
+  static constexpr int kRuns = kLanes / 16;   // runs of 128 channels that the team's j-th vectors cover
+};
+
+template <typename T, typename P, bool EIGHTS, int WAVES, int NV>
+__global__ __launch_bounds__(Team<WAVES>::kThreads) void rms_norm_kernel(RmsArgs a) {
+  using W = Team<WAVES>;
+  __shared__ float sm[WAVES > 1 ? WAVES : 1];
+  const int l16 = threadIdx.x & 15, C = a.C;
+  const int64_t row = (int64_t)blockIdx.x * W::kTeams + threadIdx.x / W::kLanes;
+  if (row >= a.rows) return;   // whole teams; never where a workgroup is one team
+  const int run0 = (int)(threadIdx.x % W::kLanes) >> 4;
+  const int runs = runs_of(C), ss = scale_stride(C);
+  const T* x = (const T*)a.x + row * a.x_stride;
+  Raw8<T> rx[NV], rr[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c0 = (run0 + W::kRuns * j) * kRun;
+    rx[j] = load_raw8<T, EIGHTS>(x, c0, l16, C);
+    if (a.r) rr[j] = load_raw8<T, EIGHTS>((const T*)a.r + row * C, c0, l16, C);
+  }
+  float v[NV][8];
+  float sq = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[j][e] = (float)rx[j].v[e];
+      if (a.r) v[j][e] = (float)(T)(v[j][e] + (float)rr[j].v[e]);
+      sq = fmaf(v[j][e], v[j][e], sq);
+    }
+    if (a.s) store8<T, EIGHTS>((T*)a.s + row * C, (run0 + W::kRuns * j) * kRun + l16 * 8, 0, C, v[j]);
+  }
+  const float rstd = 1.f / sqrtf(team_sum<WAVES>(sq, sm) / (float)C + a.eps);
+  if (a.rstd && threadIdx.x % W::kLanes == 0) a.rstd[row] = rstd;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int run = run0 + W::kRuns * j;
+    float w[8], y[8];
+    if (a.w) load8<P, EIGHTS>((const P*)a.w, run * kRun, l16, C, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = v[j][e] * rstd;
+      if (a.w) y[e] *= w[e];
+      if (run * kRun + l16 * 8 + e >= C) y[e] = 0.f;   // also where the row's rstd is not finite
+    }
+    if (a.y) store8<T, EIGHTS>((T*)a.y + row * C, run * kRun + l16 * 8, 0, C, y);
+    if (a.y8.codes) {
+      uint32_t s;
+      const uint2 c = encode8(y, s);
+      if (run < runs) store_codes(a.y8.codes + (row * runs + run) * kRun, l16, c);
+      if (WAVES > 0) {
+        if (run < ss && l16 == 0) a.y8.scales[row * ss + run] = run < runs ? (uint8_t)s : 0;
+      } else if (l16 == 0) {   // one run: the whole word of scales
+        *(uint32_t*)(a.y8.scales + row * ss) = s;
+      }
+    }
+  }
+}
+
+// Teams walk over the rows (the grid is a fixed number of workgroups), the next row on its way while one is worked on, and
+// keep their part of dw in registers; the workgroup's sum goes to `part`, and param_sum_kernel (rows8.hip) adds those up in a
+// fixed order: no atomics, the same result every time.
+template <typename T, typename P, bool EIGHTS, int WAVES, int NV, bool DS>
+__global__ __launch_bounds__(Team<WAVES>::kThreads, EIGHTS && WAVES < 16 ? 2 : 1) void rms_norm_grad_kernel(RmsGradArgs a) {
+  using W = Team<WAVES>;
+  __shared__ float sm[2][WAVES > 1 ? WAVES : 1];
+  __shared__ float join[W::kTeams > 1 ? W::kTeams * W::kLanes * 8 : 1];
+  const int l16 = threadIdx.x & 15, C = a.C;
+  const int team = threadIdx.x / W::kLanes, lane = threadIdx.x % W::kLanes, run0 = lane >> 4;
+  auto first = [&](int j) { return (run0 + W::kRuns * j) * kRun; };
+  float w[NV][8], dw[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (a.w) load8<P, EIGHTS>((const P*)a.w, first(j), l16, C, w[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!a.w) w[j][e] = 1.f;
+      dw[j][e] = 0.f;
+    }
+  }
+  Raw8<T> rdy[NV], rs[NV], rds[NV];
+  float rstd = 0.f;
+  auto load = [&](int64_t row) {
+    rstd = a.rstd[row];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      rdy[j] = load_raw8<T, EIGHTS>((const T*)a.dy + row * C, first(j), l16, C);
+      rs[j] = load_raw8<T, EIGHTS>((const T*)a.s + row * a.s_stride, first(j), l16, C);
+      if constexpr (DS) rds[j] = load_raw8<T, EIGHTS>((const T*)a.ds + row * C, first(j), l16, C);
+    }
+  };
+  int turn = 0;
+  const int64_t step = (int64_t)gridDim.x * W::kTeams;
+  int64_t row = (int64_t)blockIdx.x * W::kTeams + team;
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step, turn ^= 1) {
+    const float r = rstd;
+    float dy[NV][8], n[NV][8], ds[DS ? NV : 1][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dy[j][e] = (float)rdy[j].v[e];
+        n[j][e] = (float)rs[j].v[e];
+        if constexpr (DS) ds[j][e] = (float)rds[j].v[e];
+      }
+    if (row + step < a.rows) load(row + step);
+    float s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      // past the row's end dy and s are 0, and n has to be 0 too where rstd is not finite
+      const bool past = j == NV - 1 && first(j) + l16 * 8 >= C;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        n[j][e] *= r;
+        if (past || (!EIGHTS && first(j) + l16 * 8 + e >= C)) n[j][e] = 0.f;
+        s2 = fmaf(dy[j][e] * w[j][e], n[j][e], s2);
+        dw[j][e] = fmaf(dy[j][e], n[j][e], dw[j][e]);
+      }
+    }
+    const float m2 = team_sum<WAVES>(s2, sm[turn]) / (float)C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float dx[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dx[e] = r * (dy[j][e] * w[j][e] - n[j][e] * m2);
+        if constexpr (DS) dx[e] += ds[j][e];
+      }
+      store8<T, EIGHTS>((T*)a.dx + row * C, first(j) + l16 * 8, 0, C, dx);
+    }
+  }
+  if (!a.part) return;
+  float* const part = a.part + (int64_t)blockIdx.x * C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (W::kTeams > 1) {   // the teams hold the same channels: their sums meet in LDS
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) join[(team * 8 + e) * W::kLanes + lane] = dw[j][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < 8 * W::kLanes; i += W::kThreads) {   // element i / kLanes of lane i % kLanes
+        float s = 0.f;
+#pragma unroll
+        for (int t = 0; t < W::kTeams; ++t) s += join[t * 8 * W::kLanes + i];
+        const int l = i % W::kLanes, c = ((l >> 4) + W::kRuns * j) * kRun + (l & 15) * 8 + i / W::kLanes;
+        if (c < C) part[c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (first(j) + l16 * 8 + e < C) part[first(j) + l16 * 8 + e] = dw[j][e];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// launches
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kRmsGradBlocks = 512;   // two workgroups a CU
+
+// f(waves a row, vectors a lane). `wide`: up to 4 vectors a lane, else 2
+template <class F>
+static int pick_rms_team(int C, bool wide, F&& f) {
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  using I4 = std::integral_constant<int, 4>;
+  using I16 = std::integral_constant<int, 16>;
+  if (C <= 128) f(I0{}, I1{});
+  else if (C <= 512) f(I1{}, I1{});
+  else if (C <= 1024) f(I1{}, I2{});
+  else if (wide && C <= 1536) f(I1{}, I3{});
+  else if (wide && C <= 2048) f(I1{}, I4{});
+  else if (C <= 2048) f(I4{}, I1{});
+  else if (C <= 4096) f(I4{}, I2{});
+  else if (wide && C <= 6144) f(I4{}, I3{});
+  else if (wide && C <= 8192) f(I4{}, I4{});
+  else if (C <= 8192) f(I16{}, I1{});
+  else f(I16{}, I2{});
+  FVSR_HIP_CHECK(hipGetLastError());
+  return FVSR_OK;
+}
+
+// f(element type, parameter type, whether rows are read and written by whole vectors of 8)
+template <class F>
+static int pick_rms_types(int dtype, int param_dtype, int C, F&& f) {
+  auto with = [&](auto t, auto p) { return C % 8 == 0 ? f(t, p, std::true_type{}) : f(t, p, std::false_type{}); };
+  if (dtype == FVSR_DTYPE_BF16) return param_dtype == FVSR_DTYPE_BF16 ? with(bf16{}, bf16{}) : with(bf16{}, float{});
+  return with(float{}, float{});   // fp32 tokens take fp32 parameters
+}
+
+int launch_rms_norm(int dtype, int param_dtype, const void* x, int64_t x_stride, const void* r, int64_t rows, int C, float eps,
+                    const void* w, void* y, Out8 y8, void* s, float* rstd, hipStream_t stream) {
+  if (rows <= 0) return FVSR_OK;
+  const RmsArgs a{x, x_stride, r, rows, C, eps, w, y, y8, s, rstd};
+  return pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
+    return pick_rms_team(C, true, [&](auto waves, auto nv) {
+      using W = Team<decltype(waves)::value>;
+      hipLaunchKernelGGL((rms_norm_kernel<decltype(t), decltype(p), decltype(v)::value, decltype(waves)::value, decltype(nv)::value>),
+                         dim3((unsigned)ceil_div(rows, W::kTeams)), dim3(W::kThreads), 0, stream, a);
+    });
+  });
+}
+
+int64_t rms_grad_blocks(int64_t rows, int C) {
+  return std::min<int64_t>(kRmsGradBlocks, C <= 128 ? ceil_div(rows, 32) : C <= 2048 ? ceil_div(rows, 8) : ceil_div(rows, 2));
+}
+
+int launch_rms_norm_grad(int dtype, int param_dtype, const void* dy, const void* s, int64_t s_stride, const float* rstd,
+                         const void* ds, int64_t rows, int C, const void* w, void* dx, float* dw, float* part,
+                         hipStream_t stream) {
+  const int64_t blocks = rms_grad_blocks(rows, C);
+  if (blocks > 0) {
+    const RmsGradArgs a{dy, s, s_stride, rstd, ds, rows, C, w, dx, dw ? part : nullptr};
+    const int rc = pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
+      return pick_rms_team(C, dtype == FVSR_DTYPE_BF16, [&](auto waves, auto nv) {
+        constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
+        constexpr bool V = decltype(v)::value;
+        const dim3 grid((unsigned)blocks), block(Team<W>::kThreads);
+        if (ds) hipLaunchKernelGGL((rms_norm_grad_kernel<decltype(t), decltype(p), V, W, N, true>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((rms_norm_grad_kernel<decltype(t), decltype(p), V, W, N, false>), grid, block, 0, stream, a);
+      });
+    });
+    if (rc) return rc;
+  }
+  return dw ? launch_param_sum(part, (int)blocks, C, C, dw, nullptr, stream) : FVSR_OK;
+}
+
+}  // namespace fvsr

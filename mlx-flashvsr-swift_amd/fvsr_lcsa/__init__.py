@@ -14,7 +14,8 @@ Names mirror the reference's call surface (xocialize/mlx-flashvsr-swift):
   linear                      Linear (+ GELU tanh) on hipBLASLt                  DiT.swift:319-321,371
   DiTBlock                    DiTBlock + blockForward (streaming)               DiT.swift:363-375,491-551
 and, without a counterpart there, what training and serving the dense layers in 8 bits takes (train8.py): Blocks8, quantize8,
-dequantize8, layer_norm, layer_norm_backward, linear8, linear8_weight_grad.
+dequantize8, layer_norm, layer_norm_backward, linear8, linear8_weight_grad; and the self-attention of packed sequences (packed.py):
+rms_norm, rotary, packed_attention, their gradients, rotary_frequencies, grid_positions.
 Token tensors are (L, H*128) or (1, L, H*128), window order, float32 or bfloat16, on a HIP device, contiguous.
 Every call runs the HIP kernels of libfvsr_lcsa.so; there is no CPU fallback.
 """
@@ -34,7 +35,9 @@ __all__ = ["FVSRError", "Context", "local_block_mask", "draft_block_mask_and_pro
            "kernel_block_attention", "block_masked_attention", "block_sparse_attention", "FlashVSRAttentionOps",
            "KVRing", "window_partition", "window_reverse", "attention_mode_auto", "workspace_size",
            "rope_tables", "rope_tables_device", "qkv_epilogue", "linear", "DiTBlock", "Blocks8", "quantize8",
-           "dequantize8", "layer_norm", "layer_norm_backward", "linear8", "linear8_weight_grad",
+           "dequantize8", "layer_norm", "layer_norm_backward", "linear8", "linear8_weight_grad", "rms_norm",
+           "rms_norm_backward", "rotary", "rotary_backward", "rotary_frequencies", "grid_positions",
+           "packed_attention", "packed_attention_backward",
            "ATTN_AUTO", "ATTN_DENSE", "ATTN_KERNEL", "LAYOUT_GRID", "LAYOUT_WINDOWS", "lib"]
 
 HEAD_DIM = 128
@@ -657,5 +660,7 @@ class DiTBlock:
         return x
 
 
+from .packed import (grid_positions, packed_attention, packed_attention_backward, rms_norm,  # noqa: E402
+                     rms_norm_backward, rotary, rotary_backward, rotary_frequencies)
 from .train8 import (Blocks8, dequantize8, layer_norm, layer_norm_backward, linear8,  # noqa: E402
                      linear8_weight_grad, quantize8)

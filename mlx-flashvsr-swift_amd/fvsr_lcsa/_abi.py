@@ -67,6 +67,14 @@ SIGNATURES = {
     "fvsr_linear8": (_i, [_vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _sz, _vp]),
     "fvsr_linear8_weight_grad_workspace": (_sz, [_i64, _i, _i]),
     "fvsr_linear8_weight_grad": (_i, [_vp, _vp, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "fvsr_rms_norm": (_i, [_vp, _i, _vp, _i64, _vp, _i64, _i, C.c_float, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "fvsr_rms_norm_backward_workspace": (_sz, [_i64, _i]),
+    "fvsr_rms_norm_backward": (_i, [_vp, _i, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fvsr_rotary": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i64, _i, _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
+    "fvsr_packed_attention_workspace": (_sz, [_vp, _i, _i]),
+    "fvsr_packed_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _vp]),
+    "fvsr_packed_attention_backward_workspace": (_sz, [_vp, _i, _i]),
+    "fvsr_packed_attention_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _vp]),
     "fvsr_window_partition": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _vp]),
     "fvsr_window_reverse": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _vp]),
 }
@@ -83,6 +91,17 @@ class DiTBlockWeights(C.Structure):
     _fields_ = ([(n, _vp) for n in DIT_WEIGHT_FIELDS] + [("ctx_len", _i)] +
                 [(n, _vp) for n in ["norm3_weight", "norm3_bias", "ffn1_weight", "ffn1_bias", "ffn2_weight",
                                     "ffn2_bias"]] + [("ffn_dim", _i)])
+
+
+class Heads(C.Structure):
+    """struct fvsr_heads."""
+    _fields_ = [("data", _vp), ("heads", _i), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class Packed(C.Structure):
+    """struct fvsr_packed."""
+    _fields_ = [("cu_q", _vp), ("cu_k", _vp), ("used_k", _vp), ("sequences", _i), ("tokens_q", _i64), ("tokens_k", _i64),
+                ("channels", _i), ("causal", _i), ("scale", C.c_float)]
 
 
 class FVSRError(RuntimeError):
