@@ -24,6 +24,8 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a block: 4 waves of 32
 constexpr int kTile = 32;       // rows of a tile of the other side
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr float kRise = 4294967296.f;   // 2^32
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A tile of 32 rows of HD channels in LDS (D <= HD, zeros past D): rows of 2 HD bytes, whose 16-byte chunks are XOR-swizzled by
@@ -59,6 +61,11 @@ __device__ __forceinline__ u32x4 rows_rsrc(const bf16* base, int64_t stride, int
                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 
+// 4 bytes a lane from a buffer into LDS at lds + 4 * lane (dma16, attn_tile.hpp, otherwise)
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds, int off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
+}
+
 // the compiler moves no memory access across it
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
@@ -70,22 +77,25 @@ __device__ __forceinline__ void wait_and_sync() {
   fence();
 }
 
-// LDS offsets of a lane's operands within a tile
+// LDS offsets of a lane's operands within a tile. The swizzle being an XOR, an operand further on in the channels is the first
+// one's offset XOR a constant, made where it is used: two registers instead of 16.
 template <int HD>
 struct Lanes {
-  int row[Tile<HD>::kT];        // A operand of (tile rows) x (channels): row lane % 32, channels 16 t + 8 (lane / 32) ..
-  int tr[2][Tile<HD>::kD];      // A operand of (channels) x (tile rows), transposed: rows 16 u + 8 ab + ..
+  uint32_t row0, tr0;
   __device__ __forceinline__ Lanes() {
     using T = Tile<HD>;
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, G = lane >> 4, mm = lane & 15;
-#pragma unroll
-    for (int t = 0; t < T::kT; ++t) row[t] = l32 * T::kRow + ((2 * t + g) ^ T::swz(l32)) * 16;
-#pragma unroll
-    for (int ab = 0; ab < 2; ++ab) {
-      const int r = 8 * ab + 4 * (G >> 1) + (mm >> 2);
-#pragma unroll
-      for (int d = 0; d < T::kD; ++d) tr[ab][d] = r * T::kRow + ((4 * d + 2 * (G & 1) + (mm >> 1 & 1)) ^ T::swz(r)) * 16 + (mm & 1) * 8;
-    }
+    row0 = l32 * T::kRow + (g ^ T::swz(l32)) * 16;
+    const int r = 4 * (G >> 1) + (mm >> 2);
+    tr0 = r * T::kRow + ((2 * (G & 1) + (mm >> 1 & 1)) ^ T::swz(r)) * 16 + (mm & 1) * 8;
+  }
+  // not known to be what it was: computed where it is used, and kept in no register across a loop
+  __device__ __forceinline__ void again() { asm volatile("" : "+v"(row0), "+v"(tr0)); }
+  // A operand of (tile rows) x (channels): row lane % 32, channels 16 t + 8 (lane / 32) ..
+  __device__ __forceinline__ uint32_t row(int t) const { return row0 ^ (uint32_t)(32 * t); }
+  // A operand of (channels) x (tile rows), transposed: channels 32 d .., rows 16 u + 8 ab + ..; 8 rows on, the swizzle's bit 1 turns
+  __device__ __forceinline__ uint32_t tr(int ab, int u, int d) const {
+    return (tr0 ^ (uint32_t)(64 * d + 32 * ab)) + (uint32_t)((16 * u + 8 * ab) * Tile<HD>::kRow);
   }
 };
 
@@ -96,27 +106,43 @@ __device__ __forceinline__ f32x16 rows_times(lds_char* tile, const Lanes<HD>& at
   f32x16 s = f32x16{};
 #pragma unroll
   for (int t = 0; t < Tile<HD>::kT; ++t)
-    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const lds_bf16x8*)(tile + at.row[t]), b[t], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const lds_bf16x8*)(tile + at.row(t)), b[t], s, 0, 0, 0);
   return s;
 }
 
 // acc (channels x columns) += tile^T w, w packed from elements laid out as above
 template <int HD>
-__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&w)[2], f32x16 (&acc)[Tile<HD>::kD]) {
+__device__ __forceinline__ void add_packed(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&w)[2], f32x16 (&acc)[Tile<HD>::kD]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int d = 0; d < Tile<HD>::kD; ++d) {
-      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr[0][d] + 16 * u * Tile<HD>::kRow));
-      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr[1][d] + 16 * u * Tile<HD>::kRow));
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr(0, u, d)));
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + at.tr(1, u, d)));
       // whole-vector concatenation: element-wise assembly of the operand is mis-lowered (one dword duplicated)
       const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
       acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w[u], acc[d], 0, 0, 0);
     }
 }
 
+// whether a tile holds an infinity or NaN
+template <int HD>
+__device__ __forceinline__ bool any_odd(lds_char* tile) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < Tile<HD>::kBytes / 1024; ++i) {
+    const u32x4 x = *(const lds_u32x4*)(tile + i * 1024 + (threadIdx.x & 63) * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      most |= ((x[e] & 0x7f80u) + 0x80u) & 0x8000u;                  // an exponent of all ones carries
+      most |= ((x[e] >> 16 & 0x7f80u) + 0x80u) & 0x8000u;
+    }
+  }
+  return __ballot(most != 0) != 0;
+}
+
 // The same one tile row after another, without those that the lane's column does not see: 0 times an infinity or NaN there
-// would be NaN. `seen`: a bit a tile row. Slow, and reached only where such a value was met.
+// would be NaN. `seen`: a bit a tile row. Slow, and reached only where a tile that is not seen whole holds such a value.
 template <int HD>
 __device__ __forceinline__ void add_seen(lds_char* tile, const f32x16& w, uint32_t seen, f32x16 (&acc)[Tile<HD>::kD]) {
   using T = Tile<HD>;
@@ -142,28 +168,28 @@ __device__ __forceinline__ void add_seen(lds_char* tile, const f32x16& w, uint32
   }
 }
 
-// a bit for each tile row from a function of the row
-template <class F>
-__device__ __forceinline__ uint32_t row_bits(F&& f) {
-  uint32_t b = 0;
-#pragma unroll
-  for (int r = 0; r < kTile; ++r) b |= f(r) ? 1u << r : 0;
-  return b;
+// bits lo .. hi - 1
+__device__ __forceinline__ uint32_t bits(int lo, int hi) {
+  const uint32_t below = hi >= 32 ? ~0u : (1u << max(hi, 0)) - 1, from = lo >= 32 ? 0u : ~0u << max(lo, 0);
+  return below & from;
 }
+
+// the tile row of element i of a product, but for 4 (lane / 32)
+constexpr int elem_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
 __device__ __forceinline__ void pack(const f32x16& p, bf16x8 (&w)[2]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (bf16)p[i];
 }
 
-template <int N>
-__device__ __forceinline__ bool any_nan(const f32x16 (&acc)[N]) {
-  bool bad = false;
-#pragma unroll
-  for (int d = 0; d < N; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad |= acc[d][i] != acc[d][i];
-  return bad;
+// acc += tile^T w, of which, MASKED, the lane's column sees tile rows lo .. hi - 1 (w is 0 in the others)
+template <int HD, bool MASKED>
+__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const f32x16& w, int lo, int hi,
+                                          f32x16 (&acc)[Tile<HD>::kD]) {
+  if (MASKED && any_odd<HD>(tile)) return add_seen<HD>(tile, w, bits(lo, hi), acc);
+  bf16x8 p[2];
+  pack(w, p);
+  add_packed<HD>(tile, at, p, acc);
 }
 
 // the lane's row (channels 16 t + 8 (lane / 32) .. of it) as the other operand; zeros where there is none
@@ -266,41 +292,52 @@ struct Soft {
 #pragma unroll
     for (int d = 0; d < Tile<HD>::kD; ++d) acc[d] = f32x16{};
   }
-  // a tile of keys k0 .. k0 + 31, of which the lane's query sees those below `lim`
-  template <bool EXACT>
-  __device__ __forceinline__ void tile(lds_char* kt, lds_char* vt, const Lanes<HD>& at, const bf16x8 (&q)[Tile<HD>::kT], int k0,
-                                       int lim, bool masked, float c) {
+  // a tile of keys k0 .. k0 + 31, of which, MASKED, the lane's query sees those below `lim`
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(lds_char* kt, lds_char* vt, Lanes<HD>& at, const bf16x8 (&q)[Tile<HD>::kT], int k0, int lim,
+                                       float c) {
     const int g = (threadIdx.x & 63) >> 5;
     f32x16 s = rows_times<HD>(kt, at, q);
-    if (masked) {
+    if (MASKED) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = k0 + 8 * (i >> 2) + 4 * g + (i & 3) < lim ? s[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) s[i] = elem_row(i) < lim - k0 - 4 * g ? s[i] : -INFINITY;
     }
-    float mx = s[0];
+    // The reference is the row's maximum in the first tile that it sees. Later ones are taken as they come while their
+    // exponentials' sum stays below 2^32 (what is off a bfloat16 P or a 32-bit sum does not depend on the reference); where it does
+    // not, or is NaN, the reference rises to their maximum: rare, and a branch of the whole wave.
+    float part = 0.f;
+    f32x16 p;
+    auto take = [&] {
+      const float ref = m == -INFINITY ? 0.f : m;   // nothing seen yet
+      part = 0.f;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    const float to = fmaxf(m, pair_max(mx) * c);
-    const float ref = to == -INFINITY ? 0.f : to;   // nothing seen yet
-    const float by = __builtin_amdgcn_exp2f(m - ref);
-    m = to;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
-      sum += s[i];
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
+        part += p[i];
+      }
+    };
+    bool rise = true;
+    if (__ballot(m == -INFINITY) == 0) {
+      take();
+      rise = !(part <= kRise);
     }
-    l = fmaf(l, by, sum);
+    if (__ballot(rise) != 0) {
+      float mx = s[0];
 #pragma unroll
-    for (int d = 0; d < Tile<HD>::kD; ++d)
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      const float to = fmaxf(m, pair_max(mx) * c);
+      const float by = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+      m = to;
+      l *= by;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[d][i] *= by;
-    if (EXACT && masked) {
-      add_seen<HD>(vt, s, row_bits([&](int r) { return k0 + r < lim; }), acc);
-    } else {
-      bf16x8 w[2];
-      pack(s, w);
-      add_times<HD>(vt, at, w, acc);
+      for (int d = 0; d < Tile<HD>::kD; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= by;
+      take();
     }
+    s = p;
+    l += part;
+    add_times<HD, MASKED>(vt, at, s, 0, lim - k0, acc);
   }
 };
 
@@ -321,8 +358,9 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   const Span s = span_of(a, blk.b);
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
-  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
-  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile;
+  const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  // tiles that some row of the block sees, and that every one sees all of
+  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
   bf16x8 q[T::kT];
   load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
@@ -345,24 +383,20 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
       dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
     });
   };
-  const Lanes<HD> at;
+  Lanes<HD> at;
   Soft<HD> soft;
-  auto walk = [&](auto exact) {
-    soft.clear();
-    if (tiles > 0) issue(0);
-    for (int t = 0; t < tiles; ++t) {
-      wait_and_sync();
-      if (t + 1 < tiles) issue(t + 1);
-      lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
-      if (t * kTile < lim_max)
-        soft.template tile<decltype(exact)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, t * kTile + kTile > lim_min, a.c);
-    }
+  soft.clear();
+  if (tiles > 0) issue(0);
+  auto step = [&](auto masked, int t) {
     wait_and_sync();
+    if (t + 1 < tiles) issue(t + 1);
+    lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
+    if (!decltype(masked)::value || t * kTile < lim_max)
+      soft.template tile<decltype(masked)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, a.c);
   };
-  walk(std::false_type{});
-  // An infinity or NaN in a key's V that a row of its tile does not see makes that row NaN. Where a result is NaN, the walk is
-  // done again with those tiles' products without what is not seen.
-  if (a.causal && __syncthreads_or(any_nan(soft.acc))) walk(std::true_type{});
+  int t = 0;
+  for (; t < full; ++t) step(std::false_type{}, t);
+  for (; t < tiles; ++t) step(std::true_type{}, t);
   if (i >= s.nq) return;
   const float l = pair_sum(soft.l);
   store_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, a.D, soft.acc, l == 0.f ? 0.f : 1.f / l);
@@ -476,7 +510,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   const int begin = tile, end = parts.begin(blockIdx.x + 1);
   const uint32_t base = lds_addr(smem[wave]);
   lds_char* const lds = (lds_char*)(uintptr_t)base;
-  const Lanes<HD> at;
+  Lanes<HD> at;
   int koff[T::kCopies], voff[T::kCopies];
 #pragma unroll
   for (int p = 0; p < T::kCopies; ++p) {
@@ -496,7 +530,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
     const int hk = unit / items, r0 = (unit - hk * items) * kTile, rows = s.nq * a.group;
     // the lane's row: query i, head h
     const int r = r0 + l32, i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) % a.group;
-    const int lim = keys_seen(a, s, i), lim_min = keys_seen(a, s, r0 / a.group);
+    const int lim = keys_seen(a, s, i), full = keys_seen(a, s, r0 / a.group) / kTile;
     bf16x8 q[T::kT];
     load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + h * a.q.h, r < rows, a.D, q);
     const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + hk * a.k.h;
@@ -508,26 +542,26 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
       static_for<0, T::kCopies>([&](auto p) { dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0); });
     };
     Soft<HD> soft;
-    auto walk = [&](auto exact) {
-      soft.clear();
-      int buf = 0;
-      if (t0 + wave < t1) issue(t0 + wave, 0);
-      for (int t = t0 + wave; t < t1; t += 4, buf ^= 1) {
-        if (t + 4 < t1) {
-          issue(t + 4, buf ^ 1);
-          FVSR_WAIT_VM_LGKM0(2 * T::kCopies);
-        } else {
-          FVSR_WAIT_VM_LGKM0(0);
-        }
-        fence();
-        lds_char* const kt = lds + buf * 2 * T::kBytes;
-        soft.template tile<decltype(exact)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, t * kTile + kTile > lim_min, a.c);
-        fence();
-        FVSR_WAIT_VM_LGKM0(63);   // its reads are done before the next copies into this buffer
+    soft.clear();
+    int buf = 0, t = t0 + wave;
+    if (t < t1) issue(t, 0);
+    auto step = [&](auto masked) {
+      if (t + 4 < t1) {
+        issue(t + 4, buf ^ 1);
+        FVSR_WAIT_VM_LGKM0(2 * T::kCopies);
+      } else {
+        FVSR_WAIT_VM_LGKM0(0);
       }
+      fence();
+      lds_char* const kt = lds + buf * 2 * T::kBytes;
+      soft.template tile<decltype(masked)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, a.c);
+      fence();
+      FVSR_WAIT_VM_LGKM0(63);   // its reads are done before the next copies into this buffer
+      t += 4;
+      buf ^= 1;
     };
-    walk(std::false_type{});
-    if (a.causal && __ballot(any_nan(soft.acc)) != 0) walk(std::true_type{});   // as in packed_forward_kernel
+    while (t < min(full, t1)) step(std::false_type{});
+    while (t < t1) step(std::true_type{});
     // the waves' results meet in LDS: each its rows x channels in its own ring
     {
       const float l = pair_sum(soft.l);
@@ -637,8 +671,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   const Span s = span_of(a, blk.b);
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
-  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
-  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile;
+  const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  // tiles that some row of the block sees, and that every one sees all of
+  const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
   bf16x8 q[T::kT], d_o[T::kT];
   load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
@@ -655,7 +690,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     if (i < s.nq) {
       const int64_t at = (int64_t)head * a.tq + s.q0 + i;
       lse2 = a.lse[at] * kLog2e;
-      if (g == 0) a.delta[at] = delta;
+      if (g == 0) *(f32x2*)(a.stat + 2 * at) = f32x2{lse2, delta};
     }
   }
   const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + head / a.group * a.k.h;
@@ -677,48 +712,49 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
       dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
     });
   };
-  const Lanes<HD> at;
+  Lanes<HD> at;
   f32x16 acc[T::kD];
-  auto walk = [&](auto exact) {
 #pragma unroll
-    for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
-    if (tiles > 0) issue(0);
-    for (int t = 0; t < tiles; ++t) {
-      wait_and_sync();
-      if (t + 1 < tiles) issue(t + 1);
-      lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
-      const int k0 = t * kTile;
-      if (k0 >= lim_max) continue;
-      const bool masked = k0 + kTile > lim_min;
-      f32x16 p = rows_times<HD>(kt, at, q);
-      f32x16 dp = rows_times<HD>(kt + T::kBytes, at, d_o);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(fmaf(p[e], a.c, -lse2)) * (dp[e] - delta);
-      if (masked) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] = k0 + 8 * (e >> 2) + 4 * g + (e & 3) < lim ? dp[e] : 0.f;
-      }
-      if (decltype(exact)::value && masked) {
-        add_seen<HD>(kt, dp, row_bits([&](int r) { return k0 + r < lim; }), acc);
-      } else {
-        bf16x8 w[2];
-        pack(dp, w);
-        add_times<HD>(kt, at, w, acc);
-      }
-    }
+  for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
+  if (tiles > 0) issue(0);
+  auto step = [&](auto masked, int t) {
+    constexpr bool MASKED = decltype(masked)::value;
     wait_and_sync();
+    if (t + 1 < tiles) issue(t + 1);
+    lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
+    const int k0 = t * kTile;
+    if (MASKED && k0 >= lim_max) return;
+    at.again();
+    f32x16 p = rows_times<HD>(kt, at, q);
+    f32x16 dp = rows_times<HD>(kt + T::kBytes, at, d_o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(fmaf(p[e], a.c, -lse2)) * (dp[e] - delta);
+    if (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = elem_row(e) < lim - k0 - 4 * g ? dp[e] : 0.f;
+    }
+    add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, acc);
   };
-  walk(std::false_type{});
-  if (a.causal && __syncthreads_or(any_nan(acc))) walk(std::true_type{});
+  int t = 0;
+  for (; t < full; ++t) step(std::false_type{}, t);
+  for (; t < tiles; ++t) step(std::true_type{}, t);
   if (i < s.nq) store_row<HD>(a.dq.p + (int64_t)(s.q0 + i) * a.dq.t + head * a.dq.h, a.D, acc, a.scale);
 }
 
+// dK and dV of 128 keys: 8 waves, two to each 32 keys. One makes S, P and dV, the other, a tile of queries behind, dP, dS and dK
+// from the P that the first one leaves in LDS (in fp32: fp16 would lose the gradients of keys whose weights are all small).
+// So a wave holds one operand and one sum, not two (which with S and dP beside them pass the 256 registers that two waves a SIMD
+// have), and the two waves of a SIMD, one of each kind, are at the matrix core by turns.
 template <int HD>
-__global__ __launch_bounds__(256, 1) void packed_dkv_kernel(PackedArgs a) {
+__global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   using T = Tile<HD>;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][Q, dO]
-  __shared__ __attribute__((aligned(16))) float stat[4][2][kTile];      // [wave][lse (log2 units), delta] of a tile's queries
+  constexpr int kSlot = 2 * T::kBytes;                                                      // Q, dO
+  __shared__ __attribute__((aligned(1024))) char smem[4 * kSlot];                           // tile n in slot n % 4
+  __shared__ __attribute__((aligned(1024))) float stat[4][2][kTile];                        // its lse (log2 units) and delta
+  __shared__ __attribute__((aligned(16))) f32x4 handed[2][4][4][64];                         // P of tile n in n % 2, a wave pair each
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int pair = wave & 3;
+  const bool makes_dv = wave < 4;
   const int hk = blockIdx.x % a.kv_heads;
   const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.kv_heads);   // the first keys, which most queries see, first
   if (a.clear && blk.hi > blk.lo) {
@@ -728,111 +764,155 @@ __global__ __launch_bounds__(256, 1) void packed_dkv_kernel(PackedArgs a) {
   if (blk.b < 0 || blk.b >= a.seqs) return;
   const Span s = span_of(a, blk.b);
   if (blk.row >= s.room) return;
-  const int j0 = blk.row + wave * 32, j = j0 + l32;
+  const int j0 = blk.row + pair * 32, j = j0 + l32;
   const int off = s.nk - s.nq;   // causal: query i sees keys j <= i + off
   // tiles of queries; none for keys that are not in use
   const int tiles = blk.row < s.nk ? (s.nq + kTile - 1) / kTile : 0;
+  // the first one that sees a key of the block, and the first from which on every row sees all of them
   const int t0 = a.causal ? min(tiles, max(0, blk.row - off) / kTile) : 0;
+  const int t1 = a.causal ? min(tiles, max(0, blk.row + kRows - 1 - off + kTile - 1) / kTile) : 0;
+  const int t2 = max(t1, min(tiles, s.nq / kTile));   // the last tile may not be whole
   const int steps = (tiles - t0) * a.group;
 
-  bf16x8 k[T::kT], v[T::kT];
-  load_row<HD>(a.k.p + (int64_t)(s.k0 + j) * a.k.t + hk * a.k.h, j < s.nk, a.D, k);
-  load_row<HD>(a.v.p + (int64_t)(s.k0 + j) * a.v.t + hk * a.v.h, j < s.nk, a.D, v);
+  const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
+  bf16x8 b[T::kT];
+  load_row<HD>(kv.p + (int64_t)(s.k0 + j) * kv.t + hk * kv.h, j < s.nk, a.D, b);
+  // a tile's copies are dealt to the 8 waves: Q to the first 4, dO to the others
   constexpr int kMine = T::kCopies / 4;
-  int qoff[kMine], ooff[kMine];
+  const HeadView<const bf16> from = makes_dv ? a.q : a.d_o;
+  int voff[kMine];
 #pragma unroll
-  for (int p = 0; p < kMine; ++p) {
-    qoff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.q.t * 2, a.D);
-    ooff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.d_o.t * 2, a.D);
+  for (int p = 0; p < kMine; ++p) voff[p] = copy_off<HD>(pair * kMine + p, lane, (int)from.t * 2, a.D);
+  const int soff = l32 * 8 + g * 4;   // lse of the tile's rows, then delta
+  const uint32_t base = lds_addr(smem) + (makes_dv ? 0 : T::kBytes) + pair * kMine * 1024, sbase = lds_addr(stat);
+  auto issue = [&](int h, int t, int n) {
+    const u32x4 r = rows_rsrc(from.p + (int64_t)s.q0 * from.t + h * from.h, from.t, t * kTile, s.nq, a.D);
+    static_for<0, kMine>([&](auto p) { dma16<p * 1024>(r, base + (n & 3) * kSlot, voff[p], 0); });
+    if (wave == 0) {
+      const uint64_t at = (uint64_t)(a.stat + ((int64_t)h * a.tq + s.q0 + t * kTile) * 2);
+      const u32x4 sr = {(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)((uint32_t)(at >> 32) & 0xffffu)),
+                        (uint32_t)uniform(min(s.nq - t * kTile, kTile) * 8), 0x00020000u};
+      dma4(sr, sbase + (n & 3) * 2 * kTile * 4, soff);
+    }
+  };
+  lds_char* const lds = (lds_char*)(uintptr_t)lds_addr(smem);
+  Lanes<HD> at;
+  f32x16 acc[T::kD];
+#pragma unroll
+  for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
+  // the tile to be requested next, and the one that this wave works on
+  int ih = hk * a.group, it = t0, in = 0;
+  auto request = [&] {
+    if (in < steps) issue(ih, it, in);
+    ++in;
+    if (++it == tiles) {
+      it = t0;
+      ++ih;
+    }
+  };
+  // the copies of one step may still be under way
+  auto landed = [&](bool all) {
+    fence();
+    if (all) FVSR_WAIT_VM_LGKM0(0);
+    else if (wave == 0) FVSR_WAIT_VM_LGKM0(kMine + 1);
+    else FVSR_WAIT_VM_LGKM0(kMine);
+    __builtin_amdgcn_s_barrier();
+    fence();
+  };
+  auto first = [&](auto masked, int t, int n) {   // S, P, dV of tile t of a head, the n-th of all
+    constexpr bool MASKED = decltype(masked)::value;
+    lds_char* const qt = lds + (n & 3) * kSlot;
+    const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;   // the lane's key is seen by rows lo .. hi - 1 of the tile
+    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return;   // no query of the tile sees a key of the wave
+    at.again();
+    f32x16 p = rows_times<HD>(qt, at, b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x4 lse2 = *(const f32x4*)&stat[n & 3][0][8 * c + 4 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * c + e], a.c, -lse2[e]));
+    }
+    if (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? p[e] : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) handed[n & 1][pair][c][lane] = f32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]};
+    add_times<HD, MASKED>(qt + T::kBytes, at, p, lo, hi, acc);
+  };
+  auto second = [&](auto masked, int t, int n) {   // dP, dS, dK of tile t of a head, the n-th of all
+    constexpr bool MASKED = decltype(masked)::value;
+    lds_char* const qt = lds + (n & 3) * kSlot;
+    const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;
+    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return;
+    at.again();
+    f32x16 ds = rows_times<HD>(qt + T::kBytes, at, b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x4 p = handed[n & 1][pair][c][lane], delta = *(const f32x4*)&stat[n & 3][1][8 * c + 4 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ds[4 * c + e] = p[e] * (ds[4 * c + e] - delta[e]);
+    }
+    if (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? ds[e] : 0.f;
+    }
+    add_times<HD, MASKED>(qt, at, ds, lo, hi, acc);
+  };
+  // one loop for each kind of wave, with the same barriers: step n is the first kind's tile n and the second kind's tile n - 1
+  request();
+  request();
+  if (makes_dv) {
+    int n = 0;
+    for (int h = 0; h < a.group; ++h) {
+      int t = t0;
+      for (; t < t1; ++t, ++n) {
+        landed(n + 1 >= steps);
+        request();
+        first(std::true_type{}, t, n);
+      }
+      for (; t < t2; ++t, ++n) {
+        landed(n + 1 >= steps);
+        request();
+        first(std::false_type{}, t, n);
+      }
+      for (; t < tiles; ++t, ++n) {
+        landed(n + 1 >= steps);
+        request();
+        first(std::true_type{}, t, n);
+      }
+    }
+    landed(true);
+  } else {
+    int n = 0;
+    landed(1 >= steps);
+    request();
+    for (int h = 0; h < a.group; ++h) {
+      int t = t0;
+      for (; t < t1; ++t, ++n) {
+        landed(n + 2 >= steps);
+        request();
+        second(std::true_type{}, t, n);
+      }
+      for (; t < t2; ++t, ++n) {
+        landed(n + 2 >= steps);
+        request();
+        second(std::false_type{}, t, n);
+      }
+      for (; t < tiles; ++t, ++n) {
+        landed(n + 2 >= steps);
+        request();
+        second(std::true_type{}, t, n);
+      }
+    }
   }
-  const uint32_t base = lds_addr(smem);
-  lds_char* const lds = (lds_char*)(uintptr_t)base;
-  auto issue = [&](int h, int t, int buf) {
-    const bf16* const qb = a.q.p + (int64_t)s.q0 * a.q.t + h * a.q.h;
-    const bf16* const ob = a.d_o.p + (int64_t)s.q0 * a.d_o.t + h * a.d_o.h;
-    const u32x4 qr = rows_rsrc(qb, a.q.t, t * kTile, s.nq, a.D), dr = rows_rsrc(ob, a.d_o.t, t * kTile, s.nq, a.D);
-    const uint32_t to = base + buf * 2 * T::kBytes + wave * kMine * 1024;
-    static_for<0, kMine>([&](auto p) {
-      dma16<p * 1024>(qr, to, qoff[p], 0);
-      dma16<p * 1024>(dr, to + T::kBytes, ooff[p], 0);
-    });
-  };
-  // lanes 0-31: lse, lanes 32-63: delta, of the tile's queries
-  auto stat_of = [&](int h, int t) {
-    const int64_t at = (int64_t)h * a.tq + s.q0 + min(t * kTile + l32, s.nq - 1);
-    return g ? a.delta[at] : a.lse[at] * kLog2e;
-  };
-  const Lanes<HD> at;
-  f32x16 dk[T::kD], dv[T::kD];
-  auto walk = [&](auto exact) {
-#pragma unroll
-    for (int d = 0; d < T::kD; ++d) dk[d] = dv[d] = f32x16{};
-    int h = hk * a.group, t = t0;
-    float next = 0.f;
-    if (steps > 0) {
-      issue(h, t, 0);
-      next = stat_of(h, t);
-    }
-    for (int n = 0; n < steps; ++n) {
-      wait_and_sync();
-      const int q0 = t * kTile;
-      stat[wave][g][l32] = next;
-      if (++t == tiles) {
-        t = t0;
-        ++h;
-      }
-      if (n + 1 < steps) {
-        issue(h, t, (n + 1) & 1);
-        next = stat_of(h, t);
-      }
-      lds_char* const qt = lds + (n & 1) * 2 * T::kBytes;
-      lds_char* const ot = qt + T::kBytes;
-      const bool causal_edge = a.causal && j0 + 31 > q0 + off, masked = causal_edge || q0 + kTile > s.nq;
-      if (a.causal && j0 > q0 + 31 + off) continue;   // no query of the tile sees a key of the wave
-      auto sees = [&](int r) { return q0 + r < s.nq && (!a.causal || j <= q0 + r + off); };
-      f32x16 p = rows_times<HD>(qt, at, k);
-      f32x16 ds = rows_times<HD>(ot, at, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const f32x4 lse2 = *(const f32x4*)&stat[wave][0][8 * c + 4 * g], delta = *(const f32x4*)&stat[wave][1][8 * c + 4 * g];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(p[4 * c + e], a.c, -lse2[e]));
-          p[4 * c + e] = x;
-          ds[4 * c + e] = x * (ds[4 * c + e] - delta[e]);
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool see = sees(8 * (e >> 2) + 4 * g + (e & 3));
-          p[e] = see ? p[e] : 0.f;
-          ds[e] = see ? ds[e] : 0.f;
-        }
-      }
-      if (decltype(exact)::value && masked) {
-        const uint32_t seen = row_bits(sees);
-        add_seen<HD>(ot, p, seen, dv);
-        add_seen<HD>(qt, ds, seen, dk);
-      } else {
-        bf16x8 w[2];
-        pack(p, w);
-        add_times<HD>(ot, at, w, dv);
-        pack(ds, w);
-        add_times<HD>(qt, at, w, dk);
-      }
-    }
-    wait_and_sync();
-  };
-  walk(std::false_type{});
-  if (a.causal && __syncthreads_or(any_nan(dk) || any_nan(dv))) walk(std::true_type{});
   if (j >= s.room) return;
   if (j >= s.nk) {   // not in use: seen by none
 #pragma unroll
-    for (int d = 0; d < T::kD; ++d) dk[d] = dv[d] = f32x16{};
+    for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   }
-  store_row<HD>(a.dk.p + (int64_t)(s.k0 + j) * a.dk.t + hk * a.dk.h, a.D, dk, a.scale);
-  store_row<HD>(a.dv.p + (int64_t)(s.k0 + j) * a.dv.t + hk * a.dv.h, a.D, dv, 1.f);
+  const HeadView<bf16> to = makes_dv ? a.dv : a.dk;
+  store_row<HD>(to.p + (int64_t)(s.k0 + j) * to.t + hk * to.h, a.D, acc, makes_dv ? 1.f : a.scale);
 }
 
 int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
@@ -872,14 +952,14 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
   return FVSR_OK;
 }
 
-size_t packed_backward_workspace(int64_t tq, int heads) { return (size_t)tq * heads * sizeof(float); }
+size_t packed_backward_workspace(int64_t tq, int heads) { return (size_t)tq * heads * 2 * sizeof(float); }
 
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {
-  a.delta = (float*)ws;
+  a.stat = (float*)ws;
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3((unsigned)(slots(a.tk, a.seqs) * a.kv_heads)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3((unsigned)(slots(a.tk, a.seqs) * a.kv_heads)), dim3(512), 0, stream, a);
   };
   if (a.D <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});

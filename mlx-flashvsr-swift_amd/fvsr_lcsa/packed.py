@@ -169,8 +169,8 @@ def _out_heads(out, name: str, like: torch.Tensor):
 
 
 def _view(x) -> Heads:
-    n, h, _ = x.shape
-    return Heads(x.data_ptr(), h, x.stride(0) if n > 1 else 0, x.stride(1) if h > 1 else 0)
+    n, h, d = x.shape
+    return Heads(x.data_ptr(), h, x.stride(0) if n > 1 else h * d, x.stride(1) if h > 1 else d)
 
 
 def _ref(view):

@@ -358,6 +358,15 @@ def test_unaligned_and_overlapping_views_are_read(dev):
     ref = attention64(q, k, k, cq, causal=True)
     within(f.packed_attention(q, k, k, cu, causal=True)[0], ref["o"], ref["tol_o"])
     assert f.packed_attention(q[None], k[None], k[None], cu)[0].shape == (1, 60, 2, 64)
+    for n in (1, 40, 45):   # one token read as many: rows past the last are not zeros
+        one, do = randn(g, (1, 2, 64), dev).expand(n, 2, 64), randn(g, (1, 2, 64), dev).expand(n, 2, 64)
+        cq, cu = cu_of([n], dev)
+        for causal in (False, True):
+            ref = attention64(one, one, one, cq, causal=causal, do=do)
+            o, lse = f.packed_attention(one, one, one, cu, causal=causal, want_lse=True)
+            within(o, ref["o"], ref["tol_o"])
+            for name, x in zip(("dq", "dk", "dv"), f.packed_attention_backward(do, one, one, one, o, lse, cu, causal=causal)):
+                within(x, ref[name], ref["tol_" + name], name)
 
 
 def test_no_tokens(dev):
