@@ -28,9 +28,6 @@ namespace fvsr {
 __device__ __forceinline__ void mfma_acc(f32x16& acc, const bf16x8& a, const bf16x8& b) {
   acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
 }
-// >= 19 wait states after the last MFMA of a walk (the compiler also inserts what it needs)
-__device__ __forceinline__ void acc_drain() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
-
 // Lazy online-softmax rescale. The running reference max m_run (log2 domain, per query row) is raised only when a
 // tile's row max exceeds it by more than 8, i.e. a factor 2^8: exponentials then stay <= 256 (no overflow in fp32 or
 // bf16) and the softmax is mathematically unchanged, while the O/l rescale — a multiply over the whole accumulator —

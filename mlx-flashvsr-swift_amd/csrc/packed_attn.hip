@@ -69,10 +69,20 @@ __device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds, int off) {
 // the compiler moves no memory access across it
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
-// all of this wave's copies have landed, and every wave is past its reads
-__device__ __forceinline__ void wait_and_sync() {
+// The loads so far have landed. Before a loop whose copies (which the compiler does not count) are waited for by their number: it
+// would wait for none to be under way, every time round, where a load from before the loop might be.
+__device__ __forceinline__ void loaded() {
   fence();
   FVSR_WAIT_VM_LGKM0(0);
+  fence();
+}
+
+// The copies but the last `under_way` of this wave have landed, and every wave is past its reads.
+template <int UNDER_WAY>
+__device__ __forceinline__ void wait_and_sync_but(bool all) {
+  fence();
+  if (all) FVSR_WAIT_VM_LGKM0(0);
+  else FVSR_WAIT_VM_LGKM0(UNDER_WAY);
   __builtin_amdgcn_s_barrier();
   fence();
 }
@@ -341,10 +351,15 @@ struct Soft {
   }
 };
 
+// The walk over tiles that every row sees whole, four a turn: a step makes S of tile T + 1, P of tile T and adds P V of tile T - 1,
+// a product of the matrix core at a time with a share of the rest behind it, fenced so that this is the order they are issued in:
+// the exponentials, the reads of operands four rounds ahead, and the copies of K(T + 4) and V(T + 2) run while the matrix core
+// does. K and V have a ring of four tiles each: K(T) is read a step before, and V(T) a step after, P(T) is made.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   using T = Tile<HD>;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][K, V]
+  __shared__ __attribute__((aligned(1024))) char smem[8 * T::kBytes];   // [K, V][tile % 4]
+  constexpr int kRing = 4 * T::kBytes;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
   // a sequence's last rows, which see most where it is causal, come first
@@ -362,8 +377,6 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   // tiles that some row of the block sees, and that every one sees all of
   const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
-  bf16x8 q[T::kT];
-  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
   const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + head / a.group * a.k.h;
   const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + head / a.group * a.v.h;
   constexpr int kMine = T::kCopies / 4;   // copies of a tile a wave makes
@@ -373,35 +386,175 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     koff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.k.t * 2, a.D);
     voff[p] = copy_off<HD>(wave * kMine + p, lane, (int)a.v.t * 2, a.D);
   }
-  const uint32_t base = lds_addr(smem);
+  const uint32_t base = lds_addr(smem), mine = base + wave * kMine * 1024;
   lds_char* const lds = (lds_char*)(uintptr_t)base;
-  auto issue = [&](int t) {
-    const u32x4 kr = rows_rsrc(kb, a.k.t, t * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, t * kTile, s.nk, a.D);
-    const uint32_t to = base + (t & 1) * 2 * T::kBytes + wave * kMine * 1024;
-    static_for<0, kMine>([&](auto p) {
-      dma16<p * 1024>(kr, to, koff[p], 0);
-      dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
-    });
+  // past the last tile, and before the first: zeros
+  auto k_rsrc = [&](int t) { return rows_rsrc(kb, a.k.t, t * kTile, t < 0 ? t * kTile : s.nk, a.D); };
+  auto v_rsrc = [&](int t) { return rows_rsrc(vb, a.v.t, t * kTile, t < 0 ? t * kTile : s.nk, a.D); };
+  auto copy_k = [&](const u32x4& r, auto p, int slot) { dma16<decltype(p)::value * 1024>(r, mine + slot * T::kBytes, koff[decltype(p)::value], 0); };
+  auto copy_v = [&](const u32x4& r, auto p, int slot) { dma16<kRing + decltype(p)::value * 1024>(r, mine + slot * T::kBytes, voff[decltype(p)::value], 0); };
+  auto request = [&](int tk, int tv) {
+    const u32x4 kr = k_rsrc(tk), vr = v_rsrc(tv);
+    static_for<0, kMine>([&](auto p) { copy_k(kr, p, tk & 3); });
+    static_for<0, kMine>([&](auto p) { copy_v(vr, p, tv & 3); });
   };
+  constexpr int kStep = 2 * kMine;   // copies a step
   Lanes<HD> at;
   Soft<HD> soft;
   soft.clear();
-  if (tiles > 0) issue(0);
-  auto step = [&](auto masked, int t) {
-    wait_and_sync();
-    if (t + 1 < tiles) issue(t + 1);
-    lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
-    if (!decltype(masked)::value || t * kTile < lim_max)
-      soft.template tile<decltype(masked)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, a.c);
-  };
+  request(0, -2);
+  request(1, -1);
+  request(2, 0);
+  request(3, 1);
+  bf16x8 q[T::kT];
+  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
+  loaded();
+  __builtin_amdgcn_s_barrier();
+  fence();
   int t = 0;
-  for (; t < full; ++t) step(std::false_type{}, t);
-  for (; t < tiles; ++t) step(std::true_type{}, t);
-  if (i >= s.nq) return;
-  const float l = pair_sum(soft.l);
-  store_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, a.D, soft.acc, l == 0.f ? 0.f : 1.f / l);
-  if (a.lse && g == 0)
-    a.lse[(int64_t)head * a.tq + s.q0 + i] = l == 0.f ? -INFINITY : (soft.m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (full >= 4) {
+    uint32_t krow[T::kT], vtr[2][T::kD];
+#pragma unroll
+    for (int c = 0; c < T::kT; ++c) krow[c] = base + at.row(c);
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d) {
+      vtr[0][d] = base + kRing + at.tr(0, 0, d);
+      vtr[1][d] = base + kRing + at.tr(1, 0, d);
+    }
+    auto k_op = [&](int slot, int c) { return *(const lds_bf16x8*)((lds_char*)(uintptr_t)krow[c] + slot * T::kBytes); };
+    auto v_op = [&](int slot, int c) {   // product c: rows 16 (c / kD) .., channels 32 (c % kD) ..
+      const int u = c / T::kD, d = c % T::kD;
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[0][d] + slot * T::kBytes + 16 * u * T::kRow));
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[1][d] + slot * T::kBytes + 16 * u * T::kRow));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    f32x16 sA, sB;
+    bf16x8 pA[2], pB[2];
+    sA = rows_times<HD>(lds, at, q);
+    {
+      float mx = sA[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sA[e]);
+      soft.m = pair_max(mx) * a.c;
+    }
+    pB[0] = pB[1] = bf16x8{};
+    const float c = a.c;
+    // step T = t + SUB
+    auto step = [&](auto sub_c, f32x16& s_cur, f32x16& s_nxt, bf16x8 (&p_prev)[2], bf16x8 (&p_cur)[2]) {
+      constexpr int SUB = decltype(sub_c)::value, KS = (SUB + 1) & 3, VS = (SUB + 3) & 3;   // slots that are read
+      constexpr int kRounds = 2 * T::kT, kExp = 16 / kRounds;
+      const u32x4 kr = k_rsrc(t + SUB + 4), vr = v_rsrc(t + SUB + 2);
+      bf16x8 kk[T::kT], vv[T::kT];
+      const float negm = -soft.m;
+      float x[16], sum[2];
+      auto round = [&](auto i_c) {
+        constexpr int I = decltype(i_c)::value;
+        if constexpr (I == 0) {
+          kk[0] = k_op(KS, 0);
+          vv[0] = v_op(VS, 0);
+          kk[1] = k_op(KS, 1);
+          vv[1] = v_op(VS, 1);
+        }
+        static_for<2, T::kT>([&](auto j_c) {
+          constexpr int J = decltype(j_c)::value;
+          if constexpr ((2 * J - 4 > 0 ? 2 * J - 4 : 0) == I) {
+            kk[J] = k_op(KS, J);
+            vv[J] = v_op(VS, J);
+          }
+        });
+        if constexpr (I < kRounds) {
+          constexpr int C = I / 2;
+          if constexpr (I % 2 == 0)
+            s_nxt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk[C], q[C], C > 0 ? s_nxt : f32x16{}, 0, 0, 0);
+          else
+            soft.acc[C % T::kD] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv[C], p_prev[C / T::kD], soft.acc[C % T::kD], 0, 0, 0);
+        }
+        // the exponentials of the round before are summed and packed here, so that nothing waits for them
+        if constexpr (I >= 1) {
+#pragma unroll
+          for (int e = 0; e < kExp; ++e) {
+            constexpr int J0 = (I - 1) * kExp;
+            const int J = J0 + e;
+            if (J < 2) sum[J] = x[J];
+            else sum[J & 1] += x[J];
+            if (J & 1) {
+              p_cur[J >> 3][(J & 7) - 1] = (bf16)x[J - 1];
+              p_cur[J >> 3][J & 7] = (bf16)x[J];
+              const u32x4 w = __builtin_bit_cast(u32x4, p_cur[J >> 3]);
+              asm volatile("" ::"v"(w[(J & 7) >> 1]));   // packed here, and not sunk behind the branch below
+            }
+          }
+        }
+        if constexpr (I < kRounds) {
+#pragma unroll
+          for (int e = 0; e < kExp; ++e) x[I * kExp + e] = __builtin_amdgcn_exp2f(fmaf(s_cur[I * kExp + e], c, negm));
+        }
+        // a copy every few rounds
+        constexpr int kEvery = kRounds / kStep;
+        if constexpr (I % kEvery == 1 && I / kEvery < kStep) {
+          constexpr int R = I / kEvery;
+          if constexpr (R < kMine) copy_k(kr, std::integral_constant<int, R>{}, SUB);
+          else copy_v(vr, std::integral_constant<int, R - kMine>{}, (SUB + 2) & 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      static_for<0, kRounds + 1>(round);
+      float part = sum[0] + sum[1];
+      if (__ballot(!(part <= kRise)) != 0) {   // Soft::tile's rise, of the rows that need it
+        acc_drain();
+        float mx = s_cur[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s_cur[e]);
+        const float to = pair_max(part) <= kRise ? soft.m : fmaxf(soft.m, pair_max(mx) * c);
+        const float by = __builtin_amdgcn_exp2f(soft.m - to);
+        soft.m = to;
+        soft.l *= by;
+        part = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float y = __builtin_amdgcn_exp2f(fmaf(s_cur[e], c, -to));
+          part += y;
+          p_cur[e >> 3][e & 7] = (bf16)y;
+        }
+#pragma unroll
+        for (int d = 0; d < T::kD; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) soft.acc[d][e] *= by;
+      }
+      soft.l += part;
+      __builtin_amdgcn_sched_barrier(0);
+      wait_and_sync_but<2 * kStep>(false);   // K(T + 2) and V(T), requested two steps before, have landed
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using C2 = std::integral_constant<int, 2>;
+    using C3 = std::integral_constant<int, 3>;
+    for (; t + 4 <= full; t += 4) {
+      step(C0{}, sA, sB, pB, pA);
+      step(C1{}, sB, sA, pA, pB);
+      step(C2{}, sA, sB, pB, pA);
+      step(C3{}, sB, sA, pA, pB);
+    }
+    add_packed<HD>(lds + kRing + 3 * T::kBytes, at, pB, soft.acc);   // V(t - 1)
+    acc_drain();
+  }
+  // The tiles left: up to three whole ones, then those that some rows do not see all of. A step here reads K(t) and V(t), so K(t + 3)
+  // is the furthest that it may request (the first one does so again).
+  for (; t < tiles; ++t) {
+    wait_and_sync_but<kStep>(false);
+    request(t + 3, t + 2);
+    lds_char* const kt = lds + (t & 3) * T::kBytes;
+    if (t < full) soft.template tile<false>(kt, kt + kRing, at, q, t * kTile, lim, a.c);
+    else if (t * kTile < lim_max) soft.template tile<true>(kt, kt + kRing, at, q, t * kTile, lim, a.c);
+  }
+  if (i < s.nq) {
+    const float l = pair_sum(soft.l);
+    store_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, a.D, soft.acc, l == 0.f ? 0.f : 1.f / l);
+    if (a.lse && g == 0)
+      a.lse[(int64_t)head * a.tq + s.q0 + i] = l == 0.f ? -INFINITY : (soft.m + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+  FVSR_WAIT_VM0();   // no copy outlives the workgroup's LDS
 }
 
 // ---- few queries a sequence: the keys split over the workgroups ------------------------------------------------------------
@@ -426,6 +579,7 @@ __device__ __forceinline__ Span lane_span(const PackedArgs& a, int b) {   // spa
   return s;
 }
 
+constexpr int kMaxParts = 256;        // workgroups of the split walk: its rings leave room for one on a compute unit
 constexpr int kMinTiles = 8;          // tiles a part, at the least: two a wave
 constexpr int kMostWork = 1 << 30;    // tiles of a call (split)
 
@@ -531,8 +685,6 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
     // the lane's row: query i, head h
     const int r = r0 + l32, i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) % a.group;
     const int lim = keys_seen(a, s, i), full = keys_seen(a, s, r0 / a.group) / kTile;
-    bf16x8 q[T::kT];
-    load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + h * a.q.h, r < rows, a.D, q);
     const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + hk * a.k.h;
     const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + hk * a.v.h;
     auto issue = [&](int t, int buf) {
@@ -545,6 +697,9 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
     soft.clear();
     int buf = 0, t = t0 + wave;
     if (t < t1) issue(t, 0);
+    bf16x8 q[T::kT];
+    load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + h * a.q.h, r < rows, a.D, q);
+    loaded();
     auto step = [&](auto masked) {
       if (t + 4 < t1) {
         issue(t + 4, buf ^ 1);
@@ -623,37 +778,73 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   }
 }
 
-// Workgroup (x, y): the item cut by part x + 1's beginning, if that is the item's first cut; 256 of its rows' channels.
+// Workgroup (x, y): rows y, y + gridDim.y, .. of the item cut by part x + 1's beginning, if that is the item's first cut. All of a row's pieces are
+// asked for at once: their references and sums by a thread each, then their channels by 4 to a thread, the pieces dealt to the
+// 256 / (HD / 4) groups of threads and joined in LDS.
 template <int HD>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
+  constexpr int kCols = HD / 4, kDeal = 256 / kCols;
   __shared__ int sm[12];
+  __shared__ float weight[kMaxParts];
+  __shared__ float red[8];
+  __shared__ __attribute__((aligned(16))) f32x4 sums[kDeal][kCols];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = blockIdx.x;
   int tile, b, first;
-  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return (int)blockIdx.x + 1 < p.parts ? p.begin(blockIdx.x + 1) : -1; }, tile, b, first);
+  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return x + 1 < p.parts ? p.begin(x + 1) : -1; }, tile, b, first);
   if (b < 0) return;
   const Span s = span_of(a, b);
   const int items = items_of(a, s), tiles = tiles_of(s);
   const int unit = (tile - first) / tiles, begin = first + unit * tiles;
-  if (begin == tile || parts.owner(begin) != (int)blockIdx.x) return;   // no cut, or not the first one
-  const int last = parts.owner(begin + tiles - 1), hk = unit / items, r0 = (unit - hk * items) * kTile;
-  const int row = ((int)blockIdx.y * 256 + (int)threadIdx.x) / HD, ch = threadIdx.x % HD;
-  if (row >= min(kTile, s.nq * a.group - r0)) return;
-  auto part = [&](int w) {
-    return a.part + (int64_t)(2 * w + (w == (int)blockIdx.x && parts.begin(w) < begin ? 1 : 0)) * Partial<HD>::kFloats;
-  };
-  float m = -INFINITY;
-  for (int w = blockIdx.x; w <= last; ++w) m = fmaxf(m, part(w)[kTile * HD + row]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, x = 0.f;
-#pragma unroll 4
-  for (int w = blockIdx.x; w <= last; ++w) {
-    const float* p = part(w);
-    const float by = __builtin_amdgcn_exp2f(p[kTile * HD + row] - ref), lw = p[kTile * HD + kTile + row];
-    l = lw == 0.f ? l : fmaf(lw, by, l);
-    x = lw == 0.f ? x : fmaf(p[row * HD + ch], by, x);
+  if (begin == tile || parts.owner(begin) != x) return;   // no cut, or not the first one
+  const int hk = unit / items, r0 = (unit - hk * items) * kTile;
+  const int pieces = parts.owner(begin + tiles - 1) - x + 1, inside = parts.begin(x) < begin ? 1 : 0;   // <= kMaxParts
+  auto part = [&](int p) { return a.part + (int64_t)(2 * (x + p) + (p == 0 ? inside : 0)) * Partial<HD>::kFloats; };
+  for (int row = blockIdx.y; row < min(kTile, s.nq * a.group - r0); row += gridDim.y) {
+    __syncthreads();   // the row before is done with LDS
+    float m = -INFINITY, l = 0.f;
+    if (tid < pieces) {
+      m = part(tid)[kTile * HD + row];
+      l = part(tid)[kTile * HD + kTile + row];
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    // a piece without keys for the row counts for nothing
+    const float by = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+    if (tid < pieces) weight[tid] = by;
+    l = wave_sum(l == 0.f ? 0.f : l * by);
+    if (lane == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int col = tid % kCols, deal = tid / kCols;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int p = deal; p < pieces; p += kDeal) {
+      const f32x4 y = *(const f32x4*)(part(p) + row * HD + 4 * col);
+      const float w = weight[p];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = w == 0.f ? v[e] : fmaf(y[e], w, v[e]);
+    }
+    sums[deal][col] = v;
+    __syncthreads();
+    if (deal != 0) continue;
+#pragma unroll
+    for (int d = 1; d < kDeal; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += sums[d][col][e];
+    const int qi = (r0 + row) / a.group, qh = hk * a.group + (r0 + row) % a.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (4 * col < a.D) {
+      bf16x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (bf16)(v[e] * inv);
+      *(bf16x4*)(a.o.p + (int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + 4 * col) = o;
+    }
+    if (a.lse && col == 0) a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
   }
-  const int qi = (r0 + row) / a.group, qh = hk * a.group + (r0 + row) % a.group;
-  if (ch < a.D) a.o.p[(int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + ch] = (bf16)(l == 0.f ? 0.f : x / l);
-  if (a.lse && ch == 0) a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
@@ -662,7 +853,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   using T = Tile<HD>;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * T::kBytes];   // [buffer][K, V]
+  __shared__ __attribute__((aligned(1024))) char smem[8 * T::kBytes];   // [tile % 4][K, V]
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
   const Block blk = block_of(a.cu_q, a.tq, a.seqs, slots - 1 - (int)(blockIdx.x / a.heads));
@@ -706,7 +897,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   lds_char* const lds = (lds_char*)(uintptr_t)base;
   auto issue = [&](int t) {
     const u32x4 kr = rows_rsrc(kb, a.k.t, t * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, t * kTile, s.nk, a.D);
-    const uint32_t to = base + (t & 1) * 2 * T::kBytes + wave * kMine * 1024;
+    const uint32_t to = base + (t & 3) * 2 * T::kBytes + wave * kMine * 1024;
     static_for<0, kMine>([&](auto p) {
       dma16<p * 1024>(kr, to, koff[p], 0);
       dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
@@ -716,12 +907,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
+  loaded();
   if (tiles > 0) issue(0);
+  if (tiles > 1) issue(1);
   auto step = [&](auto masked, int t) {
     constexpr bool MASKED = decltype(masked)::value;
-    wait_and_sync();
-    if (t + 1 < tiles) issue(t + 1);
-    lds_char* const kt = lds + (t & 1) * 2 * T::kBytes;
+    wait_and_sync_but<2 * kMine>(t + 1 >= tiles);
+    if (t + 2 < tiles) issue(t + 2);
+    lds_char* const kt = lds + (t & 3) * 2 * T::kBytes;
     const int k0 = t * kTile;
     if (MASKED && k0 >= lim_max) return;
     at.again();
@@ -777,6 +970,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
   bf16x8 b[T::kT];
   load_row<HD>(kv.p + (int64_t)(s.k0 + j) * kv.t + hk * kv.h, j < s.nk, a.D, b);
+  loaded();
   // a tile's copies are dealt to the 8 waves: Q to the first 4, dO to the others
   constexpr int kMine = T::kCopies / 4;
   const HeadView<const bf16> from = makes_dv ? a.q : a.d_o;
@@ -917,8 +1111,6 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
 
 int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
 
-constexpr int kMaxParts = 256;   // workgroups of the split walk: its rings leave room for one on a compute unit
-
 // Whether the keys are split over the workgroups: where there are few queries a sequence, so that a block of 128 rows would be
 // mostly empty, and the lengths' products stay below kMostWork.
 bool split(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
@@ -940,8 +1132,9 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
     if (split(a.seqs, a.tq, a.tk, a.heads, a.kv_heads)) {
       a.part = (float*)ws;
       a.max_parts = kMaxParts;
+      const int64_t rows = std::min<int64_t>(kTile, ceil_div((int64_t)a.tq * a.group, a.seqs));   // a sequence's, on average
       hipLaunchKernelGGL((packed_split_kernel<HD>), dim3(kMaxParts), dim3(256), 0, stream, a);
-      hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(kMaxParts - 1, kTile * HD / 256), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((packed_join_kernel<HD>), dim3(kMaxParts - 1, (unsigned)rows), dim3(256), 0, stream, a);
     } else {
       hipLaunchKernelGGL((packed_forward_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
     }
