@@ -191,7 +191,9 @@ int fvsr_packed_attention(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads*
 }
 
 size_t fvsr_packed_attention_backward_workspace(const fvsr_packed* p, int heads, int kv_heads) {
-  return !p || p->tokens_q <= 0 || heads <= 0 || kv_heads <= 0 ? 0 : packed_backward_workspace(p->tokens_q, heads);
+  return !p || p->sequences <= 0 || p->tokens_q < 0 || p->tokens_k < 0 || kv_heads <= 0 || heads < kv_heads
+             ? 0
+             : packed_backward_workspace(p->sequences, p->tokens_q, p->tokens_k, heads, kv_heads, p->channels);
 }
 
 int fvsr_packed_attention_backward(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads* d_o, const fvsr_heads* q,
@@ -208,7 +210,7 @@ int fvsr_packed_attention_backward(fvsr_ctx* ctx, const fvsr_packed* p, const fv
       (rc = check_bf16_view(dk, "dk", k->heads, tk)) || (rc = check_bf16_view(dv, "dv", k->heads, tk)))
     return rc;
   if (tq == 0 && tk == 0) return FVSR_OK;
-  if ((rc = check_grid(p, tq, q->heads)) || (rc = check_grid(p, tk, k->heads))) return rc;
+  if ((rc = check_grid(p, tq, q->heads)) || (rc = check_grid(p, tk, k->heads))) return rc;   // (parts only where blocks are few)
   FVSR_REQUIRE(lse || tq == 0, FVSR_ERR_INVALID_ARG, "lse is NULL");
   const size_t need = fvsr_packed_attention_backward_workspace(p, q->heads, k->heads);
   FVSR_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), FVSR_ERR_INVALID_ARG,

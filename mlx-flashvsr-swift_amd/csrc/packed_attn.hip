@@ -948,9 +948,10 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int pair = wave & 3;
   const bool makes_dv = wave < 4;
-  const int hk = blockIdx.x % a.kv_heads;
-  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.kv_heads);   // the first keys, which most queries see, first
-  if (a.clear && blk.hi > blk.lo) {
+  const int part = blockIdx.x % a.dkv_parts, hk = blockIdx.x / a.dkv_parts % a.kv_heads;
+  // the first keys, which most queries see, first
+  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.dkv_parts / a.kv_heads);
+  if (a.clear && part == 0 && blk.hi > blk.lo) {
     clear_rows(a.dk, hk, blk.lo, blk.hi, a.D);
     clear_rows(a.dv, hk, blk.lo, blk.hi, a.D);
   }
@@ -965,7 +966,10 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   const int t0 = a.causal ? min(tiles, max(0, blk.row - off) / kTile) : 0;
   const int t1 = a.causal ? min(tiles, max(0, blk.row + kRows - 1 - off + kTile - 1) / kTile) : 0;
   const int t2 = max(t1, min(tiles, s.nq / kTile));   // the last tile may not be whole
-  const int steps = (tiles - t0) * a.group;
+  // of the tiles of all the group's heads, those of this part: the first is tile `from_t` of head `from_h`
+  const int all = (tiles - t0) * a.group, begin = (int)((int64_t)all * part / a.dkv_parts);
+  const int steps = (int)((int64_t)all * (part + 1) / a.dkv_parts) - begin;
+  const int from_h = steps > 0 ? begin / (tiles - t0) : 0, from_t = steps > 0 ? t0 + begin % (tiles - t0) : t0;
 
   const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
   bf16x8 b[T::kT];
@@ -995,7 +999,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   // the tile to be requested next, and the one that this wave works on
-  int ih = hk * a.group, it = t0, in = 0;
+  int ih = hk * a.group + from_h, it = from_t, in = 0;
   auto request = [&] {
     if (in < steps) issue(ih, it, in);
     ++in;
@@ -1005,7 +1009,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
     }
   };
   // the copies of one step may still be under way
-  auto landed = [&](bool all) {
+  auto wait_for = [&](bool all) {
     fence();
     if (all) FVSR_WAIT_VM_LGKM0(0);
     else if (wave == 0) FVSR_WAIT_VM_LGKM0(kMine + 1);
@@ -1053,60 +1057,80 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
     }
     add_times<HD, MASKED>(qt, at, ds, lo, hi, acc);
   };
-  // one loop for each kind of wave, with the same barriers: step n is the first kind's tile n and the second kind's tile n - 1
+  // The walk of one kind of wave: `work` for each tile of the part. A step is a tile of the first kind, and of the second kind
+  // the one before: `ahead` steps less are left to be waited for.
+  auto walk = [&](auto&& work, int ahead) {
+    int t = from_t;
+    for (int n = 0; n < steps;) {
+      const int end = n + min(steps - n, tiles - t);   // to the head's last tile
+      auto run = [&](auto masked, int until) {
+        for (; t < until && n < end; ++t, ++n) {
+          wait_for(n + ahead >= steps);
+          request();
+          work(masked, t, n);
+        }
+      };
+      run(std::true_type{}, t1);
+      run(std::false_type{}, t2);
+      run(std::true_type{}, tiles);
+      t = t0;
+    }
+  };
   request();
   request();
   if (makes_dv) {
-    int n = 0;
-    for (int h = 0; h < a.group; ++h) {
-      int t = t0;
-      for (; t < t1; ++t, ++n) {
-        landed(n + 1 >= steps);
-        request();
-        first(std::true_type{}, t, n);
-      }
-      for (; t < t2; ++t, ++n) {
-        landed(n + 1 >= steps);
-        request();
-        first(std::false_type{}, t, n);
-      }
-      for (; t < tiles; ++t, ++n) {
-        landed(n + 1 >= steps);
-        request();
-        first(std::true_type{}, t, n);
-      }
-    }
-    landed(true);
+    walk(first, 1);
+    wait_for(true);
   } else {
-    int n = 0;
-    landed(1 >= steps);
+    wait_for(1 >= steps);
     request();
-    for (int h = 0; h < a.group; ++h) {
-      int t = t0;
-      for (; t < t1; ++t, ++n) {
-        landed(n + 2 >= steps);
-        request();
-        second(std::true_type{}, t, n);
-      }
-      for (; t < t2; ++t, ++n) {
-        landed(n + 2 >= steps);
-        request();
-        second(std::false_type{}, t, n);
-      }
-      for (; t < tiles; ++t, ++n) {
-        landed(n + 2 >= steps);
-        request();
-        second(std::true_type{}, t, n);
-      }
-    }
+    walk(second, 2);
   }
   if (j >= s.room) return;
   if (j >= s.nk) {   // not in use: seen by none
 #pragma unroll
     for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   }
+  if (a.dkv_parts > 1) {   // for packed_dkv_join_kernel: [part][dK, dV][key][head][HD]
+    float* const row = a.part + ((((int64_t)part * 2 + (makes_dv ? 1 : 0)) * a.tk + s.k0 + j) * a.kv_heads + hk) * HD;
+#pragma unroll
+    for (int d = 0; d < T::kD; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *(f32x4*)(row + 32 * d + 8 * c + 4 * g) = f32x4{acc[d][4 * c], acc[d][4 * c + 1], acc[d][4 * c + 2], acc[d][4 * c + 3]};
+    return;
+  }
   const HeadView<bf16> to = makes_dv ? a.dv : a.dk;
   store_row<HD>(to.p + (int64_t)(s.k0 + j) * to.t + hk * to.h, a.D, acc, makes_dv ? 1.f : a.scale);
+}
+
+// adds up the parts of dK and dV of a quarter of a block of keys, in their order
+template <int HD>
+__global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
+  const int hk = blockIdx.x % a.kv_heads;
+  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.kv_heads);
+  if (blk.b < 0 || blk.b >= a.seqs) return;
+  const Span s = span_of(a, blk.b);
+  constexpr int kCols = HD / 4, kEach = kRows / 4;
+  const int64_t stride = (int64_t)2 * a.tk * a.kv_heads * HD;
+#pragma unroll 2
+  for (int e = threadIdx.x; e < 2 * kEach * kCols; e += 256) {
+    const int col = e % kCols, j = blk.row + (int)blockIdx.y * kEach + e / kCols % kEach, v = e / kCols / kEach;
+    if (j >= s.room || 4 * col >= a.D) continue;
+    const float* p = a.part + (((int64_t)v * a.tk + s.k0 + j) * a.kv_heads + hk) * HD + 4 * col;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < a.dkv_parts; ++i) {
+      const f32x4 y = *(const f32x4*)(p + i * stride);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] += y[c];
+    }
+    bf16x4 o;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = (bf16)(x[c] * (v ? 1.f : a.scale));
+    const HeadView<bf16> to = v ? a.dv : a.dk;
+    *(bf16x4*)(to.p + (int64_t)(s.k0 + j) * to.t + hk * to.h + 4 * col) = o;
+  }
 }
 
 int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
@@ -1145,14 +1169,30 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
   return FVSR_OK;
 }
 
-size_t packed_backward_workspace(int64_t tq, int heads) { return (size_t)tq * heads * 2 * sizeof(float); }
+// Parts that the queries of a block of keys are cut into, where the blocks are too few to fill the card: each costs a round trip
+// of its sums through memory, so that it is to have a few tens of steps.
+constexpr int kDkvBlocks = 1024, kDkvSteps = 32, kMostDkvParts = 16;
+int dkv_parts(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
+  const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads, steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(kDkvBlocks, std::max<int64_t>(1, blocks)), steps / kDkvSteps, kMostDkvParts}));
+}
+size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 2 * sizeof(float) + 255) & ~(size_t)255; }
+
+size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D) {
+  const int parts = dkv_parts(seqs, tq, tk, heads, kv_heads);
+  return stat_bytes(tq, heads) + (parts > 1 ? (size_t)parts * 2 * tk * kv_heads * (D <= 64 ? 64 : 128) * sizeof(float) : 0);
+}
 
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {
   a.stat = (float*)ws;
+  a.part = (float*)((char*)ws + stat_bytes(a.tq, a.heads));
+  a.dkv_parts = dkv_parts(a.seqs, a.tq, a.tk, a.heads, a.kv_heads);
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
+    const unsigned blocks = (unsigned)(slots(a.tk, a.seqs) * a.kv_heads);
     hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3((unsigned)(slots(a.tk, a.seqs) * a.kv_heads)), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3(blocks * a.dkv_parts), dim3(512), 0, stream, a);
+    if (a.dkv_parts > 1) hipLaunchKernelGGL((packed_dkv_join_kernel<HD>), dim3(blocks, 4), dim3(256), 0, stream, a);
   };
   if (a.D <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});

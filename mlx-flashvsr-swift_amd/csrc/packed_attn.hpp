@@ -15,7 +15,8 @@ struct PackedArgs {
   HeadView<bf16> o, dq, dk, dv;   // o is read by the backward pass
   float* lse;                     // (heads, tq), natural logarithms; may be null in the forward pass
   float* stat;                    // (heads, tq, 2) lse in log2 units and the sum of dO O, from the dQ kernel to the dK, dV kernel
-  float* part;                    // partial results of the split walk
+  float* part;                    // partial results of the split walk, or of dK and dV
+  int dkv_parts;                  // parts that a block's queries are cut into
   const int32_t *cu_q, *cu_k, *used_k;   // used_k may be null
   int seqs, tq, tk;
   int heads, kv_heads, group, D, causal;
@@ -26,7 +27,7 @@ struct PackedArgs {
 
 size_t packed_forward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D);
 int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream);
-size_t packed_backward_workspace(int64_t tq, int heads);
+size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D);
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream);
 
 }  // namespace fvsr

@@ -21,33 +21,24 @@ where autograd records. An `out` must not overlap what the call reads, but where
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
+import struct
+import threading
 
 import torch
 
-from . import _abi
-from ._abi import FVSRError, Heads, Packed, lib
-from .train8 import (Blocks8, _CODE, _check, _ctx, _current, _detached, _kind, _one_device, _out, _out8, _p, _p8, _param,
-                     _params, _raw_stream, _refuse, _same)
+from . import Context, _abi
+from ._abi import DTYPE_F32, Heads, Packed, lib
+from .train8 import Blocks8, _CODE, _check, _current, _detached, _kind, _out, _out8, _p, _p8, _param, _params, _raw_stream, _refuse, _same
 
 __all__ = ["rms_norm", "rms_norm_backward", "rotary", "rotary_backward", "rotary_frequencies", "grid_positions",
            "packed_attention", "packed_attention_backward"]
 
 _BF16 = (torch.bfloat16,)
-
-
-# ----------------------------------------------------------------------------------------------------------------------
-# root-mean-square norm
-# ----------------------------------------------------------------------------------------------------------------------
-def _rows(x, name: str) -> torch.Tensor:
-    """(L, C) rows of contiguous channels, at any distance from each other (a part of a wider tensor's rows)."""
-    if _kind(x, name, torch.Tensor).dtype not in _CODE:
-        _refuse(name, f"unsupported dtype {x.dtype} (float32 or bfloat16)")
-    _detached(x, name)
-    x = _unbatched(x, name, 2)
-    if x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        _refuse(name, f"expected (L, C) rows of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
-    return x
+_FLOATS = (torch.float32, torch.bfloat16)
+_Tensor = torch.Tensor
+_recording = torch.is_grad_enabled
 
 
 def _unbatched(x, name: str, dims: int):
@@ -60,8 +51,54 @@ def _unbatched(x, name: str, dims: int):
     return x
 
 
-def _row_stride(x) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _tensor(x, name: str, dtypes, dims: int):
+    """x, a tensor of one of these types that autograd does not wait for, without a leading batch of 1."""
+    if not isinstance(x, _Tensor):
+        _kind(x, name, _Tensor)
+    if x.dtype not in dtypes:
+        _refuse(name, f"unsupported dtype {x.dtype} ({' or '.join(str(d)[6:] for d in dtypes)})")
+    if x.requires_grad and _recording():
+        _detached(x, name)
+    return x if x.dim() == dims else _unbatched(x, name, dims)
+
+
+def _device(first, name: str, *more) -> int:
+    """The index of the HIP device of the first operand, which the others (None: skipped) share. Checked after every shape, before a
+    pointer reaches the library."""
+    if not first.is_cuda:
+        _refuse(name, f"expected a tensor on a HIP device, got {first.device}")
+    index = first.get_device()
+    for t, n in more:
+        if t is not None and (t.get_device() if isinstance(t, _Tensor) else t.codes.get_device()) != index:
+            _refuse(n, f"expected a tensor on {first.device}, got {t.device}")
+    return index
+
+
+def _handle(index: int):
+    found = Context._by_device.get(index)
+    return (Context.get(index) if found is None else found).handle
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# root-mean-square norm
+# ----------------------------------------------------------------------------------------------------------------------
+def _rows(x, name: str):
+    """((L, C) rows of contiguous channels, L, C, elements between rows): a part of a wider tensor's rows, maybe."""
+    x = _tensor(x, name, _FLOATS, 2)
+    rows, c = x.shape
+    if x.is_contiguous() and c > 0:
+        return x, rows, c, c
+    if c < 1 or (c > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < c):
+        _refuse(name, f"expected (L, C) rows of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
+    return x, rows, c, (x.stride(0) if rows > 1 else c)
+
+
+def _like(x, name: str, rows: int, c: int, dtype):
+    """A contiguous (rows, c) operand or output of this type, or None."""
+    if x is None or (isinstance(x, _Tensor) and x.dtype is dtype and x.dim() == 2 and x.shape == (rows, c) and x.is_contiguous()
+                     and not x.requires_grad):
+        return x
+    return _out(x, name, (rows, c), dtype)
 
 
 def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, want_stats: bool = False, quantized: bool = False,
@@ -74,33 +111,37 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
     if stream is not None:
         with _current(stream, x):
             return rms_norm(x, weight, eps, residual, want_stats, quantized, out=out, out_sum=out_sum)
-    x2 = _rows(x, "x")
-    rows, c = x2.shape
-    weight = _param(weight, "weight", c)
-    r = _out(residual, "residual", (rows, c), x2.dtype)
+    x2, rows, c, stride = _rows(x, "x")
+    dtype = x2.dtype
+    w = _param(weight, "weight", c)
+    r = _like(residual, "residual", rows, c, dtype)
     if r is None and out_sum is not None:
         _refuse("out_sum", "there is no sum without a residual")
-    s = _out(out_sum, "out_sum", (rows, c), x2.dtype)
-    y = _out8(out, "out", (rows, c)) if quantized else _out(out, "out", (rows, c), x2.dtype)
-    dev = _one_device(x2, "x", (weight, "weight"), (r, "residual"), (out, "out"), (s, "out_sum"))
-    kind, w, _ = _params(x2.dtype, weight)
-    total = out_sum
+    s = _like(out_sum, "out_sum", rows, c, dtype)
+    y = _out8(out, "out", (rows, c)) if quantized else _like(out, "out", rows, c, dtype)
+    dev = _device(x2, "x", (w, "weight"), (r, "residual"), (y, "out"), (s, "out_sum"))
+    kind = DTYPE_F32
+    if w is not None and w.dtype is not torch.float32:
+        kind, w, _ = _params(dtype, w)
+    total, result = out_sum, out
     if r is not None and s is None:
-        total = s = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if want_stats else None
-    result = out
+        total = s = x.new_empty(x.shape)
+    rstd = x.new_empty(rows, dtype=torch.float32) if want_stats else None
+    yp = yc = ys = None
     if quantized:
-        if result is None:
-            result = Blocks8.empty(rows, c, dev)
-        yp, (yc, ys) = None, _p8(result)
+        if y is None:
+            result = y = Blocks8.empty(rows, c, x2.device)
+        yc, ys = _p8(y)
     else:
         if y is None:
-            result = y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if s is not None and y.data_ptr() == s.data_ptr() and rows:
+            result = y = x.new_empty(x.shape)
+        yp = y.data_ptr()
+        if s is out_sum is not None and yp == s.data_ptr() and rows:
             _refuse("out", "the norm and the sum need memory of their own")
-        yp, yc, ys = y.data_ptr(), None, None
-    _check(lib.fvsr_rms_norm(_ctx(dev), _CODE[x2.dtype], x2.data_ptr(), _row_stride(x2), _p(r), rows, c, float(eps), kind, _p(w),
-                             yp, yc, ys, _p(s), _p(rstd), _raw_stream(dev.index)), "fvsr_rms_norm")
+    rc = lib.fvsr_rms_norm(_handle(dev), _CODE[dtype], x2.data_ptr(), stride, _p(r), rows, c, eps, kind, _p(w), yp, yc, ys, _p(s),
+                           _p(rstd), _raw_stream(dev))
+    if rc:
+        _check(rc, "fvsr_rms_norm")
     return result, total, rstd
 
 
@@ -113,68 +154,86 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
     if stream is not None:
         with _current(stream, dy):
             return rms_norm_backward(dy, total, rstd, weight, dsum, want_weight, out=out)
-    d2 = _rows(dy, "dy")
-    if not d2.is_contiguous():
+    d2, rows, c, stride = _rows(dy, "dy")
+    dtype = d2.dtype
+    if stride != c:
         _refuse("dy", "expected a contiguous tensor")
-    rows, c = d2.shape
-    t2 = _rows(total, "total")
-    _same("total", t2.shape, (rows, c), t2.dtype, d2.dtype)
-    _same("rstd", _kind(rstd, "rstd", torch.Tensor).shape, (rows,), rstd.dtype, torch.float32)
+    t2, n, m, stride = _rows(total, "total")
+    if (n, m) != (rows, c) or t2.dtype is not dtype:
+        _same("total", t2.shape, (rows, c), t2.dtype, dtype)
+    if not isinstance(rstd, _Tensor) or rstd.shape != (rows,) or rstd.dtype is not torch.float32:
+        _same("rstd", _kind(rstd, "rstd", _Tensor).shape, (rows,), rstd.dtype, torch.float32)
     _detached(rstd, "rstd")
     if not rstd.is_contiguous():
         _refuse("rstd", "expected a contiguous tensor")
-    weight = _param(weight, "weight", c)
-    ds = _out(dsum, "dsum", (rows, c), d2.dtype)
-    o = _out(out, "out", (rows, c), d2.dtype)
-    dev = _one_device(d2, "dy", (t2, "total"), (rstd, "rstd"), (weight, "weight"), (ds, "dsum"), (o, "out"))
-    kind, w, _ = _params(d2.dtype, weight)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev) if o is None else o
+    w = _param(weight, "weight", c)
+    ds = _like(dsum, "dsum", rows, c, dtype)
+    o = _like(out, "out", rows, c, dtype)
+    dev = _device(d2, "dy", (t2, "total"), (rstd, "rstd"), (w, "weight"), (ds, "dsum"), (o, "out"))
+    kind = DTYPE_F32
+    if w is not None and w.dtype is not torch.float32:
+        kind, w, _ = _params(dtype, w)
+    dx = out
+    if o is None:
+        dx = o = dy.new_empty(dy.shape)
     dw = ws = None
     nbytes = 0
     if want_weight:
         nbytes = lib.fvsr_rms_norm_backward_workspace(rows, c)
-        dw = torch.empty(c, dtype=torch.float32, device=dev)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _check(lib.fvsr_rms_norm_backward(_ctx(dev), _CODE[d2.dtype], d2.data_ptr(), t2.data_ptr(), _row_stride(t2), rstd.data_ptr(),
-                                      _p(ds), rows, c, kind, _p(w), dx.data_ptr(), _p(dw), _p(ws), nbytes, _raw_stream(dev.index)),
-           "fvsr_rms_norm_backward")
-    return (dx if out is None else out), dw
+        dw = dy.new_empty(c, dtype=torch.float32)
+        ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    rc = lib.fvsr_rms_norm_backward(_handle(dev), _CODE[dtype], d2.data_ptr(), t2.data_ptr(), stride, rstd.data_ptr(), _p(ds), rows,
+                                    c, kind, _p(w), o.data_ptr(), _p(dw), _p(ws), nbytes, _raw_stream(dev))
+    if rc:
+        _check(rc, "fvsr_rms_norm_backward")
+    return dx, dw
 
 
 # ----------------------------------------------------------------------------------------------------------------------
 # heads
 # ----------------------------------------------------------------------------------------------------------------------
-def _heads(x, name: str, dtypes) -> torch.Tensor:
-    """(L, H, D) with contiguous channels; heads and tokens at any distance (parts of one projection's rows)."""
-    if _kind(x, name, torch.Tensor).dtype not in dtypes:
-        _refuse(name, f"unsupported dtype {x.dtype} ({' or '.join(str(d)[6:] for d in dtypes)})")
-    _detached(x, name)
-    x = _unbatched(x, name, 3)
-    if x.shape[1] < 1 or x.shape[2] < 1 or (x.shape[2] > 1 and x.stride(2) != 1):
-        _refuse(name, f"expected (L, H, D) heads of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
-    return x
+class _Structs(threading.local):
+    """A thread's memory for the structs of one call, which the library reads before it returns: filled by struct.pack_into, at a
+    tenth of the time that ctypes' fields take."""
+    view, packed = struct.Struct("@Piqq"), struct.Struct("@PPPiqqiif")
+
+    def __init__(self):
+        self.memory = C.create_string_buffer(1024)
+        at = C.addressof(self.memory)
+        self.views, self.seqs = [at + 64 * i for i in range(9)], at + 640
+
+    def heads(self, i: int, t, h: int, ts: int, hs: int) -> int:
+        self.view.pack_into(self.memory, 64 * i, t.data_ptr(), h, ts, hs)
+        return self.views[i]
+
+    def sequences(self, *fields) -> int:
+        self.packed.pack_into(self.memory, 640, *fields)
+        return self.seqs
 
 
-def _out_heads(out, name: str, like: torch.Tensor):
-    """A caller's output of heads (or None): no two elements at one address."""
-    if out is None:
-        return None
-    o = _heads(out, name, (like.dtype,))
-    _same(name, o.shape, like.shape)
-    n, h, d = o.shape
-    ts, hs = (o.stride(0) if n > 1 else 1 << 62), (o.stride(1) if h > 1 else 1 << 62)
-    if not (hs >= d and (n == 1 or h == 1 or ts >= (h - 1) * hs + d or hs >= (n - 1) * ts + d) and ts >= d):
-        _refuse(name, f"rows that overlap: {tuple(o.shape)} with strides {o.stride()}")
-    return o
+_structs = _Structs()
+assert _Structs.view.size == C.sizeof(Heads) <= 64 and _Structs.packed.size <= C.sizeof(Packed) <= 384
 
 
-def _view(x) -> Heads:
+def _heads(x, name: str, dtypes):
+    """((L, H, D) heads of contiguous channels, L, H, D, elements between tokens, between heads): heads and tokens at any distance
+    (parts of one projection's rows)."""
+    x = _tensor(x, name, dtypes, 3)
     n, h, d = x.shape
-    return Heads(x.data_ptr(), h, x.stride(0) if n > 1 else h * d, x.stride(1) if h > 1 else d)
+    ts, hs, cs = x.stride()
+    if h < 1 or d < 1 or (d > 1 and cs != 1):
+        _refuse(name, f"expected (L, H, D) heads of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
+    return x, n, h, d, (ts if n > 1 else h * d), (hs if h > 1 else d)
 
 
-def _ref(view):
-    return None if view is None else C.byref(view)
+def _out_heads(out, name: str, n: int, h: int, d: int, dtype):
+    """A caller's output of heads, as _heads gives it: no two elements at one address."""
+    o = _heads(out, name, (dtype,))
+    _same(name, o[0].shape, (n, h, d))
+    ts, hs = (o[4] if n > 1 else 1 << 62), (o[5] if h > 1 else 1 << 62)
+    if not (hs >= d and ts >= d and (n == 1 or h == 1 or ts >= (h - 1) * hs + d or hs >= (n - 1) * ts + d)):
+        _refuse(name, f"rows that overlap: {tuple(o[0].shape)} with strides {o[0].stride()}")
+    return o
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -209,96 +268,138 @@ def rotary_backward(dq: torch.Tensor, dk, positions: torch.Tensor, frequencies: 
     return _turn(dq, dk, positions, frequencies, axes, halves, stream, out, 1)
 
 
+@functools.lru_cache(64)
+def _axes(axes: tuple):
+    """(number of axes, pairs, the pairs of each as the library reads them)."""
+    axes = tuple(int(p) for p in axes)
+    if not 1 <= len(axes) <= 3 or min(axes) < 0 or sum(axes) < 1:
+        raise ValueError
+    return len(axes), sum(axes), struct.pack(f"{len(axes)}i", *axes)
+
+
 def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
     if stream is not None:
         with _current(stream, q):
             return _turn(q, k, positions, frequencies, axes, halves, None, out, back)
-    q3 = _heads(q, "q", tuple(_CODE))
-    k3 = None if k is None else _heads(k, "k", (q3.dtype,))
-    n, _, d = q3.shape
-    if k3 is not None and (k3.shape[0], k3.shape[2]) != (n, d):
-        _refuse("k", f"expected {n} tokens and {d} channels a head as q has, got {tuple(k3.shape)}")
+    q3, n, h, d, qt, qh = _heads(q, "q", _FLOATS)
+    dtype = q3.dtype
+    k3 = None
+    if k is not None:
+        k3, kn, hk, kd, kt, kh = _heads(k, "k", (dtype,))
+        if kn != n or kd != d:
+            _refuse("k", f"expected {n} tokens and {d} channels a head as q has, got {tuple(k3.shape)}")
     try:
-        axes = tuple(int(p) for p in axes)
+        count, pairs, packed = _axes(tuple(axes))
     except (TypeError, ValueError):
-        _refuse("axes", "expected the pairs of each axis")
-    if not 1 <= len(axes) <= 3 or min(axes) < 0 or not 1 <= sum(axes) <= d // 2 or d % 2:
+        count, pairs = 0, 0
+    if not count or 2 * pairs > d or d % 2:
         _refuse("axes", f"expected 1 to 3 axes of 1 to {d // 2} pairs together, got {axes} for {d} channels")
-    if _kind(positions, "positions", torch.Tensor).dtype not in (torch.int32, torch.int64):
+    wide = _kind(positions, "positions", _Tensor).dtype is torch.int64
+    if not wide and positions.dtype is not torch.int32:
         _refuse("positions", f"unsupported dtype {positions.dtype} (int32 or int64)")
-    if tuple(positions.shape) != (len(axes), n) and not (len(axes) == 1 and tuple(positions.shape) == (n,)):
-        _refuse("positions", f"expected ({len(axes)}, {n}), got {tuple(positions.shape)}")
-    _same("frequencies", _kind(frequencies, "frequencies", torch.Tensor).shape, (sum(axes),), frequencies.dtype, torch.float64)
+    if positions.shape != (count, n) and not (count == 1 and positions.shape == (n,)):
+        _refuse("positions", f"expected ({count}, {n}), got {tuple(positions.shape)}")
+    if not isinstance(frequencies, _Tensor) or frequencies.shape != (pairs,) or frequencies.dtype is not torch.float64:
+        _same("frequencies", _kind(frequencies, "frequencies", _Tensor).shape, (pairs,), frequencies.dtype, torch.float64)
     _detached(frequencies, "frequencies")
     if not (positions.is_contiguous() and frequencies.is_contiguous()):
         _refuse("positions", "expected contiguous positions and frequencies")
-    oq, ok = out if out is not None else (None, None)
-    if ok is not None and k3 is None:
-        _refuse("out", "there is no k to write")
-    yq, yk = _out_heads(oq, "out", q3), None if k3 is None else _out_heads(ok, "out", k3)
-    dev = _one_device(q3, "q", (k3, "k"), (positions, "positions"), (frequencies, "frequencies"), (yq, "out"), (yk, "out"))
+    oq = ok = yq = yk = None
+    if out is not None:
+        oq, ok = out
+        if ok is not None and k3 is None:
+            _refuse("out", "there is no k to write")
+        yq = None if oq is None else _out_heads(oq, "out", n, h, d, dtype)
+        yk = None if ok is None else _out_heads(ok, "out", n, hk, d, dtype)
+    dev = _device(q3, "q", (k3, "k"), (positions, "positions"), (frequencies, "frequencies"), (yq and yq[0], "out"),
+                  (yk and yk[0], "out"))
+    st = _structs
+    a = st.heads(0, q3, h, qt, qh)
     if yq is None:
-        oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        yq = oq.view(q3.shape)
-    if k3 is not None and yk is None:
-        ok = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        yk = ok.view(k3.shape)
-    a, b = _view(q3), _view(yq)
-    e, f = (None, None) if k3 is None else (_view(k3), _view(yk))
-    _check(lib.fvsr_rotary(_ctx(dev), _CODE[q3.dtype], C.byref(a), C.byref(b), _ref(e), _ref(f), n, d, positions.data_ptr(),
-                           positions.dtype == torch.int64, frequencies.data_ptr(), len(axes), (C.c_int32 * len(axes))(*axes),
-                           bool(halves), back, _raw_stream(dev.index)), "fvsr_rotary")
+        oq = q.new_empty(q.shape)
+        b = st.heads(1, oq, h, h * d, d)
+    else:
+        b = st.heads(1, yq[0], h, yq[4], yq[5])
+    e = f = None
+    if k3 is not None:
+        e = st.heads(2, k3, hk, kt, kh)
+        if yk is None:
+            ok = k.new_empty(k.shape)
+            f = st.heads(3, ok, hk, hk * d, d)
+        else:
+            f = st.heads(3, yk[0], hk, yk[4], yk[5])
+    rc = lib.fvsr_rotary(_handle(dev), _CODE[dtype], a, b, e, f, n, d, positions.data_ptr(), wide, frequencies.data_ptr(), count, packed,
+                         bool(halves), back, _raw_stream(dev))
+    if rc:
+        _check(rc, "fvsr_rotary")
     return oq, ok
 
 
 # ----------------------------------------------------------------------------------------------------------------------
 # attention over packed sequences
 # ----------------------------------------------------------------------------------------------------------------------
-def _aligned(x):
-    """x, or a copy of it, as the kernels read it: 16-byte aligned rows."""
-    n, h, _ = x.shape
-    if x.data_ptr() & 15 or (n > 1 and x.stride(0) & 7) or (h > 1 and x.stride(1) & 7):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+def _aligned(x) -> bool:
+    """Whether the kernels can read heads as they lie: 16-byte aligned rows."""
+    return not (x[0].data_ptr() & 15 or x[4] & 7 or x[5] & 7)
+
+
+def _ready(x):
+    """Heads as the kernels read them: as they lie, or a copy."""
+    if _aligned(x):
+        return x
+    _, n, h, d, _, _ = x
+    return x[0].clone(memory_format=torch.contiguous_format), n, h, d, h * d, d
 
 
 def _offsets(cu, name: str, n=None):
-    if _kind(cu, name, torch.Tensor).dtype != torch.int32:
-        _refuse(name, f"unsupported dtype {cu.dtype} (int32)")
-    if cu.dim() != 1 or not cu.is_contiguous() or (cu.numel() < 2 if n is None else cu.numel() != n):
+    if not isinstance(cu, _Tensor) or cu.dtype is not torch.int32:
+        _refuse(name, f"unsupported dtype {_kind(cu, name, _Tensor).dtype} (int32)")
+    m = cu.numel()
+    if cu.dim() != 1 or not cu.is_contiguous() or (m < 2 if n is None else m != n):
         _refuse(name, f"expected {'at least 2' if n is None else n} contiguous offsets, got {tuple(cu.shape)}")
-    return cu
+    return m
 
 
 def _sequences(q, k, v, cu_q, cu_k, used_k, scale):
-    """(q, k, v, cu_k, scale), checked."""
+    """(q, k, v, as _heads gives them, cu_k, offsets, scale), checked."""
     q, k, v = _heads(q, "q", _BF16), _heads(k, "k", _BF16), _heads(v, "v", _BF16)
-    d = q.shape[2]
+    n, h, d = q[1:4]
     if d % 8 or d > 128:
         _refuse("q", f"{d} channels a head: a multiple of 8, at most 128, is needed", _abi.ERR_UNSUPPORTED)
-    if k.shape[2] != d or q.shape[1] % k.shape[1]:
-        _refuse("k", f"expected heads of {d} channels that divide q's {q.shape[1]}, got {tuple(k.shape)}")
-    _same("v", v.shape, k.shape)
-    _offsets(cu_q, "cu_q")
+    if k[3] != d or h % k[2]:
+        _refuse("k", f"expected heads of {d} channels that divide q's {h}, got {tuple(k[0].shape)}")
+    if v[1:4] != k[1:4]:
+        _same("v", v[0].shape, k[0].shape)
+    m = _offsets(cu_q, "cu_q")
     if cu_k is None:
-        if k.shape[0] != q.shape[0]:
-            _refuse("k", f"expected q's {q.shape[0]} tokens where there is no cu_k, got {k.shape[0]}")
+        if k[1] != n:
+            _refuse("k", f"expected q's {n} tokens where there is no cu_k, got {k[1]}")
         cu_k = cu_q
     else:
-        _offsets(cu_k, "cu_k", cu_q.numel())
+        _offsets(cu_k, "cu_k", m)
     if used_k is not None:
-        _offsets(used_k, "used_k", cu_q.numel() - 1)
-    scale = 1 / math.sqrt(d) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        _refuse("scale", f"expected a positive finite number, got {scale}")
-    return q, k, v, cu_k, scale
+        _offsets(used_k, "used_k", m - 1)
+    if scale is None:
+        scale = d ** -0.5
+    else:
+        scale = float(scale)
+        if not (scale > 0 and math.isfinite(scale)):
+            _refuse("scale", f"expected a positive finite number, got {scale}")
+    return q, k, v, cu_k, m, scale
 
 
-def _out_aligned(out, name: str, like):
-    o = _out_heads(out, name, like)
-    if o is not None and _aligned(o) is not o:
+def _out_ready(out, name: str, like):
+    o = _out_heads(out, name, *like[1:4], like[0].dtype)
+    if not _aligned(o):
         _refuse(name, "expected 16-byte aligned rows")
     return o
+
+
+@functools.lru_cache(256)
+def _workspace(backward: bool, sequences: int, tokens_q: int, tokens_k: int, channels: int, heads: int, kv_heads: int) -> int:
+    p = Packed(None, None, None, sequences, tokens_q, tokens_k, channels, 0, 1.0)
+    size = lib.fvsr_packed_attention_backward_workspace if backward else lib.fvsr_packed_attention_workspace
+    return size(C.byref(p), heads, kv_heads)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k=None, causal: bool = False,
@@ -314,23 +415,24 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if stream is not None:
         with _current(stream, q):
             return packed_attention(q, k, v, cu_q, cu_k, causal, scale, used_k, want_lse, out=out)
-    q3, k3, v3, ck, scale = _sequences(q, k, v, cu_q, cu_k, used_k, scale)
-    o3 = _out_aligned(out, "out", q3)
-    dev = _one_device(q3, "q", (k3, "k"), (v3, "v"), (cu_q, "cu_q"), (ck, "cu_k"), (used_k, "used_k"), (o3, "out"))
-    q3, k3, v3 = _aligned(q3), _aligned(k3), _aligned(v3)
-    n, h, d = q3.shape
+    q3, k3, v3, ck, m, scale = _sequences(q, k, v, cu_q, cu_k, used_k, scale)
+    o3 = None if out is None else _out_ready(out, "out", q3)
+    dev = _device(q3[0], "q", (k3[0], "k"), (v3[0], "v"), (cu_q, "cu_q"), (ck, "cu_k"), (used_k, "used_k"), (o3 and o3[0], "out"))
+    n, h, d = q3[1:4]
     o = out
     if o3 is None:
-        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        o3 = o.view(n, h, d)
-    lse = torch.empty(h, n, dtype=torch.float32, device=dev) if want_lse else None
-    p = Packed(cu_q.data_ptr(), ck.data_ptr(), _p(used_k), cu_q.numel() - 1, n, k3.shape[0], d, bool(causal), scale)
-    hk = k3.shape[1]
-    nbytes = lib.fvsr_packed_attention_workspace(C.byref(p), h, hk)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    a, b, c, e = _view(q3), _view(k3), _view(v3), _view(o3)
-    _check(lib.fvsr_packed_attention(_ctx(dev), C.byref(p), C.byref(a), C.byref(b), C.byref(c), C.byref(e), _p(lse), out is None,
-                                     _p(ws), nbytes, _raw_stream(dev.index)), "fvsr_packed_attention")
+        o = q.new_empty(q.shape)
+        o3 = o, n, h, d, h * d, d
+    lse = q.new_empty((h, n), dtype=torch.float32) if want_lse else None
+    nbytes = _workspace(False, m - 1, n, k3[1], d, h, k3[2])
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    q3, k3, v3 = _ready(q3), _ready(k3), _ready(v3)
+    st = _structs
+    p = st.sequences(cu_q.data_ptr(), ck.data_ptr(), 0 if used_k is None else used_k.data_ptr(), m - 1, n, k3[1], d, bool(causal), scale)
+    views = [st.heads(i, x[0], x[2], x[4], x[5]) for i, x in enumerate((q3, k3, v3, o3))]
+    rc = lib.fvsr_packed_attention(_handle(dev), p, *views, _p(lse), out is None, _p(ws), nbytes, _raw_stream(dev))
+    if rc:
+        _check(rc, "fvsr_packed_attention")
     return o, lse
 
 
@@ -343,31 +445,37 @@ def packed_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor
     if stream is not None:
         with _current(stream, q):
             return packed_attention_backward(do, q, k, v, o, lse, cu_q, cu_k, causal, scale, used_k, out=out)
-    q3, k3, v3, ck, scale = _sequences(q, k, v, cu_q, cu_k, used_k, scale)
+    q3, k3, v3, ck, m, scale = _sequences(q, k, v, cu_q, cu_k, used_k, scale)
+    n, h, d = q3[1:4]
     g3, o3 = _heads(do, "do", _BF16), _heads(o, "o", _BF16)
-    _same("do", g3.shape, q3.shape)
-    _same("o", o3.shape, q3.shape)
-    n, h, d = q3.shape
-    _same("lse", _kind(lse, "lse", torch.Tensor).shape, (h, n), lse.dtype, torch.float32)
+    for x, name in ((g3, "do"), (o3, "o")):
+        if x[1:4] != q3[1:4]:
+            _same(name, x[0].shape, q3[0].shape)
+    if not isinstance(lse, _Tensor) or lse.shape != (h, n) or lse.dtype is not torch.float32:
+        _same("lse", _kind(lse, "lse", _Tensor).shape, (h, n), lse.dtype, torch.float32)
     _detached(lse, "lse")
     if not lse.is_contiguous():
         _refuse("lse", "expected a contiguous tensor")
-    outs = (None, None, None) if out is None else tuple(out)
-    if len(outs) != 3 or (out is not None and any(x is None for x in outs)):
-        _refuse("out", "expected three tensors, for dq, dk and dv")
-    views = [_out_aligned(x, "out", like) for x, like in zip(outs, (q3, k3, v3))]
-    dev = _one_device(q3, "q", (k3, "k"), (v3, "v"), (g3, "do"), (o3, "o"), (lse, "lse"), (cu_q, "cu_q"), (ck, "cu_k"),
-                      (used_k, "used_k"), *((x, "out") for x in views))
+    made = (None, None, None)
+    if out is not None:
+        out = tuple(out)
+        if len(out) != 3 or any(x is None for x in out):
+            _refuse("out", "expected three tensors, for dq, dk and dv")
+        made = [_out_ready(x, "out", like) for x, like in zip(out, (q3, k3, v3))]
+    dev = _device(q3[0], "q", (k3[0], "k"), (v3[0], "v"), (g3[0], "do"), (o3[0], "o"), (lse, "lse"), (cu_q, "cu_q"), (ck, "cu_k"),
+                  (used_k, "used_k"), *((x and x[0], "out") for x in made))
+    grads = out
     if out is None:
-        outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
-        views = [x.view(y.shape) for x, y in zip(outs, (q3, k3, v3))]
-    q3, k3, v3, g3, o3 = (_aligned(x) for x in (q3, k3, v3, g3, o3))
-    p = Packed(cu_q.data_ptr(), ck.data_ptr(), _p(used_k), cu_q.numel() - 1, n, k3.shape[0], d, bool(causal), scale)
-    nbytes = lib.fvsr_packed_attention_backward_workspace(C.byref(p), h, k3.shape[1])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    given = [_view(x) for x in (g3, q3, k3, v3, o3)]
-    made = [_view(x) for x in views]
-    _check(lib.fvsr_packed_attention_backward(_ctx(dev), C.byref(p), *map(C.byref, given), lse.data_ptr(), *map(C.byref, made),
-                                              out is None, _p(ws), nbytes, _raw_stream(dev.index)),
-           "fvsr_packed_attention_backward")
-    return outs
+        grads = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        made = [(x, *y[1:4], y[2] * d, d) for x, y in zip(grads, (q3, k3, v3))]
+    nbytes = _workspace(True, m - 1, n, k3[1], d, h, k3[2])
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    g3, q3, k3, v3, o3 = _ready(g3), _ready(q3), _ready(k3), _ready(v3), _ready(o3)
+    st = _structs
+    p = st.sequences(cu_q.data_ptr(), ck.data_ptr(), 0 if used_k is None else used_k.data_ptr(), m - 1, n, k3[1], d, bool(causal), scale)
+    a = [st.heads(i, x[0], x[2], x[4], x[5]) for i, x in enumerate((g3, q3, k3, v3, o3, *made))]
+    rc = lib.fvsr_packed_attention_backward(_handle(dev), p, *a[:5], lse.data_ptr(), *a[5:], out is None, ws.data_ptr(), nbytes,
+                                            _raw_stream(dev))
+    if rc:
+        _check(rc, "fvsr_packed_attention_backward")
+    return grads
