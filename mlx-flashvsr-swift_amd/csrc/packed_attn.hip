@@ -580,11 +580,11 @@ __device__ __forceinline__ Span lane_span(const PackedArgs& a, int b) {   // spa
 }
 
 constexpr int kMaxParts = 256;        // workgroups of the split walk: its rings leave room for one on a compute unit
-constexpr int kMinTiles = 8;          // tiles a part, at the least: two a wave
+constexpr int kMinTiles = 8;          // tiles a part, at the least (two a wave), but where items are shorter: each costs a round trip
 constexpr int kMostWork = 1 << 30;    // tiles of a call (split)
 
 // The parts, and for the tile `of(parts)` its sequence and that one's first tile. Called by the whole workgroup of 256;
-// `sm` is LDS for 12 ints. The sequence is -1 where there is no such tile. Offsets that fall could make sequences overlap and
+// `sm` is LDS for 16 ints. The sequence is -1 where there is no such tile. Offsets that fall could make sequences overlap and
 // their work pass 31 bits: none is done then.
 template <class F>
 __device__ __forceinline__ Parts find_tile(const PackedArgs& a, int* sm, F&& of, int& tile, int& b, int& first) {
@@ -595,17 +595,20 @@ __device__ __forceinline__ Parts find_tile(const PackedArgs& a, int* sm, F&& of,
     return items_of(a, s) * tiles_of(s) * a.kv_heads;
   };
   int mine = 0;
-  float about = 0.f;
+  float about = 0.f, items = 0.f;
   for (int i = b0; i < b1; ++i) {
     const int n = work_of(i);
     mine += n;
     about += (float)n;
+    items += (float)(items_of(a, lane_span(a, i)) * a.kv_heads);
   }
   about = wave_sum(about);
+  items = wave_sum(items);
   int at = wave_scan_dpp(mine);
   if (lane == 63) {
     sm[wave] = at;
     sm[8 + wave] = __float_as_int(about);
+    sm[12 + wave] = __float_as_int(items);
   }
   if (tid == 0) sm[4] = -1;
   __syncthreads();
@@ -615,7 +618,8 @@ __device__ __forceinline__ Parts find_tile(const PackedArgs& a, int* sm, F&& of,
   p.work = uniform(sm[0] + sm[1] + sm[2] + sm[3]);
   about = __int_as_float(sm[8]) + __int_as_float(sm[9]) + __int_as_float(sm[10]) + __int_as_float(sm[11]);
   if (about > 1.5f * kMostWork) p.work = 0;
-  p.parts = max(1, min(a.max_parts, p.work / kMinTiles));
+  items = __int_as_float(sm[12]) + __int_as_float(sm[13]) + __int_as_float(sm[14]) + __int_as_float(sm[15]);
+  p.parts = max(1, min(a.max_parts, max(p.work / kMinTiles, uniform((int)fminf(items, 1e6f)))));
   tile = p.work > 0 ? of(p) : -1;
   if (tile >= at && tile < at + mine) {
     for (int i = b0; i < b1; ++i) {
@@ -635,7 +639,13 @@ __device__ __forceinline__ Parts find_tile(const PackedArgs& a, int* sm, F&& of,
   return p;
 }
 
-// partial results: of slot x, 32 rows of HD floats, then the rows' references and sums
+// Partial results: of slot x, 32 rows of HD floats, then the rows' references and sums. In front of them, for each part, the item
+// that begins in it and ends in a later one.
+struct Cut {
+  int pieces, inside;        // 0 pieces: no such item; whether the part begins before the item (its piece then is the second slot)
+  int hk, r0, rows, q0;      // its key head, first row, rows in the sequence, and the sequence's first query
+  int pad[2];
+};
 template <int HD>
 struct Partial {
   static constexpr int kFloats = kTile * HD + 2 * kTile;
@@ -646,7 +656,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   using T = Tile<HD>;
   __shared__ __attribute__((aligned(1024))) char smem[4][4 * T::kBytes];   // [wave][buffer][K, V]
   __shared__ float ml[4][2][kTile];
-  __shared__ int sm[12];
+  __shared__ int sm[16];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(tid >> 6);
   if (a.clear) {   // rows of no sequence, a head a turn
     const int lo = within(uniform(a.cu_q[0]), 0, a.tq), hi = within(uniform(a.cu_q[a.seqs]), lo, a.tq);
@@ -660,6 +670,9 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   }
   int tile, b, first;
   const Parts parts = find_tile(a, sm, [&](const Parts& p) { return (int)blockIdx.x < p.parts ? p.begin(blockIdx.x) : -1; }, tile, b, first);
+  Cut* const cut = (Cut*)a.part + blockIdx.x;
+  float* const partial = a.part + kMaxParts * sizeof(Cut) / 4;
+  if (tid == 0) cut->pieces = 0;
   if (b < 0) return;
   const int begin = tile, end = parts.begin(blockIdx.x + 1);
   const uint32_t base = lds_addr(smem[wave]);
@@ -735,7 +748,8 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
     }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == tiles;
-    float* const part = a.part + (int64_t)(2 * blockIdx.x + (tile == begin ? 0 : 1)) * Partial<HD>::kFloats;
+    float* const part = partial + (int64_t)(2 * blockIdx.x + (tile == begin ? 0 : 1)) * Partial<HD>::kFloats;
+    if (tid == 0 && t0 == 0 && t1 < tiles) *cut = Cut{parts.owner(tile + tiles - 1) - (int)blockIdx.x + 1, tile > begin, hk, r0, rows, s.q0, {}};
     const int here = min(kTile, rows - r0);
     for (int e = tid; e < here * (HD / 4); e += 256) {
       const int row = e / (HD / 4), piece = e % (HD / 4);
@@ -778,28 +792,22 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   }
 }
 
-// Workgroup (x, y): rows y, y + gridDim.y, .. of the item cut by part x + 1's beginning, if that is the item's first cut. All of a row's pieces are
+// Workgroup (x, y): rows y, y + gridDim.y, .. of the item that begins in part x and ends in a later one. All of a row's pieces are
 // asked for at once: their references and sums by a thread each, then their channels by 4 to a thread, the pieces dealt to the
 // 256 / (HD / 4) groups of threads and joined in LDS.
 template <int HD>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
   constexpr int kCols = HD / 4, kDeal = 256 / kCols;
-  __shared__ int sm[12];
   __shared__ float weight[kMaxParts];
   __shared__ float red[8];
   __shared__ __attribute__((aligned(16))) f32x4 sums[kDeal][kCols];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = blockIdx.x;
-  int tile, b, first;
-  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return x + 1 < p.parts ? p.begin(x + 1) : -1; }, tile, b, first);
-  if (b < 0) return;
-  const Span s = span_of(a, b);
-  const int items = items_of(a, s), tiles = tiles_of(s);
-  const int unit = (tile - first) / tiles, begin = first + unit * tiles;
-  if (begin == tile || parts.owner(begin) != x) return;   // no cut, or not the first one
-  const int hk = unit / items, r0 = (unit - hk * items) * kTile;
-  const int pieces = parts.owner(begin + tiles - 1) - x + 1, inside = parts.begin(x) < begin ? 1 : 0;   // <= kMaxParts
-  auto part = [&](int p) { return a.part + (int64_t)(2 * (x + p) + (p == 0 ? inside : 0)) * Partial<HD>::kFloats; };
-  for (int row = blockIdx.y; row < min(kTile, s.nq * a.group - r0); row += gridDim.y) {
+  const Cut cut = ((const Cut*)a.part)[x];
+  if (cut.pieces <= 0) return;
+  const int pieces = cut.pieces;   // <= kMaxParts
+  const float* const partial = a.part + kMaxParts * sizeof(Cut) / 4;
+  auto part = [&](int p) { return partial + (int64_t)(2 * (x + p) + (p == 0 ? cut.inside : 0)) * Partial<HD>::kFloats; };
+  for (int row = blockIdx.y; row < min(kTile, cut.rows - cut.r0); row += gridDim.y) {
     __syncthreads();   // the row before is done with LDS
     float m = -INFINITY, l = 0.f;
     if (tid < pieces) {
@@ -835,15 +843,15 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
     for (int d = 1; d < kDeal; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += sums[d][col][e];
-    const int qi = (r0 + row) / a.group, qh = hk * a.group + (r0 + row) % a.group;
+    const int qi = cut.q0 + (cut.r0 + row) / a.group, qh = cut.hk * a.group + (cut.r0 + row) % a.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (4 * col < a.D) {
       bf16x4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (bf16)(v[e] * inv);
-      *(bf16x4*)(a.o.p + (int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + 4 * col) = o;
+      *(bf16x4*)(a.o.p + (int64_t)qi * a.o.t + qh * a.o.h + 4 * col) = o;
     }
-    if (a.lse && col == 0) a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
+    if (a.lse && col == 0) a.lse[(int64_t)qh * a.tq + qi] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
@@ -866,24 +874,6 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   // tiles that some row of the block sees, and that every one sees all of
   const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
-  bf16x8 q[T::kT], d_o[T::kT];
-  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
-  load_row<HD>(a.d_o.p + (int64_t)(s.q0 + i) * a.d_o.t + head * a.d_o.h, i < s.nq, a.D, d_o);
-  float lse2 = 0.f, delta = 0.f;
-  {
-    bf16x8 o[T::kT];
-    load_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, i < s.nq, a.D, o);
-#pragma unroll
-    for (int t = 0; t < T::kT; ++t)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf((float)d_o[t][e], (float)o[t][e], delta);
-    delta = pair_sum(delta);
-    if (i < s.nq) {
-      const int64_t at = (int64_t)head * a.tq + s.q0 + i;
-      lse2 = a.lse[at] * kLog2e;
-      if (g == 0) *(f32x2*)(a.stat + 2 * at) = f32x2{lse2, delta};
-    }
-  }
   const bf16* const kb = a.k.p + (int64_t)s.k0 * a.k.t + head / a.group * a.k.h;
   const bf16* const vb = a.v.p + (int64_t)s.k0 * a.v.t + head / a.group * a.v.h;
   constexpr int kMine = T::kCopies / 4;
@@ -903,13 +893,31 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
       dma16<p * 1024>(vr, to + T::kBytes, voff[p], 0);
     });
   };
+  if (tiles > 0) issue(0);
+  if (tiles > 1) issue(1);
+  bf16x8 q[T::kT], d_o[T::kT];
+  load_row<HD>(a.q.p + (int64_t)(s.q0 + i) * a.q.t + head * a.q.h, i < s.nq, a.D, q);
+  load_row<HD>(a.d_o.p + (int64_t)(s.q0 + i) * a.d_o.t + head * a.d_o.h, i < s.nq, a.D, d_o);
+  float lse2 = 0.f, delta = 0.f;
+  {
+    bf16x8 o[T::kT];
+    load_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, i < s.nq, a.D, o);
+#pragma unroll
+    for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)d_o[t][e], (float)o[t][e], delta);
+    delta = pair_sum(delta);
+    if (i < s.nq) {
+      const int64_t at = (int64_t)head * a.tq + s.q0 + i;
+      lse2 = a.lse[at] * kLog2e;
+      if (g == 0) *(f32x2*)(a.stat + 2 * at) = f32x2{lse2, delta};
+    }
+  }
   Lanes<HD> at;
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   loaded();
-  if (tiles > 0) issue(0);
-  if (tiles > 1) issue(1);
   auto step = [&](auto masked, int t) {
     constexpr bool MASKED = decltype(masked)::value;
     wait_and_sync_but<2 * kMine>(t + 1 >= tiles);
@@ -971,10 +979,6 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   const int steps = (int)((int64_t)all * (part + 1) / a.dkv_parts) - begin;
   const int from_h = steps > 0 ? begin / (tiles - t0) : 0, from_t = steps > 0 ? t0 + begin % (tiles - t0) : t0;
 
-  const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
-  bf16x8 b[T::kT];
-  load_row<HD>(kv.p + (int64_t)(s.k0 + j) * kv.t + hk * kv.h, j < s.nk, a.D, b);
-  loaded();
   // a tile's copies are dealt to the 8 waves: Q to the first 4, dO to the others
   constexpr int kMine = T::kCopies / 4;
   const HeadView<const bf16> from = makes_dv ? a.q : a.d_o;
@@ -1008,6 +1012,12 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
       ++ih;
     }
   };
+  request();
+  request();
+  const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
+  bf16x8 b[T::kT];
+  load_row<HD>(kv.p + (int64_t)(s.k0 + j) * kv.t + hk * kv.h, j < s.nk, a.D, b);
+  loaded();
   // the copies of one step may still be under way
   auto wait_for = [&](bool all) {
     fence();
@@ -1076,8 +1086,6 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
       t = t0;
     }
   };
-  request();
-  request();
   if (makes_dv) {
     walk(first, 1);
     wait_for(true);
@@ -1147,7 +1155,7 @@ bool split(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
 
 size_t packed_forward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D) {
   if (!split(seqs, tq, tk, heads, kv_heads)) return 0;
-  return (size_t)2 * kMaxParts * (D <= 64 ? Partial<64>::kFloats : Partial<128>::kFloats) * sizeof(float);
+  return kMaxParts * (sizeof(Cut) + 2 * sizeof(float) * (D <= 64 ? Partial<64>::kFloats : Partial<128>::kFloats));
 }
 
 int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
