@@ -917,28 +917,110 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
-  loaded();
-  auto step = [&](auto masked, int t) {
-    constexpr bool MASKED = decltype(masked)::value;
-    wait_and_sync_but<2 * kMine>(t + 1 >= tiles);
-    if (t + 2 < tiles) issue(t + 2);
-    lds_char* const kt = lds + (t & 3) * 2 * T::kBytes;
-    const int k0 = t * kTile;
-    if (MASKED && k0 >= lim_max) return;
-    at.again();
-    f32x16 p = rows_times<HD>(kt, at, q);
-    f32x16 dp = rows_times<HD>(kt + T::kBytes, at, d_o);
+  // tiles 0 and 1 have landed, for every wave
+  __builtin_amdgcn_s_barrier();
+  fence();
+  uint32_t row[T::kT], tr[2][T::kD];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(fmaf(p[e], a.c, -lse2)) * (dp[e] - delta);
-    if (MASKED) {
+  for (int c = 0; c < T::kT; ++c) row[c] = base + at.row(c);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dp[e] = elem_row(e) < lim - k0 - 4 * g ? dp[e] : 0.f;
+  for (int d = 0; d < T::kD; ++d) {
+    tr[0][d] = base + at.tr(0, 0, d);
+    tr[1][d] = base + at.tr(1, 0, d);
+  }
+  constexpr int kSlot = 2 * T::kBytes;
+  // operand x of a step on slot SLOT: rows of V (dP), rows of the next tile's K (its S), K transposed (dQ)
+  auto operand = [&](auto slot, auto x) {
+    constexpr int SLOT = decltype(slot)::value, X = decltype(x)::value, C = X % T::kT;
+    if constexpr (X < T::kT) {
+      return *(const lds_bf16x8*)((lds_char*)(uintptr_t)row[C] + SLOT * kSlot + T::kBytes);
+    } else if constexpr (X < 2 * T::kT) {
+      return *(const lds_bf16x8*)((lds_char*)(uintptr_t)row[C] + ((SLOT + 1) & 3) * kSlot);
+    } else {
+      constexpr int U = C / T::kD, D = C % T::kD, OFF = SLOT * kSlot + 16 * U * T::kRow;
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)tr[0][D] + OFF));
+      const i16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)tr[1][D] + OFF));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, acc);
   };
+  f32x16 sA = f32x16{}, sB = f32x16{};
+  if (tiles > 0) sA = rows_times<HD>(lds, at, q);
   int t = 0;
-  for (; t < full; ++t) step(std::false_type{}, t);
-  for (; t < tiles; ++t) step(std::true_type{}, t);
+  // A step on a tile that every row sees whole: dP of it while its P is made, S of the next tile while dS is, then dQ; a product at a
+  // time with a share of the rest behind it, as in packed_forward_kernel.
+  auto step = [&](auto slot, f32x16& s_cur, f32x16& s_nxt) {
+    constexpr int kRounds = 3 * T::kT, kAhead = 4, kExp = 16 / T::kT, kDs = (16 + T::kT - 3) / (T::kT - 2);
+    const int tt = t + decltype(slot)::value + 3;
+    const u32x4 kr = rows_rsrc(kb, a.k.t, tt * kTile, s.nk, a.D), vr = rows_rsrc(vb, a.v.t, tt * kTile, s.nk, a.D);
+    constexpr uint32_t kTo = ((decltype(slot)::value + 3) & 3) * kSlot;
+    bf16x8 op[kRounds], w[2];
+    f32x16 dp;
+    float p[16];
+    auto round = [&](auto i_c) {
+      constexpr int I = decltype(i_c)::value, C = I % T::kT;
+      if constexpr (I == 0)
+        static_for<0, kAhead>([&](auto x) { op[decltype(x)::value] = operand(slot, x); });
+      if constexpr (I + kAhead < kRounds) op[I + kAhead] = operand(slot, std::integral_constant<int, I + kAhead>{});
+      if constexpr (I < T::kT) {
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[I], d_o[C], C > 0 ? dp : f32x16{}, 0, 0, 0);
+#pragma unroll
+        for (int e = C * kExp; e < (C + 1) * kExp; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s_cur[e], a.c, -lse2));
+      } else if constexpr (I < 2 * T::kT) {
+        s_nxt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[I], q[C], C > 0 ? s_nxt : f32x16{}, 0, 0, 0);
+        if constexpr (C >= 2) {   // the last product of dP takes two rounds
+          constexpr int e0 = (C - 2) * kDs < 16 ? (C - 2) * kDs : 16, e1 = e0 + kDs < 16 ? e0 + kDs : 16;
+#pragma unroll
+          for (int e = e0; e < e1; ++e) w[e >> 3][e & 7] = (bf16)(p[e] * (dp[e] - delta));
+        }
+      } else {
+        acc[C % T::kD] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[I], w[C / T::kD], acc[C % T::kD], 0, 0, 0);
+        if constexpr (C % 2 == 0 && C / 2 < 2 * kMine) {
+          constexpr int R = C / 2;
+          if constexpr (R < kMine) dma16<R * 1024>(kr, base + kTo + wave * kMine * 1024, koff[R], 0);
+          else dma16<(R - kMine) * 1024>(vr, base + kTo + T::kBytes + wave * kMine * 1024, voff[R - kMine], 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    static_for<0, kRounds>(round);
+    wait_and_sync_but<2 * kMine>(false);   // tile t + 2, requested a step before, has landed
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (tiles > 2) issue(2);
+  if (full >= 4) {
+    wait_and_sync_but<2 * kMine>(false);
+    for (; t + 4 <= full; t += 4) {
+      step(std::integral_constant<int, 0>{}, sA, sB);
+      step(std::integral_constant<int, 1>{}, sB, sA);
+      step(std::integral_constant<int, 2>{}, sA, sB);
+      step(std::integral_constant<int, 3>{}, sB, sA);
+    }
+    acc_drain();
+  }
+  // the tiles left: up to three whole ones, then those that some rows do not see all of
+  auto last = [&](auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    wait_and_sync_but<2 * kMine>(t + 2 >= tiles);   // tiles t and t + 1 have landed
+    if (t + 3 < tiles) issue(t + 3);
+    lds_char* const kt = lds + (t & 3) * kSlot;
+    const int k0 = t * kTile;
+    if (!MASKED || k0 < lim_max) {
+      at.again();
+      f32x16 dp = rows_times<HD>(kt + T::kBytes, at, d_o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(fmaf(sA[e], a.c, -lse2)) * (dp[e] - delta);
+      if (MASKED) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = elem_row(e) < lim - k0 - 4 * g ? dp[e] : 0.f;
+      }
+      add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, acc);
+    }
+    ++t;
+    if (t < tiles) sA = rows_times<HD>(lds + (t & 3) * kSlot, at, q);
+  };
+  while (t < full) last(std::false_type{});
+  while (t < tiles) last(std::true_type{});
+  FVSR_WAIT_VM0();   // no copy outlives the workgroup's LDS
   if (i < s.nq) store_row<HD>(a.dq.p + (int64_t)(s.q0 + i) * a.dq.t + head * a.dq.h, a.D, acc, a.scale);
 }
 
