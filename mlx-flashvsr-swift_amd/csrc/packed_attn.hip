@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a block: 4 waves of 32
 constexpr int kTile = 32;       // rows of a tile of the other side
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float kRise = 4294967296.f;   // 2^32
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -59,11 +58,6 @@ __device__ __forceinline__ u32x4 rows_rsrc(const bf16* base, int64_t stride, int
   return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-}
-
-// 4 bytes a lane from a buffer into LDS at lds + 4 * lane (dma16, attn_tile.hpp, otherwise)
-__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds, int off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
 }
 
 // the compiler moves no memory access across it
@@ -112,8 +106,8 @@ struct Lanes {
 // (32 tile rows) x (32 columns, one a lane pair): the tile's rows times the lane's row b. Element i of the result is tile row
 // 8 (i / 4) + 4 (lane / 32) + i % 4.
 template <int HD>
-__device__ __forceinline__ f32x16 rows_times(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&b)[Tile<HD>::kT]) {
-  f32x16 s = f32x16{};
+__device__ __forceinline__ f32x16 rows_times(lds_char* tile, const Lanes<HD>& at, const bf16x8 (&b)[Tile<HD>::kT],
+                                             f32x16 s = f32x16{}) {
 #pragma unroll
   for (int t = 0; t < Tile<HD>::kT; ++t)
     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const lds_bf16x8*)(tile + at.row(t)), b[t], s, 0, 0, 0);
@@ -858,6 +852,19 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 // ---- backward ------------------------------------------------------------------------------------------------------------
 // Two kernels, so that nothing is added with atomics: dQ walks over the keys like the forward pass (and leaves delta), dK and dV
 // walk over the queries of the group's heads. Each makes S and dP again: 7 products in all where one kernel would make 5.
+// What dK and dV need of a query beside its rows: -lse / scale and -delta, each as three bf16 numbers whose sum is the fp32 one.
+// A product with ones adds them to S and dP in the matrix core: as operands of an addition they would have to be in 16 registers,
+// read from LDS at eight times the bytes.
+__device__ __forceinline__ bf16x8 stat_parts(float lse, float delta) {
+  auto part = [](float& x) {
+    const bf16 y = (bf16)x;
+    x -= (float)y;
+    return y;
+  };
+  const bf16 a = part(lse), b = part(lse), c = part(lse), d = part(delta), e = part(delta), f = part(delta);
+  return bf16x8{a, b, c, (bf16)0.f, d, e, f, (bf16)0.f};
+}
+
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   using T = Tile<HD>;
@@ -910,7 +917,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     if (i < s.nq) {
       const int64_t at = (int64_t)head * a.tq + s.q0 + i;
       lse2 = a.lse[at] * kLog2e;
-      if (g == 0) *(f32x2*)(a.stat + 2 * at) = f32x2{lse2, delta};
+      if (g == 0) *(bf16x8*)(a.stat + 8 * at) = stat_parts(-a.lse[at] / a.scale, -delta);
     }
   }
   Lanes<HD> at;
@@ -1024,17 +1031,26 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   if (i < s.nq) store_row<HD>(a.dq.p + (int64_t)(s.q0 + i) * a.dq.t + head * a.dq.h, a.D, acc, a.scale);
 }
 
+// Two weights, from 0 to below 2, in 16 bits each: of fp32's bits the sign and the exponent's first are 0, the next 16 are kept, rounded.
+// Off by at most 2^-10 of itself, an eighth of what rounding dS to bf16 costs in the mean square, down to 2^-126 (fp16 would lose the
+// gradients of keys whose weights are all small). An infinity or NaN does not survive, but reaches dS by delta.
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  return __builtin_amdgcn_perm((__float_as_uint(hi) << 2) + 0x8000u, (__float_as_uint(lo) << 2) + 0x8000u, 0x07060302u);
+}
+__device__ __forceinline__ float low_weight(uint32_t w) { return __uint_as_float((w & 0xffffu) << 14); }
+__device__ __forceinline__ float high_weight(uint32_t w) { return __uint_as_float((w >> 16) << 14); }
+
 // dK and dV of 128 keys: 8 waves, two to each 32 keys. One makes S, P and dV, the other, a tile of queries behind, dP, dS and dK
-// from the P that the first one leaves in LDS (in fp32: fp16 would lose the gradients of keys whose weights are all small).
+// from the P that the first one leaves in LDS (in 16 bits of its own, pack_weights).
 // So a wave holds one operand and one sum, not two (which with S and dP beside them pass the 256 registers that two waves a SIMD
 // have), and the two waves of a SIMD, one of each kind, are at the matrix core by turns.
 template <int HD>
-__global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
+__global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(PackedArgs a) {
   using T = Tile<HD>;
   constexpr int kSlot = 2 * T::kBytes;                                                      // Q, dO
   __shared__ __attribute__((aligned(1024))) char smem[4 * kSlot];                           // tile n in slot n % 4
-  __shared__ __attribute__((aligned(1024))) float stat[4][2][kTile];                        // its lse (log2 units) and delta
-  __shared__ __attribute__((aligned(16))) f32x4 handed[2][4][4][64];                         // P of tile n in n % 2, a wave pair each
+  __shared__ __attribute__((aligned(1024))) bf16x8 stat[4][64];                             // its rows' stat_parts
+  __shared__ __attribute__((aligned(16))) u32x4 handed[2][4][2][64];                         // P of tile n in n % 2, a wave pair each
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int pair = wave & 3;
   const bool makes_dv = wave < 4;
@@ -1067,31 +1083,42 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
   int voff[kMine];
 #pragma unroll
   for (int p = 0; p < kMine; ++p) voff[p] = copy_off<HD>(pair * kMine + p, lane, (int)from.t * 2, a.D);
-  const int soff = l32 * 8 + g * 4;   // lse of the tile's rows, then delta
+  const int soff = g == 0 ? l32 * 16 : (int)0x80000000;   // the tile's rows; the other lanes copy zeros
   const uint32_t base = lds_addr(smem) + (makes_dv ? 0 : T::kBytes) + pair * kMine * 1024, sbase = lds_addr(stat);
-  auto issue = [&](int h, int t, int n) {
-    const u32x4 r = rows_rsrc(from.p + (int64_t)s.q0 * from.t + h * from.h, from.t, t * kTile, s.nq, a.D);
-    static_for<0, kMine>([&](auto p) { dma16<p * 1024>(r, base + (n & 3) * kSlot, voff[p], 0); });
-    if (wave == 0) {
-      const uint64_t at = (uint64_t)(a.stat + ((int64_t)h * a.tq + s.q0 + t * kTile) * 2);
-      const u32x4 sr = {(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)((uint32_t)(at >> 32) & 0xffffu)),
-                        (uint32_t)uniform(min(s.nq - t * kTile, kTile) * 8), 0x00020000u};
-      dma4(sr, sbase + (n & 3) * 2 * kTile * 4, soff);
-    }
-  };
   lds_char* const lds = (lds_char*)(uintptr_t)lds_addr(smem);
   Lanes<HD> at;
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
-  // the tile to be requested next, and the one that this wave works on
+  // The tile that is requested next: its rows, and those left of its head. Kept from one to the next, for a scalar multiplication or
+  // two at the head of each step is a hundred cycles before the first product.
   int ih = hk * a.group + from_h, it = from_t, in = 0;
+  const bf16* rows = nullptr;
+  const bf16* stats = nullptr;
+  auto go_to = [&](int h, int t) {
+    rows = from.p + (int64_t)(s.q0 + t * kTile) * from.t + h * from.h;
+    stats = a.stat + ((int64_t)h * a.tq + s.q0 + t * kTile) * 8;
+  };
+  go_to(ih, it);
+  const int64_t tile_rows = kTile * from.t;
+  const int whole = ((kTile - 1) * (int)from.t + a.D) * 2, rest = s.nq % kTile, ragged = ((rest - 1) * (int)from.t + a.D) * 2;
+  auto rsrc = [&](const bf16* at, int bytes) {
+    return u32x4{(uint32_t)uniform((int)(uint32_t)(uint64_t)at), (uint32_t)uniform((int)((uint64_t)at >> 32 & 0xffffu)),
+                 (uint32_t)uniform(bytes), 0x00020000u};
+  };
   auto request = [&] {
-    if (in < steps) issue(ih, it, in);
+    if (in < steps) {
+      const bool end = it == tiles - 1 && rest != 0;
+      const u32x4 r = rsrc(rows, end ? ragged : whole);
+      static_for<0, kMine>([&](auto p) { dma16<p * 1024>(r, base + (in & 3) * kSlot, voff[p], 0); });
+      if (wave == 0) dma16<0>(rsrc(stats, end ? rest * 16 : kTile * 16), sbase + (in & 3) * 1024, soff, 0);
+    }
     ++in;
+    rows += tile_rows;
+    stats += kTile * 8;
     if (++it == tiles) {
       it = t0;
-      ++ih;
+      go_to(++ih, it);
     }
   };
   request();
@@ -1109,39 +1136,48 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
     __builtin_amdgcn_s_barrier();
     fence();
   };
+  // minus the rows' lse / scale (0) or delta (1), for every key: what S and dP of a tile begin with
+  const bf16x8 ones = g == 0 ? bf16x8{(bf16)1.f, (bf16)1.f, (bf16)1.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f} : bf16x8{};
+  auto minus = [&](int n, int which) {
+    const bf16x4 x = *(const bf16x4*)((const char*)&stat[n & 3][l32] + 8 * which);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(x, bf16x4{}, 0, 1, 2, 3, 4, 5, 6, 7), ones, f32x16{}, 0, 0, 0);
+  };
   auto first = [&](auto masked, int t, int n) {   // S, P, dV of tile t of a head, the n-th of all
     constexpr bool MASKED = decltype(masked)::value;
     lds_char* const qt = lds + (n & 3) * kSlot;
     const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;   // the lane's key is seen by rows lo .. hi - 1 of the tile
-    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return;   // no query of the tile sees a key of the wave
+    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return request();   // no query of the tile sees a key of the wave
     at.again();
-    f32x16 p = rows_times<HD>(qt, at, b);
+    f32x16 p = rows_times<HD>(qt, at, b, minus(n, 0));
+    request();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const f32x4 lse2 = *(const f32x4*)&stat[n & 3][0][8 * c + 4 * g];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * c + e], a.c, -lse2[e]));
-    }
+    for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(p[e] * a.c);
     if (MASKED) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? p[e] : 0.f;
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) handed[n & 1][pair][c][lane] = f32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]};
+    for (int c = 0; c < 2; ++c)
+      handed[n & 1][pair][c][lane] = u32x4{pack_weights(p[8 * c], p[8 * c + 1]), pack_weights(p[8 * c + 2], p[8 * c + 3]),
+                                           pack_weights(p[8 * c + 4], p[8 * c + 5]), pack_weights(p[8 * c + 6], p[8 * c + 7])};
     add_times<HD, MASKED>(qt + T::kBytes, at, p, lo, hi, acc);
   };
   auto second = [&](auto masked, int t, int n) {   // dP, dS, dK of tile t of a head, the n-th of all
     constexpr bool MASKED = decltype(masked)::value;
     lds_char* const qt = lds + (n & 3) * kSlot;
     const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;
-    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return;
+    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return request();
     at.again();
-    f32x16 ds = rows_times<HD>(qt + T::kBytes, at, b);
+    f32x16 ds = rows_times<HD>(qt + T::kBytes, at, b, minus(n, 1));
+    request();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const f32x4 p = handed[n & 1][pair][c][lane], delta = *(const f32x4*)&stat[n & 3][1][8 * c + 4 * g];
+    for (int c = 0; c < 2; ++c) {
+      const u32x4 p = handed[n & 1][pair][c][lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ds[4 * c + e] = p[e] * (ds[4 * c + e] - delta[e]);
+      for (int e = 0; e < 4; ++e) {
+        ds[8 * c + 2 * e] *= low_weight(p[e]);
+        ds[8 * c + 2 * e + 1] *= high_weight(p[e]);
+      }
     }
     if (MASKED) {
 #pragma unroll
@@ -1158,8 +1194,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv_kernel(PackedArgs a) {
       auto run = [&](auto masked, int until) {
         for (; t < until && n < end; ++t, ++n) {
           wait_for(n + ahead >= steps);
-          request();
-          work(masked, t, n);
+          work(masked, t, n);   // which requests a tile
         }
       };
       run(std::true_type{}, t1);
@@ -1266,7 +1301,7 @@ int dkv_parts(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
   const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads, steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);
   return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(kDkvBlocks, std::max<int64_t>(1, blocks)), steps / kDkvSteps, kMostDkvParts}));
 }
-size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 2 * sizeof(float) + 255) & ~(size_t)255; }
+size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 16 + 255) & ~(size_t)255; }
 
 size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D) {
   const int parts = dkv_parts(seqs, tq, tk, heads, kv_heads);
@@ -1274,7 +1309,7 @@ size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, in
 }
 
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {
-  a.stat = (float*)ws;
+  a.stat = (bf16*)ws;
   a.part = (float*)((char*)ws + stat_bytes(a.tq, a.heads));
   a.dkv_parts = dkv_parts(a.seqs, a.tq, a.tk, a.heads, a.kv_heads);
   auto go = [&](auto hd) {

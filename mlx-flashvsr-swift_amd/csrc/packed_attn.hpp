@@ -14,7 +14,7 @@ struct PackedArgs {
   HeadView<const bf16> q, k, v, d_o;
   HeadView<bf16> o, dq, dk, dv;   // o is read by the backward pass
   float* lse;                     // (heads, tq), natural logarithms; may be null in the forward pass
-  float* stat;                    // (heads, tq, 2) lse in log2 units and the sum of dO O, from the dQ kernel to the dK, dV kernel
+  bf16* stat;                     // (heads, tq, 8) stat_parts of the queries, from the dQ kernel to the dK, dV kernel
   float* part;                    // partial results of the split walk, or of dK and dV
   int dkv_parts;                  // parts that a block's queries are cut into
   const int32_t *cu_q, *cu_k, *used_k;   // used_k may be null
