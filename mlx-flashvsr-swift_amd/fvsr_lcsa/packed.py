@@ -39,6 +39,7 @@ _BF16 = (torch.bfloat16,)
 _FLOATS = (torch.float32, torch.bfloat16)
 _Tensor = torch.Tensor
 _recording = torch.is_grad_enabled
+_empty_like = torch.empty_like   # a third faster than new_empty; of rows and heads it gives rows and heads, channels innermost
 
 
 def _unbatched(x, name: str, dims: int):
@@ -125,7 +126,7 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
         kind, w, _ = _params(dtype, w)
     total, result = out_sum, out
     if r is not None and s is None:
-        total = s = x.new_empty(x.shape)
+        total = s = _empty_like(residual)
     rstd = x.new_empty(rows, dtype=torch.float32) if want_stats else None
     yp = yc = ys = None
     if quantized:
@@ -134,7 +135,7 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
         yc, ys = _p8(y)
     else:
         if y is None:
-            result = y = x.new_empty(x.shape)
+            result = y = _empty_like(x) if stride == c else x.new_empty(x.shape)
         yp = y.data_ptr()
         if s is out_sum is not None and yp == s.data_ptr() and rows:
             _refuse("out", "the norm and the sum need memory of their own")
@@ -175,12 +176,12 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
         kind, w, _ = _params(dtype, w)
     dx = out
     if o is None:
-        dx = o = dy.new_empty(dy.shape)
+        dx = o = _empty_like(dy)
     dw = ws = None
     nbytes = 0
     if want_weight:
         nbytes = lib.fvsr_rms_norm_backward_workspace(rows, c)
-        dw = dy.new_empty(c, dtype=torch.float32)
+        dw = _empty_like(w) if kind == DTYPE_F32 and w is not None and w.dim() == 1 else dy.new_empty(c, dtype=torch.float32)
         ws = dy.new_empty(nbytes, dtype=torch.uint8)
     rc = lib.fvsr_rms_norm_backward(_handle(dev), _CODE[dtype], d2.data_ptr(), t2.data_ptr(), stride, rstd.data_ptr(), _p(ds), rows,
                                     c, kind, _p(w), o.data_ptr(), _p(dw), _p(ws), nbytes, _raw_stream(dev))
@@ -224,6 +225,14 @@ def _heads(x, name: str, dtypes):
     if h < 1 or d < 1 or (d > 1 and cs != 1):
         _refuse(name, f"expected (L, H, D) heads of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
     return x, n, h, d, (ts if n > 1 else h * d), (hs if h > 1 else d)
+
+
+def _made(x):
+    """(a new tensor like x, elements between its tokens, between its heads)"""
+    o = _empty_like(x)
+    n, h, d = o.shape[-3:]
+    ts, hs, _ = o.stride()[-3:]
+    return o, (ts if n > 1 else h * d), (hs if h > 1 else d)
 
 
 def _out_heads(out, name: str, n: int, h: int, d: int, dtype):
@@ -316,16 +325,16 @@ def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
     st = _structs
     a = st.heads(0, q3, h, qt, qh)
     if yq is None:
-        oq = q.new_empty(q.shape)
-        b = st.heads(1, oq, h, h * d, d)
+        oq, qt, qh = _made(q)
+        b = st.heads(1, oq, h, qt, qh)
     else:
         b = st.heads(1, yq[0], h, yq[4], yq[5])
     e = f = None
     if k3 is not None:
         e = st.heads(2, k3, hk, kt, kh)
         if yk is None:
-            ok = k.new_empty(k.shape)
-            f = st.heads(3, ok, hk, hk * d, d)
+            ok, kt, kh = _made(k)
+            f = st.heads(3, ok, hk, kt, kh)
         else:
             f = st.heads(3, yk[0], hk, yk[4], yk[5])
     rc = lib.fvsr_rotary(_handle(dev), _CODE[dtype], a, b, e, f, n, d, positions.data_ptr(), wide, frequencies.data_ptr(), count, packed,
@@ -421,8 +430,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     n, h, d = q3[1:4]
     o = out
     if o3 is None:
-        o = q.new_empty(q.shape)
-        o3 = o, n, h, d, h * d, d
+        o, ts, hs = _made(q)
+        o3 = o, n, h, d, ts, hs
     lse = q.new_empty((h, n), dtype=torch.float32) if want_lse else None
     nbytes = _workspace(False, m - 1, n, k3[1], d, h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
@@ -466,8 +475,8 @@ def packed_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor
                   (used_k, "used_k"), *((x and x[0], "out") for x in made))
     grads = out
     if out is None:
-        grads = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        made = [(x, *y[1:4], y[2] * d, d) for x, y in zip(grads, (q3, k3, v3))]
+        made = [(x, *y[1:4], ts, hs) for (x, ts, hs), y in zip(map(_made, (q, k, v)), (q3, k3, v3))]
+        grads = tuple(x[0] for x in made)
     nbytes = _workspace(True, m - 1, n, k3[1], d, h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     g3, q3, k3, v3, o3 = _ready(g3), _ready(q3), _ready(k3), _ready(v3), _ready(o3)

@@ -358,6 +358,22 @@ def test_unaligned_and_overlapping_views_are_read(dev):
     ref = attention64(q, k, k, cq, causal=True)
     within(f.packed_attention(q, k, k, cu, causal=True)[0], ref["o"], ref["tol_o"])
     assert f.packed_attention(q[None], k[None], k[None], cu)[0].shape == (1, 60, 2, 64)
+    # heads that lie one behind another, a lone token far from the next, no stride at all
+    q, k = randn(g, (4, 60, 64), dev).transpose(0, 1), randn(g, (2, 60, 64), dev).transpose(0, 1)
+    ref = attention64(q, k, k, cq, causal=True, do=q)
+    o, lse = f.packed_attention(q, k, k, cu, causal=True, want_lse=True)
+    within(o, ref["o"], ref["tol_o"])
+    for name, x in zip(("dq", "dk", "dv"), f.packed_attention_backward(q, q, k, k, o, lse, cu, causal=True)):
+        within(x, ref[name], ref["tol_" + name], name)
+    far = torch.empty((2, 1 << 24), dtype=bf, device=dev)
+    lone = far.as_strided((1, 4, 64), (1 << 24, 64, 1))
+    lone.copy_(randn(g, (1, 4, 64), dev))
+    _, c1 = cu_of([1], dev)
+    assert torch.equal(f.packed_attention(lone, lone, lone, c1)[0], lone)
+    freq, pos = f.rotary_frequencies((32,), device=dev), torch.arange(60, dtype=torch.int32, device=dev)
+    a, b = f.rotary(q, k, pos, freq, (32,))
+    c, d = f.rotary(q.contiguous(), k.contiguous(), pos, freq, (32,))
+    assert torch.equal(a, c) and torch.equal(b, d)
     for n in (1, 40, 45):   # one token read as many: rows past the last are not zeros
         one, do = randn(g, (1, 2, 64), dev).expand(n, 2, 64), randn(g, (1, 2, 64), dev).expand(n, 2, 64)
         cq, cu = cu_of([n], dev)
