@@ -142,7 +142,7 @@ int fvsr_rotary(fvsr_ctx* ctx, int dtype, const fvsr_heads* q, const fvsr_heads*
   FVSR_REQUIRE(ctx != nullptr, FVSR_ERR_INVALID_ARG, "ctx is NULL");
   FVSR_REQUIRE(dtype_ok(dtype), FVSR_ERR_INVALID_ARG, "dtype must be FVSR_DTYPE_F32 or FVSR_DTYPE_BF16");
   FVSR_REQUIRE(tokens >= 0 && channels > 0 && channels % 2 == 0, FVSR_ERR_INVALID_ARG, "tokens must be >= 0, channels even and > 0");
-  FVSR_REQUIRE(tokens <= (int64_t)1 << 32 && channels <= 4096, FVSR_ERR_UNSUPPORTED, "at most 2^32 tokens of 4096 channels a head");
+  FVSR_REQUIRE(tokens <= (int64_t)1 << 32 && channels <= 1024, FVSR_ERR_UNSUPPORTED, "at most 2^32 tokens of 1024 channels a head");
   FVSR_REQUIRE(axes >= 1 && axes <= 3 && axis_pairs, FVSR_ERR_INVALID_ARG, "1 to 3 axes, with the pairs of each, are needed");
   int64_t pairs = 0;
   for (int i = 0; i < axes; ++i) {

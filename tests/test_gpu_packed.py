@@ -133,7 +133,8 @@ def test_rms_norm_of_rows_that_are_not_finite(dev):
 @pytest.mark.parametrize("halves", [False, True])
 @pytest.mark.parametrize("n,h,hk,d,axes,far", [(1, 12, 2, 128, (22, 21, 21), 1024), (5, 3, 1, 16, (8,), 10), (33, 4, 4, 64, (16, 16), 500),
                                                (7, 2, 0, 80, (16, 17), 10 ** 6), (100, 9, 3, 104, (25, 27), 2 ** 31 - 1),
-                                               (3, 5, 1, 6, (1,), 3), (19, 20, 4, 30, (0, 11, 2), 77), (2100, 2, 1, 256, (40, 40, 40), 9000)])
+                                               (3, 5, 1, 6, (1,), 3), (19, 20, 4, 30, (0, 11, 2), 77), (2100, 2, 1, 256, (40, 40, 40), 9000), (3, 1, 1, 1024, (512,), 50),
+                                               (2, 2, 1, 1022, (3, 200, 307), 2 ** 20)])
 def test_rotary_and_gradient(dev, dtype, halves, n, h, hk, d, axes, far):
     g = gen_of(n, h, d, halves)
     qkv = randn(g, (n, h + 2 * hk + 1, d), dev, dtype)

@@ -157,7 +157,7 @@ def test_c_entry_points_refuse_before_device_work():
         "fvsr_rotary", ctx, 1, view(), view(), k, ko, tokens, ch, p, 0, p, len(axes), (C.c_int32 * 4)(*axes), 0, 0, None)
     for kw in ({"tokens": -1}, {"ch": 63}, {"axes": ()}, {"axes": (1, 1, 1, 1)}, {"axes": (-1, 2)}, {"axes": (32, 1)}, {"k": view()}):
         assert rot(**kw)[0] == _abi.ERR_INVALID_ARG, kw
-    assert rot(ch=4098)[0] == _abi.ERR_UNSUPPORTED
+    assert rot(ch=1026)[0] == _abi.ERR_UNSUPPORTED
 
 
 def test_workspaces():
