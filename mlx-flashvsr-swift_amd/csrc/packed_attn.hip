@@ -231,14 +231,18 @@ __device__ __forceinline__ int within(int x, int lo, int hi) { return min(max(x,
 struct Span {
   int q0, nq, k0, nk, room;   // room: keys up to the next sequence's, nk of them in use
 };
-__device__ __forceinline__ Span span_of(const PackedArgs& a, int b) {
+__device__ __forceinline__ Span span_from(const PackedArgs& a, int q0, int q1, int k0, int k1, int used) {
   Span s;
-  s.q0 = within(uniform(a.cu_q[b]), 0, a.tq);
-  s.nq = within(uniform(a.cu_q[b + 1]), s.q0, a.tq) - s.q0;
-  s.k0 = within(uniform(a.cu_k[b]), 0, a.tk);
-  s.room = within(uniform(a.cu_k[b + 1]), s.k0, a.tk) - s.k0;
-  s.nk = a.used_k ? within(uniform(a.used_k[b]), 0, s.room) : s.room;
+  s.q0 = within(q0, 0, a.tq);
+  s.nq = within(q1, s.q0, a.tq) - s.q0;
+  s.k0 = within(k0, 0, a.tk);
+  s.room = within(k1, s.k0, a.tk) - s.k0;
+  s.nk = a.used_k ? within(used, 0, s.room) : s.room;
   return s;
+}
+__device__ __forceinline__ Span span_of(const PackedArgs& a, int b) {
+  return span_from(a, uniform(a.cu_q[b]), uniform(a.cu_q[b + 1]), uniform(a.cu_k[b]), uniform(a.cu_k[b + 1]),
+                   a.used_k ? uniform(a.used_k[b]) : 0);
 }
 
 // The block of kRows rows in `slot`: of sequence b (then its first row, `row`, in the sequence), or rows of no sequence: then
@@ -247,16 +251,31 @@ struct Block {
   int b, row;
   int lo, hi;
 };
-__device__ __forceinline__ Block block_of(const int32_t* cu, int total, int seqs, int slot) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int i = 0; i <= seqs; i += 64) {
+// And the sequence's span. Offsets of up to 63 sequences are held by the lanes of a wave, which look for theirs side by side: one
+// round trip to memory, where the blocks of short sequences spend much of their time.
+template <bool KEYS>   // blocks of keys, or of queries
+__device__ __forceinline__ Block block_of(const PackedArgs& a, int slot, Span& span) {
+  const int lane = threadIdx.x & 63, seqs = a.seqs, total = KEYS ? a.tk : a.tq;
+  const int at = min(lane, seqs);
+  const int q = a.cu_q[at], k = a.cu_k[at], used = a.used_k ? a.used_k[min(lane, seqs - 1)] : 0;
+  const int32_t* const cu = KEYS ? a.cu_k : a.cu_q;
+  int n = __popcll(__ballot(lane <= seqs && within(KEYS ? k : q, 0, total) / kRows + lane <= slot));
+  for (int i = 64; i <= seqs; i += 64) {
     const bool before = i + lane <= seqs && within(cu[min(i + lane, seqs)], 0, total) / kRows + i + lane <= slot;
     n += __popcll(__ballot(before));
   }
   Block x;
   x.b = uniform(n) - 1;
-  const int first = within(uniform(cu[max(x.b, 0)]), 0, total);   // of the sequence, or behind the last one
+  const int b = max(x.b, 0);   // <= seqs
+  int first;                   // row of the sequence, or behind the last one
+  if (seqs < 64) {
+    auto of = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+    first = within(of(KEYS ? k : q, b), 0, total);
+    span = span_from(a, of(q, b), of(q, b + 1), of(k, b), of(k, b + 1), of(used, b));   // of no use where b is seqs
+  } else {
+    first = within(uniform(cu[b]), 0, total);
+    span = span_of(a, min(b, seqs - 1));
+  }
   x.row = x.b < 0 ? 0 : (slot - (first / kRows + x.b)) * kRows;
   x.lo = x.hi = 0;
   if (x.b < 0) {
@@ -357,14 +376,14 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
   // a sequence's last rows, which see most where it is causal, come first
-  const Block blk = block_of(a.cu_q, a.tq, a.seqs, slots - 1 - (int)(blockIdx.x / a.heads));
+  Span s;
+  const Block blk = block_of<false>(a, slots - 1 - (int)(blockIdx.x / a.heads), s);
   if (a.clear && blk.hi > blk.lo) {
     clear_rows(a.o, head, blk.lo, blk.hi, a.D);
     if (a.lse)
       for (int r = blk.lo + (int)threadIdx.x; r < blk.hi; r += 256) a.lse[(int64_t)head * a.tq + r] = -INFINITY;
   }
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  const Span s = span_of(a, blk.b);
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
   const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
@@ -564,13 +583,7 @@ struct Parts {
 __device__ __forceinline__ int items_of(const PackedArgs& a, const Span& s) { return (s.nq * a.group + kTile - 1) / kTile; }
 __device__ __forceinline__ int tiles_of(const Span& s) { return max(1, (s.nk + kTile - 1) / kTile); }
 __device__ __forceinline__ Span lane_span(const PackedArgs& a, int b) {   // span_of, for a sequence of the lane's own
-  Span s;
-  s.q0 = within(a.cu_q[b], 0, a.tq);
-  s.nq = within(a.cu_q[b + 1], s.q0, a.tq) - s.q0;
-  s.k0 = within(a.cu_k[b], 0, a.tk);
-  s.room = within(a.cu_k[b + 1], s.k0, a.tk) - s.k0;
-  s.nk = a.used_k ? within(a.used_k[b], 0, s.room) : s.room;
-  return s;
+  return span_from(a, a.cu_q[b], a.cu_q[b + 1], a.cu_k[b], a.cu_k[b + 1], a.used_k ? a.used_k[b] : 0);
 }
 
 constexpr int kMaxParts = 256;        // workgroups of the split walk: its rings leave room for one on a compute unit
@@ -871,10 +884,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[8 * T::kBytes];   // [tile % 4][K, V]
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
-  const Block blk = block_of(a.cu_q, a.tq, a.seqs, slots - 1 - (int)(blockIdx.x / a.heads));
+  Span s;
+  const Block blk = block_of<false>(a, slots - 1 - (int)(blockIdx.x / a.heads), s);
   if (a.clear && blk.hi > blk.lo) clear_rows(a.dq, head, blk.lo, blk.hi, a.D);
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  const Span s = span_of(a, blk.b);
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
   const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
@@ -914,19 +927,34 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf((float)d_o[t][e], (float)o[t][e], delta);
     delta = pair_sum(delta);
-    if (i < s.nq) {
-      const int64_t at = (int64_t)head * a.tq + s.q0 + i;
-      lse2 = a.lse[at] * kLog2e;
-      if (g == 0) *(bf16x8*)(a.stat + 8 * at) = stat_parts(-a.lse[at] / a.scale, -delta);
-    }
+    if (i < s.nq) lse2 = a.lse[(int64_t)head * a.tq + s.q0 + i] * kLog2e;
   }
   Lanes<HD> at;
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
-  // tiles 0 and 1 have landed, for every wave
-  __builtin_amdgcn_s_barrier();
+  loaded();
+  __builtin_amdgcn_s_barrier();   // tiles 0 and 1 have landed, for every wave
   fence();
+  constexpr int kSlot = 2 * T::kBytes;
+  if (tiles <= 4) {
+    // Where a row sees few keys, O is as large as V, and the rounding of O to bf16 would be a large part of what dS is off by: delta is
+    // made of P and dP here, as the ring holds all the tiles.
+    for (int t = 2; t < tiles; ++t) issue(t);
+    wait_and_sync_but<0>(true);
+    delta = 0.f;
+    for (int t = 0; t < tiles; ++t) {
+      const f32x16 x = rows_times<HD>(lds + t * kSlot, at, q), dp = rows_times<HD>(lds + t * kSlot + T::kBytes, at, d_o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        delta += elem_row(e) < lim - t * kTile - 4 * g ? __builtin_amdgcn_exp2f(fmaf(x[e], a.c, -lse2)) * dp[e] : 0.f;
+    }
+    delta = pair_sum(delta);
+  }
+  if (i < s.nq && g == 0) {
+    const int64_t to = (int64_t)head * a.tq + s.q0 + i;
+    *(bf16x8*)(a.stat + 8 * to) = stat_parts(-a.lse[to] / a.scale, -delta);
+  }
   uint32_t row[T::kT], tr[2][T::kD];
 #pragma unroll
   for (int c = 0; c < T::kT; ++c) row[c] = base + at.row(c);
@@ -935,7 +963,6 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     tr[0][d] = base + at.tr(0, 0, d);
     tr[1][d] = base + at.tr(1, 0, d);
   }
-  constexpr int kSlot = 2 * T::kBytes;
   // operand x of a step on slot SLOT: rows of V (dP), rows of the next tile's K (its S), K transposed (dQ)
   auto operand = [&](auto slot, auto x) {
     constexpr int SLOT = decltype(slot)::value, X = decltype(x)::value, C = X % T::kT;
@@ -993,7 +1020,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     wait_and_sync_but<2 * kMine>(false);   // tile t + 2, requested a step before, has landed
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (tiles > 2) issue(2);
+  if (tiles > 4) issue(2);
   if (full >= 4) {
     wait_and_sync_but<2 * kMine>(false);
     for (; t + 4 <= full; t += 4) {
@@ -1007,8 +1034,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   // the tiles left: up to three whole ones, then those that some rows do not see all of
   auto last = [&](auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
-    wait_and_sync_but<2 * kMine>(t + 2 >= tiles);   // tiles t and t + 1 have landed
-    if (t + 3 < tiles) issue(t + 3);
+    wait_and_sync_but<2 * kMine>(t + 2 >= tiles);   // tiles t and t + 1 have landed (up to four all have)
+    if (tiles > 4 && t + 3 < tiles) issue(t + 3);
     lds_char* const kt = lds + (t & 3) * kSlot;
     const int k0 = t * kTile;
     if (!MASKED || k0 < lim_max) {
@@ -1056,13 +1083,13 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   const bool makes_dv = wave < 4;
   const int part = blockIdx.x % a.dkv_parts, hk = blockIdx.x / a.dkv_parts % a.kv_heads;
   // the first keys, which most queries see, first
-  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.dkv_parts / a.kv_heads);
+  Span s;
+  const Block blk = block_of<true>(a, blockIdx.x / a.dkv_parts / a.kv_heads, s);
   if (a.clear && part == 0 && blk.hi > blk.lo) {
     clear_rows(a.dk, hk, blk.lo, blk.hi, a.D);
     clear_rows(a.dv, hk, blk.lo, blk.hi, a.D);
   }
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  const Span s = span_of(a, blk.b);
   if (blk.row >= s.room) return;
   const int j0 = blk.row + pair * 32, j = j0 + l32;
   const int off = s.nk - s.nq;   // causal: query i sees keys j <= i + off
@@ -1233,9 +1260,9 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
 template <int HD>
 __global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
   const int hk = blockIdx.x % a.kv_heads;
-  const Block blk = block_of(a.cu_k, a.tk, a.seqs, blockIdx.x / a.kv_heads);
+  Span s;
+  const Block blk = block_of<true>(a, blockIdx.x / a.kv_heads, s);
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  const Span s = span_of(a, blk.b);
   constexpr int kCols = HD / 4, kEach = kRows / 4;
   const int64_t stride = (int64_t)2 * a.tk * a.kv_heads * HD;
 #pragma unroll 2

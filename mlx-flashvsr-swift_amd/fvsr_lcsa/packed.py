@@ -139,7 +139,7 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
         yp = y.data_ptr()
         if s is out_sum is not None and yp == s.data_ptr() and rows:
             _refuse("out", "the norm and the sum need memory of their own")
-    rc = lib.fvsr_rms_norm(_handle(dev), _CODE[dtype], x2.data_ptr(), stride, _p(r), rows, c, eps, kind, _p(w), yp, yc, ys, _p(s),
+    rc = lib.fvsr_rms_norm(_handle(dev), _CODE[dtype], x2.data_ptr(), stride, _p(r), rows, c, float(eps), kind, _p(w), yp, yc, ys, _p(s),
                            _p(rstd), _raw_stream(dev))
     if rc:
         _check(rc, "fvsr_rms_norm")

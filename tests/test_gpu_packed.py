@@ -258,6 +258,13 @@ def test_packed_attention_rows_of_no_sequence(dev, causal):
         check_attention(dev, lengths, None, 4, 2, 128, causal, start=5, tail=1)
 
 
+@pytest.mark.parametrize("n", [62, 63, 64, 65, 130])
+def test_packed_attention_of_many_sequences(dev, n):
+    """Around the number that a wave's lanes hold, and past it."""
+    check_attention(dev, [40 + i % 3 for i in range(n)], None, 4, 1, 64, True)
+    check_attention(dev, [i % 4 for i in range(n)], [i % 7 for i in range(n)], 2, 2, 128, False)
+
+
 def test_packed_attention_scales(dev):
     check_attention(dev, [70, 33], None, 2, 1, 64, True, scale=1.0)      # sharp weights
     check_attention(dev, [70, 33], None, 2, 1, 64, False, scale=1e-4)
