@@ -1074,10 +1074,13 @@ __device__ __forceinline__ float high_weight(uint32_t w) { return __uint_as_floa
 template <int HD>
 __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(PackedArgs a) {
   using T = Tile<HD>;
-  constexpr int kSlot = 2 * T::kBytes;                                                      // Q, dO
-  __shared__ __attribute__((aligned(1024))) char smem[4 * kSlot];                           // tile n in slot n % 4
-  __shared__ __attribute__((aligned(1024))) bf16x8 stat[4][64];                             // its rows' stat_parts
-  __shared__ __attribute__((aligned(16))) u32x4 handed[2][4][2][64];                         // P of tile n in n % 2, a wave pair each
+  // A step's tiles of queries: two, where they and their neighbours' fit (a step begins and ends with waiting), one where that leaves
+  // room for a second workgroup on the compute unit.
+  constexpr int kN = HD == 128 ? 2 : 1, kRowsN = kN * kTile, kSlots = kN == 2 ? 3 : 4, kEarly = kSlots - 2;
+  constexpr int kSlot = 2 * kN * T::kBytes;                                               // Q, dO
+  __shared__ __attribute__((aligned(1024))) char smem[kSlots * kSlot];                    // step n in slot n % kSlots
+  __shared__ __attribute__((aligned(1024))) bf16x8 stat[kSlots][kN][64];                  // its rows' stat_parts
+  __shared__ __attribute__((aligned(16))) u32x4 handed[2][4][kN][2][64];                  // P of step n in n % 2, a wave pair each
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int pair = wave & 3;
   const bool makes_dv = wave < 4;
@@ -1093,141 +1096,163 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   if (blk.row >= s.room) return;
   const int j0 = blk.row + pair * 32, j = j0 + l32;
   const int off = s.nk - s.nq;   // causal: query i sees keys j <= i + off
-  // tiles of queries; none for keys that are not in use
-  const int tiles = blk.row < s.nk ? (s.nq + kTile - 1) / kTile : 0;
-  // the first one that sees a key of the block, and the first from which on every row sees all of them
-  const int t0 = a.causal ? min(tiles, max(0, blk.row - off) / kTile) : 0;
-  const int t1 = a.causal ? min(tiles, max(0, blk.row + kRows - 1 - off + kTile - 1) / kTile) : 0;
-  const int t2 = max(t1, min(tiles, s.nq / kTile));   // the last tile may not be whole
-  // of the tiles of all the group's heads, those of this part: the first is tile `from_t` of head `from_h`
-  const int all = (tiles - t0) * a.group, begin = (int)((int64_t)all * part / a.dkv_parts);
+  // The first query that sees a key of the block, down to a tile; the steps of a head from there on (none for keys that are not in
+  // use), those before the first from which on every row sees all of the block, and those before the last one that may not be whole.
+  const int q0 = a.causal ? min(s.nq, max(0, blk.row - off) / kTile * kTile) : 0;
+  const int units = blk.row < s.nk ? (s.nq - q0 + kRowsN - 1) / kRowsN : 0;
+  const int u1 = a.causal ? min(units, max(0, blk.row + kRows - 1 - off - q0 + kRowsN - 1) / kRowsN) : 0;
+  const int u2 = max(u1, min(units, (s.nq - q0) / kRowsN));
+  // of the steps of all the group's heads, those of this part: the first is `from_u` of head `from_h`
+  const int all = units * a.group, begin = (int)((int64_t)all * part / a.dkv_parts);
   const int steps = (int)((int64_t)all * (part + 1) / a.dkv_parts) - begin;
-  const int from_h = steps > 0 ? begin / (tiles - t0) : 0, from_t = steps > 0 ? t0 + begin % (tiles - t0) : t0;
+  const int from_h = steps > 0 ? begin / units : 0, from_u = steps > 0 ? begin % units : 0;
 
-  // a tile's copies are dealt to the 8 waves: Q to the first 4, dO to the others
+  // a step's copies are dealt to the 8 waves: Q to the first 4, dO to the others
   constexpr int kMine = T::kCopies / 4;
   const HeadView<const bf16> from = makes_dv ? a.q : a.d_o;
   int voff[kMine];
 #pragma unroll
   for (int p = 0; p < kMine; ++p) voff[p] = copy_off<HD>(pair * kMine + p, lane, (int)from.t * 2, a.D);
-  const int soff = g == 0 ? l32 * 16 : (int)0x80000000;   // the tile's rows; the other lanes copy zeros
-  const uint32_t base = lds_addr(smem) + (makes_dv ? 0 : T::kBytes) + pair * kMine * 1024, sbase = lds_addr(stat);
+  const int soff = g == 0 ? l32 * 16 : (int)0x80000000;   // a tile's rows; the other lanes copy zeros
+  const uint32_t base = lds_addr(smem) + (makes_dv ? 0 : kN * T::kBytes) + pair * kMine * 1024, sbase = lds_addr(stat);
   lds_char* const lds = (lds_char*)(uintptr_t)lds_addr(smem);
   Lanes<HD> at;
   f32x16 acc[T::kD];
 #pragma unroll
   for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
-  // The tile that is requested next: its rows, and those left of its head. Kept from one to the next, for a scalar multiplication or
+  // The step that is requested next: its rows, and those left of its head. Kept from one to the next, for a scalar multiplication or
   // two at the head of each step is a hundred cycles before the first product.
-  int ih = hk * a.group + from_h, it = from_t, in = 0;
+  int ih = hk * a.group + from_h, iu = from_u, in = 0, islot = 0;
   const bf16* rows = nullptr;
   const bf16* stats = nullptr;
-  auto go_to = [&](int h, int t) {
-    rows = from.p + (int64_t)(s.q0 + t * kTile) * from.t + h * from.h;
-    stats = a.stat + ((int64_t)h * a.tq + s.q0 + t * kTile) * 8;
+  auto go_to = [&](int h, int u) {
+    rows = from.p + (int64_t)(s.q0 + q0 + u * kRowsN) * from.t + h * from.h;
+    stats = a.stat + ((int64_t)h * a.tq + s.q0 + q0 + u * kRowsN) * 8;
   };
-  go_to(ih, it);
-  const int64_t tile_rows = kTile * from.t;
-  const int whole = ((kTile - 1) * (int)from.t + a.D) * 2, rest = s.nq % kTile, ragged = ((rest - 1) * (int)from.t + a.D) * 2;
+  go_to(ih, iu);
+  const int tile_bytes = kTile * (int)from.t * 2, rest = (s.nq - q0) % kRowsN;
+  const int whole = ((kRowsN - 1) * (int)from.t + a.D) * 2, ragged = ((rest - 1) * (int)from.t + a.D) * 2;
   auto rsrc = [&](const bf16* at, int bytes) {
     return u32x4{(uint32_t)uniform((int)(uint32_t)(uint64_t)at), (uint32_t)uniform((int)((uint64_t)at >> 32 & 0xffffu)),
                  (uint32_t)uniform(bytes), 0x00020000u};
   };
   auto request = [&] {
     if (in < steps) {
-      const bool end = it == tiles - 1 && rest != 0;
+      const bool end = iu == units - 1 && rest != 0;
       const u32x4 r = rsrc(rows, end ? ragged : whole);
-      static_for<0, kMine>([&](auto p) { dma16<p * 1024>(r, base + (in & 3) * kSlot, voff[p], 0); });
-      if (wave == 0) dma16<0>(rsrc(stats, end ? rest * 16 : kTile * 16), sbase + (in & 3) * 1024, soff, 0);
+#pragma unroll
+      for (int k = 0; k < kN; ++k)
+        static_for<0, kMine>([&](auto p) { dma16<p * 1024>(r, base + islot * kSlot + k * T::kBytes, voff[p], k * tile_bytes); });
+      if (wave == 0) {
+        const u32x4 sr = rsrc(stats, end ? rest * 16 : kRowsN * 16);
+#pragma unroll
+        for (int k = 0; k < kN; ++k) dma16<0>(sr, sbase + (islot * kN + k) * 1024, soff, k * kTile * 16);
+      }
     }
     ++in;
-    rows += tile_rows;
-    stats += kTile * 8;
-    if (++it == tiles) {
-      it = t0;
-      go_to(++ih, it);
+    if (++islot == kSlots) islot = 0;
+    rows += kRowsN * from.t;
+    stats += kRowsN * 8;
+    if (++iu == units) {
+      iu = 0;
+      go_to(++ih, iu);
     }
   };
-  request();
-  request();
+  for (int n = 0; n < kEarly; ++n) request();
   const HeadView<const bf16> kv = makes_dv ? a.k : a.v;
   bf16x8 b[T::kT];
   load_row<HD>(kv.p + (int64_t)(s.k0 + j) * kv.t + hk * kv.h, j < s.nk, a.D, b);
   loaded();
-  // the copies of one step may still be under way
+  // the copies of kEarly - 1 steps may still be under way
   auto wait_for = [&](bool all) {
     fence();
-    if (all) FVSR_WAIT_VM_LGKM0(0);
-    else if (wave == 0) FVSR_WAIT_VM_LGKM0(kMine + 1);
-    else FVSR_WAIT_VM_LGKM0(kMine);
+    if (all || kEarly == 1) FVSR_WAIT_VM_LGKM0(0);
+    else if (wave == 0) FVSR_WAIT_VM_LGKM0((kEarly - 1) * (kMine + 1) * kN);
+    else FVSR_WAIT_VM_LGKM0((kEarly - 1) * kMine * kN);
     __builtin_amdgcn_s_barrier();
     fence();
   };
   // minus the rows' lse / scale (0) or delta (1), for every key: what S and dP of a tile begin with
   const bf16x8 ones = g == 0 ? bf16x8{(bf16)1.f, (bf16)1.f, (bf16)1.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f} : bf16x8{};
-  auto minus = [&](int n, int which) {
-    const bf16x4 x = *(const bf16x4*)((const char*)&stat[n & 3][l32] + 8 * which);
+  auto minus = [&](int slot, int k, int which) {
+    const bf16x4 x = *(const bf16x4*)((const char*)&stat[slot][k][l32] + 8 * which);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(x, bf16x4{}, 0, 1, 2, 3, 4, 5, 6, 7), ones, f32x16{}, 0, 0, 0);
   };
-  auto first = [&](auto masked, int t, int n) {   // S, P, dV of tile t of a head, the n-th of all
+  // the lane's key is seen by rows lo .. hi - 1 of a tile that begins with query r; whether any key of the wave is seen by the tile
+  auto lo_of = [&](int r) { return a.causal ? j - off - r : 0; };
+  auto hi_of = [&](int r) { return s.nq - r; };
+  auto any_of = [&](int r) { return r < s.nq && (!a.causal || j0 <= r + 31 + off); };
+  auto first = [&](auto masked, int u, int n, int slot) {   // S, P and dV of step u of a head, the n-th of all
     constexpr bool MASKED = decltype(masked)::value;
-    lds_char* const qt = lds + (n & 3) * kSlot;
-    const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;   // the lane's key is seen by rows lo .. hi - 1 of the tile
-    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return request();   // no query of the tile sees a key of the wave
+    lds_char* const qt = lds + slot * kSlot;
+    lds_char* const ot = qt + kN * T::kBytes;
     at.again();
-    f32x16 p = rows_times<HD>(qt, at, b, minus(n, 0));
+    f32x16 p[kN];
+#pragma unroll
+    for (int k = 0; k < kN; ++k) p[k] = rows_times<HD>(qt + k * T::kBytes, at, b, minus(slot, k, 0));
     request();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(p[e] * a.c);
-    if (MASKED) {
+    for (int k = 0; k < kN; ++k) {
+      const int r = q0 + u * kRowsN + k * kTile, lo = lo_of(r), hi = hi_of(r);
+      if (MASKED && !any_of(r)) continue;   // neither here nor in `second`
 #pragma unroll
-      for (int e = 0; e < 16; ++e) p[e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? p[e] : 0.f;
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      handed[n & 1][pair][c][lane] = u32x4{pack_weights(p[8 * c], p[8 * c + 1]), pack_weights(p[8 * c + 2], p[8 * c + 3]),
-                                           pack_weights(p[8 * c + 4], p[8 * c + 5]), pack_weights(p[8 * c + 6], p[8 * c + 7])};
-    add_times<HD, MASKED>(qt + T::kBytes, at, p, lo, hi, acc);
-  };
-  auto second = [&](auto masked, int t, int n) {   // dP, dS, dK of tile t of a head, the n-th of all
-    constexpr bool MASKED = decltype(masked)::value;
-    lds_char* const qt = lds + (n & 3) * kSlot;
-    const int lo = a.causal ? j - off - t * kTile : 0, hi = s.nq - t * kTile;
-    if (MASKED && a.causal && j0 > t * kTile + 31 + off) return request();
-    at.again();
-    f32x16 ds = rows_times<HD>(qt + T::kBytes, at, b, minus(n, 1));
-    request();
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const u32x4 p = handed[n & 1][pair][c][lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ds[8 * c + 2 * e] *= low_weight(p[e]);
-        ds[8 * c + 2 * e + 1] *= high_weight(p[e]);
+      for (int e = 0; e < 16; ++e) {
+        p[k][e] = __builtin_amdgcn_exp2f(p[k][e] * a.c);
+        if (MASKED) p[k][e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? p[k][e] : 0.f;
       }
-    }
-    if (MASKED) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? ds[e] : 0.f;
+      for (int c = 0; c < 2; ++c)
+        handed[n & 1][pair][k][c][lane] = u32x4{pack_weights(p[k][8 * c], p[k][8 * c + 1]), pack_weights(p[k][8 * c + 2], p[k][8 * c + 3]),
+                                                pack_weights(p[k][8 * c + 4], p[k][8 * c + 5]), pack_weights(p[k][8 * c + 6], p[k][8 * c + 7])};
+      add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, acc);
     }
-    add_times<HD, MASKED>(qt, at, ds, lo, hi, acc);
   };
-  // The walk of one kind of wave: `work` for each tile of the part. A step is a tile of the first kind, and of the second kind
-  // the one before: `ahead` steps less are left to be waited for.
+  auto second = [&](auto masked, int u, int n, int slot) {   // dP, dS and dK of step u of a head, the n-th of all
+    constexpr bool MASKED = decltype(masked)::value;
+    lds_char* const qt = lds + slot * kSlot;
+    lds_char* const ot = qt + kN * T::kBytes;
+    at.again();
+    f32x16 ds[kN];
+#pragma unroll
+    for (int k = 0; k < kN; ++k) ds[k] = rows_times<HD>(ot + k * T::kBytes, at, b, minus(slot, k, 1));
+    request();
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const int r = q0 + u * kRowsN + k * kTile, lo = lo_of(r), hi = hi_of(r);
+      if (MASKED && !any_of(r)) continue;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const u32x4 p = handed[n & 1][pair][k][c][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ds[k][8 * c + 2 * e] *= low_weight(p[e]);
+          ds[k][8 * c + 2 * e + 1] *= high_weight(p[e]);
+        }
+      }
+      if (MASKED) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[k][e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? ds[k][e] : 0.f;
+      }
+      add_times<HD, MASKED>(qt + k * T::kBytes, at, ds[k], lo, hi, acc);
+    }
+  };
+  // The walk of one kind of wave: `work` for each step of the part. The second kind is a step behind the first: `ahead` steps less are
+  // left to be waited for.
   auto walk = [&](auto&& work, int ahead) {
-    int t = from_t;
+    int u = from_u, slot = 0;
     for (int n = 0; n < steps;) {
-      const int end = n + min(steps - n, tiles - t);   // to the head's last tile
+      const int end = n + min(steps - n, units - u);   // to the head's last step
       auto run = [&](auto masked, int until) {
-        for (; t < until && n < end; ++t, ++n) {
+        for (; u < until && n < end; ++u, ++n) {
           wait_for(n + ahead >= steps);
-          work(masked, t, n);   // which requests a tile
+          work(masked, u, n, slot);   // which requests a step
+          if (++slot == kSlots) slot = 0;
         }
       };
-      run(std::true_type{}, t1);
-      run(std::false_type{}, t2);
-      run(std::true_type{}, tiles);
-      t = t0;
+      run(std::true_type{}, u1);
+      run(std::false_type{}, u2);
+      run(std::true_type{}, units);
+      u = 0;
     }
   };
   if (makes_dv) {
@@ -1325,7 +1350,7 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
 // of its sums through memory, so that it is to have a few tens of steps.
 constexpr int kDkvBlocks = 1024, kDkvSteps = 32, kMostDkvParts = 16;
 int dkv_parts(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
-  const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads, steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);
+  const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads, steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);   // of a tile
   return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(kDkvBlocks, std::max<int64_t>(1, blocks)), steps / kDkvSteps, kMostDkvParts}));
 }
 size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 16 + 255) & ~(size_t)255; }
