@@ -1312,12 +1312,19 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
 
 int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
 
-// Whether the keys are split over the workgroups: where there are few queries a sequence, so that a block of 128 rows would be
-// mostly empty, and the lengths' products stay below kMostWork.
+// Whether the keys are split over the workgroups, or a workgroup walks over all keys of 128 queries of a head: by what each takes, in
+// microseconds, for sequences of the average lengths. A walk of few blocks takes 0.39 us a tile of keys after 10; from 230 on they
+// share the card. Split, there are two launches, and 256 workgroups take 0.24 us for each of the tiles of all items. That is from
+// 12 heads of 128 over 12 and 2, 1 to 64 sequences of 1 to 1024 queries and 512 to 43200 keys: one query over 43200 keys 17 us
+// split, 526 not; 256 queries 143 and 537; 1024 queries 489 and 547, over 4096 keys 83 and 66; 64 queries each of 64 sequences over
+// 4096 keys, 12 heads over 2, 244 and 204, 32 queries 132 and 184. The lengths' products have to stay below kMostWork.
 bool split(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
   const int64_t group = heads / kv_heads;
-  if (tq * group > (int64_t)64 * seqs) return false;
-  return (ceil_div(tq * group, kTile) + seqs) * (ceil_div(tk, kTile) + seqs) * kv_heads < kMostWork;
+  if ((ceil_div(tq * group, kTile) + seqs) * (ceil_div(tk, kTile) + seqs) * kv_heads >= kMostWork) return false;
+  const double tiles = (double)ceil_div(tk, (int64_t)kTile * seqs);
+  const double items = (double)ceil_div(tq * group, (int64_t)kTile * seqs) * seqs * kv_heads;
+  const double blocks = (double)ceil_div(tq, (int64_t)kRows * seqs) * seqs * heads;
+  return 18 + items * tiles * (0.24 / kMaxParts) < 10 + 0.39 * tiles * std::max(1., blocks / 230);
 }
 
 }  // namespace

@@ -10,12 +10,14 @@ Others, per value, with U = 2^-24 and h half a step of the output's type:
   rotary: an angle's fraction of a turn is exact to 2^-25 turns (rounded to 32 bits below half a turn): 2^-22.3 radians; sine and
       cosine 4 U more; products and sums 3 U: below (|a| + |b|) 2^-21 + h |result|
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
 import fvsr_lcsa as f
+from fvsr_lcsa import _abi
 from packed_reference import H, U, attention64, rms64, rms_grad64, turn64, within
 from train8_reference import RUN, quantize64
 
@@ -233,6 +235,12 @@ def check_attention(dev, lengths_q, lengths_k, h, hk, d, causal, used=None, trai
         assert torch.equal(m[rows], x[rows]) and (m[~rows] == 7).all()
 
 
+def workspace(lengths_q, lengths_k, h, hk, d, causal):
+    """Bytes of workspace of a forward call, where the keys are split over the workgroups."""
+    packed = _abi.Packed(0, 0, None, len(lengths_q), sum(lengths_q), sum(lengths_k), d, int(causal), 1.0)
+    return _abi.lib.fvsr_packed_attention_workspace(ctypes.byref(packed), h, hk)
+
+
 LENGTHS = [[1], [2, 1, 3], [31, 32, 33], [128], [129, 0, 127, 1], [300, 64], [5, 257, 0, 0, 40, 128, 31]]
 
 
@@ -290,6 +298,53 @@ def test_single_tokens_over_a_cache(dev, h, hk, d, m):
     o, lse = f.packed_attention(q, k, v, args[0], args[1], causal=True, used_k=args[2], want_lse=True)
     within(o, ref["o"], ref["tol_o"], "o")
     within(lse, ref["lse"], ref["tol_lse"], "lse")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 128), (3, 1, 64), (16, 1, 40)])
+@pytest.mark.parametrize("lq,lk", [([2], [700]), ([131], [5000]), ([200, 5], [90, 9000]), ([3, 1, 40], [2, 1, 9000]),
+                                   ([64, 0, 30], [0, 9000, 31]), ([33, 32, 1], [3000, 4001, 2990])], ids=str)
+def test_few_queries_over_long_keys(dev, lq, lk, h, hk, d, causal):
+    """Calls whose keys are split over the workgroups: sizes that have a workspace."""
+    assert workspace(lq, lk, h, hk, d, causal)
+    check_attention(dev, lq, lk, h, hk, d, causal, train=h == 4, strided=True)
+    check_attention(dev, lq, lk, h, hk, d, causal, train=False, start=150, tail=200, used=[max(0, n - 40) for n in lk])
+
+
+@pytest.mark.parametrize("n", [62, 63, 64, 65, 130])
+def test_few_queries_of_many_sequences(dev, n):
+    lq, lk = [i % 3 for i in range(n)], [(i * 379) % 1500 for i in range(n)]
+    for more in (0, 1500):      # either way, and split
+        lk = [k + more for k in lk]
+        assert workspace(lq, lk, 4, 1, 64, True) or not more
+        check_attention(dev, lq, lk, 4, 1, 64, True, train=False)
+        check_attention(dev, lq, lk, 2, 2, 128, False, train=False, used=[k // 2 for k in lk])
+
+
+def test_few_queries_and_keys_that_are_not_finite(dev):
+    """Where the keys are split: an infinity or NaN in the keys and values of one token, of a sequence before or past the used keys."""
+    g = gen_of("split nan")
+    lq, room, used, h, hk, d = [2, 40, 3], [1000, 5000, 800], [1000, 4900, 790], 4, 2, 64
+    assert workspace(lq, room, h, hk, d, True)
+    (cq, cu_q), (ck, cu_k) = cu_of(lq, dev), cu_of(room, dev)
+    us = torch.tensor(used, dtype=torch.int32, device=dev)
+    q = randn(g, (cq[-1], h, d), dev)
+    k, v = (randn(g, (ck[-1], hk, d), dev) for _ in range(2))
+    ref = attention64(q, k, v, cq, ck, True, used=used)
+    for i, n in enumerate(used):
+        k[ck[i] + n:ck[i + 1]] = math.nan
+        v[ck[i] + n:ck[i + 1]] = math.inf
+    for value in (math.inf, math.nan):
+        for x in (k, v):
+            keep = x.clone()
+            x[ck[1] + used[1] - 20] = value      # queries 20 .. 39 of the second sequence see it
+            o, lse = f.packed_attention(q, k, v, cu_q, cu_k, causal=True, used_k=us, want_lse=True)
+            blind = [i for i in range(cq[-1]) if not cq[1] + 20 <= i < cq[2]]
+            within(o[blind], ref["o"][blind], ref["tol_o"][blind], "o")
+            within(lse[:, blind], ref["lse"][:, blind], ref["tol_lse"][:, blind], "lse")
+            if x is v or value != math.inf:      # a key's infinity may leave a weight of zero
+                assert not torch.isfinite(o[cq[1] + 20:cq[2]]).flatten(1).all(1).any()
+            x.copy_(keep)
 
 
 def test_long_sequences(dev):

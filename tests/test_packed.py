@@ -150,7 +150,7 @@ def test_c_entry_points_refuse_before_device_work():
     assert call(packed(), q=view(data=24))[0] == _abi.ERR_INVALID_ARG
     assert call(packed(), q=view(ts=252))[0] == _abi.ERR_INVALID_ARG
     assert call(packed(), q=view(ts=1 << 23))[0] == _abi.ERR_UNSUPPORTED
-    assert "workspace" in call(packed())[1]      # few queries: the keys are split
+    assert "workspace" in call(packed(tokens_k=60000))[1]      # few queries: the keys are split
     assert status("fvsr_packed_attention_backward", ctx, packed(), view(), view(), view(2), view(2), view(), None, view(), view(2), view(2), 0,
                   None, 0, None)[0] == _abi.ERR_INVALID_ARG
     rot = lambda tokens=4, ch=64, axes=(8, 8), k=None, ko=None: status(
@@ -162,9 +162,9 @@ def test_c_entry_points_refuse_before_device_work():
 
 def test_workspaces():
     def size(**kw):
-        a = dict(cu_q=16, cu_k=16, used_k=None, sequences=2, tokens_q=2, tokens_k=600, channels=128, causal=0, scale=0.125) | kw
+        a = dict(cu_q=16, cu_k=16, used_k=None, sequences=2, tokens_q=2, tokens_k=60000, channels=128, causal=0, scale=0.125) | kw
         return _abi.lib.fvsr_packed_attention_workspace(C.byref(Packed(*a.values())), 4, 2)
-    assert size() > 0 and size(tokens_q=1000, tokens_k=1000) == 0 and size(tokens_q=0) == 0
+    assert size() > 0 and size(tokens_q=4000, tokens_k=4000) == 0 and size(tokens_k=600) == 0 and size(tokens_q=0) == 0
     assert 0 < size(channels=64) < size()
 
 
