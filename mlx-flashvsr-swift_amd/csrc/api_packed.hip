@@ -62,7 +62,7 @@ static int check_packed(const fvsr_ctx* ctx, const fvsr_packed* p) {
 }
 
 static int check_grid(const fvsr_packed* p, int64_t tokens, int heads) {
-  FVSR_REQUIRE((tokens / 128 + p->sequences + 1) * heads < (int64_t)1 << 24, FVSR_ERR_UNSUPPORTED,
+  FVSR_REQUIRE((tokens / 128 + p->sequences + 1) * heads < kMostRows, FVSR_ERR_UNSUPPORTED,
                "too many blocks of queries or keys for one launch");
   return FVSR_OK;
 }
@@ -193,7 +193,7 @@ int fvsr_packed_attention(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads*
 size_t fvsr_packed_attention_backward_workspace(const fvsr_packed* p, int heads, int kv_heads) {
   return !p || p->sequences <= 0 || p->tokens_q < 0 || p->tokens_k < 0 || kv_heads <= 0 || heads < kv_heads
              ? 0
-             : packed_backward_workspace(p->sequences, p->tokens_q, p->tokens_k, heads, kv_heads, p->channels);
+             : packed_backward_workspace(p->sequences, p->tokens_q, p->tokens_k, heads, kv_heads, p->channels, p->causal != 0);
 }
 
 int fvsr_packed_attention_backward(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads* d_o, const fvsr_heads* q,

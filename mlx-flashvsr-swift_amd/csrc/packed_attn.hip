@@ -1084,10 +1084,12 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
   const int pair = wave & 3;
   const bool makes_dv = wave < 4;
-  const int part = blockIdx.x % a.dkv_parts, hk = blockIdx.x / a.dkv_parts % a.kv_heads;
+  // from block `dkv_whole` on, a block is cut
+  const int over = max(0, (int)blockIdx.x - a.dkv_whole), parts = (int)blockIdx.x < a.dkv_whole ? 1 : a.dkv_parts;
+  const int part = over % parts, block = (int)blockIdx.x - over + over / parts, hk = block % a.kv_heads;
   // the first keys, which most queries see, first
   Span s;
-  const Block blk = block_of<true>(a, blockIdx.x / a.dkv_parts / a.kv_heads, s);
+  const Block blk = block_of<true>(a, block / a.kv_heads, s);
   if (a.clear && part == 0 && blk.hi > blk.lo) {
     clear_rows(a.dk, hk, blk.lo, blk.hi, a.D);
     clear_rows(a.dv, hk, blk.lo, blk.hi, a.D);
@@ -1103,8 +1105,8 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   const int u1 = a.causal ? min(units, max(0, blk.row + kRows - 1 - off - q0 + kRowsN - 1) / kRowsN) : 0;
   const int u2 = max(u1, min(units, (s.nq - q0) / kRowsN));
   // of the steps of all the group's heads, those of this part: the first is `from_u` of head `from_h`
-  const int all = units * a.group, begin = (int)((int64_t)all * part / a.dkv_parts);
-  const int steps = (int)((int64_t)all * (part + 1) / a.dkv_parts) - begin;
+  const int all = units * a.group, begin = (int)((int64_t)all * part / parts);
+  const int steps = (int)((int64_t)all * (part + 1) / parts) - begin;
   const int from_h = steps > 0 ? begin / units : 0, from_u = steps > 0 ? begin % units : 0;
 
   // a step's copies are dealt to the 8 waves: Q to the first 4, dO to the others
@@ -1268,8 +1270,9 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
 #pragma unroll
     for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   }
-  if (a.dkv_parts > 1) {   // for packed_dkv_join_kernel: [part][dK, dV][key][head][HD]
-    float* const row = a.part + ((((int64_t)part * 2 + (makes_dv ? 1 : 0)) * a.tk + s.k0 + j) * a.kv_heads + hk) * HD;
+  if (parts > 1) {   // for packed_dkv_join_kernel: [block][part][dK, dV][key][HD]
+    const int64_t at = ((int64_t)(block - a.dkv_whole) * parts + part) * 2 + (makes_dv ? 1 : 0);
+    float* const row = a.part + (at * kRows + j - blk.row) * HD;
 #pragma unroll
     for (int d = 0; d < T::kD; ++d)
 #pragma unroll
@@ -1284,21 +1287,21 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
 // adds up the parts of dK and dV of a quarter of a block of keys, in their order
 template <int HD>
 __global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
-  const int hk = blockIdx.x % a.kv_heads;
+  const int block = a.dkv_whole + blockIdx.x, hk = block % a.kv_heads;
   Span s;
-  const Block blk = block_of<true>(a, blockIdx.x / a.kv_heads, s);
+  const Block blk = block_of<true>(a, block / a.kv_heads, s);
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  constexpr int kCols = HD / 4, kEach = kRows / 4;
-  const int64_t stride = (int64_t)2 * a.tk * a.kv_heads * HD;
+  constexpr int kCols = HD / 4, kEach = kRows / 4, kStride = 2 * kRows * HD;
+  const float* const parts = a.part + (int64_t)blockIdx.x * a.dkv_parts * kStride;
 #pragma unroll 2
   for (int e = threadIdx.x; e < 2 * kEach * kCols; e += 256) {
-    const int col = e % kCols, j = blk.row + (int)blockIdx.y * kEach + e / kCols % kEach, v = e / kCols / kEach;
+    const int col = e % kCols, row = (int)blockIdx.y * kEach + e / kCols % kEach, v = e / kCols / kEach, j = blk.row + row;
     if (j >= s.room || 4 * col >= a.D) continue;
-    const float* p = a.part + (((int64_t)v * a.tk + s.k0 + j) * a.kv_heads + hk) * HD + 4 * col;
+    const float* p = parts + (v * kRows + row) * HD + 4 * col;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < a.dkv_parts; ++i) {
-      const f32x4 y = *(const f32x4*)(p + i * stride);
+      const f32x4 y = *(const f32x4*)(p + i * kStride);
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] += y[c];
     }
@@ -1353,30 +1356,46 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
   return FVSR_OK;
 }
 
-// Parts that the queries of a block of keys are cut into, where the blocks are too few to fill the card: each costs a round trip
-// of its sums through memory, so that it is to have a few tens of steps.
+// Blocks of keys from `whole` on have their queries cut into `parts`, which costs a round trip of each part's sums through memory, so
+// that a part is to have a few tens of steps: all blocks, where they are too few to fill the card, or those left over for a last round
+// of workgroups, where all queries see all keys (causal, the last blocks are short), and the lengths of few sequences leave little doubt
+// which blocks these are.
 constexpr int kDkvBlocks = 1024, kDkvSteps = 32, kMostDkvParts = 16;
-int dkv_parts(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
-  const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads, steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);   // of a tile
-  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(kDkvBlocks, std::max<int64_t>(1, blocks)), steps / kDkvSteps, kMostDkvParts}));
+struct DkvCut {
+  int64_t whole;
+  int parts;
+};
+DkvCut dkv_cut(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D, bool causal) {
+  if (tk == 0) return {0, 1};
+  const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads;
+  const int64_t steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);   // of a tile
+  const int64_t most = std::min<int64_t>(steps / kDkvSteps, kMostDkvParts);
+  if (blocks < kDkvBlocks) return {0, (int)std::max<int64_t>(1, std::min(ceil_div(kDkvBlocks, blocks), most))};
+  const int64_t at_once = D <= 64 ? 512 : 256, left = blocks % at_once;
+  const int parts = causal || left == 0 || (int64_t)seqs * kv_heads >= at_once / 4 ? 1 : (int)std::min(at_once / left, most);
+  return parts > 1 ? DkvCut{blocks - left, parts} : DkvCut{0, 1};
 }
 size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 16 + 255) & ~(size_t)255; }
 
-size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D) {
-  const int parts = dkv_parts(seqs, tq, tk, heads, kv_heads);
-  return stat_bytes(tq, heads) + (parts > 1 ? (size_t)parts * 2 * tk * kv_heads * (D <= 64 ? 64 : 128) * sizeof(float) : 0);
+size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D, bool causal) {
+  const DkvCut cut = dkv_cut(seqs, tq, tk, heads, kv_heads, D, causal);
+  if (cut.parts == 1) return stat_bytes(tq, heads);
+  const size_t rows = (size_t)(slots(tk, seqs) * kv_heads - cut.whole) * cut.parts * 2 * kRows;
+  return stat_bytes(tq, heads) + rows * (D <= 64 ? 64 : 128) * sizeof(float);
 }
 
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {
   a.stat = (bf16*)ws;
   a.part = (float*)((char*)ws + stat_bytes(a.tq, a.heads));
-  a.dkv_parts = dkv_parts(a.seqs, a.tq, a.tk, a.heads, a.kv_heads);
+  const DkvCut cut = dkv_cut(a.seqs, a.tq, a.tk, a.heads, a.kv_heads, a.D, a.causal);
+  a.dkv_parts = cut.parts;
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
-    const unsigned blocks = (unsigned)(slots(a.tk, a.seqs) * a.kv_heads);
+    const unsigned blocks = (unsigned)(slots(a.tk, a.seqs) * a.kv_heads), whole = cut.parts > 1 ? (unsigned)cut.whole : blocks;
+    a.dkv_whole = (int)whole;
     hipLaunchKernelGGL((packed_dq_kernel<HD>), dim3((unsigned)(slots(a.tq, a.seqs) * a.heads)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3(blocks * a.dkv_parts), dim3(512), 0, stream, a);
-    if (a.dkv_parts > 1) hipLaunchKernelGGL((packed_dkv_join_kernel<HD>), dim3(blocks, 4), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((packed_dkv_kernel<HD>), dim3(whole + (blocks - whole) * cut.parts), dim3(512), 0, stream, a);
+    if (whole < blocks) hipLaunchKernelGGL((packed_dkv_join_kernel<HD>), dim3(blocks - whole, 4), dim3(256), 0, stream, a);
   };
   if (a.D <= 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});

@@ -16,7 +16,7 @@ struct PackedArgs {
   float* lse;                     // (heads, tq), natural logarithms; may be null in the forward pass
   bf16* stat;                     // (heads, tq, 8) stat_parts of the queries, from the dQ kernel to the dK, dV kernel
   float* part;                    // partial results of the split walk, or of dK and dV
-  int dkv_parts;                  // parts that a block's queries are cut into
+  int dkv_whole, dkv_parts;       // blocks of keys before the first whose queries are cut, and the parts that they are cut into
   const int32_t *cu_q, *cu_k, *used_k;   // used_k may be null
   int seqs, tq, tk;
   int heads, kv_heads, group, D, causal;
@@ -27,7 +27,7 @@ struct PackedArgs {
 
 size_t packed_forward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D);
 int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream);
-size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D);
+size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D, bool causal);
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream);
 
 }  // namespace fvsr

@@ -405,8 +405,8 @@ def _out_ready(out, name: str, like):
 
 
 @functools.lru_cache(256)
-def _workspace(backward: bool, sequences: int, tokens_q: int, tokens_k: int, channels: int, heads: int, kv_heads: int) -> int:
-    p = Packed(None, None, None, sequences, tokens_q, tokens_k, channels, 0, 1.0)
+def _workspace(backward: bool, sequences: int, tokens_q: int, tokens_k: int, channels: int, causal: bool, heads: int, kv_heads: int) -> int:
+    p = Packed(None, None, None, sequences, tokens_q, tokens_k, channels, causal, 1.0)
     size = lib.fvsr_packed_attention_backward_workspace if backward else lib.fvsr_packed_attention_workspace
     return size(C.byref(p), heads, kv_heads)
 
@@ -433,7 +433,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         o, ts, hs = _made(q)
         o3 = o, n, h, d, ts, hs
     lse = q.new_empty((h, n), dtype=torch.float32) if want_lse else None
-    nbytes = _workspace(False, m - 1, n, k3[1], d, h, k3[2])
+    nbytes = _workspace(False, m - 1, n, k3[1], d, bool(causal), h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     q3, k3, v3 = _ready(q3), _ready(k3), _ready(v3)
     st = _structs
@@ -477,7 +477,7 @@ def packed_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor
     if out is None:
         made = [(x, *y[1:4], ts, hs) for (x, ts, hs), y in zip(map(_made, (q, k, v)), (q3, k3, v3))]
         grads = tuple(x[0] for x in made)
-    nbytes = _workspace(True, m - 1, n, k3[1], d, h, k3[2])
+    nbytes = _workspace(True, m - 1, n, k3[1], d, bool(causal), h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     g3, q3, k3, v3, o3 = _ready(g3), _ready(q3), _ready(k3), _ready(v3), _ready(o3)
     st = _structs

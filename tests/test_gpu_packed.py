@@ -353,6 +353,33 @@ def test_long_sequences(dev):
     check_attention(dev, [1], [20000], 6, 1, 128, True, train=False)
 
 
+@pytest.mark.parametrize("d,lq,lk,used", [(64, [2100], [3400], None), (128, [2100], [3400], None), (64, [2100, 2049], [1700, 1601], [1690, 1555]),
+                                          (40, [2100], [3330], [3300])])
+def test_blocks_of_keys_left_for_a_last_round(dev, d, lq, lk, used):
+    """dK and dV where the queries of the last blocks of keys are cut into parts, and no others'."""
+    h, sel = 40, [0, 17, 39]
+    bytes_of = lambda h, causal: _abi.lib.fvsr_packed_attention_backward_workspace(
+        ctypes.byref(_abi.Packed(0, 0, None, len(lq), sum(lq), sum(lk), d, causal, 1.0)), h, h)
+    parts = bytes_of(h, 0) - bytes_of(h, 1)
+    assert 0 < parts < 2 * 4 * sum(lk) * h * d
+    g = gen_of("last round", d, len(lq))
+    (cq, cu_q), (ck, cu_k) = cu_of(lq, dev), cu_of(lk, dev)
+    us = None if used is None else torch.tensor(used, dtype=torch.int32, device=dev)
+    q, do = (randn(g, (cq[-1], h, d), dev) for _ in range(2))
+    k, v = (randn(g, (ck[-1], h, d), dev) for _ in range(2))
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, used_k=us, want_lse=True)
+    got = f.packed_attention_backward(do, q, k, v, o, lse, cu_q, cu_k, used_k=us)
+    ref = attention64(*(x[:, sel] for x in (q, k, v)), cq, ck, used=used, do=do[:, sel])
+    for n, x in zip(("dq", "dk", "dv"), got):
+        within(x[:, sel], ref[n], ref["tol_" + n], n)
+    again = f.packed_attention_backward(do, q, k, v, o, lse, cu_q, cu_k, used_k=us)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    # a few heads by themselves: cut otherwise, or not at all, and off by what the bounds allow each
+    few = f.packed_attention_backward(*(x[:, sel] for x in (do, q, k, v, o)), lse[sel], cu_q, cu_k, used_k=us)
+    for n, x in zip(("dq", "dk", "dv"), few):
+        within(x, ref[n], ref["tol_" + n], n)
+
+
 def test_offsets_past_32_bits(dev):
     """A cache whose rows lie more than 2^32 bytes from its first: the last of its sequences."""
     n, stride = 600, 1 << 22

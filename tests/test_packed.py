@@ -144,7 +144,7 @@ def test_c_entry_points_refuse_before_device_work():
                                                      None, 0, None, 0, None)
     for kw in ({"sequences": 0}, {"cu_q": None}, {"cu_k": None}, {"tokens_q": -1}, {"scale": 0.0}, {"scale": math.nan}):
         assert call(packed(**kw))[0] == _abi.ERR_INVALID_ARG, kw
-    for kw in ({"channels": 60}, {"channels": 136}, {"tokens_k": 1 << 31}, {"tokens_q": 0x7ffffe00}):
+    for kw in ({"channels": 60}, {"channels": 136}, {"tokens_k": 1 << 31}, {"tokens_q": 0x7ffffe00}, {"sequences": 1 << 21}):
         assert call(packed(**kw))[0] == _abi.ERR_UNSUPPORTED, kw
     assert call(packed(), k=view(3))[0] == _abi.ERR_INVALID_ARG
     assert call(packed(), q=view(data=24))[0] == _abi.ERR_INVALID_ARG
@@ -166,6 +166,14 @@ def test_workspaces():
         return _abi.lib.fvsr_packed_attention_workspace(C.byref(Packed(*a.values())), 4, 2)
     assert size() > 0 and size(tokens_q=4000, tokens_k=4000) == 0 and size(tokens_k=600) == 0 and size(tokens_q=0) == 0
     assert 0 < size(channels=64) < size()
+
+    def back(tq, tk, heads, seqs=1, causal=0, channels=128):
+        p = Packed(16, 16, None, seqs, tq, tk, channels, causal, 0.125)
+        return _abi.lib.fvsr_packed_attention_backward_workspace(C.byref(p), heads, heads) - tq * heads * 16
+    block = 2 * 128 * 128 * 4      # a part's sums of a block of 128 keys
+    assert back(17280, 17280, 12) == (137 * 12 - 6 * 256) * 3 * block      # what is left of 137 slots after six rounds, three parts each
+    assert back(17280, 17280, 12, causal=1) == 0 and back(16384, 16384, 12) == 0 and back(17280, 17280, 12, seqs=6) == 0
+    assert back(4096, 1280, 1) == 12 * 4 * block and back(4096, 0, 1) == 0 and back(64, 64, 12) == 0
 
 
 # ---- the plain forms against differences ---------------------------------------------------------------------------------
