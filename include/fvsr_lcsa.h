@@ -361,7 +361,7 @@ int fvsr_rotary(fvsr_ctx* ctx, int dtype, const fvsr_heads* q, const fvsr_heads*
  * cu_k[b + 1] - 1 of tokens_k, the first used_k[b] of them where used_k is given (a cache with room for more). Offsets are device
  * int32 and do not fall; they are read when the kernels run (a captured call follows them), and taken into the tensors' range
  * where they leave it. Query i of m sees all n keys, or with `causal` the first i + 1 + n - m; one that sees none gives zeros (and an
- * lse of -inf). `scale` (> 0) multiplies the scores. channels a head: a multiple of 8, at most 128. */
+ * lse of -inf). `scale` (1e-30 to 1e30) multiplies the scores. channels a head: a multiple of 8, at most 128. */
 typedef struct fvsr_packed {
   const int32_t *cu_q, *cu_k, *used_k;
   int sequences;

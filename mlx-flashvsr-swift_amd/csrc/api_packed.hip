@@ -58,6 +58,7 @@ static int check_packed(const fvsr_ctx* ctx, const fvsr_packed* p) {
   FVSR_REQUIRE(p->channels > 0 && p->channels % 8 == 0 && p->channels <= 128, FVSR_ERR_UNSUPPORTED,
                "channels of a head must be a multiple of 8, at most 128");
   FVSR_REQUIRE(std::isfinite(p->scale) && p->scale > 0.f, FVSR_ERR_INVALID_ARG, "scale must be positive and finite");
+  FVSR_REQUIRE(p->scale >= 1e-30f && p->scale <= 1e30f, FVSR_ERR_UNSUPPORTED, "scale must be from 1e-30 to 1e30");   // lse / scale stays finite
   return FVSR_OK;
 }
 

@@ -448,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
       float mx = sA[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sA[e]);
-      soft.m = pair_max(mx) * a.c;
+      soft.m = fmaxf(pair_max(mx) * a.c, -3e38f);   // finite, also where infinities in K leave nothing of this tile
     }
     pB[0] = pB[1] = bf16x8{};
     const float c = a.c;

@@ -172,7 +172,7 @@ int launch_rotary(int dtype, const fvsr_heads* q, const fvsr_heads* q_out, const
   const int heads = a.q.heads + a.k.heads;
   // heads a thread: as many as leave the card 2^18 threads, since each repeats the angles of its pairs
   const int64_t threads = tokens * a.units;
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(heads, ((int64_t)1 << 18) / threads));
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min(heads, 65535), ((int64_t)1 << 18) / threads));
   a.span = (int)ceil_div(heads, parts);
   const int64_t blocks = ceil_div(tokens, a.each);
   if (blocks >= ((int64_t)1 << 24)) return set_error(FVSR_ERR_UNSUPPORTED, "too many tokens for one launch");

@@ -484,6 +484,28 @@ def test_no_tokens(dev):
     q = torch.ones((3, 4, 64), dtype=bf, device=dev)
     o, lse = f.packed_attention(q, e[:, :2], e[:, :2], torch.tensor([0, 1, 3], dtype=torch.int32, device=dev), cu, want_lse=True)
     assert not o.any() and (lse == -math.inf).all()
+    cu_q = torch.tensor([0, 1, 3], dtype=torch.int32, device=dev)
+    dq, dk, dv = f.packed_attention_backward(q, q, e[:, :2], e[:, :2], o, lse, cu_q, cu)      # no keys
+    assert not dq.any() and dk.shape == dv.shape == (0, 2, 64)
+    dq, dk, dv = f.packed_attention_backward(e, e, q[:, :2], q[:, :2], e, lse[:, :0], cu, cu_q)      # no queries
+    assert dq.shape == e.shape and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize("nq", [1, 200])
+@pytest.mark.parametrize("h", [1, 40])
+def test_keys_whose_scores_are_all_minus_infinity(dev, nq, h):
+    """An infinity in the first keys that gives them no weight, in tiles that are seen whole: as if they were not there."""
+    g = gen_of("minus", nq, h)
+    n, blind = 1500, 70
+    q, (k, v) = randn(g, (nq, h, 64), dev), (randn(g, (n, 1, 64), dev) for _ in range(2))
+    q[..., 5] = q[..., 5].abs() + 0.1
+    _, cu_q = cu_of([nq], dev)
+    _, cu_k = cu_of([n], dev)
+    ref = attention64(q, k[blind:], v[blind:], [0, nq], [0, n - blind])
+    k[:blind, :, 5] = -math.inf
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, want_lse=True)
+    within(o, ref["o"], ref["tol_o"], "o")
+    within(lse, ref["lse"], ref["tol_lse"], "lse")
 
 
 # ---- together, as they are used ------------------------------------------------------------------------------------------

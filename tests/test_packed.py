@@ -144,7 +144,8 @@ def test_c_entry_points_refuse_before_device_work():
                                                      None, 0, None, 0, None)
     for kw in ({"sequences": 0}, {"cu_q": None}, {"cu_k": None}, {"tokens_q": -1}, {"scale": 0.0}, {"scale": math.nan}):
         assert call(packed(**kw))[0] == _abi.ERR_INVALID_ARG, kw
-    for kw in ({"channels": 60}, {"channels": 136}, {"tokens_k": 1 << 31}, {"tokens_q": 0x7ffffe00}, {"sequences": 1 << 21}):
+    for kw in ({"channels": 60}, {"channels": 136}, {"tokens_k": 1 << 31}, {"tokens_q": 0x7ffffe00}, {"sequences": 1 << 21},
+               {"scale": 1e-31}, {"scale": 1e31}):
         assert call(packed(**kw))[0] == _abi.ERR_UNSUPPORTED, kw
     assert call(packed(), k=view(3))[0] == _abi.ERR_INVALID_ARG
     assert call(packed(), q=view(data=24))[0] == _abi.ERR_INVALID_ARG
