@@ -137,12 +137,9 @@ __device__ __forceinline__ bool any_odd(lds_char* tile) {
   for (int i = 0; i < Tile<HD>::kBytes / 1024; ++i) {
     const u32x4 x = *(const lds_u32x4*)(tile + i * 1024 + (threadIdx.x & 63) * 16);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      most |= ((x[e] & 0x7f80u) + 0x80u) & 0x8000u;                  // an exponent of all ones carries
-      most |= ((x[e] >> 16 & 0x7f80u) + 0x80u) & 0x8000u;
-    }
+    for (int e = 0; e < 4; ++e) most |= (x[e] & 0x7f807f80u) + 0x00800080u;   // an exponent of all ones carries into the sign's place
   }
-  return __ballot(most != 0) != 0;
+  return __ballot((most & 0x80008000u) != 0) != 0;
 }
 
 // The same one tile row after another, without those that the lane's column does not see: 0 times an infinity or NaN there
@@ -186,11 +183,12 @@ __device__ __forceinline__ void pack(const f32x16& p, bf16x8 (&w)[2]) {
   for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (bf16)p[i];
 }
 
-// acc += tile^T w, of which, MASKED, the lane's column sees tile rows lo .. hi - 1 (w is 0 in the others)
+// acc += tile^T w, of which, MASKED, the lane's column sees tile rows lo .. hi - 1 (w is 0 in the others); `whole`: all of the wave's see
+// all
 template <int HD, bool MASKED>
-__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const f32x16& w, int lo, int hi,
+__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const f32x16& w, int lo, int hi, bool whole,
                                           f32x16 (&acc)[Tile<HD>::kD]) {
-  if (MASKED && any_odd<HD>(tile)) return add_seen<HD>(tile, w, bits(lo, hi), acc);
+  if (MASKED && !whole && any_odd<HD>(tile)) return add_seen<HD>(tile, w, bits(lo, hi), acc);
   bf16x8 p[2];
   pack(w, p);
   add_packed<HD>(tile, at, p, acc);
@@ -315,9 +313,9 @@ struct Soft {
 #pragma unroll
     for (int d = 0; d < Tile<HD>::kD; ++d) acc[d] = f32x16{};
   }
-  // a tile of keys k0 .. k0 + 31, of which, MASKED, the lane's query sees those below `lim`
+  // a tile of keys k0 .. k0 + 31, of which, MASKED, the lane's query sees those below `lim`, and every one of the wave those below `all`
   template <bool MASKED>
-  __device__ __forceinline__ void tile(lds_char* kt, lds_char* vt, Lanes<HD>& at, const bf16x8 (&q)[Tile<HD>::kT], int k0, int lim,
+  __device__ __forceinline__ void tile(lds_char* kt, lds_char* vt, Lanes<HD>& at, const bf16x8 (&q)[Tile<HD>::kT], int k0, int lim, int all,
                                        float c) {
     const int g = (threadIdx.x & 63) >> 5;
     f32x16 s = rows_times<HD>(kt, at, q);
@@ -360,7 +358,7 @@ struct Soft {
     }
     s = p;
     l += part;
-    add_times<HD, MASKED>(vt, at, s, 0, lim - k0, acc);
+    add_times<HD, MASKED>(vt, at, s, 0, lim - k0, k0 + kTile <= all, acc);
   }
 };
 
@@ -386,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   if (blk.b < 0 || blk.b >= a.seqs) return;
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
-  const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
   // tiles that some row of the block sees, and that every one sees all of
   const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
@@ -558,8 +556,8 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     wait_and_sync_but<kStep>(false);
     request(t + 3, t + 2);
     lds_char* const kt = lds + (t & 3) * T::kBytes;
-    if (t < full) soft.template tile<false>(kt, kt + kRing, at, q, t * kTile, lim, a.c);
-    else if (t * kTile < lim_max) soft.template tile<true>(kt, kt + kRing, at, q, t * kTile, lim, a.c);
+    if (t < full) soft.template tile<false>(kt, kt + kRing, at, q, t * kTile, lim, lim_min, a.c);
+    else if (t * kTile < lim_max) soft.template tile<true>(kt, kt + kRing, at, q, t * kTile, lim, lim_min, a.c);
   }
   if (i < s.nq) {
     const float l = pair_sum(soft.l);
@@ -729,7 +727,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
       }
       fence();
       lds_char* const kt = lds + buf * 2 * T::kBytes;
-      soft.template tile<decltype(masked)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, a.c);
+      soft.template tile<decltype(masked)::value>(kt, kt + T::kBytes, at, q, t * kTile, lim, 0, a.c);
       fence();
       FVSR_WAIT_VM_LGKM0(63);   // its reads are done before the next copies into this buffer
       t += 4;
@@ -890,7 +888,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   if (blk.b < 0 || blk.b >= a.seqs) return;
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
-  const int lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
+  const int lim_min = keys_seen(a, s, blk.row + wave * 32), lim_max = keys_seen(a, s, blk.row + wave * 32 + 31);
   // tiles that some row of the block sees, and that every one sees all of
   const int tiles = (keys_seen(a, s, blk.row + kRows - 1) + kTile - 1) / kTile, full = keys_seen(a, s, blk.row) / kTile;
 
@@ -1047,7 +1045,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = elem_row(e) < lim - k0 - 4 * g ? dp[e] : 0.f;
       }
-      add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, acc);
+      add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, k0 + kTile <= lim_min, acc);
     }
     ++t;
     if (t < tiles) sA = rows_times<HD>(lds + (t & 3) * kSlot, at, q);
@@ -1066,6 +1064,10 @@ __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
 }
 __device__ __forceinline__ float low_weight(uint32_t w) { return __uint_as_float((w & 0xffffu) << 14); }
 __device__ __forceinline__ float high_weight(uint32_t w) { return __uint_as_float((w >> 16) << 14); }
+
+// a part's sums of a block of keys, dK and dV; the parts of a block do not lie a power of two apart
+template <int HD>
+constexpr int kPartFloats = 2 * kRows * HD + 256;
 
 // dK and dV of 128 keys: 8 waves, two to each 32 keys. One makes S, P and dV, the other, a tile of queries behind, dP, dS and dK
 // from the P that the first one leaves in LDS (in 16 bits of its own, pack_weights).
@@ -1183,6 +1185,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   // the lane's key is seen by rows lo .. hi - 1 of a tile that begins with query r; whether any key of the wave is seen by the tile
   auto lo_of = [&](int r) { return a.causal ? j - off - r : 0; };
   auto hi_of = [&](int r) { return s.nq - r; };
+  auto all_of = [&](int r) { return r + kTile <= s.nq && (!a.causal || j0 + 31 <= r + off); };
   auto any_of = [&](int r) { return r < s.nq && (!a.causal || j0 <= r + 31 + off); };
   auto first = [&](auto masked, int u, int n, int slot) {   // S, P and dV of step u of a head, the n-th of all
     constexpr bool MASKED = decltype(masked)::value;
@@ -1206,7 +1209,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
       for (int c = 0; c < 2; ++c)
         handed[n & 1][pair][k][c][lane] = u32x4{pack_weights(p[k][8 * c], p[k][8 * c + 1]), pack_weights(p[k][8 * c + 2], p[k][8 * c + 3]),
                                                 pack_weights(p[k][8 * c + 4], p[k][8 * c + 5]), pack_weights(p[k][8 * c + 6], p[k][8 * c + 7])};
-      add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, acc);
+      add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, all_of(r), acc);
     }
   };
   auto second = [&](auto masked, int u, int n, int slot) {   // dP, dS and dK of step u of a head, the n-th of all
@@ -1235,7 +1238,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[k][e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? ds[k][e] : 0.f;
       }
-      add_times<HD, MASKED>(qt + k * T::kBytes, at, ds[k], lo, hi, acc);
+      add_times<HD, MASKED>(qt + k * T::kBytes, at, ds[k], lo, hi, all_of(r), acc);
     }
   };
   // The walk of one kind of wave: `work` for each step of the part. The second kind is a step behind the first: `ahead` steps less are
@@ -1271,8 +1274,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
     for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   }
   if (parts > 1) {   // for packed_dkv_join_kernel: [block][part][dK, dV][key][HD]
-    const int64_t at = ((int64_t)(block - a.dkv_whole) * parts + part) * 2 + (makes_dv ? 1 : 0);
-    float* const row = a.part + (at * kRows + j - blk.row) * HD;
+    float* const row = a.part + ((int64_t)(block - a.dkv_whole) * parts + part) * kPartFloats<HD> + ((makes_dv ? kRows : 0) + j - blk.row) * HD;
 #pragma unroll
     for (int d = 0; d < T::kD; ++d)
 #pragma unroll
@@ -1291,8 +1293,8 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
   Span s;
   const Block blk = block_of<true>(a, block / a.kv_heads, s);
   if (blk.b < 0 || blk.b >= a.seqs) return;
-  constexpr int kCols = HD / 4, kEach = kRows / 4, kStride = 2 * kRows * HD;
-  const float* const parts = a.part + (int64_t)blockIdx.x * a.dkv_parts * kStride;
+  constexpr int kCols = HD / 4, kEach = kRows / 4;
+  const float* const parts = a.part + (int64_t)blockIdx.x * a.dkv_parts * kPartFloats<HD>;
 #pragma unroll 2
   for (int e = threadIdx.x; e < 2 * kEach * kCols; e += 256) {
     const int col = e % kCols, row = (int)blockIdx.y * kEach + e / kCols % kEach, v = e / kCols / kEach, j = blk.row + row;
@@ -1301,7 +1303,7 @@ __global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedArgs a) {
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < a.dkv_parts; ++i) {
-      const f32x4 y = *(const f32x4*)(p + i * kStride);
+      const f32x4 y = *(const f32x4*)(p + i * kPartFloats<HD>);
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] += y[c];
     }
@@ -1380,8 +1382,8 @@ size_t stat_bytes(int64_t tq, int heads) { return ((size_t)tq * heads * 16 + 255
 size_t packed_backward_workspace(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D, bool causal) {
   const DkvCut cut = dkv_cut(seqs, tq, tk, heads, kv_heads, D, causal);
   if (cut.parts == 1) return stat_bytes(tq, heads);
-  const size_t rows = (size_t)(slots(tk, seqs) * kv_heads - cut.whole) * cut.parts * 2 * kRows;
-  return stat_bytes(tq, heads) + rows * (D <= 64 ? 64 : 128) * sizeof(float);
+  const size_t parts = (size_t)(slots(tk, seqs) * kv_heads - cut.whole) * cut.parts;
+  return stat_bytes(tq, heads) + parts * (D <= 64 ? kPartFloats<64> : kPartFloats<128>) * sizeof(float);
 }
 
 int launch_packed_backward(PackedArgs a, void* ws, hipStream_t stream) {

@@ -146,6 +146,9 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
     return result, total, rstd
 
 
+_grad_workspace = functools.lru_cache(256)(lib.fvsr_rms_norm_backward_workspace)
+
+
 def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor, weight=None, dsum=None,
                       want_weight: bool = True, stream=None, out=None):
     """(dx, dweight) of rms_norm; dx is the gradient of x and of the residual alike. total: the sum that it returned, or the x that
@@ -180,7 +183,7 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
     dw = ws = None
     nbytes = 0
     if want_weight:
-        nbytes = lib.fvsr_rms_norm_backward_workspace(rows, c)
+        nbytes = _grad_workspace(rows, c)
         dw = _empty_like(w) if kind == DTYPE_F32 and w is not None and w.dim() == 1 else dy.new_empty(c, dtype=torch.float32)
         ws = dy.new_empty(nbytes, dtype=torch.uint8)
     rc = lib.fvsr_rms_norm_backward(_handle(dev), _CODE[dtype], d2.data_ptr(), t2.data_ptr(), stride, rstd.data_ptr(), _p(ds), rows,

@@ -171,7 +171,7 @@ def test_workspaces():
     def back(tq, tk, heads, seqs=1, causal=0, channels=128):
         p = Packed(16, 16, None, seqs, tq, tk, channels, causal, 0.125)
         return _abi.lib.fvsr_packed_attention_backward_workspace(C.byref(p), heads, heads) - tq * heads * 16
-    block = 2 * 128 * 128 * 4      # a part's sums of a block of 128 keys
+    block = (2 * 128 * 128 + 256) * 4      # a part's sums of a block of 128 keys
     assert back(17280, 17280, 12) == (137 * 12 - 6 * 256) * 3 * block      # what is left of 137 slots after six rounds, three parts each
     assert back(17280, 17280, 12, causal=1) == 0 and back(16384, 16384, 12) == 0 and back(17280, 17280, 12, seqs=6) == 0
     assert back(4096, 1280, 1) == 12 * 4 * block and back(4096, 0, 1) == 0 and back(64, 64, 12) == 0
