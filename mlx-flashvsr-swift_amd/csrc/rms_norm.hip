@@ -51,6 +51,30 @@ struct Team {
   static constexpr int kRuns = kLanes / 16;   // runs of 128 channels that the team's j-th vectors cover
 };
 
+// Values c0 + 8 l16 .. of a row, as load_raw8 gives them once `settle` has been called. The last part of 8 of a bf16 row is read as the
+// row's last 8 values, by one load like the others, and moved into its place when it is needed: values read one by one are put together
+// by waiting for them, which a row on its way ahead must not do (8000 x 4001: the gradient 94 us so, 56 at 4000).
+template <typename T, bool EIGHTS>
+__device__ __forceinline__ Raw8<T> load_part(const T* row, int c0, int l16, int C) {
+  if (EIGHTS || sizeof(T) == 4 || C < 8) return load_raw8<T, EIGHTS>(row, c0, l16, C);
+  Raw8<T> r;
+  *(u32x4*)r.v = u32x4{0, 0, 0, 0};
+  const int c = c0 + l16 * 8;
+  if (c < C) *(u32x4*)r.v = *(const any16*)(row + min(c, C - 8));
+  return r;
+}
+template <typename T, bool EIGHTS>
+__device__ __forceinline__ void settle(Raw8<T>& r, int c0, int l16, int C) {
+  if constexpr (!EIGHTS && sizeof(T) == 2) {
+    const int c = c0 + l16 * 8, by = C >= 8 && c < C ? max(0, c + 8 - C) : 0;   // values too many in front
+    u32x4 x = *(const u32x4*)r.v;
+    if (by & 4) x = u32x4{x[2], x[3], 0, 0};
+    if (by & 2) x = u32x4{x[1], x[2], x[3], 0};
+    if (by & 1) x = u32x4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16, x[3] >> 16};
+    *(u32x4*)r.v = x;
+  }
+}
+
 template <typename T, typename P, bool EIGHTS, int WAVES, int NV>
 __global__ __launch_bounds__(Team<WAVES>::kThreads) void rms_norm_kernel(RmsArgs a) {
   using W = Team<WAVES>;
@@ -65,9 +89,11 @@ __global__ __launch_bounds__(Team<WAVES>::kThreads) void rms_norm_kernel(RmsArgs
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c0 = (run0 + W::kRuns * j) * kRun;
-    rx[j] = load_raw8<T, EIGHTS>(x, c0, l16, C);
-    if (a.r) rr[j] = load_raw8<T, EIGHTS>((const T*)a.r + row * C, c0, l16, C);
+    rx[j] = load_part<T, EIGHTS>(x, c0, l16, C);
+    if (a.r) rr[j] = load_part<T, EIGHTS>((const T*)a.r + row * C, c0, l16, C);
   }
+  settle<T, EIGHTS>(rx[NV - 1], (run0 + W::kRuns * (NV - 1)) * kRun, l16, C);   // no vector before it is a row's last
+  if (a.r) settle<T, EIGHTS>(rr[NV - 1], (run0 + W::kRuns * (NV - 1)) * kRun, l16, C);
   float v[NV][8];
   float sq = 0.f;
 #pragma unroll
@@ -118,64 +144,87 @@ __global__ __launch_bounds__(Team<WAVES>::kThreads, EIGHTS && WAVES < 16 ? 2 : 1
   const int l16 = threadIdx.x & 15, C = a.C;
   const int team = threadIdx.x / W::kLanes, lane = threadIdx.x % W::kLanes, run0 = lane >> 4;
   auto first = [&](int j) { return (run0 + W::kRuns * j) * kRun; };
+  // the rows as they lie stay in registers, and are widened in each pass: a row's and the next one's are half, or a quarter, of the floats.
+  // The widest rows take the weights from the cache for each row, and keep dw in LDS, where they pass what a lane of 16 waves has.
+  constexpr bool kLean = WAVES == 16 && NV > 1, kAhead = DS && !(kLean && (sizeof(T) == 4 || !EIGHTS));
+  __shared__ __attribute__((aligned(16))) f32x4 held[kLean ? 2 * NV * W::kThreads : 1];
   float w[NV][8], dw[NV][8];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
+  auto weights = [&](int j) {
     if (a.w) load8<P, EIGHTS>((const P*)a.w, first(j), l16, C, w[j]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 8; ++e)
       if (!a.w) w[j][e] = 1.f;
-      dw[j][e] = 0.f;
-    }
+  };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (!kLean) weights(j);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[j][e] = 0.f;
+    if constexpr (kLean) held[2 * j * W::kThreads + lane] = held[(2 * j + 1) * W::kThreads + lane] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  Raw8<T> rdy[NV], rs[NV], rds[NV];
-  float rstd = 0.f;
-  auto load = [&](int64_t row) {
-    rstd = a.rstd[row];
+  struct Row {
+    float rstd;
+    Raw8<T> dy[NV], s[NV], ds[DS ? NV : 1];
+  };
+  auto load_ds = [&](Row& x, int64_t row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x.ds[j] = load_part<T, EIGHTS>((const T*)a.ds + row * C, first(j), l16, C);
+  };
+  auto load = [&](Row& x, int64_t row) {
+    x.rstd = a.rstd[row];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      rdy[j] = load_raw8<T, EIGHTS>((const T*)a.dy + row * C, first(j), l16, C);
-      rs[j] = load_raw8<T, EIGHTS>((const T*)a.s + row * a.s_stride, first(j), l16, C);
-      if constexpr (DS) rds[j] = load_raw8<T, EIGHTS>((const T*)a.ds + row * C, first(j), l16, C);
+      x.dy[j] = load_part<T, EIGHTS>((const T*)a.dy + row * C, first(j), l16, C);
+      x.s[j] = load_part<T, EIGHTS>((const T*)a.s + row * a.s_stride, first(j), l16, C);
     }
+    if constexpr (kAhead) load_ds(x, row);
   };
   int turn = 0;
   const int64_t step = (int64_t)gridDim.x * W::kTeams;
   int64_t row = (int64_t)blockIdx.x * W::kTeams + team;
-  if (row < a.rows) load(row);
+  Row next;
+  if (row < a.rows) load(next, row);
   for (; row < a.rows; row += step, turn ^= 1) {
-    const float r = rstd;
-    float dy[NV][8], n[NV][8], ds[DS ? NV : 1][8];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        dy[j][e] = (float)rdy[j].v[e];
-        n[j][e] = (float)rs[j].v[e];
-        if constexpr (DS) ds[j][e] = (float)rds[j].v[e];
-      }
-    if (row + step < a.rows) load(row + step);
+    Row x = next;
+    if constexpr (DS && !kAhead) load_ds(x, row);
+    if (row + step < a.rows) load(next, row + step);
+    settle<T, EIGHTS>(x.dy[NV - 1], first(NV - 1), l16, C);
+    settle<T, EIGHTS>(x.s[NV - 1], first(NV - 1), l16, C);
+    if constexpr (DS) settle<T, EIGHTS>(x.ds[NV - 1], first(NV - 1), l16, C);
+    // past the row's end (in the last vectors only) dy and s are 0, and n has to be 0 too where rstd is not finite
+    auto normed = [&](int j, int e) {
+      const float n = (float)x.s[j].v[e] * x.rstd;
+      return j == NV - 1 && first(j) + l16 * 8 + (EIGHTS ? 0 : e) >= C ? 0.f : n;
+    };
     float s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      // past the row's end dy and s are 0, and n has to be 0 too where rstd is not finite
-      const bool past = j == NV - 1 && first(j) + l16 * 8 >= C;
+      if constexpr (kLean) {
+        weights(j);
+        *(f32x4*)&dw[j][0] = held[2 * j * W::kThreads + lane];
+        *(f32x4*)&dw[j][4] = held[(2 * j + 1) * W::kThreads + lane];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[j][e] *= r;
-        if (past || (!EIGHTS && first(j) + l16 * 8 + e >= C)) n[j][e] = 0.f;
-        s2 = fmaf(dy[j][e] * w[j][e], n[j][e], s2);
-        dw[j][e] = fmaf(dy[j][e], n[j][e], dw[j][e]);
+        const float dy = (float)x.dy[j].v[e], n = normed(j, e);
+        s2 = fmaf(dy * w[j][e], n, s2);
+        dw[j][e] = fmaf(dy, n, dw[j][e]);
+      }
+      if constexpr (kLean) {
+        held[2 * j * W::kThreads + lane] = *(const f32x4*)&dw[j][0];
+        held[(2 * j + 1) * W::kThreads + lane] = *(const f32x4*)&dw[j][4];
       }
     }
     const float m2 = team_sum<WAVES>(s2, sm[turn]) / (float)C;
+    if constexpr (kLean) asm volatile("" ::: "memory");   // the weights again, not kept from above
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if constexpr (kLean) weights(j);
       float dx[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        dx[e] = r * (dy[j][e] * w[j][e] - n[j][e] * m2);
-        if constexpr (DS) dx[e] += ds[j][e];
+        dx[e] = x.rstd * ((float)x.dy[j].v[e] * w[j][e] - normed(j, e) * m2);
+        if constexpr (DS) dx[e] += (float)x.ds[j].v[e];
       }
       store8<T, EIGHTS>((T*)a.dx + row * C, first(j) + l16 * 8, 0, C, dx);
     }
@@ -199,7 +248,7 @@ __global__ __launch_bounds__(Team<WAVES>::kThreads, EIGHTS && WAVES < 16 ? 2 : 1
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (first(j) + l16 * 8 + e < C) part[first(j) + l16 * 8 + e] = dw[j][e];
+        if (first(j) + l16 * 8 + e < C) part[first(j) + l16 * 8 + e] = kLean ? held[(2 * j + e / 4) * W::kThreads + lane][e % 4] : dw[j][e];
     }
   }
 }
@@ -265,7 +314,7 @@ int launch_rms_norm_grad(int dtype, int param_dtype, const void* dy, const void*
   if (blocks > 0) {
     const RmsGradArgs a{dy, s, s_stride, rstd, ds, rows, C, w, dx, dw ? part : nullptr};
     const int rc = pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
-      return pick_rms_team(C, dtype == FVSR_DTYPE_BF16, [&](auto waves, auto nv) {
+      return pick_rms_team(C, dtype == FVSR_DTYPE_BF16 && C <= 6144, [&](auto waves, auto nv) {
         constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
         constexpr bool V = decltype(v)::value;
         const dim3 grid((unsigned)blocks), block(Team<W>::kThreads);

@@ -52,7 +52,8 @@ def stream_of(gen, rows, c, dtype, dev):
 
 @pytest.mark.parametrize("dtype", [bf, f32])
 @pytest.mark.parametrize("rows,c", [(1, 1), (3, 7), (5, 8), (65, 64), (17, 128), (4, 129), (33, 520), (9, 1003), (130, 1536), (3, 2047),
-                                    (5, 4096), (2, 6000), (3, 8192), (2, 8961), (2, 16384)])
+                                    (5, 4096), (2, 6000), (3, 8192), (2, 8961), (2, 16384), (3, 1026), (4, 1004), (3, 10), (4, 13), (3, 4102),
+                                    (7, 9214), (600, 9), (1100, 8195)])
 def test_rms_norm_and_gradient(dev, dtype, rows, c):
     g = gen_of(rows, c)
     x, r, dy, ds = (stream_of(g, rows, c, dtype, dev) for _ in range(4))
