@@ -29,7 +29,7 @@ struct RotaryArgs {
   int end1, end2;           // pairs [0, end1) are of axis 0, [end1, end2) of axis 1, the others of axis 2
   const double* freq;       // (pairs)
   int back;                 // the gradient
-  int units, span;          // units of kPairs pairs (then of 8 copied channels) a head; heads a thread
+  int units, span;          // units of a head; heads a thread
   int each;                 // tokens a workgroup
   uint32_t by_units;        // 2^16 / units, rounded up: a thread's number (below 256) times it, >> 16, is the quotient
 };
@@ -53,15 +53,38 @@ __device__ __forceinline__ void sincos_turns(double turns, float& sine, float& c
   cosine = (q + 1) & 2 ? -b : b;
 }
 
-// kPairs: 4 neighbours (16 bytes of bf16 a thread, adjacent threads adjacent) or 8 in halves (16 bytes of either)
-template <typename T, bool HALVES>
+// The first `by` of 8 values taken out, the others moved to the front.
+template <typename T, typename V>
+__device__ __forceinline__ V moved(V v, int by) {
+  if constexpr (sizeof(T) == 2) {
+    u32x4 x = __builtin_bit_cast(u32x4, v);
+    if (by & 4) x = u32x4{x[2], x[3], 0, 0};
+    if (by & 2) x = u32x4{x[1], x[2], x[3], 0};
+    if (by & 1) x = u32x4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16, x[3] >> 16};
+    return __builtin_bit_cast(V, x);
+  } else {
+#pragma unroll
+    for (int b = 4; b > 0; b >>= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = !(by & b) ? v[e] : e + b < 8 ? v[e + b] : 0;
+    return v;
+  }
+}
+
+// A thread's unit is 8 channels of neighbouring pairs (kPairs 4, the last of them perhaps past the pairs, and copied), or 8 channels
+// of either half (kPairs 8), or, behind the halves, 8 channels that are copied. All are read by whole vectors, several heads at once,
+// those that would pass the head's end from 8 before it: a unit that went channel by channel, head after head, would be what the
+// others wait for (17280 tokens, 20 heads of 80 channels, 33 pairs: 78 us so, 31 now).
+// WHOLE: units of whole vectors only, either turned or copied.
+template <typename T, bool HALVES, bool WHOLE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   constexpr int kPairs = HALVES ? 8 : 4;
   typedef T any_half __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  typedef T half8 __attribute__((ext_vector_type(8)));
   const int mine = (int)(threadIdx.x * a.by_units >> 16);
   const int64_t token = (int64_t)blockIdx.x * a.each + mine;
   if (mine >= a.each || token >= a.tokens) return;
-  const int unit = (int)threadIdx.x - mine * a.units, first = unit * kPairs;
+  const int unit = (int)threadIdx.x - mine * a.units, first = unit * kPairs, D = a.D;
   const int heads = a.q.heads + a.k.heads, h0 = (int)blockIdx.y * a.span, h1 = min(heads, h0 + a.span);
   const T* const qx = (const T*)a.q.x + token * a.q.xt;
   const T* const kx = (const T*)a.k.x + token * a.k.xt;
@@ -69,86 +92,92 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   T* const ko = (T*)a.k.out + token * a.k.ot;
   auto from = [&](int h) { return h < a.q.heads ? qx + h * a.q.xh : kx + (h - a.q.heads) * a.k.xh; };
   auto to = [&](int h) { return h < a.q.heads ? qo + h * a.q.oh : ko + (h - a.q.heads) * a.k.oh; };
-  if (first >= a.pairs) {   // channels past the pairs: 8 a unit
-    const int c0 = 2 * a.pairs + 8 * (unit - (a.pairs + kPairs - 1) / kPairs), n = min(8, a.D - c0);
-    for (int h = h0; h < h1; ++h) {
-      const T* x = from(h) + c0;
-      T* o = to(h) + c0;
-      if (x == o) continue;
-      if (n == 8) {
-        *(any_half*)o = *(const any_half*)x;
-      } else {
-        for (int e = 0; e < n; ++e) o[e] = x[e];
-      }
-    }
+  // pairs that turn, first channel, channels (of either half); the first channel of the other half
+  const int turned = max(0, min(kPairs, a.pairs - first)), n = WHOLE ? kPairs : turned, beyond = unit - (a.pairs + kPairs - 1) / kPairs;
+  const int c0 = !HALVES ? 2 * first : turned > 0 ? first : 2 * a.pairs + 8 * beyond, count = WHOLE ? 8 : HALVES && n > 0 ? n : min(8, D - c0);
+  const int d0 = a.pairs + first;
+  constexpr int kAhead = sizeof(T) == 2 && !HALVES ? 8 : 4;   // heads whose loads are under way together
+  half8 u[kAhead], v[kAhead];
+  if (WHOLE && turned == 0) {
+    for (int h = h0; h < h1; ++h)
+      if (to(h) != from(h)) *(any_half*)(to(h) + c0) = *(const any_half*)(from(h) + c0);
     return;
   }
-  const int n = min(kPairs, a.pairs - first);
-  constexpr int kAhead = sizeof(T) == 2 && !HALVES ? 8 : 4;   // heads whose loads are under way together
-  any_half u[kAhead], v[kAhead];
+  const int at0 = WHOLE ? c0 : max(0, min(c0, D - 8)), at1 = WHOLE ? d0 : max(0, min(d0, D - 8));
+  auto fetch = [&](const T* x, int at) {
+    half8 r;
+    if (WHOLE || D >= 8) {
+      r = *(const any_half*)(x + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = e < D ? x[e] : (T)0.f;
+    }
+    return r;
+  };
   auto load = [&](int h) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (h + j < h1) {
-        const T* x = from(h + j) + (HALVES ? first : 2 * first);
-        u[j] = *(const any_half*)x;
-        if constexpr (HALVES) v[j] = *(const any_half*)(x + a.pairs);
+        u[j] = fetch(from(h + j), at0);
+        if constexpr (HALVES)
+          if (n > 0) v[j] = fetch(from(h + j), at1);
       }
     }
   };
-  if (n == kPairs) load(h0);   // on their way while the angles are made
+  load(h0);   // on their way while the angles are made
   float c[kPairs], s[kPairs];
 #pragma unroll
   for (int e = 0; e < kPairs; ++e) {
-    const int p = min(first + e, a.pairs - 1), axis = p < a.end1 ? 0 : p < a.end2 ? 1 : 2;
+    c[e] = s[e] = 0.f;
+    if (e >= n) continue;   // WHOLE: all or none
+    const int p = first + e, axis = p < a.end1 ? 0 : p < a.end2 ? 1 : 2;
     const int64_t at = axis * a.tokens + token;
     const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
     sincos_turns(pos * a.freq[p] * 0.15915494309189535, s[e], c[e]);   // 1 / (2 pi)
     if (a.back) s[e] = -s[e];
   }
-  if (n == kPairs) {
-    for (int h = h0; h < h1; h += kAhead) {
-      any_half x[kAhead], y[kAhead];
+  auto store = [&](T* o, half8 x) {
+    if (count == 8) {
+      *(any_half*)o = x;
+    } else {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if constexpr (HALVES) {
+      for (int e = 0; e < 8; ++e)
+        if (e < count) o[e] = x[e];
+    }
+  };
+  for (int h = h0; h < h1; h += kAhead) {
+    half8 x[kAhead], y[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      x[j] = WHOLE || at0 == c0 ? u[j] : moved<T>(u[j], c0 - at0);
+      if constexpr (HALVES) {
+        y[j] = WHOLE || at1 == d0 ? v[j] : moved<T>(v[j], d0 - at1);
+        if (n > 0) {   // past n: not stored
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float p = (float)u[j][e], q = (float)v[j][e];
+            const float p = (float)x[j][e], q = (float)y[j][e];
             x[j][e] = (T)(p * c[e] - q * s[e]);
             y[j][e] = (T)(p * s[e] + q * c[e]);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = (float)u[j][2 * e], q = (float)u[j][2 * e + 1];
-            x[j][2 * e] = (T)(p * c[e] - q * s[e]);
-            x[j][2 * e + 1] = (T)(p * s[e] + q * c[e]);
-          }
         }
-      }
-      load(h + kAhead);
+      } else if (n > 0) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (h + j < h1) {
-          T* o = to(h + j) + (HALVES ? first : 2 * first);
-          *(any_half*)o = x[j];
-          if constexpr (HALVES) *(any_half*)(o + a.pairs) = y[j];
+        for (int e = 0; e < 4; ++e) {
+          const float p = (float)x[j][2 * e], q = (float)x[j][2 * e + 1];
+          const T p2 = (T)(p * c[e] - q * s[e]), q2 = (T)(p * s[e] + q * c[e]);
+          x[j][2 * e] = WHOLE || e < n ? p2 : x[j][2 * e];
+          x[j][2 * e + 1] = WHOLE || e < n ? q2 : x[j][2 * e + 1];
         }
       }
     }
-    return;
-  }
-  for (int h = h0; h < h1; ++h) {   // the last unit of a number of pairs that does not divide
-    const T* x = from(h);
-    T* o = to(h);
+    load(h + kAhead);
 #pragma unroll
-    for (int e = 0; e < kPairs; ++e) {
-      if (e < n) {
-        const int i0 = HALVES ? first + e : 2 * (first + e), i1 = HALVES ? i0 + a.pairs : i0 + 1;
-        const float p = (float)x[i0], q = (float)x[i1];
-        o[i0] = (T)(p * c[e] - q * s[e]);
-        o[i1] = (T)(p * s[e] + q * c[e]);
+    for (int j = 0; j < kAhead; ++j) {
+      if (h + j < h1) {
+        T* const o = to(h + j);
+        if (n > 0 || o != from(h + j)) store(o + c0, x[j]);
+        if constexpr (HALVES)
+          if (n > 0) store(o + d0, y[j]);
       }
     }
   }
@@ -165,8 +194,7 @@ int launch_rotary(int dtype, const fvsr_heads* q, const fvsr_heads* q_out, const
   for (int i = 0; i < axes; ++i) a.pairs += axis_pairs[i];
   a.end1 = axis_pairs[0];
   a.end2 = a.end1 + (axes > 1 ? axis_pairs[1] : 0);
-  const int per = halves ? 8 : 4;
-  a.units = (int)(ceil_div(a.pairs, per) + ceil_div(D - 2 * a.pairs, 8));
+  a.units = (int)(halves ? ceil_div(a.pairs, 8) + ceil_div(D - 2 * a.pairs, 8) : ceil_div(D, 8));
   a.each = 256 / a.units;
   a.by_units = 65536 / a.units + 1;
   const int heads = a.q.heads + a.k.heads;
@@ -179,8 +207,14 @@ int launch_rotary(int dtype, const fvsr_heads* q, const fvsr_heads* q_out, const
   const dim3 grid((unsigned)blocks, (unsigned)ceil_div(heads, a.span));
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (halves) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, dim3(256), 0, stream, a);
+    const bool whole = a.pairs % (halves ? 8 : 4) == 0 && D % 8 == 0;
+    auto with = [&](auto h) {
+      constexpr bool H = decltype(h)::value;
+      if (whole) hipLaunchKernelGGL((rotary_kernel<T, H, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((rotary_kernel<T, H, false>), grid, dim3(256), 0, stream, a);
+    };
+    if (halves) with(std::true_type{});
+    else with(std::false_type{});
   };
   if (dtype == FVSR_DTYPE_BF16) go(bf16{});
   else go(float{});

@@ -137,7 +137,8 @@ def test_rms_norm_of_rows_that_are_not_finite(dev):
 @pytest.mark.parametrize("n,h,hk,d,axes,far", [(1, 12, 2, 128, (22, 21, 21), 1024), (5, 3, 1, 16, (8,), 10), (33, 4, 4, 64, (16, 16), 500),
                                                (7, 2, 0, 80, (16, 17), 10 ** 6), (100, 9, 3, 104, (25, 27), 2 ** 31 - 1),
                                                (3, 5, 1, 6, (1,), 3), (19, 20, 4, 30, (0, 11, 2), 77), (2100, 2, 1, 256, (40, 40, 40), 9000), (3, 1, 1, 1024, (512,), 50),
-                                               (2, 2, 1, 1022, (3, 200, 307), 2 ** 20)])
+                                               (2, 2, 1, 1022, (3, 200, 307), 2 ** 20), (9, 2, 1, 12, (6,), 50), (9, 3, 1, 20, (3, 4), 50),
+                                               (5, 4, 2, 44, (9, 10), 1000), (6, 9, 9, 72, (33,), 100), (40, 3, 2, 18, (2, 3, 4), 9), (300, 5, 5, 72, (17, 15), 60)])
 def test_rotary_and_gradient(dev, dtype, halves, n, h, hk, d, axes, far):
     g = gen_of(n, h, d, halves)
     qkv = randn(g, (n, h + 2 * hk + 1, d), dev, dtype)
@@ -168,6 +169,32 @@ def test_rotary_and_gradient(dev, dtype, halves, n, h, hk, d, axes, far):
     same = f.rotary(q, k, *how, out=(q, k))
     assert same[0] is q and torch.equal(q, got[0]) and (k is None or torch.equal(k, got[1]))
     assert torch.equal(qkv[:, h + hk:], keep[:, h + hk:])
+
+
+@pytest.mark.parametrize("dtype", [bf, f32])
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("d,pairs", [(16, 5), (80, 33), (24, 8), (72, 33)])
+def test_rotary_of_channels_that_are_not_finite(dev, dtype, halves, d, pairs):
+    """Channels past the pairs are copied whatever they hold, and a pair's values stay in the pair."""
+    g = gen_of("not finite", d, pairs, halves)
+    n, m = 7, 2 * pairs
+    q, pos = randn(g, (n, 3, d), dev, dtype), torch.randint(0, 50, (n,), generator=g, dtype=torch.int32).to(dev)
+    freq = f.rotary_frequencies((pairs,), device=dev)
+    want = f.rotary(q, None, pos, freq, (pairs,), halves)[0]
+    q[:, 1, m:] = math.inf
+    q[:, 1, m::2] = math.nan
+    got = f.rotary(q, None, pos, freq, (pairs,), halves)[0]
+    assert torch.equal(got[..., :m], want[..., :m])
+    assert torch.equal(got[..., m:].view(torch.int16 if dtype == bf else torch.int32), q[..., m:].view(torch.int16 if dtype == bf else torch.int32))
+    same = q.clone()
+    f.rotary(same, None, pos, freq, (pairs,), halves, out=(same, None))
+    assert torch.equal(same[..., :m], want[..., :m])
+    i = pairs - 1
+    a, b = (i, i + pairs) if halves else (2 * i, 2 * i + 1)
+    q[:, 1, a] = math.nan
+    got = f.rotary(q, None, pos, freq, (pairs,), halves)[0]
+    rest = [c for c in range(m) if c not in (a, b)]
+    assert got[:, 1, [a, b]].isnan().all() and torch.equal(got[:, 1, rest], want[:, 1, rest])
 
 
 def test_rotary_is_the_fused_epilogues(dev):
