@@ -347,9 +347,9 @@ typedef struct fvsr_heads {
   int64_t token_stride, head_stride;
 } fvsr_heads;
 
-/* Rotary positions: of each head (channels wide, even, at most 1024), pair i turns by positions[axis of i][token] * frequencies[i] radians: (a, b)
- * becomes (a cos - b sin, a sin + b cos), or with `back` (the gradient) (a cos + b sin, b cos - a sin). Pairs are channels (2 i,
- * 2 i + 1), or with `halves` (i, pairs + i); the first axis_pairs[0] pairs are of axis 0, and so on (1 to 3 axes); channels
+/* Rotary positions: of each head (channels wide, even, at most 1024), pair i turns by positions[axis of i][token] * frequencies[i]
+ * radians: (a, b) becomes (a cos - b sin, a sin + b cos), or with `back` (the gradient) (a cos + b sin, b cos - a sin). Pairs are
+ * channels (2 i, 2 i + 1), or with `halves` (i, pairs + i); the first axis_pairs[0] pairs are of axis 0, and so on (1 to 3 axes); channels
  * past the pairs are copied. Angles in 64 bits (positions below 2^53 in magnitude), the rest in fp32, rounded once. positions:
  * (axes, tokens), int32, or int64 with positions64; frequencies: (pairs) fp64. k and k_out may be NULL. An output may be its
  * input. */

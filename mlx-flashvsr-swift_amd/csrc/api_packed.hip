@@ -52,13 +52,15 @@ static int check_bf16_view(const fvsr_heads* x, const char* what, int heads, int
 static int check_packed(const fvsr_ctx* ctx, const fvsr_packed* p) {
   FVSR_REQUIRE(ctx != nullptr, FVSR_ERR_INVALID_ARG, "ctx is NULL");
   FVSR_REQUIRE(p != nullptr, FVSR_ERR_INVALID_ARG, "the sequences are NULL");
-  FVSR_REQUIRE(p->sequences > 0 && p->cu_q && p->cu_k, FVSR_ERR_INVALID_ARG, "at least one sequence, with offsets of queries and keys, is needed");
+  FVSR_REQUIRE(p->sequences > 0 && p->cu_q && p->cu_k, FVSR_ERR_INVALID_ARG,
+               "at least one sequence, with offsets of queries and keys, is needed");
   FVSR_REQUIRE(p->tokens_q >= 0 && p->tokens_k >= 0, FVSR_ERR_INVALID_ARG, "tokens must be >= 0");
   FVSR_REQUIRE(p->tokens_q <= 0x7fffff00 && p->tokens_k <= 0x7fffff00, FVSR_ERR_UNSUPPORTED, "more tokens than 31-bit offsets hold");
   FVSR_REQUIRE(p->channels > 0 && p->channels % 8 == 0 && p->channels <= 128, FVSR_ERR_UNSUPPORTED,
                "channels of a head must be a multiple of 8, at most 128");
   FVSR_REQUIRE(std::isfinite(p->scale) && p->scale > 0.f, FVSR_ERR_INVALID_ARG, "scale must be positive and finite");
-  FVSR_REQUIRE(p->scale >= 1e-30f && p->scale <= 1e30f, FVSR_ERR_UNSUPPORTED, "scale must be from 1e-30 to 1e30");   // lse / scale stays finite
+  FVSR_REQUIRE(p->scale >= 1e-30f && p->scale <= 1e30f, FVSR_ERR_UNSUPPORTED,
+               "scale must be from 1e-30 to 1e30");   // lse / scale stays finite
   return FVSR_OK;
 }
 

@@ -12,7 +12,10 @@
 //
 // bf16 operands, fp32 sums on v_mfma_f32_32x32x16_bf16: S^T = K Q^T, so a lane owns a query, P packed to bf16 goes
 // straight back in as the operand of O^T += V^T P^T, V^T read transposed from row-major LDS (ds_read_b64_tr_b16). P and dS are
-// rounded to bf16 for those products (off by at most 2^-9 of themselves each); sums of P, the softmax and delta stay fp32.
+// rounded to bf16 for those products (off by at most 2^-8 of themselves each); sums of P, the softmax and delta stay fp32.
+//
+// Figures below are of 12 heads of 128 over 17280 x 17280 rows, whole, unless said otherwise; a bf16 library product of 16384^3 reaches
+// 1345 TFLOP/s on the same card.
 #include <algorithm>
 
 #include "attn_tile.hpp"
@@ -366,6 +369,12 @@ struct Soft {
 // a product of the matrix core at a time with a share of the rest behind it, fenced so that this is the order they are issued in:
 // the exponentials, the reads of operands four rounds ahead, and the copies of K(T + 4) and V(T + 2) run while the matrix core
 // does. K and V have a ring of four tiles each: K(T) is read a step before, and V(T) a step after, P(T) is made.
+//
+// Bound by the matrix core (63 % of the card's cycles; 16 products of 32 cycles a tile and wave, two waves a SIMD) at the clock that such
+// work leaves, 1.6 GHz: 1.60 ms, 1.15 PFLOP/s. Without the pipeline, one tile's S, P and P V after another: 1.88 ms; the rows' maximum in
+// every tile instead of Soft's reference: 2.46 ms. 4 waves of 32 queries share the tiles, since a wave of 64 has no registers
+// left for the next S beside its sums. Of 64 channels there are half the products for as many exponentials: 0.95 PFLOP/s. Causal, 808 us.
+// Sequences of 512 read and write 201 MB in 73 us: near the copy's rate.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   using T = Tile<HD>;
@@ -402,8 +411,12 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   // past the last tile, and before the first: zeros
   auto k_rsrc = [&](int t) { return rows_rsrc(kb, a.k.t, t * kTile, t < 0 ? t * kTile : s.nk, a.D); };
   auto v_rsrc = [&](int t) { return rows_rsrc(vb, a.v.t, t * kTile, t < 0 ? t * kTile : s.nk, a.D); };
-  auto copy_k = [&](const u32x4& r, auto p, int slot) { dma16<decltype(p)::value * 1024>(r, mine + slot * T::kBytes, koff[decltype(p)::value], 0); };
-  auto copy_v = [&](const u32x4& r, auto p, int slot) { dma16<kRing + decltype(p)::value * 1024>(r, mine + slot * T::kBytes, voff[decltype(p)::value], 0); };
+  auto copy_k = [&](const u32x4& r, auto p, int slot) {
+    dma16<decltype(p)::value * 1024>(r, mine + slot * T::kBytes, koff[decltype(p)::value], 0);
+  };
+  auto copy_v = [&](const u32x4& r, auto p, int slot) {
+    dma16<kRing + decltype(p)::value * 1024>(r, mine + slot * T::kBytes, voff[decltype(p)::value], 0);
+  };
   auto request = [&](int tk, int tv) {
     const u32x4 kr = k_rsrc(tk), vr = v_rsrc(tv);
     static_for<0, kMine>([&](auto p) { copy_k(kr, p, tk & 3); });
@@ -434,9 +447,9 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     }
     auto k_op = [&](int slot, int c) { return *(const lds_bf16x8*)((lds_char*)(uintptr_t)krow[c] + slot * T::kBytes); };
     auto v_op = [&](int slot, int c) {   // product c: rows 16 (c / kD) .., channels 32 (c % kD) ..
-      const int u = c / T::kD, d = c % T::kD;
-      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[0][d] + slot * T::kBytes + 16 * u * T::kRow));
-      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[1][d] + slot * T::kBytes + 16 * u * T::kRow));
+      const int d = c % T::kD, off = slot * T::kBytes + 16 * (c / T::kD) * T::kRow;
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[0][d] + off));
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((lds_char*)(uintptr_t)vtr[1][d] + off));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     f32x16 sA, sB;
@@ -573,6 +586,11 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
 // stand in one order (sequence, key head, item, tile) and are cut into equal parts, one a workgroup, whatever the lengths are:
 // a part begins and ends inside items, whose results it leaves for packed_join_kernel, and finishes those in between. Of an
 // item's tiles each of the 4 waves takes every fourth, with a ring of its own and no barrier.
+//
+// Memory-bound: K and V move once. 24 sequences of up to 17280 keys, 16 heads of 128 over 4: 260 MB in 63 us, 4.1 TB/s, and 4.8 to join;
+// one of 43200 keys, 12 heads over 2: 44 MB in 12.7 us and 4.3, where the offsets' two round trips, the rings' first tiles and the meeting
+// of the waves in LDS stand beside the 9 that its bytes take. One workgroup a compute unit, with 128 KB of K and V under way or in use:
+// three waves with rings of three tiles had the same bytes and took longer.
 struct Parts {
   int work, parts;   // tiles of all items; workgroups that share them
   __device__ __forceinline__ int begin(int w) const { return (int)((int64_t)work * w / parts); }
@@ -585,7 +603,9 @@ __device__ __forceinline__ Span lane_span(const PackedArgs& a, int b) {   // spa
 }
 
 constexpr int kMaxParts = 256;        // workgroups of the split walk: its rings leave room for one on a compute unit
-constexpr int kMinTiles = 8;          // tiles a part, at the least (two a wave), but where items are shorter: each costs a round trip
+// Tiles a part, at the least (two a wave), but where items are shorter: each costs a round trip. One query over 4096 keys, 12 heads of
+// 128: 11.4 us a call of a graph with 8, 13.2 with 4, 13.0 with 16; over 1024 keys and 2 key heads 11.3, 10.4 and 13.1.
+constexpr int kMinTiles = 8;
 constexpr int kMostWork = 1 << 30;    // tiles of a call (split)
 
 // The parts, and for the tile `of(parts)` its sequence and that one's first tile. Called by the whole workgroup of 256;
@@ -674,7 +694,8 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
     }
   }
   int tile, b, first;
-  const Parts parts = find_tile(a, sm, [&](const Parts& p) { return (int)blockIdx.x < p.parts ? p.begin(blockIdx.x) : -1; }, tile, b, first);
+  const auto of = [&](const Parts& p) { return (int)blockIdx.x < p.parts ? p.begin(blockIdx.x) : -1; };
+  const Parts parts = find_tile(a, sm, of, tile, b, first);
   Cut* const cut = (Cut*)a.part + blockIdx.x;
   float* const partial = a.part + kMaxParts * sizeof(Cut) / 4;
   if (tid == 0) cut->pieces = 0;
@@ -748,13 +769,15 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {   // 16-byte pieces of a row, XOR-swizzled by row
           const int piece = (8 * d + 2 * c + g) ^ (l32 & 7);
-          *(f32x4*)(mine + l32 * HD + 4 * piece) = f32x4{soft.acc[d][4 * c], soft.acc[d][4 * c + 1], soft.acc[d][4 * c + 2], soft.acc[d][4 * c + 3]};
+          const auto& x = soft.acc[d];
+          *(f32x4*)(mine + l32 * HD + 4 * piece) = f32x4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
         }
     }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == tiles;
     float* const part = partial + (int64_t)(2 * blockIdx.x + (tile == begin ? 0 : 1)) * Partial<HD>::kFloats;
-    if (tid == 0 && t0 == 0 && t1 < tiles) *cut = Cut{parts.owner(tile + tiles - 1) - (int)blockIdx.x + 1, tile > begin, hk, r0, rows, s.q0, {}};
+    if (tid == 0 && t0 == 0 && t1 < tiles)
+      *cut = Cut{parts.owner(tile + tiles - 1) - (int)blockIdx.x + 1, tile > begin, hk, r0, rows, s.q0, {}};
     const int here = min(kTile, rows - r0);
     for (int e = tid; e < here * (HD / 4); e += 256) {
       const int row = e / (HD / 4), piece = e % (HD / 4);
@@ -799,7 +822,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
 
 // Workgroup (x, y): rows y, y + gridDim.y, .. of the item that begins in part x and ends in a later one. All of a row's pieces are
 // asked for at once: their references and sums by a thread each, then their channels by 4 to a thread, the pieces dealt to the
-// 256 / (HD / 4) groups of threads and joined in LDS.
+// 256 / (HD / 4) groups of threads and joined in LDS. 4.3 us, a launch and three round trips; one row's pieces one after another took 60.
 template <int HD>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
   constexpr int kCols = HD / 4, kDeal = 256 / kCols;
@@ -863,6 +886,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 // ---- backward ------------------------------------------------------------------------------------------------------------
 // Two kernels, so that nothing is added with atomics: dQ walks over the keys like the forward pass (and leaves delta), dK and dV
 // walk over the queries of the group's heads. Each makes S and dP again: 7 products in all where one kernel would make 5.
+//
+// dQ is bound like the forward pass: 2.20 ms, 1.25 PFLOP/s for its three products, the matrix core busy for 71 % of the cycles.
 // What dK and dV need of a query beside its rows: -lse / scale and -delta, each as three bf16 numbers whose sum is the fp32 one.
 // A product with ones adds them to S and dP in the matrix core: as operands of an addition they would have to be in 16 registers,
 // read from LDS at eight times the bytes.
@@ -937,7 +962,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   constexpr int kSlot = 2 * T::kBytes;
   if (tiles <= 4) {
     // Where a row sees few keys, O is as large as V, and the rounding of O to bf16 would be a large part of what dS is off by: delta is
-    // made of P and dP here, as the ring holds all the tiles.
+    // made of P and dP here, as the ring holds all the tiles. (Causal sequences of 17 to 4097 tokens: a gradient is at most 0.053 from a plain
+    // form's, 0.093 without; the time is the same.)
     for (int t = 2; t < tiles; ++t) issue(t);
     wait_and_sync_but<0>(true);
     delta = 0.f;
@@ -1057,8 +1083,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 }
 
 // Two weights, from 0 to below 2, in 16 bits each: of fp32's bits the sign and the exponent's first are 0, the next 16 are kept, rounded.
-// Off by at most 2^-10 of itself, an eighth of what rounding dS to bf16 costs in the mean square, down to 2^-126 (fp16 would lose the
-// gradients of keys whose weights are all small). An infinity or NaN does not survive, but reaches dS by delta.
+// Off by at most 2^-10 of itself, a sixteenth of what rounding dS to bf16 costs in the mean square, down to 2^-126 (fp16 would lose the
+// gradients of keys whose weights are all small; fp32 took twice the LDS, and the room for two tiles a step). An infinity or NaN does not
+// survive, but reaches dS by delta.
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   return __builtin_amdgcn_perm((__float_as_uint(hi) << 2) + 0x8000u, (__float_as_uint(lo) << 2) + 0x8000u, 0x07060302u);
 }
@@ -1073,6 +1100,10 @@ constexpr int kPartFloats = 2 * kRows * HD + 256;
 // from the P that the first one leaves in LDS (in 16 bits of its own, pack_weights).
 // So a wave holds one operand and one sum, not two (which with S and dP beside them pass the 256 registers that two waves a SIMD
 // have), and the two waves of a SIMD, one of each kind, are at the matrix core by turns.
+//
+// 3.18 ms, 1.15 PFLOP/s for its four products; the matrix core is busy for 59 % of the cycles, the rest are the barrier of a step and the
+// reads behind it. Steps of two tiles: 3.57 before the last round's blocks were cut (dkv_cut), 3.80 with steps of one. S and dP of the
+// next tile before this one's rest, as the other kernels have it, was worth 2 % here and cost 40 % with 64 channels a head.
 template <int HD>
 __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(PackedArgs a) {
   using T = Tile<HD>;
@@ -1177,7 +1208,8 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
     fence();
   };
   // minus the rows' lse / scale (0) or delta (1), for every key: what S and dP of a tile begin with
-  const bf16x8 ones = g == 0 ? bf16x8{(bf16)1.f, (bf16)1.f, (bf16)1.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f} : bf16x8{};
+  const bf16 one = (bf16)(g == 0 ? 1.f : 0.f), zero = (bf16)0.f;
+  const bf16x8 ones = bf16x8{one, one, one, zero, zero, zero, zero, zero};
   auto minus = [&](int slot, int k, int which) {
     const bf16x4 x = *(const bf16x4*)((const char*)&stat[slot][k][l32] + 8 * which);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(x, bf16x4{}, 0, 1, 2, 3, 4, 5, 6, 7), ones, f32x16{}, 0, 0, 0);
@@ -1207,8 +1239,9 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        handed[n & 1][pair][k][c][lane] = u32x4{pack_weights(p[k][8 * c], p[k][8 * c + 1]), pack_weights(p[k][8 * c + 2], p[k][8 * c + 3]),
-                                                pack_weights(p[k][8 * c + 4], p[k][8 * c + 5]), pack_weights(p[k][8 * c + 6], p[k][8 * c + 7])};
+        handed[n & 1][pair][k][c][lane] =
+            u32x4{pack_weights(p[k][8 * c], p[k][8 * c + 1]), pack_weights(p[k][8 * c + 2], p[k][8 * c + 3]),
+                  pack_weights(p[k][8 * c + 4], p[k][8 * c + 5]), pack_weights(p[k][8 * c + 6], p[k][8 * c + 7])};
       add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, all_of(r), acc);
     }
   };
@@ -1274,7 +1307,8 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
     for (int d = 0; d < T::kD; ++d) acc[d] = f32x16{};
   }
   if (parts > 1) {   // for packed_dkv_join_kernel: [block][part][dK, dV][key][HD]
-    float* const row = a.part + ((int64_t)(block - a.dkv_whole) * parts + part) * kPartFloats<HD> + ((makes_dv ? kRows : 0) + j - blk.row) * HD;
+    float* const sums = a.part + ((int64_t)(block - a.dkv_whole) * parts + part) * kPartFloats<HD>;
+    float* const row = sums + ((makes_dv ? kRows : 0) + j - blk.row) * HD;
 #pragma unroll
     for (int d = 0; d < T::kD; ++d)
 #pragma unroll
@@ -1362,6 +1396,10 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
 // that a part is to have a few tens of steps: all blocks, where they are too few to fill the card, or those left over for a last round
 // of workgroups, where all queries see all keys (causal, the last blocks are short), and the lengths of few sequences leave little doubt
 // which blocks these are.
+// Gradients cut and not cut, us: 16 heads of 64 over 4, causal sequences of 17 to 4097 tokens 279 and 425; 2048 tokens of 16 heads over 2,
+// causal, 127 and 462; 17280 queries over 512 keys 261 and 513; 4096 tokens of 12 heads, causal, 267 and 234. With 512 blocks instead
+// of kDkvBlocks 313, 124, 280, 252; with 2048 294, 126, 260, 304; with 16 or 64 steps within 10 %. The last round's blocks: 17280 tokens
+// of 12 heads 5405 and 5647, of 64 channels 3109 and 3255; 4000, 5000 and 6000 tokens of 16 heads 1926 and 1951.
 constexpr int kDkvBlocks = 1024, kDkvSteps = 32, kMostDkvParts = 16;
 struct DkvCut {
   int64_t whole;

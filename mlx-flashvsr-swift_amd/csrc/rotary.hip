@@ -7,6 +7,9 @@
 // Memory-bound: q and k move once. The angle is taken in 64 bits, in turns, and only what is left of its quarter in 32: a
 // position of 10^5 keeps its angle to 10^-11, and the sine and cosine to their own last bits. A thread computes those of its
 // pairs once and uses them for as many heads as it holds.
+//
+// bf16 17280 tokens, 12 + 12 heads of 128: 47.6 us, 4.5 TB/s (a copy: 4.7), with the operands in the memory-side cache 33.8; in halves 51.
+// 4001 tokens of 9 + 3 heads of 80 in fp32: 11.2, a launch, the chain from a position to its sine, and 31 MB.
 #include <algorithm>
 
 #include "blocks8.hpp"
@@ -93,8 +96,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   auto from = [&](int h) { return h < a.q.heads ? qx + h * a.q.xh : kx + (h - a.q.heads) * a.k.xh; };
   auto to = [&](int h) { return h < a.q.heads ? qo + h * a.q.oh : ko + (h - a.q.heads) * a.k.oh; };
   // pairs that turn, first channel, channels (of either half); the first channel of the other half
-  const int turned = max(0, min(kPairs, a.pairs - first)), n = WHOLE ? kPairs : turned, beyond = unit - (a.pairs + kPairs - 1) / kPairs;
-  const int c0 = !HALVES ? 2 * first : turned > 0 ? first : 2 * a.pairs + 8 * beyond, count = WHOLE ? 8 : HALVES && n > 0 ? n : min(8, D - c0);
+  const int turned = max(0, min(kPairs, a.pairs - first)), n = WHOLE ? kPairs : turned;
+  const int beyond = unit - (a.pairs + kPairs - 1) / kPairs;
+  const int c0 = !HALVES ? 2 * first : turned > 0 ? first : 2 * a.pairs + 8 * beyond;
+  const int count = WHOLE ? 8 : HALVES && n > 0 ? n : min(8, D - c0);
   const int d0 = a.pairs + first;
   constexpr int kAhead = sizeof(T) == 2 && !HALVES ? 8 : 4;   // heads whose loads are under way together
   half8 u[kAhead], v[kAhead];
@@ -198,7 +203,9 @@ int launch_rotary(int dtype, const fvsr_heads* q, const fvsr_heads* q_out, const
   a.each = 256 / a.units;
   a.by_units = 65536 / a.units + 1;
   const int heads = a.q.heads + a.k.heads;
-  // heads a thread: as many as leave the card 2^18 threads, since each repeats the angles of its pairs
+  // Heads a thread: as many as leave the card 2^18 threads, since each repeats the angles of its pairs. 2000 and 8000 tokens of 24 heads,
+  // 4000 of 40 in halves, us: 7.2, 17.0, 16.9; with 2^16 threads 7.1, 17.3, 19.7; 2^17 6.4, 17.3, 17.7; 2^19 8.9, 20.9, 19.4; 2^20 11.9,
+  // 25.6, 21.7.
   const int64_t threads = tokens * a.units;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min(heads, 65535), ((int64_t)1 << 18) / threads));
   a.span = (int)ceil_div(heads, parts);
