@@ -318,11 +318,15 @@ def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
         _refuse("positions", "expected contiguous positions and frequencies")
     oq = ok = yq = yk = None
     if out is not None:
+        if not isinstance(out, (tuple, list)) or len(out) != 2:
+            _refuse("out", "expected a pair of tensors (or None), for q and k")
         oq, ok = out
         if ok is not None and k3 is None:
             _refuse("out", "there is no k to write")
         yq = None if oq is None else _out_heads(oq, "out", n, h, d, dtype)
         yk = None if ok is None else _out_heads(ok, "out", n, hk, d, dtype)
+        if n and yq and yk and yq[0].data_ptr() == yk[0].data_ptr():
+            _refuse("out", "q's and k's results need memory of their own")
     dev = _device(q3, "q", (k3, "k"), (positions, "positions"), (frequencies, "frequencies"), (yq and yq[0], "out"),
                   (yk and yk[0], "out"))
     st = _structs
@@ -470,10 +474,13 @@ def packed_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor
         _refuse("lse", "expected a contiguous tensor")
     made = (None, None, None)
     if out is not None:
-        out = tuple(out)
-        if len(out) != 3 or any(x is None for x in out):
+        if not isinstance(out, (tuple, list)) or len(out) != 3 or any(x is None for x in out):
             _refuse("out", "expected three tensors, for dq, dk and dv")
+        out = tuple(out)
         made = [_out_ready(x, "out", like) for x, like in zip(out, (q3, k3, v3))]
+        at = [x[0].data_ptr() for x in made if x[1]]
+        if len(set(at)) < len(at):
+            _refuse("out", "the gradients need memory of their own")
     dev = _device(q3[0], "q", (k3[0], "k"), (v3[0], "v"), (g3[0], "do"), (o3[0], "o"), (lse, "lse"), (cu_q, "cu_q"), (ck, "cu_k"),
                   (used_k, "used_k"), *((x and x[0], "out") for x in made))
     grads = out

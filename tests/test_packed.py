@@ -73,6 +73,9 @@ def test_rotary_refusals():
         f.rotary(q, k, pos, freq, (10, 10), out=(q[:, :1].expand(6, 4, 64), k))
     with pytest.raises(E, match="out"):
         f.rotary(q, None, pos, freq, (10, 10), out=(q, k))
+    for bad in (q, (q,), (q, k, k), (q, q[:, :2])):
+        with pytest.raises(E, match="out"):
+            f.rotary(q, k, pos, freq, (10, 10), out=bad)
     with pytest.raises(E, match="q"):
         f.rotary(q.transpose(1, 2), k, pos, freq, (10, 10))
     with pytest.raises(E, match="HIP device"):
@@ -113,8 +116,9 @@ def test_packed_attention_refusals():
         f.packed_attention_backward(q, q, k, k, q, lse.t(), c)
     with pytest.raises(E, match="do"):
         f.packed_attention_backward(q[:5], q, k, k, q, lse, c)
-    with pytest.raises(E, match="out"):
-        f.packed_attention_backward(q, q, k, k, q, lse, c, out=(q, k))
+    for bad in ((q, k), q, (q, k, None), (q, k, k[:5]), (q, k, k)):
+        with pytest.raises(E, match="out"):
+            f.packed_attention_backward(q, q, k, k, q, lse, c, out=bad)
     with pytest.raises(E, match="HIP device"):
         f.packed_attention_backward(q, q, k, k, q, lse, c)
 
