@@ -94,6 +94,11 @@ def _rows(x, name: str):
     return x, rows, c, (x.stride(0) if rows > 1 else c)
 
 
+def _plain(w, c: int) -> bool:
+    """Whether a weight is what _param gives of it, seen at a third of its time."""
+    return isinstance(w, _Tensor) and w.dtype is torch.float32 and w.shape == (c,) and w.is_contiguous() and not w.requires_grad
+
+
 def _like(x, name: str, rows: int, c: int, dtype):
     """A contiguous (rows, c) operand or output of this type, or None."""
     if x is None or (isinstance(x, _Tensor) and x.dtype is dtype and x.dim() == 2 and x.shape == (rows, c) and x.is_contiguous()
@@ -114,7 +119,7 @@ def rms_norm(x: torch.Tensor, weight=None, eps: float = 1e-6, residual=None, wan
             return rms_norm(x, weight, eps, residual, want_stats, quantized, out=out, out_sum=out_sum)
     x2, rows, c, stride = _rows(x, "x")
     dtype = x2.dtype
-    w = _param(weight, "weight", c)
+    w = weight if _plain(weight, c) else _param(weight, "weight", c)
     r = _like(residual, "residual", rows, c, dtype)
     if r is None and out_sum is not None:
         _refuse("out_sum", "there is no sum without a residual")
@@ -170,7 +175,7 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
     _detached(rstd, "rstd")
     if not rstd.is_contiguous():
         _refuse("rstd", "expected a contiguous tensor")
-    w = _param(weight, "weight", c)
+    w = weight if _plain(weight, c) else _param(weight, "weight", c)
     ds = _like(dsum, "dsum", rows, c, dtype)
     o = _like(out, "out", rows, c, dtype)
     dev = _device(d2, "dy", (t2, "total"), (rstd, "rstd"), (w, "weight"), (ds, "dsum"), (o, "out"))
@@ -199,16 +204,21 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
 class _Structs(threading.local):
     """A thread's memory for the structs of one call, which the library reads before it returns: filled by struct.pack_into, at a
     tenth of the time that ctypes' fields take."""
-    view, packed = struct.Struct("@Piqq"), struct.Struct("@PPPiqqiif")
+    views = [struct.Struct("@" + n * "Piqq") for n in range(9)]
+    packed = struct.Struct("@PPPiqqiif")
 
     def __init__(self):
         self.memory = C.create_string_buffer(1024)
-        at = C.addressof(self.memory)
-        self.views, self.seqs = [at + 64 * i for i in range(9)], at + 640
+        self.at = [C.addressof(self.memory) + C.sizeof(Heads) * i for i in range(9)]
+        self.seqs = C.addressof(self.memory) + 640
 
-    def heads(self, i: int, t, h: int, ts: int, hs: int) -> int:
-        self.view.pack_into(self.memory, 64 * i, t.data_ptr(), h, ts, hs)
-        return self.views[i]
+    def heads(self, *x):
+        """The addresses of the structs of these heads, as _heads gives them."""
+        fields = []
+        for t, _, h, _, ts, hs in x:
+            fields += (t.data_ptr(), h, ts, hs)
+        self.views[len(x)].pack_into(self.memory, 0, *fields)
+        return self.at[:len(x)]
 
     def sequences(self, *fields) -> int:
         self.packed.pack_into(self.memory, 640, *fields)
@@ -216,26 +226,31 @@ class _Structs(threading.local):
 
 
 _structs = _Structs()
-assert _Structs.view.size == C.sizeof(Heads) <= 64 and _Structs.packed.size <= C.sizeof(Packed) <= 384
+assert all(s.size == n * C.sizeof(Heads) <= 640 for n, s in enumerate(_Structs.views)) and _Structs.packed.size <= C.sizeof(Packed) <= 384
 
 
 def _heads(x, name: str, dtypes):
     """((L, H, D) heads of contiguous channels, L, H, D, elements between tokens, between heads): heads and tokens at any distance
     (parts of one projection's rows)."""
-    x = _tensor(x, name, dtypes, 3)
+    if not isinstance(x, _Tensor) or x.dim() != 3 or x.dtype not in dtypes or x.requires_grad:
+        x = _tensor(x, name, dtypes, 3)
     n, h, d = x.shape
+    if x.is_contiguous() and h > 0 and d > 0:
+        return x, n, h, d, h * d, d
     ts, hs, cs = x.stride()
     if h < 1 or d < 1 or (d > 1 and cs != 1):
         _refuse(name, f"expected (L, H, D) heads of contiguous channels, got {tuple(x.shape)} with strides {x.stride()}")
     return x, n, h, d, (ts if n > 1 else h * d), (hs if h > 1 else d)
 
 
-def _made(x):
-    """(a new tensor like x, elements between its tokens, between its heads)"""
+def _made(x, heads):
+    """New heads like x, whose `heads` _heads has given, as it gives them."""
     o = _empty_like(x)
-    n, h, d = o.shape[-3:]
+    _, n, h, d, ts, hs = heads
+    if ts == h * d and hs == d and x.is_contiguous():
+        return o, n, h, d, ts, hs
     ts, hs, _ = o.stride()[-3:]
-    return o, (ts if n > 1 else h * d), (hs if h > 1 else d)
+    return o, n, h, d, (ts if n > 1 else h * d), (hs if h > 1 else d)
 
 
 def _out_heads(out, name: str, n: int, h: int, d: int, dtype):
@@ -293,13 +308,14 @@ def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
     if stream is not None:
         with _current(stream, q):
             return _turn(q, k, positions, frequencies, axes, halves, None, out, back)
-    q3, n, h, d, qt, qh = _heads(q, "q", _FLOATS)
-    dtype = q3.dtype
+    q3 = _heads(q, "q", _FLOATS)
+    _, n, h, d, _, _ = q3
+    dtype = q3[0].dtype
     k3 = None
     if k is not None:
-        k3, kn, hk, kd, kt, kh = _heads(k, "k", (dtype,))
-        if kn != n or kd != d:
-            _refuse("k", f"expected {n} tokens and {d} channels a head as q has, got {tuple(k3.shape)}")
+        k3 = _heads(k, "k", (dtype,))
+        if k3[1] != n or k3[3] != d:
+            _refuse("k", f"expected {n} tokens and {d} channels a head as q has, got {tuple(k3[0].shape)}")
     try:
         count, pairs, packed = _axes(tuple(axes))
     except (TypeError, ValueError):
@@ -324,26 +340,21 @@ def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
         if ok is not None and k3 is None:
             _refuse("out", "there is no k to write")
         yq = None if oq is None else _out_heads(oq, "out", n, h, d, dtype)
-        yk = None if ok is None else _out_heads(ok, "out", n, hk, d, dtype)
+        yk = None if ok is None else _out_heads(ok, "out", n, k3[2], d, dtype)
         if n and yq and yk and yq[0].data_ptr() == yk[0].data_ptr():
             _refuse("out", "q's and k's results need memory of their own")
-    dev = _device(q3, "q", (k3, "k"), (positions, "positions"), (frequencies, "frequencies"), (yq and yq[0], "out"),
+    dev = _device(q3[0], "q", (k3 and k3[0], "k"), (positions, "positions"), (frequencies, "frequencies"), (yq and yq[0], "out"),
                   (yk and yk[0], "out"))
-    st = _structs
-    a = st.heads(0, q3, h, qt, qh)
     if yq is None:
-        oq, qt, qh = _made(q)
-        b = st.heads(1, oq, h, qt, qh)
+        yq = _made(q, q3)
+        oq = yq[0]
+    if k3 is None:
+        (a, b), e, f = _structs.heads(q3, yq), None, None
     else:
-        b = st.heads(1, yq[0], h, yq[4], yq[5])
-    e = f = None
-    if k3 is not None:
-        e = st.heads(2, k3, hk, kt, kh)
         if yk is None:
-            ok, kt, kh = _made(k)
-            f = st.heads(3, ok, hk, kt, kh)
-        else:
-            f = st.heads(3, yk[0], hk, yk[4], yk[5])
+            yk = _made(k, k3)
+            ok = yk[0]
+        a, b, e, f = _structs.heads(q3, yq, k3, yk)
     rc = lib.fvsr_rotary(_handle(dev), _CODE[dtype], a, b, e, f, n, d, positions.data_ptr(), wide, frequencies.data_ptr(), count, packed,
                          bool(halves), back, _raw_stream(dev))
     if rc:
@@ -437,16 +448,15 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     n, h, d = q3[1:4]
     o = out
     if o3 is None:
-        o, ts, hs = _made(q)
-        o3 = o, n, h, d, ts, hs
+        o3 = _made(q, q3)
+        o = o3[0]
     lse = q.new_empty((h, n), dtype=torch.float32) if want_lse else None
     nbytes = _workspace(False, m - 1, n, k3[1], d, bool(causal), h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     q3, k3, v3 = _ready(q3), _ready(k3), _ready(v3)
     st = _structs
     p = st.sequences(cu_q.data_ptr(), ck.data_ptr(), 0 if used_k is None else used_k.data_ptr(), m - 1, n, k3[1], d, bool(causal), scale)
-    views = [st.heads(i, x[0], x[2], x[4], x[5]) for i, x in enumerate((q3, k3, v3, o3))]
-    rc = lib.fvsr_packed_attention(_handle(dev), p, *views, _p(lse), out is None, _p(ws), nbytes, _raw_stream(dev))
+    rc = lib.fvsr_packed_attention(_handle(dev), p, *st.heads(q3, k3, v3, o3), _p(lse), out is None, _p(ws), nbytes, _raw_stream(dev))
     if rc:
         _check(rc, "fvsr_packed_attention")
     return o, lse
@@ -485,14 +495,14 @@ def packed_attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor
                   (used_k, "used_k"), *((x and x[0], "out") for x in made))
     grads = out
     if out is None:
-        made = [(x, *y[1:4], ts, hs) for (x, ts, hs), y in zip(map(_made, (q, k, v)), (q3, k3, v3))]
+        made = _made(q, q3), _made(k, k3), _made(v, v3)
         grads = tuple(x[0] for x in made)
     nbytes = _workspace(True, m - 1, n, k3[1], d, bool(causal), h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     g3, q3, k3, v3, o3 = _ready(g3), _ready(q3), _ready(k3), _ready(v3), _ready(o3)
     st = _structs
     p = st.sequences(cu_q.data_ptr(), ck.data_ptr(), 0 if used_k is None else used_k.data_ptr(), m - 1, n, k3[1], d, bool(causal), scale)
-    a = [st.heads(i, x[0], x[2], x[4], x[5]) for i, x in enumerate((g3, q3, k3, v3, o3, *made))]
+    a = st.heads(g3, q3, k3, v3, o3, *made)
     rc = lib.fvsr_packed_attention_backward(_handle(dev), p, *a[:5], lse.data_ptr(), *a[5:], out is None, ws.data_ptr(), nbytes,
                                             _raw_stream(dev))
     if rc:
