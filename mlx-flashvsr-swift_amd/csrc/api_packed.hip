@@ -118,7 +118,8 @@ int fvsr_rms_norm(fvsr_ctx* ctx, int dtype, const void* x, int64_t x_stride, con
 }
 
 size_t fvsr_rms_norm_backward_workspace(int64_t rows, int channels) {
-  return rows <= 0 || channels <= 0 ? 0 : (size_t)rms_grad_blocks(rows, channels) * channels * sizeof(float);
+  const int64_t blocks = rows <= 0 || channels <= 0 ? 0 : rms_grad_blocks(rows, channels);
+  return blocks > 1 ? (size_t)blocks * channels * sizeof(float) : 0;
 }
 
 int fvsr_rms_norm_backward(fvsr_ctx* ctx, int dtype, const void* dy, const void* s, int64_t s_stride, const float* rstd,
@@ -130,8 +131,8 @@ int fvsr_rms_norm_backward(fvsr_ctx* ctx, int dtype, const void* dy, const void*
   FVSR_REQUIRE(s_stride >= channels, FVSR_ERR_INVALID_ARG, "s_stride must be at least the channels");
   if (rows > 0) {
     FVSR_REQUIRE(dy && s && rstd && dx, FVSR_ERR_INVALID_ARG, "dy, s, rstd and dx must be non-NULL");
-    FVSR_REQUIRE(!dweight || (workspace && aligned(workspace, 16) &&
-                              workspace_bytes >= fvsr_rms_norm_backward_workspace(rows, channels)),
+    const size_t need = dweight ? fvsr_rms_norm_backward_workspace(rows, channels) : 0;
+    FVSR_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need),
                  FVSR_ERR_INVALID_ARG, "dweight needs a 16-byte aligned workspace of fvsr_rms_norm_backward_workspace bytes");
   }
   FVSR_ON_DEVICE(ctx);

@@ -310,7 +310,12 @@ int launch_rms_norm(int dtype, int param_dtype, const void* x, int64_t x_stride,
   });
 }
 
+// Workgroups of the gradient. One, for a few rows a team, has dw in it and needs no second launch. One and more, us of a graph's
+// calls, and with the host's: 128 rows of 128 5.8, 10.1 and 5.1, 13.7; 32 of 512 5.9, 10.0 and 5.2, 14.0; 16 of 1000 5.6, 10.0 and 6.3,
+// 13.9; 8 of 1536 5.1, 10.0 and 7.1, 14.2; 4 of 4096 7.4, 9.7 and 7.6, 13.8. Twice the rows lose: 64 of 512 9.6 and 5.4, 32 of 1000 9.3 and
+// 6.6, 8 of 4096 11.1 and 7.6, 4 of 8960 13.5 and 12.2.
 int64_t rms_grad_blocks(int64_t rows, int C) {
+  if (rows <= (C <= 128 ? 128 : C <= 512 ? 32 : C <= 1024 ? 16 : C <= 2048 ? 8 : C <= 8192 ? 4 : 1)) return std::min<int64_t>(rows, 1);
   return std::min<int64_t>(kRmsGradBlocks, C <= 128 ? ceil_div(rows, 32) : C <= 2048 ? ceil_div(rows, 8) : ceil_div(rows, 2));
 }
 
@@ -319,7 +324,7 @@ int launch_rms_norm_grad(int dtype, int param_dtype, const void* dy, const void*
                          hipStream_t stream) {
   const int64_t blocks = rms_grad_blocks(rows, C);
   if (blocks > 0) {
-    const RmsGradArgs a{dy, s, s_stride, rstd, ds, rows, C, w, dx, dw ? part : nullptr};
+    const RmsGradArgs a{dy, s, s_stride, rstd, ds, rows, C, w, dx, !dw ? nullptr : blocks == 1 ? dw : part};
     const int rc = pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
       return pick_rms_team(C, dtype == FVSR_DTYPE_BF16 && C <= 6144, [&](auto waves, auto nv) {
         constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
@@ -331,7 +336,7 @@ int launch_rms_norm_grad(int dtype, int param_dtype, const void* dy, const void*
     });
     if (rc) return rc;
   }
-  return dw ? launch_param_sum(part, (int)blocks, C, C, dw, nullptr, stream) : FVSR_OK;
+  return dw && blocks != 1 ? launch_param_sum(part, (int)blocks, C, C, dw, nullptr, stream) : FVSR_OK;
 }
 
 }  // namespace fvsr

@@ -190,7 +190,7 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, rstd: torch.Tensor,
     if want_weight:
         nbytes = _grad_workspace(rows, c)
         dw = _empty_like(w) if kind == DTYPE_F32 and w is not None and w.dim() == 1 else dy.new_empty(c, dtype=torch.float32)
-        ws = dy.new_empty(nbytes, dtype=torch.uint8)
+        ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = lib.fvsr_rms_norm_backward(_handle(dev), _CODE[dtype], d2.data_ptr(), t2.data_ptr(), stride, rstd.data_ptr(), _p(ds), rows,
                                     c, kind, _p(w), o.data_ptr(), _p(dw), _p(ws), nbytes, _raw_stream(dev))
     if rc:

@@ -135,7 +135,7 @@ def test_c_entry_points_refuse_before_device_work():
                       None)[0] == _abi.ERR_INVALID_ARG
     assert status("fvsr_rms_norm", ctx, 1, p, 16385, None, 1, 16385, 1e-6, 0, None, p, None, None, None, None, None)[0] == _abi.ERR_UNSUPPORTED
     assert status("fvsr_rms_norm", ctx, 1, p, 8, None, 1 << 40, 8, 1e-6, 0, None, p, None, None, None, None, None)[0] == _abi.ERR_UNSUPPORTED
-    assert "workspace" in status("fvsr_rms_norm_backward", ctx, 1, p, p, 8, p, None, 4, 8, 0, None, p, p, None, 0, None)[1]
+    assert "workspace" in status("fvsr_rms_norm_backward", ctx, 1, p, p, 8, p, None, 4000, 8, 0, None, p, p, None, 0, None)[1]
 
     def view(heads=4, ts=256, hs=64, data=16):
         return C.byref(Heads(data, heads, ts, hs))
@@ -178,6 +178,9 @@ def test_workspaces():
     block = (2 * 128 * 128 + 256) * 4      # a part's sums of a block of 128 keys
     assert back(17280, 17280, 12) == (137 * 12 - 6 * 256) * 3 * block      # what is left of 137 slots after six rounds, three parts each
     assert back(17280, 17280, 12, causal=1) == 0 and back(16384, 16384, 12) == 0 and back(17280, 17280, 12, seqs=6) == 0
+    norm = _abi.lib.fvsr_rms_norm_backward_workspace      # none where one workgroup has all rows
+    assert norm(128, 128) == norm(32, 512) == norm(8, 1536) == norm(1, 16384) == norm(0, 64) == 0 and norm(129, 128) == 5 * 128 * 4
+    assert norm(2, 16384) == 0 and norm(3, 16384) == 2 * 16384 * 4
     assert back(4096, 1280, 1) == 12 * 4 * block and back(4096, 0, 1) == 0 and back(64, 64, 12) == 0
 
 
