@@ -12,6 +12,7 @@ Others, per value, with U = 2^-24 and h half a step of the output's type:
 """
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -349,6 +350,15 @@ def test_few_queries_of_many_sequences(dev, n):
         check_attention(dev, lq, lk, 2, 2, 128, False, train=False, used=[k // 2 for k in lk])
 
 
+def test_hundreds_of_sequences(dev):
+    """More than a workgroup has threads: blocks that look for their sequence, and the split walk that counts its tiles."""
+    check_attention(dev, [i % 4 for i in range(700)], None, 2, 1, 64, True)
+    check_attention(dev, [(i * 7) % 40 for i in range(300)], [(i * 11) % 50 for i in range(300)], 2, 2, 128, True, start=3, tail=5)
+    lq, lk = [i % 2 for i in range(700)], [(i * 379) % 1500 + 100 for i in range(700)]
+    assert workspace(lq, lk, 2, 1, 64, True)
+    check_attention(dev, lq, lk, 2, 1, 64, True, train=False)
+
+
 def test_few_queries_and_keys_that_are_not_finite(dev):
     """Where the keys are split: an infinity or NaN in the keys and values of one token, of a sequence before or past the used keys."""
     g = gen_of("split nan")
@@ -655,6 +665,62 @@ def test_single_tokens_captured_and_on_another_stream(dev):
         ref = attention64(q, k, v, list(range(n + 1)), [room * j for j in range(n + 1)], True, used=used.tolist())
         within(o, ref["o"], ref["tol_o"], str(i))
         assert torch.equal(o, call())
+
+
+def test_calls_of_several_threads(dev):
+    """Threads with streams of their own, at the same time."""
+    g = gen_of("threads")
+    q, do = (randn(g, (300, 4, 64), dev) for _ in range(2))
+    k, v = (randn(g, (300, 2, 64), dev) for _ in range(2))
+    x, w = randn(g, (300, 256), dev), torch.ones(256, device=dev)
+    cu = [torch.tensor(c, dtype=torch.int32, device=dev) for c in ([0, 300], [0, 1, 200, 300])]
+    freq, pos = f.rotary_frequencies((32,), device=dev), torch.arange(300, dtype=torch.int32, device=dev)
+
+    def once(i):
+        a, b = f.rotary(q, k, pos + i, freq, (32,))
+        o, lse = f.packed_attention(a, b, v, cu[i % 2], causal=True, want_lse=True)
+        grads = f.packed_attention_backward(do, a, b, v, o, lse, cu[i % 2], causal=True)
+        y, _, rstd = f.rms_norm(x, w, residual=x, want_stats=True)
+        return (a, b, o, lse, *grads, y, *f.rms_norm_backward(y, x, rstd, w))
+
+    want, wrong = [once(i) for i in range(4)], []
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = once(i)
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(i for a, b in zip(got, want[i]) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_whatever_a_workspace_holds(dev):
+    """Temporaries from memory full of NaN: nothing is read before it is written."""
+    g = gen_of("workspace")
+    (_, c1), (_, ck), (_, c2) = cu_of([1, 2, 40], dev), cu_of([3000, 1, 4000], dev), cu_of([2000, 500, 60], dev)
+    q, k = randn(g, (43, 4, 128), dev), randn(g, (7001, 2, 128), dev)
+    x, y = randn(g, (2560, 4, 64), dev), randn(g, (2560, 1, 64), dev)
+    r, w = randn(g, (700, 640), dev), torch.ones(640, device=dev)
+
+    def run():
+        o, lse = f.packed_attention(x, y, y, c2, causal=True, want_lse=True)
+        n, _, rstd = f.rms_norm(r, w, want_stats=True)
+        return (*f.packed_attention(q, k, k, c1, ck, causal=True, want_lse=True), o, *f.packed_attention_backward(x, x, y, y, o, lse, c2, causal=True),
+                *f.rms_norm_backward(n, r, rstd, w))
+
+    want = run()
+    torch.cuda.synchronize()
+    for size in (1 << 18, 1 << 22, 1 << 25, 1 << 27):
+        held = [torch.full((size // 4,), math.nan, device=dev) for _ in range(4)]
+        del held
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
 
 
 def test_norm_to_8_bits_into_a_linear_layer(dev):
