@@ -161,7 +161,8 @@ __device__ __forceinline__ void add_seen(lds_char* tile, const f32x16& w, uint32
     const float p = __uint_as_float((r >> 2 & 1) ? both[1] : both[0]);   // held by the half of lanes that owns row r
     const bool see = seen >> r & 1;
 #pragma unroll
-    for (int d = 0; d < T::kD; ++d)
+    for (int d = 0; d < T::kD; ++d) {
+      __builtin_amdgcn_sched_barrier(0);   // a few registers at a time: not to spill for what is rare
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int chunk = 4 * d + c;   // channels 32 d + 8 c + 4 g ..
@@ -169,6 +170,7 @@ __device__ __forceinline__ void add_seen(lds_char* tile, const f32x16& w, uint32
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[d][4 * c + e] = see ? fmaf(p, (float)v[e], acc[d][4 * c + e]) : acc[d][4 * c + e];
       }
+    }
   }
 }
 
@@ -569,8 +571,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     wait_and_sync_but<kStep>(false);
     request(t + 3, t + 2);
     lds_char* const kt = lds + (t & 3) * T::kBytes;
-    if (t < full) soft.template tile<false>(kt, kt + kRing, at, q, t * kTile, lim, lim_min, a.c);
-    else if (t * kTile < lim_max) soft.template tile<true>(kt, kt + kRing, at, q, t * kTile, lim, lim_min, a.c);
+    if (t * kTile < lim_max) soft.template tile<true>(kt, kt + kRing, at, q, t * kTile, lim, lim_min, a.c);
   }
   if (i < s.nq) {
     const float l = pair_sum(soft.l);
