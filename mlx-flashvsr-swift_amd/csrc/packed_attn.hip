@@ -189,14 +189,21 @@ __device__ __forceinline__ void pack(const f32x16& p, bf16x8 (&w)[2]) {
 }
 
 // acc += tile^T w, of which, MASKED, the lane's column sees tile rows lo .. hi - 1 (w is 0 in the others); `whole`: all of the wave's see
-// all
+// all; `fine`: what rounding w to bf16 leaves is added too
 template <int HD, bool MASKED>
-__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const f32x16& w, int lo, int hi, bool whole,
+__device__ __forceinline__ void add_times(lds_char* tile, const Lanes<HD>& at, const f32x16& w, int lo, int hi, bool whole, bool fine,
                                           f32x16 (&acc)[Tile<HD>::kD]) {
   if (MASKED && !whole && any_odd<HD>(tile)) return add_seen<HD>(tile, w, bits(lo, hi), acc);
   bf16x8 p[2];
   pack(w, p);
   add_packed<HD>(tile, at, p, acc);
+  if (MASKED && fine) {
+    f32x16 left;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) left[i] = w[i] - (float)p[i >> 3][i & 7];
+    pack(left, p);
+    add_packed<HD>(tile, at, p, acc);
+  }
 }
 
 // the lane's row (channels 16 t + 8 (lane / 32) .. of it) as the other operand; zeros where there is none
@@ -363,7 +370,7 @@ struct Soft {
     }
     s = p;
     l += part;
-    add_times<HD, MASKED>(vt, at, s, 0, lim - k0, k0 + kTile <= all, acc);
+    add_times<HD, MASKED>(vt, at, s, 0, lim - k0, k0 + kTile <= all, false, acc);
   }
 };
 
@@ -961,10 +968,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   __builtin_amdgcn_s_barrier();   // tiles 0 and 1 have landed, for every wave
   fence();
   constexpr int kSlot = 2 * T::kBytes;
-  if (tiles <= 4) {
+  const bool few = tiles <= 4;
+  if (few) {
     // Where a row sees few keys, O is as large as V, and the rounding of O to bf16 would be a large part of what dS is off by: delta is
     // made of P and dP here, as the ring holds all the tiles. (Causal sequences of 17 to 4097 tokens: a gradient is at most 0.053 from a plain
-    // form's, 0.093 without; the time is the same.)
+    // form's, 0.093 without; the time is the same.) A sum of few dS is also off by what rounding them to bf16 leaves, which is added (`last`).
     for (int t = 2; t < tiles; ++t) issue(t);
     wait_and_sync_but<0>(true);
     delta = 0.f;
@@ -1046,7 +1054,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
   if (tiles > 4) issue(2);
-  if (full >= 4) {
+  if (!few && full >= 4) {
     wait_and_sync_but<2 * kMine>(false);
     for (; t + 4 <= full; t += 4) {
       step(std::integral_constant<int, 0>{}, sA, sB);
@@ -1072,12 +1080,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = elem_row(e) < lim - k0 - 4 * g ? dp[e] : 0.f;
       }
-      add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, k0 + kTile <= lim_min, acc);
+      add_times<HD, MASKED>(kt, at, dp, 0, lim - k0, k0 + kTile <= lim_min, few, acc);
     }
     ++t;
     if (t < tiles) sA = rows_times<HD>(lds + (t & 3) * kSlot, at, q);
   };
-  while (t < full) last(std::false_type{});
+  while (!few && t < full) last(std::false_type{});
   while (t < tiles) last(std::true_type{});
   FVSR_WAIT_VM0();   // no copy outlives the workgroup's LDS
   if (i < s.nq) store_row<HD>(a.dq.p + (int64_t)(s.q0 + i) * a.dq.t + head * a.dq.h, a.D, acc, a.scale);
@@ -1136,7 +1144,9 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   // use), those before the first from which on every row sees all of the block, and those before the last one that may not be whole.
   const int q0 = a.causal ? min(s.nq, max(0, blk.row - off) / kTile * kTile) : 0;
   const int units = blk.row < s.nk ? (s.nq - q0 + kRowsN - 1) / kRowsN : 0;
-  const int u1 = a.causal ? min(units, max(0, blk.row + kRows - 1 - off - q0 + kRowsN - 1) / kRowsN) : 0;
+  // where few queries see the block, what rounding P and dS to bf16 leaves is added as well: by the steps that may not be whole
+  const bool few = s.nq - q0 <= kRows;
+  const int u1 = few ? units : a.causal ? min(units, max(0, blk.row + kRows - 1 - off - q0 + kRowsN - 1) / kRowsN) : 0;
   const int u2 = max(u1, min(units, (s.nq - q0) / kRowsN));
   // of the steps of all the group's heads, those of this part: the first is `from_u` of head `from_h`
   const int all = units * a.group, begin = (int)((int64_t)all * part / parts);
@@ -1243,7 +1253,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
         handed[n & 1][pair][k][c][lane] =
             u32x4{pack_weights(p[k][8 * c], p[k][8 * c + 1]), pack_weights(p[k][8 * c + 2], p[k][8 * c + 3]),
                   pack_weights(p[k][8 * c + 4], p[k][8 * c + 5]), pack_weights(p[k][8 * c + 6], p[k][8 * c + 7])};
-      add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, all_of(r), acc);
+      add_times<HD, MASKED>(ot + k * T::kBytes, at, p[k], lo, hi, all_of(r), few, acc);
     }
   };
   auto second = [&](auto masked, int u, int n, int slot) {   // dP, dS and dK of step u of a head, the n-th of all
@@ -1272,7 +1282,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[k][e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? ds[k][e] : 0.f;
       }
-      add_times<HD, MASKED>(qt + k * T::kBytes, at, ds[k], lo, hi, all_of(r), acc);
+      add_times<HD, MASKED>(qt + k * T::kBytes, at, ds[k], lo, hi, all_of(r), few, acc);
     }
   };
   // The walk of one kind of wave: `work` for each step of the part. The second kind is a step behind the first: `ahead` steps less are
