@@ -263,11 +263,11 @@ __global__ __launch_bounds__(Team<WAVES>::kThreads, EIGHTS && WAVES < 16 ? 2 : 1
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kRmsGradBlocks = 512;   // two workgroups a CU: 768 took 51 us for 47.6 (17280 x 1536), and 140 for 116 (fp32 8000 x 4001)
 
-// f(waves a row, vectors a lane). `wide`: up to 4 vectors a lane, else 2. Fewer waves a row meet less; the gradient of fp32 rows and of
-// those past 6144 channels has no registers for it (bf16 17280 x 1536, forward and back: 83.6 us with 3 vectors, 88.3 with 4 waves; 4000 x
-// 8192, back: 73 with 4 vectors, 62 with 16 waves).
-template <class F>
-static int pick_rms_team(int C, bool wide, F&& f) {
+// f(waves a row, vectors a lane): up to 4 vectors a lane up to WIDE channels, else 2. Fewer waves a row meet less; the gradient of fp32 rows
+// and of those past 6144 channels has no registers for it (bf16 17280 x 1536, forward and back: 83.6 us with 3 vectors, 88.3 with 4 waves;
+// 4000 x 8192, back: 73 with 4 vectors, 62 with 16 waves).
+template <int WIDE, class F>
+static int pick_rms_team(int C, F&& f) {
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -277,14 +277,17 @@ static int pick_rms_team(int C, bool wide, F&& f) {
   if (C <= 128) f(I0{}, I1{});
   else if (C <= 512) f(I1{}, I1{});
   else if (C <= 1024) f(I1{}, I2{});
-  else if (wide && C <= 1536) f(I1{}, I3{});
-  else if (wide && C <= 2048) f(I1{}, I4{});
-  else if (C <= 2048) f(I4{}, I1{});
-  else if (C <= 4096) f(I4{}, I2{});
-  else if (wide && C <= 6144) f(I4{}, I3{});
-  else if (wide && C <= 8192) f(I4{}, I4{});
-  else if (C <= 8192) f(I16{}, I1{});
-  else f(I16{}, I2{});
+  else if (C <= 2048) {
+    if constexpr (WIDE == 0) f(I4{}, I1{});
+    else if (C <= 1536) f(I1{}, I3{});
+    else f(I1{}, I4{});
+  } else if (C <= 4096) f(I4{}, I2{});
+  else if (C <= 8192) {
+    if constexpr (WIDE == 0) f(I16{}, I1{});
+    else if (C <= 6144) f(I4{}, I3{});
+    else if constexpr (WIDE == 8192) f(I4{}, I4{});
+    else f(I16{}, I1{});
+  } else f(I16{}, I2{});
   FVSR_HIP_CHECK(hipGetLastError());
   return FVSR_OK;
 }
@@ -302,7 +305,7 @@ int launch_rms_norm(int dtype, int param_dtype, const void* x, int64_t x_stride,
   if (rows <= 0) return FVSR_OK;
   const RmsArgs a{x, x_stride, r, rows, C, eps, w, y, y8, s, rstd};
   return pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
-    return pick_rms_team(C, true, [&](auto waves, auto nv) {
+    return pick_rms_team<8192>(C, [&](auto waves, auto nv) {
       using W = Team<decltype(waves)::value>;
       hipLaunchKernelGGL((rms_norm_kernel<decltype(t), decltype(p), decltype(v)::value, decltype(waves)::value, decltype(nv)::value>),
                          dim3((unsigned)ceil_div(rows, W::kTeams)), dim3(W::kThreads), 0, stream, a);
@@ -326,7 +329,7 @@ int launch_rms_norm_grad(int dtype, int param_dtype, const void* dy, const void*
   if (blocks > 0) {
     const RmsGradArgs a{dy, s, s_stride, rstd, ds, rows, C, w, dx, !dw ? nullptr : blocks == 1 ? dw : part};
     const int rc = pick_rms_types(dtype, param_dtype, C, [&](auto t, auto p, auto v) {
-      return pick_rms_team(C, dtype == FVSR_DTYPE_BF16 && C <= 6144, [&](auto waves, auto nv) {
+      return pick_rms_team<sizeof(t) == 2 ? 6144 : 0>(C, [&](auto waves, auto nv) {
         constexpr int W = decltype(waves)::value, N = decltype(nv)::value;
         constexpr bool V = decltype(v)::value;
         const dim3 grid((unsigned)blocks), block(Team<W>::kThreads);
