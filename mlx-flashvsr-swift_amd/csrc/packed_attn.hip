@@ -6,9 +6,8 @@
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO          (dK and dV summed over the group's query heads)
 //
 // Sequence b has queries cu_q[b] .. cu_q[b + 1] - 1 and keys from cu_k[b] on. Query i of m sees all n keys, or, causal, the
-// first i + 1 + n - m. The lengths are on the device only: a workgroup finds its sequence from the number of its block (a
-// sequence of m rows takes the slots from cu[b] / rows + b on, rows being the block's, so that slots never collide and the
-// grid is known from the totals).
+// first i + 1 + n - m. The lengths are on the device only: a workgroup finds its sequence from its number (block_of), and the grid is known
+// from the totals.
 //
 // bf16 operands, fp32 sums on v_mfma_f32_32x32x16_bf16: S^T = K Q^T, so a lane owns a query, P packed to bf16 goes
 // straight back in as the operand of O^T += V^T P^T, V^T read transposed from row-major LDS (ds_read_b64_tr_b16). P and dS are
@@ -255,31 +254,68 @@ __device__ __forceinline__ Span span_of(const PackedArgs& a, int b) {
                    a.used_k ? uniform(a.used_k[b]) : 0);
 }
 
-// The block of kRows rows in `slot`: of sequence b (then its first row, `row`, in the sequence), or rows of no sequence: then
-// [lo, hi), which are cleared where the call asks for it.
+// A block of kRows rows: of sequence b, from its row `row` on (b below 0, or not below the sequences: of none). Rows of no sequence,
+// which are cleared where the call asks for it: [lo, hi), or of those below `lo` and from `hi` on every `step`-th kRows, from chunk `at`.
 struct Block {
   int b, row;
-  int lo, hi;
+  int lo, hi, at, step;
 };
-// And the sequence's span. Offsets of up to 63 sequences are held by the lanes of a wave, which look for theirs side by side: one
-// round trip to memory, where the blocks of short sequences spend much of their time.
+template <class F>
+__device__ __forceinline__ void for_outside(const Block& x, int total, F&& f) {
+  if (x.step == 0) {
+    if (x.hi > x.lo) f(x.lo, x.hi);
+    return;
+  }
+  const int lead = (x.lo + kRows - 1) / kRows, tail = (total - x.hi + kRows - 1) / kRows;
+  for (int c = x.at; c < lead + tail; c += x.step) {
+    const int from = c < lead ? c * kRows : x.hi + (c - lead) * kRows;
+    f(from, min(from + kRows, c < lead ? x.lo : total));
+  }
+}
+
+// Workgroup n's block, and the sequence's span; blocks of queries in falling order, since a sequence's last rows see most where it is
+// causal. Offsets of up to 63 sequences are held by the lanes of a wave, which look for theirs side by side: one round trip to memory,
+// where the blocks of short sequences spend much of their time.
+//
+// Blocks of sequence b begin in slot first row / kRows + b, so that slots never collide, or, short sequences, one behind another: then the
+// lanes count their blocks first. Workgroups without work among the others leave two on one compute unit and none on the next, which
+// costs the more the shorter the sequences: forward and gradient of 12 heads of 128, us, dense and with gaps: 40 sequences of 128 15.5, 61
+// and 21.5, 87; 32 of 512 67, 241 and 71, 260; 5 of 512 15.8 and 20.7 (forward); but 40 causal ones of 1024 206, 694 and 200, 667.
 template <bool KEYS>   // blocks of keys, or of queries
-__device__ __forceinline__ Block block_of(const PackedArgs& a, int slot, Span& span) {
-  const int lane = threadIdx.x & 63, seqs = a.seqs, total = KEYS ? a.tk : a.tq;
+__device__ __forceinline__ Block block_of(const PackedArgs& a, int n, Span& span) {
+  const int lane = threadIdx.x & 63, seqs = a.seqs, total = KEYS ? a.tk : a.tq, slots = total / kRows + seqs + 1;
   const int at = min(lane, seqs);
   const int q = a.cu_q[at], k = a.cu_k[at], used = a.used_k ? a.used_k[min(lane, seqs - 1)] : 0;
-  const int32_t* const cu = KEYS ? a.cu_k : a.cu_q;
-  int n = __popcll(__ballot(lane <= seqs && within(KEYS ? k : q, 0, total) / kRows + lane <= slot));
-  for (int i = 64; i <= seqs; i += 64) {
-    const bool before = i + lane <= seqs && within(cu[min(i + lane, seqs)], 0, total) / kRows + i + lane <= slot;
-    n += __popcll(__ballot(before));
+  Block x{-1, 0, 0, 0, 0, 0};
+  auto of = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+  if (seqs < 64 && total <= 4 * kRows * seqs) {
+    const int mine = KEYS ? k : q, next = __shfl_down(mine, 1), from = within(mine, 0, total);   // by every lane
+    const int rows = lane < seqs ? within(next, from, total) - from : 0;
+    const int blocks = (rows + kRows - 1) / kRows, upto = wave_scan_dpp(blocks);
+    const int all = of(upto, 63), slot = KEYS ? n : all - 1 - n;
+    if (n < all) {
+      x.b = uniform(__popcll(__ballot(upto <= slot)));   // < seqs: the last lane's is all
+      x.row = (slot - (of(upto, x.b) - of(blocks, x.b))) * kRows;
+      span = span_from(a, of(q, x.b), of(q, x.b + 1), of(k, x.b), of(k, x.b + 1), of(used, x.b));
+    } else {
+      x.lo = of(from, 0);
+      x.hi = within(of(mine, seqs), x.lo, total);
+      x.at = n - all;
+      x.step = max(1, slots - all);
+    }
+    return x;
   }
-  Block x;
-  x.b = uniform(n) - 1;
+  const int32_t* const cu = KEYS ? a.cu_k : a.cu_q;
+  const int slot = KEYS ? n : slots - 1 - n;
+  int before = __popcll(__ballot(lane <= seqs && within(KEYS ? k : q, 0, total) / kRows + lane <= slot));
+  for (int i = 64; i <= seqs; i += 64) {
+    const bool is = i + lane <= seqs && within(cu[min(i + lane, seqs)], 0, total) / kRows + i + lane <= slot;
+    before += __popcll(__ballot(is));
+  }
+  x.b = uniform(before) - 1;
   const int b = max(x.b, 0);   // <= seqs
   int first;                   // row of the sequence, or behind the last one
   if (seqs < 64) {
-    auto of = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
     first = within(of(KEYS ? k : q, b), 0, total);
     span = span_from(a, of(q, b), of(q, b + 1), of(k, b), of(k, b + 1), of(used, b));   // of no use where b is seqs
   } else {
@@ -287,7 +323,6 @@ __device__ __forceinline__ Block block_of(const PackedArgs& a, int slot, Span& s
     span = span_of(a, min(b, seqs - 1));
   }
   x.row = x.b < 0 ? 0 : (slot - (first / kRows + x.b)) * kRows;
-  x.lo = x.hi = 0;
   if (x.b < 0) {
     x.lo = slot * kRows;
     x.hi = min(x.lo + kRows, first);
@@ -383,7 +418,7 @@ struct Soft {
 // work leaves, 1.6 GHz: 1.60 ms, 1.15 PFLOP/s. Without the pipeline, one tile's S, P and P V after another: 1.88 ms; the rows' maximum in
 // every tile instead of Soft's reference: 2.46 ms. 4 waves of 32 queries share the tiles, since a wave of 64 has no registers
 // left for the next S beside its sums. Of 64 channels there are half the products for as many exponentials: 0.96 PFLOP/s. Causal, 783 us.
-// 32 sequences of 512 read and write 201 MB in 71 us, 2.8 TB/s. The tiles behind the walk have one form, masked: with a second for whole
+// 32 sequences of 512 read and write 201 MB in 66 us, 3.0 TB/s. The tiles behind the walk have one form, masked: with a second for whole
 // ones the sums were in registers twice, and what that spilled was reloaded behind the copies under way (40 causal sequences of 1024 228 us,
 // 199 now; of 512 90 and 74).
 template <int HD>
@@ -392,15 +427,15 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[8 * T::kBytes];   // [K, V][tile % 4]
   constexpr int kRing = 4 * T::kBytes;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
-  const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
-  // a sequence's last rows, which see most where it is causal, come first
+  const int head = blockIdx.x % a.heads;
   Span s;
-  const Block blk = block_of<false>(a, slots - 1 - (int)(blockIdx.x / a.heads), s);
-  if (a.clear && blk.hi > blk.lo) {
-    clear_rows(a.o, head, blk.lo, blk.hi, a.D);
-    if (a.lse)
-      for (int r = blk.lo + (int)threadIdx.x; r < blk.hi; r += 256) a.lse[(int64_t)head * a.tq + r] = -INFINITY;
-  }
+  const Block blk = block_of<false>(a, blockIdx.x / a.heads, s);
+  if (a.clear)
+    for_outside(blk, a.tq, [&](int lo, int hi) {
+      clear_rows(a.o, head, lo, hi, a.D);
+      if (a.lse)
+        for (int r = lo + (int)threadIdx.x; r < hi; r += 256) a.lse[(int64_t)head * a.tq + r] = -INFINITY;
+    });
   if (blk.b < 0 || blk.b >= a.seqs) return;
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
@@ -916,10 +951,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
   using T = Tile<HD>;
   __shared__ __attribute__((aligned(1024))) char smem[8 * T::kBytes];   // [tile % 4][K, V]
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = uniform(threadIdx.x >> 6);
-  const int slots = gridDim.x / a.heads, head = blockIdx.x % a.heads;
+  const int head = blockIdx.x % a.heads;
   Span s;
-  const Block blk = block_of<false>(a, slots - 1 - (int)(blockIdx.x / a.heads), s);
-  if (a.clear && blk.hi > blk.lo) clear_rows(a.dq, head, blk.lo, blk.hi, a.D);
+  const Block blk = block_of<false>(a, blockIdx.x / a.heads, s);
+  if (a.clear) for_outside(blk, a.tq, [&](int lo, int hi) { clear_rows(a.dq, head, lo, hi, a.D); });
   if (blk.b < 0 || blk.b >= a.seqs) return;
   if (blk.row >= s.nq) return;
   const int i = blk.row + wave * 32 + l32, lim = keys_seen(a, s, i);
@@ -1136,10 +1171,11 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
   // the first keys, which most queries see, first
   Span s;
   const Block blk = block_of<true>(a, block / a.kv_heads, s);
-  if (a.clear && part == 0 && blk.hi > blk.lo) {
-    clear_rows(a.dk, hk, blk.lo, blk.hi, a.D);
-    clear_rows(a.dv, hk, blk.lo, blk.hi, a.D);
-  }
+  if (a.clear && part == 0)
+    for_outside(blk, a.tk, [&](int lo, int hi) {
+      clear_rows(a.dk, hk, lo, hi, a.D);
+      clear_rows(a.dv, hk, lo, hi, a.D);
+    });
   if (blk.b < 0 || blk.b >= a.seqs) return;
   if (blk.row >= s.room) return;
   const int j0 = blk.row + pair * 32, j = j0 + l32;
