@@ -1449,7 +1449,9 @@ int launch_packed_forward(PackedArgs a, void* ws, hipStream_t stream) {
 // which blocks these are.
 // Gradients cut and not cut, us: 16 heads of 64 over 4, causal sequences of 17 to 4097 tokens 279 and 425; 2048 tokens of 16 heads over 2,
 // causal, 127 and 462; 17280 queries over 512 keys 261 and 513; 4096 tokens of 12 heads, causal, 267 and 234. With 512 blocks instead
-// of kDkvBlocks 313, 124, 280, 252; with 2048 294, 126, 260, 304; with 16 or 64 steps within 10 %. The last round's blocks: 17280 tokens
+// of kDkvBlocks 313, 124, 280, 252; with 2048 294, 126, 260, 304; with 16 or 64 steps within 10 %. Half of kDkvSteps where the blocks
+// leave half of the card idle: 4, 490 and 895 tokens of 24 heads over 6, causal, 89 and 140; 669 of 32 over 8 59 and 79; 1024 of 12 63 and
+// 63; a quarter 88, 68, 65; and of 192 blocks (2048 tokens of 12) half 122, all 100. The last round's blocks: 17280 tokens
 // of 12 heads 5405 and 5647, of 64 channels 3109 and 3255; 4000, 5000 and 6000 tokens of 16 heads 1926 and 1951.
 constexpr int kDkvBlocks = 1024, kDkvSteps = 32, kMostDkvParts = 16;
 struct DkvCut {
@@ -1460,7 +1462,7 @@ DkvCut dkv_cut(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads, int D,
   if (tk == 0) return {0, 1};
   const int64_t blocks = (ceil_div(tk, kRows) + seqs / 2) * kv_heads;
   const int64_t steps = ceil_div(tq, (int64_t)kTile * seqs) * (heads / kv_heads);   // of a tile
-  const int64_t most = std::min<int64_t>(steps / kDkvSteps, kMostDkvParts);
+  const int64_t most = std::min<int64_t>(steps / (blocks <= 128 ? kDkvSteps / 2 : kDkvSteps), kMostDkvParts);
   if (blocks < kDkvBlocks) return {0, (int)std::max<int64_t>(1, std::min(ceil_div(kDkvBlocks, blocks), most))};
   const int64_t at_once = D <= 64 ? 512 : 256, left = blocks % at_once;
   const int parts = causal || left == 0 || (int64_t)seqs * kv_heads >= at_once / 4 ? 1 : (int)std::min(at_once / left, most);

@@ -181,7 +181,7 @@ def test_workspaces():
     norm = _abi.lib.fvsr_rms_norm_backward_workspace      # none where one workgroup has all rows
     assert norm(128, 128) == norm(32, 512) == norm(8, 1536) == norm(1, 16384) == norm(0, 64) == 0 and norm(129, 128) == 5 * 128 * 4
     assert norm(2, 16384) == 0 and norm(3, 16384) == 2 * 16384 * 4
-    assert back(4096, 1280, 1) == 12 * 4 * block and back(4096, 0, 1) == 0 and back(64, 64, 12) == 0
+    assert back(4096, 1280, 1) == 12 * 8 * block and back(4096, 0, 1) == 0 and back(64, 64, 12) == 0
 
 
 # ---- the plain forms against differences ---------------------------------------------------------------------------------
