@@ -501,6 +501,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     f32x16 sA, sB;
     bf16x8 pA[2], pB[2];
     sA = rows_times<HD>(lds, at, q);
+    wait_and_sync_but<0>(true);   // every wave has read K(0): the first step's copies of K(4) go into its place
     {
       float mx = sA[0];
 #pragma unroll
