@@ -249,7 +249,10 @@ def _made(x, heads):
     _, n, h, d, ts, hs = heads
     if ts == h * d and hs == d and x.is_contiguous():
         return o, n, h, d, ts, hs
-    ts, hs, _ = o.stride()[-3:]
+    ts, hs, cs = o.stride()[-3:]
+    if cs != 1:   # of windows that overlap, the dimension with the shortest stride is innermost
+        o = x.new_empty(x.shape)
+        ts, hs = h * d, d
     return o, n, h, d, (ts if n > 1 else h * d), (hs if h > 1 else d)
 
 

@@ -37,3 +37,27 @@ def test_the_first_tile_is_read_before_its_place_is_filled_again(dev, d, keys):
     ref = attention64(q[:, sel], k[:, sel], v[:, sel], [0, m], [0, keys])
     within(o[:, sel], ref["o"], ref["tol_o"], "o")
     within(lse[sel], ref["lse"], ref["tol_lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", [bf, torch.float32])
+@pytest.mark.parametrize("shape,strides", [((4, 2, 8), (16, 1, 1)), ((4, 2, 8), (1, 16, 1)), ((9, 3, 8), (2, 1, 1)), ((1, 4, 8), (1, 1, 1)),
+                                           ((40, 1, 64), (1, 1, 1)), ((5, 4, 64), (0, 1, 1))])
+def test_windows_that_overlap_are_read(dev, dtype, shape, strides):
+    """Heads, or tokens, one element apart: results have their own layout, with the channels innermost."""
+    g = gen_of("windows", shape, strides)
+    n, h, d = shape
+    x = randn(g, (4096,), dev, dtype).as_strided(shape, strides)
+    own = x.contiguous()
+    freq, pos = f.rotary_frequencies((d // 2,), device=dev), torch.arange(n, dtype=torch.int32, device=dev)
+    for call in (f.rotary, f.rotary_backward):
+        for a, b in zip(call(x, x, pos, freq, (d // 2,)), call(own, own, pos, freq, (d // 2,))):
+            assert a.stride(-1) == 1 and torch.equal(a, b)
+    if dtype != bf:
+        return
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    o, lse = f.packed_attention(x, x, x, cu, causal=True, want_lse=True)
+    want, wlse = f.packed_attention(own, own, own, cu, causal=True, want_lse=True)
+    assert o.stride(-1) == 1 and torch.equal(o, want) and torch.equal(lse, wlse)
+    got = f.packed_attention_backward(x, x, x, x, o, lse, cu, causal=True)
+    for a, b in zip(got, f.packed_attention_backward(own, own, own, own, want, wlse, cu, causal=True)):
+        assert a.stride(-1) == 1 and torch.equal(a, b)
