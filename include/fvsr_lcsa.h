@@ -371,9 +371,11 @@ typedef struct fvsr_packed {
   float scale;
 } fvsr_packed;
 
+enum { FVSR_CLEAR_LSE = 2 };   /* of `clear` below; any other value but 0 clears o as well */
 /* o = softmax(scale q k^T) v, bf16; lse (heads, tokens_q) fp32, log(sum exp(scores)), or NULL. k and v have the same heads, q and o a
  * multiple of them, whose neighbours share one. Data 16-byte and strides 8-element aligned, 128 tokens' strides below 2^31 bytes.
- * Rows of no sequence are left as they were, or with `clear` zeros (lse -inf). */
+ * Rows of no sequence are left as they were, or with `clear` zeros (lse -inf); with FVSR_CLEAR_LSE, for a new lse beside an o
+ * whose rows are to stay, only those of lse are set. */
 size_t fvsr_packed_attention_workspace(const fvsr_packed* p, int heads, int kv_heads);
 int fvsr_packed_attention(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads* q, const fvsr_heads* k, const fvsr_heads* v,
                           const fvsr_heads* o, float* lse, int clear, void* workspace, size_t workspace_bytes, void* stream);

@@ -190,7 +190,7 @@ int fvsr_packed_attention(fvsr_ctx* ctx, const fvsr_packed* p, const fvsr_heads*
   PackedArgs a = args_of(p, q, k, v);
   a.o = out_of(o);
   a.lse = lse;
-  a.clear = clear ? 1 : 0;
+  a.clear = clear == FVSR_CLEAR_LSE ? 2 : clear ? 3 : 0;
   return launch_packed_forward(a, workspace, (hipStream_t)stream);
 }
 

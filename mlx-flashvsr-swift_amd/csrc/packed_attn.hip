@@ -432,7 +432,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
   const Block blk = block_of<false>(a, blockIdx.x / a.heads, s);
   if (a.clear)
     for_outside(blk, a.tq, [&](int lo, int hi) {
-      clear_rows(a.o, head, lo, hi, a.D);
+      if (a.clear & 1) clear_rows(a.o, head, lo, hi, a.D);
       if (a.lse)
         for (int r = lo + (int)threadIdx.x; r < hi; r += 256) a.lse[(int64_t)head * a.tq + r] = -INFINITY;
     });
@@ -732,8 +732,10 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
   if (a.clear) {   // rows of no sequence, a head a turn
     const int lo = within(uniform(a.cu_q[0]), 0, a.tq), hi = within(uniform(a.cu_q[a.seqs]), lo, a.tq);
     for (int h = blockIdx.x; h < a.heads; h += gridDim.x) {
-      clear_rows(a.o, h, 0, lo, a.D);
-      clear_rows(a.o, h, hi, a.tq, a.D);
+      if (a.clear & 1) {
+        clear_rows(a.o, h, 0, lo, a.D);
+        clear_rows(a.o, h, hi, a.tq, a.D);
+      }
       if (a.lse)
         for (int r = tid; r < a.tq; r += 256)
           if (r < lo || r >= hi) a.lse[(int64_t)h * a.tq + r] = -INFINITY;

@@ -20,7 +20,7 @@ struct PackedArgs {
   const int32_t *cu_q, *cu_k, *used_k;   // used_k may be null
   int seqs, tq, tk;
   int heads, kv_heads, group, D, causal;
-  int clear;                      // rows of no sequence are set to zeros
+  int clear;                      // rows of no sequence: 1, o's or the gradients' are set to zeros; 2, lse's to -inf; or both
   int max_parts;                  // workgroups of the split walk
   float c, scale;                 // scale * log2(e), scale
 };

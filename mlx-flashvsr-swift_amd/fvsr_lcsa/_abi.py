@@ -12,6 +12,7 @@ OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_HIP, ERR_OUT_OF_MEMORY, ERR_CAPACITY, 
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ATTN_AUTO, ATTN_DENSE, ATTN_KERNEL = 0, 1, 3
 LAYOUT_WINDOWS, LAYOUT_GRID = 0, 1
+CLEAR_LSE = 2
 
 _vp = C.c_void_p
 _i = C.c_int

@@ -440,7 +440,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     given (a cache with room); all int32, read on the device when the kernels run. Query i of m sees all n keys, or, `causal`, the
     first i + 1 + n - m: a query over a cache that holds its own key is causal. One that sees none gives zeros. scale: 1 / sqrt(D)
     unless given. lse: (H, Lq) float32, log(sum(exp(scores))), which packed_attention_backward reads (None unless wanted). Rows of no
-    sequence are zeros, in an `out` as they were. Operands may be parts of wider rows; parts that are not 16-byte aligned
+    sequence are zeros, in an `out` as they were, and -inf in lse. Operands may be parts of wider rows; parts that are not 16-byte aligned
     are copied first."""
     if stream is not None:
         with _current(stream, q):
@@ -457,9 +457,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     nbytes = _workspace(False, m - 1, n, k3[1], d, bool(causal), h, k3[2])
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     q3, k3, v3 = _ready(q3), _ready(k3), _ready(v3)
+    clear = 1 if out is None else _abi.CLEAR_LSE if want_lse else 0   # a new lse has -inf for rows of no sequence either way
     st = _structs
     p = st.sequences(cu_q.data_ptr(), ck.data_ptr(), 0 if used_k is None else used_k.data_ptr(), m - 1, n, k3[1], d, bool(causal), scale)
-    rc = lib.fvsr_packed_attention(_handle(dev), p, *st.heads(q3, k3, v3, o3), _p(lse), out is None, _p(ws), nbytes, _raw_stream(dev))
+    rc = lib.fvsr_packed_attention(_handle(dev), p, *st.heads(q3, k3, v3, o3), _p(lse), clear, _p(ws), nbytes, _raw_stream(dev))
     if rc:
         _check(rc, "fvsr_packed_attention")
     return o, lse

@@ -1,5 +1,6 @@
 """Calls of the packed operators at the edges of what their documentation allows: the packed pass' rings at their shortest, views that
 overlap, rows of no sequence, very large scores and values, offsets that fall. Against the float64 forms of tests/packed_reference.py."""
+import math
 import zlib
 
 import pytest
@@ -61,3 +62,30 @@ def test_windows_that_overlap_are_read(dev, dtype, shape, strides):
     got = f.packed_attention_backward(x, x, x, x, o, lse, cu, causal=True)
     for a, b in zip(got, f.packed_attention_backward(own, own, own, own, want, wlse, cu, causal=True)):
         assert a.stride(-1) == 1 and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lengths,keys", [([40, 100], [40, 100]), ([700], [700]), ([1, 2], [3000, 4000]), ([3] * 70, [200] * 70)], ids=str)
+def test_lse_of_rows_of_no_sequence_is_minus_infinity_beside_a_callers_output(dev, lengths, keys):
+    """`out` keeps the rows of no sequence, an lse made by the call has -inf there, whatever its memory held."""
+    g = gen_of("lse", lengths)
+    start, tail, h, hk, d = 150, 200, 4, 2, 64
+    at = [start + sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    ak = [sum(keys[:i]) for i in range(len(keys) + 1)]
+    n = at[-1] + tail
+    q, k, v = randn(g, (n, h, d), dev), randn(g, (ak[-1], hk, d), dev), randn(g, (ak[-1], hk, d), dev)
+    cu_q, cu_k = (torch.tensor(x, dtype=torch.int32, device=dev) for x in (at, ak))
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, want_lse=True)
+    outside = torch.ones(n, dtype=torch.bool, device=dev)
+    outside[at[0]:at[-1]] = False
+    assert (lse[:, outside] == -math.inf).all() and not o[outside].any()
+    mark = torch.full_like(o, 7.0)
+    held = [torch.full((h, n), 7.0, device=dev) for _ in range(8)]      # what the next allocations of this size will hold
+    torch.cuda.synchronize()
+    del held
+    for _ in range(4):
+        out, lse2 = f.packed_attention(q, k, v, cu_q, cu_k, want_lse=True, out=mark)
+        assert out is mark and torch.equal(lse2, lse)
+        assert (mark[outside] == 7).all() and torch.equal(mark[~outside], o[~outside])
+    mark.fill_(7)
+    assert f.packed_attention(q, k, v, cu_q, cu_k, out=mark)[1] is None
+    assert (mark[outside] == 7).all() and torch.equal(mark[~outside], o[~outside])
