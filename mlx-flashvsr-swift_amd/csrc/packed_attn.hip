@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a block: 4 waves of 32
 constexpr int kTile = 32;       // rows of a tile of the other side
-constexpr float kRise = 4294967296.f;   // 2^32
+constexpr float kRise = 256.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A tile of 32 rows of HD channels in LDS (D <= HD, zeros past D): rows of 2 HD bytes, whose 16-byte chunks are XOR-swizzled by
@@ -371,8 +371,9 @@ struct Soft {
       for (int i = 0; i < 16; ++i) s[i] = elem_row(i) < lim - k0 - 4 * g ? s[i] : -INFINITY;
     }
     // The reference is the row's maximum in the first tile that it sees. Later ones are taken as they come while their
-    // exponentials' sum stays below 2^32 (what is off a bfloat16 P or a 32-bit sum does not depend on the reference); where it does
-    // not, or is NaN, the reference rises to their maximum: rare, and a branch of the whole wave.
+    // exponentials' sum stays below kRise (what is off a bfloat16 P or a 32-bit sum does not depend on the reference); where it does
+    // not, or is NaN, the reference rises to their maximum: rare, and a branch of the whole wave. The sums on the way then stay below
+    // 16 n |V| over n keys: finite for every |V| below 2^124 / n. (With a reference that only rises at 2^32 they were finite below 2^100 / n.)
     float part = 0.f;
     f32x16 p;
     auto take = [&] {

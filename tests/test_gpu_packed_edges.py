@@ -89,3 +89,20 @@ def test_lse_of_rows_of_no_sequence_is_minus_infinity_beside_a_callers_output(de
     mark.fill_(7)
     assert f.packed_attention(q, k, v, cu_q, cu_k, out=mark)[1] is None
     assert (mark[outside] == 7).all() and torch.equal(mark[~outside], o[~outside])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("m,n,causal", [(900, 700, False), (300, 700, False), (300, 300, True), (1, 6000, False), (20, 50, True)])
+def test_large_values_stay_finite(dev, d, m, n, causal):
+    """Values near 2^108 under weights that grow by 2^30 from one tile of keys to a later one: the sums on the way stay in range."""
+    g = gen_of("large", d, m, n)
+    h = 12 if m == 900 else 2      # no split of the keys, and a split, and neither
+    q, k, v = randn(g, (m, h, d), dev), randn(g, (n, 1, d), dev), randn(g, (n, 1, d), dev, scale=2.0 ** 108)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[2 * n // 3 + 8::97, :, 0] = 20.0 * d ** 0.5 / 8.0
+    cu_q, cu_k = (torch.tensor([0, x], dtype=torch.int32, device=dev) for x in (m, n))
+    ref = attention64(q, k, v, [0, m], [0, n], causal)
+    assert torch.isfinite(ref["o"]).all()
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, causal=causal, want_lse=True)
+    within(o, ref["o"], ref["tol_o"], "o")
+    within(lse, ref["lse"], ref["tol_lse"], "lse")
