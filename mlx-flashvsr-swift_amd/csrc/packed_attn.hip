@@ -1136,8 +1136,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedArgs a) {
 
 // Two weights, from 0 to below 2, in 16 bits each: of fp32's bits the sign and the exponent's first are 0, the next 16 are kept, rounded.
 // Off by at most 2^-10 of itself, a sixteenth of what rounding dS to bf16 costs in the mean square, down to 2^-126 (fp16 would lose the
-// gradients of keys whose weights are all small; fp32 took twice the LDS, and the room for two tiles a step). An infinity or NaN does not
-// survive, but reaches dS by delta.
+// gradients of keys whose weights are all small; fp32 took twice the LDS, and the room for two tiles a step). NaN does not survive, but
+// reaches dS by delta. Weights are below 2 because they are held to 2^0.5 where they are made: made again from a row's lse, one may pass 1 by
+// what rounding does to large scores, by a factor of e and more from 2^24 on, and what passed 2 was lost from dK here. That minimum takes
+// 1.0 to 1.5 % of the gradient; one of each weight as it is packed took 0.8 to 3, three-way maxima and a branch to it 0.8 to 1.5.
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   return __builtin_amdgcn_perm((__float_as_uint(hi) << 2) + 0x8000u, (__float_as_uint(lo) << 2) + 0x8000u, 0x07060302u);
 }
@@ -1289,7 +1291,7 @@ __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(Packe
       if (MASKED && !any_of(r)) continue;   // neither here nor in `second`
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        p[k][e] = __builtin_amdgcn_exp2f(p[k][e] * a.c);
+        p[k][e] = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(p[k][e] * a.c, 0.5f));   // NaN stays NaN
         if (MASKED) p[k][e] = elem_row(e) >= lo - 4 * g && elem_row(e) < hi - 4 * g ? p[k][e] : 0.f;
       }
 #pragma unroll

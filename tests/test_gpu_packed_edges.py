@@ -106,3 +106,31 @@ def test_large_values_stay_finite(dev, d, m, n, causal):
     o, lse = f.packed_attention(q, k, v, cu_q, cu_k, causal=causal, want_lse=True)
     within(o, ref["o"], ref["tol_o"], "o")
     within(lse, ref["lse"], ref["tol_lse"], "lse")
+
+
+@pytest.mark.parametrize("nq", [1, 300])
+@pytest.mark.parametrize("d", [64, 128])
+def test_weights_that_round_above_two_keep_their_gradient(dev, nq, d):
+    """Scores from 2^26 to 2^27, where a weight comes back from lse off by e^8 either way: it is held to 2^0.5, and dK loses no term. Each
+    sequence's queries see two keys of the same score (weights of a half) among others of none; dV shows the weight w that the pass
+    used, since dV of a key is w dO, and dK is w (dP - delta) q scale."""
+    seqs, keys = 128, 160
+    a = (1 + torch.arange(seqs) / 128).to(bf)                            # exact scores: q is a everywhere, k a power of two
+    q = a[:, None, None].expand(seqs, 1, d).repeat_interleave(nq, 0).to(dev)
+    k = torch.zeros((seqs, keys, 1, d), dtype=bf)
+    k[:, [40, 100]] = 2.0 ** 26 / d
+    v = torch.zeros((seqs, keys, 1, d), dtype=bf)
+    v[:, 40], v[:, 100] = 1.0, -1.0
+    k, v = (x.view(-1, 1, d).to(dev) for x in (k, v))
+    do = torch.zeros((seqs, nq, 1, d), dtype=bf)
+    do[:, 0] = 1.0                                                       # one query of a sequence
+    do = do.view(-1, 1, d).to(dev)
+    cu_q, cu_k = (n * torch.arange(seqs + 1, dtype=torch.int32, device=dev) for n in (nq, keys))
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, scale=1.0, want_lse=True)
+    assert not o.any()                                                   # a half of 1 and a half of -1
+    _, dk, dv = f.packed_attention_backward(do, q, k, v, o, lse, cu_q, cu_k, scale=1.0)
+    w = dv.view(seqs, keys, d)[:, 40, 0].double().cpu()
+    got = dk.view(seqs, keys, d)[:, 40, 0].double().cpu() / (d * a.double())      # dP = d, delta = 0
+    assert (w > 1.4).any() and (w < 0.1).any() and w.max() < 1.42        # both sides are met
+    # dV and dK are rounded to bfloat16, w to 10 bits on its way and to bfloat16 for the product: 2^-8 each
+    assert ((got - w).abs() <= 2.0 ** -6 * w).all(), (w, got)
