@@ -16,7 +16,7 @@ A training pass from one projection's rows to the next, and back:
 Rows are (L, C), heads (L, H, D), either with a leading batch of 1, on a HIP device. As in train8.py the calls keep no state,
 take their temporaries from torch's allocator on the stream they run on (the current one, or `stream`), overlap and are
 captured into graphs, and are plain functions: gradients are asked for by name, and a tensor that requires one is refused
-where autograd records. An `out` must not overlap what the call reads, but where it says so.
+where autograd records, as is one that carries a tangent. An `out` must not overlap what the call reads, but where it says so.
 """
 from __future__ import annotations
 
@@ -27,10 +27,11 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import Context, _abi
 from ._abi import DTYPE_F32, Heads, Packed, lib
-from .train8 import Blocks8, _CODE, _check, _current, _detached, _kind, _out, _out8, _p, _p8, _param, _params, _raw_stream, _refuse, _same
+from .train8 import Blocks8, _CODE, _check, _current, _detached, _kind, _no_tangents, _out, _out8, _p, _p8, _param, _params, _raw_stream, _refuse, _same
 
 __all__ = ["rms_norm", "rms_norm_backward", "rotary", "rotary_backward", "rotary_frequencies", "grid_positions",
            "packed_attention", "packed_attention_backward"]
@@ -66,6 +67,8 @@ def _tensor(x, name: str, dtypes, dims: int):
 def _device(first, name: str, *more) -> int:
     """The index of the HIP device of the first operand, which the others (None: skipped) share. Checked after every shape, before a
     pointer reaches the library."""
+    if forward_ad._current_level >= 0:
+        _no_tangents((first, name), *more)
     if not first.is_cuda:
         _refuse(name, f"expected a tensor on a HIP device, got {first.device}")
     index = first.get_device()

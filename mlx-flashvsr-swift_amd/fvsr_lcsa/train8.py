@@ -15,7 +15,8 @@ Tokens are (L, C) or (1, L, C), contiguous, on a HIP device; L may be 0. The cal
 torch's allocator on the stream that the call runs on (the current one, or `stream`), so calls may overlap on several
 streams and be captured into graphs. They are plain functions: gradients are asked for by name, and no result is part of
 an autograd graph; a tensor that requires a gradient is refused where autograd records (call them under torch.no_grad()
-or inside an autograd function). An `out` must not overlap what the call reads (but layer_norm_backward's may be dy).
+or inside an autograd function), as is one that carries a forward-mode tangent outside an autograd function. An `out` must
+not overlap what the call reads (but layer_norm_backward's may be dy).
 Norms take up to 16384 channels, the others 2^20.
 """
 from __future__ import annotations
@@ -23,6 +24,7 @@ from __future__ import annotations
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import Context, _abi
 from ._abi import DTYPE_BF16, DTYPE_F32, FVSRError, lib
@@ -101,6 +103,15 @@ def _detached(t: torch.Tensor, name: str):
                 _abi.ERR_UNSUPPORTED)
 
 
+def _no_tangents(*operands):
+    """Refuses a tensor that carries a tangent of forward-mode differentiation, which would be lost as well. None is to be had outside
+    a dual level (forward_ad._current_level below 0: the callers look at that first), nor inside an autograd function."""
+    for t, name in operands:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(name, "carries a tangent, which this call would drop: call it on forward_ad.unpack_dual(...).primal",
+                    _abi.ERR_UNSUPPORTED)
+
+
 def _tokens(x, name: str, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tensor:
     if not isinstance(x, torch.Tensor):
         _refuse(name, f"expected a tensor, got {type(x).__name__}")
@@ -150,6 +161,8 @@ def _out(out, name: str, shape, dtype):
 def _one_device(first: torch.Tensor, name: str, *more) -> torch.device:
     """The HIP device of the first operand, which the others (None: skipped) share. Checked after every shape, before a pointer
     reaches the library."""
+    if forward_ad._current_level >= 0:
+        _no_tangents((first, name), *more)
     dev = first.device
     if dev.type != "cuda":
         _refuse(name, f"expected a tensor on a HIP device, got {dev}")
