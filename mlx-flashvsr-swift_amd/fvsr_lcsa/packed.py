@@ -303,8 +303,7 @@ def rotary_backward(dq: torch.Tensor, dk, positions: torch.Tensor, frequencies: 
 
 @functools.lru_cache(64)
 def _axes(axes: tuple):
-    """(number of axes, pairs, the pairs of each as the library reads them)."""
-    axes = tuple(int(p) for p in axes)
+    """(number of axes, pairs, the pairs of each as the library reads them) of whole numbers."""
     if not 1 <= len(axes) <= 3 or min(axes) < 0 or sum(axes) < 1:
         raise ValueError
     return len(axes), sum(axes), struct.pack(f"{len(axes)}i", *axes)
@@ -323,8 +322,12 @@ def _turn(q, k, positions, frequencies, axes, halves, stream, out, back):
         if k3[1] != n or k3[3] != d:
             _refuse("k", f"expected {n} tokens and {d} channels a head as q has, got {tuple(k3[0].shape)}")
     try:
-        count, pairs, packed = _axes(tuple(axes))
-    except (TypeError, ValueError):
+        axes = tuple(axes)
+        whole = tuple(map(int, axes))   # plain numbers: what the cache knows them by
+        if whole != axes:
+            raise ValueError
+        count, pairs, packed = _axes(whole)
+    except (TypeError, ValueError, OverflowError, struct.error):
         count, pairs = 0, 0
     if not count or 2 * pairs > d or d % 2:
         _refuse("axes", f"expected 1 to 3 axes of 1 to {d // 2} pairs together, got {axes} for {d} channels")

@@ -60,3 +60,19 @@ def test_a_tensor_with_a_tangent_is_refused():
                 Inside.apply(call, dual)
             with pytest.raises(f.FVSRError, match="HIP device"):
                 call(t)
+
+
+def test_axes_are_whole_numbers_as_they_are_now():
+    """Pairs that are no whole numbers are refused, not cut off; numbers that change in place are read anew in each call."""
+    q = torch.zeros((6, 2, 64), dtype=bf)
+    pos, freq = torch.zeros((2, 6), dtype=torch.int32), torch.zeros(20, dtype=torch.float64)
+    for axes in ((10.5, 10.5), (10.9, 10), ("10", "10"), "aa", (10, float("nan")), (10, float("inf")), (10, 2 ** 40), ((10,), 10), 20, None):
+        with pytest.raises(f.FVSRError, match="axes"):
+            f.rotary(q, None, pos, freq, axes)
+    held = [torch.tensor(10), torch.tensor(10)]
+    for axes in ((10, 10), [4, 16], (10.0, 10.0), torch.tensor([10, 10]), held):
+        with pytest.raises(f.FVSRError, match="HIP device"):
+            f.rotary(q, None, pos, freq, axes)
+    held[0].fill_(9)
+    with pytest.raises(f.FVSRError, match="frequencies.*19"):
+        f.rotary(q, None, pos, freq, held)
