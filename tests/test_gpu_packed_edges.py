@@ -1,5 +1,6 @@
 """Calls of the packed operators at the edges of what their documentation allows: the packed pass' rings at their shortest, views that
 overlap, rows of no sequence, very large scores and values, offsets that fall. Against the float64 forms of tests/packed_reference.py."""
+import ctypes
 import math
 import zlib
 
@@ -134,3 +135,37 @@ def test_weights_that_round_above_two_keep_their_gradient(dev, nq, d):
     assert (w > 1.4).any() and (w < 0.1).any() and w.max() < 1.42        # both sides are met
     # dV and dK are rounded to bfloat16, w to 10 bits on its way and to bfloat16 for the product: 2^-8 each
     assert ((got - w).abs() <= 2.0 ** -6 * w).all(), (w, got)
+
+
+@pytest.mark.parametrize("n,offsets,cache", [
+    (200, [[0, 500], [-50, 100, 99999], [0, 150, 20, 200], [2 ** 31 - 1, -2 ** 31]], None),                 # blocks one behind another
+    (1500, [[0, 99999], [-7, 1499, 300, 1500], [1500, 0], [700, 2 ** 31 - 1]], None),                        # in slots
+    (300, [[(i * 97) % 331 - 15 for i in range(65)], [300 - 4 * i for i in range(76)], [0] * 64 + [2 ** 31 - 1]], None),   # of many sequences
+    (6, [[0, 99], [5, 1, 6], [-3, 2, 1, 2 ** 31 - 1]], 9000),                                                # the keys split
+], ids=["dense", "slots", "many", "split"])
+def test_offsets_that_fall_or_leave_the_tensors_write_between_the_guards(dev, n, offsets, cache):
+    """Offsets are taken into the tensors' range: results are of no use, but every row outside an output stays, the gradients' too."""
+    g = gen_of("guards", n)
+    h, hk, d, room = 4, 2, 64, cache or n
+    q, k = randn(g, (n, h, d), dev), randn(g, (room, hk, d), dev)
+
+    def guarded(like):
+        whole = torch.full((like.shape[0] + 300, *like.shape[1:]), 7.0, dtype=bf, device=dev)
+        return whole, whole[150:150 + like.shape[0]]
+
+    for cu in offsets:
+        c = torch.tensor(cu, dtype=torch.int32, device=dev)
+        ck = c if cache is None else torch.tensor([x * 1000 % 2 ** 31 for x in cu], dtype=torch.int32, device=dev)
+        if cache:
+            p = f._abi.Packed(None, None, None, len(cu) - 1, n, room, d, 1, 1.0)
+            assert f._abi.lib.fvsr_packed_attention_workspace(ctypes.byref(p), h, hk) > 0
+        for used in (None, [(-1) ** i * 40 * i for i in range(len(cu) - 1)], [2 ** 31 - 1] * (len(cu) - 1)):
+            us = None if used is None else torch.tensor(used, dtype=torch.int32, device=dev)
+            for causal in (False, True):
+                how = dict(causal=causal, used_k=us)
+                wholes, outs = zip(*(guarded(x) for x in (q, q, k, k)))
+                o, lse = f.packed_attention(q, k, k, c, ck, want_lse=True, out=outs[0], **how)
+                f.packed_attention_backward(q, q, k, k, o, lse, c, ck, out=outs[1:], **how)
+                torch.cuda.synchronize()
+                for w in wholes:
+                    assert (w[:150] == 7).all() and (w[-150:] == 7).all()
