@@ -280,7 +280,8 @@ __device__ __forceinline__ void for_outside(const Block& x, int total, F&& f) {
 // Blocks of sequence b begin in slot first row / kRows + b, so that slots never collide, or, short sequences, one behind another: then the
 // lanes count their blocks first. Workgroups without work among the others leave two on one compute unit and none on the next, which
 // costs the more the shorter the sequences: forward and gradient of 12 heads of 128, us, dense and with gaps: 40 sequences of 128 15.5, 61
-// and 21.5, 87; 32 of 512 67, 241 and 71, 260; 5 of 512 15.8 and 20.7 (forward); but 40 causal ones of 1024 206, 694 and 200, 667.
+// and 21.5, 87; 32 of 512 67, 241 and 71, 260; 5 of 512 15.8 and 20.7 (forward); but 40 causal ones of 1024 206, 694 and 200, 667. From 64
+// sequences on, which the lanes do not hold, all have gaps: dense blocks of so many are not built, and not measured.
 template <bool KEYS>   // blocks of keys, or of queries
 __device__ __forceinline__ Block block_of(const PackedArgs& a, int n, Span& span) {
   const int lane = threadIdx.x & 63, seqs = a.seqs, total = KEYS ? a.tk : a.tq, slots = total / kRows + seqs + 1;
@@ -415,7 +416,7 @@ struct Soft {
 // the exponentials, the reads of operands four rounds ahead, and the copies of K(T + 4) and V(T + 2) run while the matrix core
 // does. K and V have a ring of four tiles each: K(T) is read a step before, and V(T) a step after, P(T) is made.
 //
-// Bound by the matrix core (63 % of the card's cycles; 16 products of 32 cycles a tile and wave, two waves a SIMD) at the clock that such
+// Bound by the matrix core (64 % of the card's cycles; 16 products of 32 cycles a tile and wave, two waves a SIMD) at the clock that such
 // work leaves, 1.6 GHz: 1.60 ms, 1.15 PFLOP/s. Without the pipeline, one tile's S, P and P V after another: 1.88 ms; the rows' maximum in
 // every tile instead of Soft's reference: 2.46 ms. 4 waves of 32 queries share the tiles, since a wave of 64 has no registers
 // left for the next S beside its sums. Of 64 channels there are half the products for as many exponentials: 0.96 PFLOP/s. Causal, 783 us.
@@ -936,7 +937,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
 // Two kernels, so that nothing is added with atomics: dQ walks over the keys like the forward pass (and leaves delta), dK and dV
 // walk over the queries of the group's heads. Each makes S and dP again: 7 products in all where one kernel would make 5.
 //
-// dQ is bound like the forward pass: 2.20 ms, 1.25 PFLOP/s for its three products, the matrix core busy for 71 % of the cycles.
+// dQ is bound like the forward pass: 2.20 ms, 1.25 PFLOP/s for its three products, the matrix core busy for 72 % of the cycles.
 // What dK and dV need of a query beside its rows: -lse / scale and -delta, each as three bf16 numbers whose sum is the fp32 one.
 // A product with ones adds them to S and dP in the matrix core: as operands of an addition they would have to be in 16 registers,
 // read from LDS at eight times the bytes.
@@ -1155,8 +1156,9 @@ constexpr int kPartFloats = 2 * kRows * HD + 256;
 // So a wave holds one operand and one sum, not two (which with S and dP beside them pass the 256 registers that two waves a SIMD
 // have), and the two waves of a SIMD, one of each kind, are at the matrix core by turns.
 //
-// 3.18 ms, 1.15 PFLOP/s for its four products; the matrix core is busy for 59 % of the cycles, the rest are the barrier of a step and the
-// reads behind it. Steps of two tiles: 3.57 before the last round's blocks were cut (dkv_cut), 3.80 with steps of one. S and dP of the
+// 3.25 ms, 1.13 PFLOP/s for its four products; the matrix core is busy for 57 % of the cycles, the rest are the barrier of a step and the
+// reads behind it (3.18 without the minimum that holds weights below 2). Before that, steps of two tiles: 3.57 before the last round's blocks
+// were cut (dkv_cut), 3.80 with steps of one. S and dP of the
 // next tile before this one's rest, as the other kernels have it, was worth 2 % here and cost 40 % with 64 channels a head.
 template <int HD>
 __global__ __launch_bounds__(512, HD == 64 ? 4 : 2) void packed_dkv_kernel(PackedArgs a) {
@@ -1413,7 +1415,8 @@ int64_t slots(int64_t rows, int seqs) { return rows / kRows + seqs + 1; }
 // share the card. Split, there are two launches, and 256 workgroups take 0.24 us for each of the tiles of all items. That is from
 // 12 heads of 128 over 12 and 2, 1 to 64 sequences of 1 to 1024 queries and 512 to 43200 keys: one query over 43200 keys 17 us
 // split, 526 not; 256 queries 143 and 537; 1024 queries 489 and 547, over 4096 keys 83 and 66; 64 queries each of 64 sequences over
-// 4096 keys, 12 heads over 2, 244 and 204, 32 queries 132 and 184. The lengths' products have to stay below kMostWork.
+// 4096 keys, 12 heads over 2, 244 and 204, 32 queries 132 and 184. Heads of 64 channels go by the same figures, which were not taken for
+// them. The lengths' products have to stay below kMostWork.
 bool split(int seqs, int64_t tq, int64_t tk, int heads, int kv_heads) {
   const int64_t group = heads / kv_heads;
   if ((ceil_div(tq * group, kTile) + seqs) * (ceil_div(tk, kTile) + seqs) * kv_heads >= kMostWork) return false;
