@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a block: 4 waves of 32
 constexpr int kTile = 32;       // rows of a tile of the other side
-constexpr float kRise = 256.f;
+constexpr float kRise = 4096.f, kAbove = 20.f, kAbove2 = 1048576.f;   // kAbove2 = 2^kAbove
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A tile of 32 rows of HD channels in LDS (D <= HD, zeros past D): rows of 2 HD bytes, whose 16-byte chunks are XOR-swizzled by
@@ -349,6 +349,11 @@ __device__ __forceinline__ int keys_seen(const PackedArgs& a, const Span& s, int
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
+// lse of a row from its reference and sum; kAbove is taken off both, for the logarithm to keep its last bits
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m - kAbove + __builtin_amdgcn_logf(l * kAbove2)) * kLn2;
+}
+
 // A softmax in progress for the lane's query: reference m (log2 units), sum l of this lane's half of the keys, unnormalised
 // output (channels x queries).
 template <int HD>
@@ -371,10 +376,13 @@ struct Soft {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = elem_row(i) < lim - k0 - 4 * g ? s[i] : -INFINITY;
     }
-    // The reference is the row's maximum in the first tile that it sees. Later ones are taken as they come while their
-    // exponentials' sum stays below kRise (what is off a bfloat16 P or a 32-bit sum does not depend on the reference); where it does
-    // not, or is NaN, the reference rises to their maximum: rare, and a branch of the whole wave. The sums on the way then stay below
-    // 16 n |V| over n keys: finite for every |V| below 2^124 / n. (With a reference that only rises at 2^32 they were finite below 2^100 / n.)
+    // The reference is kAbove more than the row's maximum in the first tile that it sees. Later ones are taken as they come while their
+    // exponentials' sum stays below kRise (a bfloat16 P and a 32-bit sum are as near whatever the reference is); where it does not, or is
+    // NaN, the reference rises to kAbove more than their maximum: rare, as it takes scores 32 above the first ones, and a branch of the whole
+    // wave. The sums on the way stay below 2^8 n |V| over n keys, finite for every |V| below 2^120 / n; a row's largest term is 2^-20 |V| or
+    // more, which fp32 holds to bfloat16's precision for values from 2^-120 on. With the maximum itself as the reference, rising at 2^8 took
+    // 29 % where scores have a deviation of 8 (4096 x 4096, 12 heads of 64: 74 -> 95 us, 74 so), and rising at 2^32 values from 2^100 / n
+    // on passed the largest float.
     float part = 0.f;
     f32x16 p;
     auto take = [&] {
@@ -395,7 +403,7 @@ struct Soft {
       float mx = s[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      const float to = fmaxf(m, pair_max(mx) * c);
+      const float to = fmaxf(m, fmaf(pair_max(mx), c, kAbove));
       const float by = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
       m = to;
       l *= by;
@@ -508,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
       float mx = sA[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sA[e]);
-      soft.m = fmaxf(pair_max(mx) * a.c, -3e38f);   // finite, also where infinities in K leave nothing of this tile
+      soft.m = fmaxf(fmaf(pair_max(mx), a.c, kAbove), -3e38f);   // finite, also where infinities in K leave nothing of this tile
     }
     pB[0] = pB[1] = bf16x8{};
     const float c = a.c;
@@ -578,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
         float mx = s_cur[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s_cur[e]);
-        const float to = pair_max(part) <= kRise ? soft.m : fmaxf(soft.m, pair_max(mx) * c);
+        const float to = pair_max(part) <= kRise ? soft.m : fmaxf(soft.m, fmaf(pair_max(mx), c, kAbove));
         const float by = __builtin_amdgcn_exp2f(soft.m - to);
         soft.m = to;
         soft.l *= by;
@@ -624,7 +632,7 @@ __global__ __launch_bounds__(256, 2) void packed_forward_kernel(PackedArgs a) {
     const float l = pair_sum(soft.l);
     store_row<HD>(a.o.p + (int64_t)(s.q0 + i) * a.o.t + head * a.o.h, a.D, soft.acc, l == 0.f ? 0.f : 1.f / l);
     if (a.lse && g == 0)
-      a.lse[(int64_t)head * a.tq + s.q0 + i] = l == 0.f ? -INFINITY : (soft.m + __builtin_amdgcn_logf(l)) * kLn2;
+      a.lse[(int64_t)head * a.tq + s.q0 + i] = lse_of(soft.m, l);
   }
   FVSR_WAIT_VM0();   // no copy outlives the workgroup's LDS
 }
@@ -856,7 +864,7 @@ __global__ __launch_bounds__(256, 1) void packed_split_kernel(PackedArgs a) {
           *(bf16x4*)(a.o.p + (int64_t)(s.q0 + qi) * a.o.t + qh * a.o.h + 4 * piece) = o;
         }
         if (a.lse && piece == 0)
-          a.lse[(int64_t)qh * a.tq + s.q0 + qi] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+          a.lse[(int64_t)qh * a.tq + s.q0 + qi] = lse_of(m, l);
       } else {
         *(f32x4*)(part + row * HD + 4 * piece) = x;
         if (piece == 0) {
@@ -929,7 +937,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedArgs a) {
       for (int e = 0; e < 4; ++e) o[e] = (bf16)(v[e] * inv);
       *(bf16x4*)(a.o.p + (int64_t)qi * a.o.t + qh * a.o.h + 4 * col) = o;
     }
-    if (a.lse && col == 0) a.lse[(int64_t)qh * a.tq + qi] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
+    if (a.lse && col == 0) a.lse[(int64_t)qh * a.tq + qi] = lse_of(top, l);
   }
 }
 

@@ -109,6 +109,21 @@ def test_large_values_stay_finite(dev, d, m, n, causal):
     within(lse, ref["lse"], ref["tol_lse"], "lse")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("m,n,causal", [(900, 700, False), (300, 300, True), (1, 3000, False), (2, 2, True)])
+def test_small_values_keep_their_precision(dev, d, m, n, causal):
+    """Values near 2^-112: products with the smallest unnormalised weights that count are below fp32's normal numbers. An addition there is
+    off by 2^-150 at most, and a row's sum of weights is 2^-20 or more: n 2^-130 beside the other errors."""
+    g = gen_of("small", d, m, n)
+    h = 12 if m == 900 else 2
+    q, k, v = randn(g, (m, h, d), dev, scale=1.5), randn(g, (n, 1, d), dev), randn(g, (n, 1, d), dev, scale=2.0 ** -112)
+    cu_q, cu_k = (torch.tensor([0, x], dtype=torch.int32, device=dev) for x in (m, n))
+    ref = attention64(q, k, v, [0, m], [0, n], causal)
+    o, lse = f.packed_attention(q, k, v, cu_q, cu_k, causal=causal, want_lse=True)
+    within(o, ref["o"], ref["tol_o"] + n * 2.0 ** -130, "o")
+    within(lse, ref["lse"], ref["tol_lse"], "lse")
+
+
 @pytest.mark.parametrize("nq", [1, 300])
 @pytest.mark.parametrize("d", [64, 128])
 def test_weights_that_round_above_two_keep_their_gradient(dev, nq, d):
